@@ -256,6 +256,114 @@ NSFPS_API int nsfps_group_points_device(const float *d_xyz, const uint64_t *poin
                               uint64_t count, uint32_t nsample, const int64_t *d_idx,
                               float *d_out, void *stream);
 
+/* ---- Features of sampled clouds: row lookup by index with its gradient, the
+ * choice of the nearest blocks of a cloud, and attention over chosen blocks
+ * with its gradient.  No counterpart in the reference, which stops at the
+ * sample indices; these are what a point network does with them next.
+ *
+ * All of these calls are asynchronous: they issue kernels on `stream` of the
+ * current device and return.  They keep no state and allocate nothing; scratch
+ * comes from the caller (`d_work`, at least the bytes the matching _workspace
+ * call gives, 256-byte aligned), so calls on different streams, or captured
+ * into different graphs, need only have different scratch.  Results do not
+ * depend on how the work is scheduled: the same inputs give the same bits. */
+enum nsfps_dtype { NSFPS_F32 = 0, NSFPS_F16 = 1, NSFPS_BF16 = 2 };
+
+/* Lookup of `count` rows per batch entry in a table of `rows` rows of `width`
+ * elements, times `scale` (the product taken in fp32 and rounded once):
+ *   out[b][p][:] = scale * table[b][idx[b][p]][:]
+ * A negative index stands for no row: zeros, and no gradient.  An index of
+ * `rows` or more reads nothing: its output row is NaN, its gradient goes
+ * nowhere.  The table's elements are contiguous within a row; batch_stride
+ * and row_stride are in elements.  idx (batch x count int64) and out are
+ * dense. */
+typedef struct nsfps_rows_desc {
+  uint64_t batch, rows, width, count;
+  int64_t batch_stride, row_stride;
+  float scale;
+  int32_t dtype; /* nsfps_dtype of table and out */
+} nsfps_rows_desc;
+
+NSFPS_API int nsfps_gather_rows_device(const nsfps_rows_desc *desc, const void *d_table,
+                                       const int64_t *d_idx, void *d_out, void *stream);
+
+/* Gradient of the lookup with respect to the table (dense, batch x rows x
+ * width; the strides of `desc` are not used):
+ *   dtable[b][n][:] = scale * sum over p with idx[b][p] == n of dout[b][p][:]
+ * summed in fp32 in a fixed order of p and rounded once; rows that no index
+ * names are written as zeros.  batch * count and batch * rows below 2^31. */
+NSFPS_API int nsfps_gather_rows_grad_workspace(const nsfps_rows_desc *desc, uint64_t *bytes);
+NSFPS_API int nsfps_gather_rows_grad_device(const nsfps_rows_desc *desc, const void *d_dout,
+                                            const int64_t *d_idx, void *d_dtable, void *d_work,
+                                            uint64_t work_bytes, void *stream);
+
+/* Nearest blocks of a cloud.  Block j of a cloud is its points [j * block,
+ * (j + 1) * block) below the cloud's length; its distance to a centre is that
+ * of the block's bounding box, squared, in the sampler's arithmetic:
+ *   dx = max(max(lo_x - c_x, c_x - hi_x), 0), ...  d2 = (dx*dx + dy*dy) + dz*dz
+ * every operation fp32 rounded to nearest without contraction.  d_blocks
+ * receives, per centre, the `top` blocks of smallest (d2, j), ascending, and
+ * d_d2 (may be NULL) their d2; slots beyond the cloud's blocks get -1 and
+ * +inf.  d_xyz: batch x n x 3 and d_centers: batch x m x 3 floats, dense;
+ * d_lengths: batch int32 (clamped to 0..n), or NULL when every cloud has n
+ * points.  A NaN point coordinate is left out of its box, a NaN centre
+ * coordinate counts as inside every box.  block: 16, 32, 64 or 128; top:
+ * 1..NSFPS_MAX_TOP; batch * m and batch * n below 2^31. */
+#define NSFPS_MAX_TOP 64u
+typedef struct nsfps_select_desc {
+  uint64_t batch, points, centers;
+  uint32_t block, top;
+} nsfps_select_desc;
+
+NSFPS_API int nsfps_select_blocks_workspace(const nsfps_select_desc *desc, uint64_t *bytes);
+NSFPS_API int nsfps_select_blocks_device(const nsfps_select_desc *desc, const float *d_xyz,
+                                         const int32_t *d_lengths, const float *d_centers,
+                                         int64_t *d_blocks, float *d_d2, void *d_work,
+                                         uint64_t work_bytes, void *stream);
+
+/* Attention of every query over the blocks chosen for it:
+ *   out[b][m][h] = sum_t p_t v[b][t][g], p = softmax_t(scale * q[b][m][h] . k[b][t][g]),
+ * g = h / (heads / kv_heads), t over the keys below the cloud's length of the
+ * blocks that blocks[b][m][0 .. top) lists.  The list is a set: an entry that
+ * occurs again, is negative or names no block of the cloud counts for nothing.
+ * A query without a key gets zeros (and no gradient).  What lies behind a
+ * cloud's length is never part of a result, whatever its value.
+ * q, k and v: F16 or BF16, elements of a head contiguous, 16-byte aligned, the
+ * strides (batch, row, head, in elements) multiples of 8.  blocks (batch x
+ * queries x top int64), out (batch x queries x heads x head_dim) and lse
+ * (batch x queries x heads fp32: log of the softmax sum, -inf without a key;
+ * may be NULL) are dense.  head_dim: a multiple of 8 up to 128; block: 16, 32,
+ * 64 or 128; top: 1..NSFPS_MAX_TOP; heads a multiple of kv_heads, at most 256.
+ * batch * queries * top and batch * keys below 2^30. */
+typedef struct nsfps_attention_desc {
+  uint64_t batch, queries, keys;
+  uint32_t heads, kv_heads, head_dim, block, top;
+  int32_t dtype;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  float scale;
+  uint32_t reserved; /* 0 */
+} nsfps_attention_desc;
+
+/* Scratch of the forward (backward == 0) or the gradient call. */
+NSFPS_API int nsfps_block_attention_workspace(const nsfps_attention_desc *desc, int backward,
+                                              uint64_t *bytes);
+NSFPS_API int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d_q,
+                                           const void *d_k, const void *d_v,
+                                           const int64_t *d_blocks, const int32_t *d_lengths,
+                                           void *d_out, float *d_lse, void *d_work,
+                                           uint64_t work_bytes, void *stream);
+
+/* Gradient: dq (dense, like out), dk and dv (dense, batch x keys x kv_heads x
+ * head_dim; keys that no query reads get zeros) from dout (dense, like out,
+ * 16-byte aligned) and the forward's out and lse. */
+NSFPS_API int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const void *d_q,
+                                                const void *d_k, const void *d_v,
+                                                const int64_t *d_blocks,
+                                                const int32_t *d_lengths, const void *d_out,
+                                                const float *d_lse, const void *d_dout,
+                                                void *d_dq, void *d_dk, void *d_dv, void *d_work,
+                                                uint64_t work_bytes, void *stream);
+
 /* Timing and work counters of the last call on this thread: stage times in
  * milliseconds measured with CUDA events on the launching stream (setup =
  * binning, sort and leaf build; loop = the persistent sampling kernel;

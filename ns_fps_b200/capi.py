@@ -277,3 +277,113 @@ def group_points_device(d_xyz_ptr: int, point_offsets, d_centers_ptr: int, cente
         ctypes.c_void_p(d_idx_ptr), ctypes.c_void_p(d_out_ptr), ctypes.c_void_p(stream_ptr))
     if rc != OK:
         raise RuntimeError(f"nsfps_group_points_device rc={rc}: {last_error()}")
+
+
+# ---------------------------------------------------------------- features
+
+F32, F16, BF16 = range(3)
+
+
+class RowsDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("rows", ctypes.c_uint64), ("width", ctypes.c_uint64),
+                ("count", ctypes.c_uint64), ("batch_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("dtype", ctypes.c_int32)]
+
+
+class SelectDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("points", ctypes.c_uint64),
+                ("centers", ctypes.c_uint64), ("block", ctypes.c_uint32),
+                ("top", ctypes.c_uint32)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("queries", ctypes.c_uint64),
+                ("keys", ctypes.c_uint64), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("block", ctypes.c_uint32), ("top", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_uint32)]
+
+
+def _ok(rc, name):
+    if rc != OK:
+        raise RuntimeError(f"{name} rc={rc}: {last_error()}")
+
+
+def _ptr(p):
+    return ctypes.c_void_p(p or None)
+
+
+def gather_rows_device(desc: RowsDesc, d_table_ptr: int, d_idx_ptr: int, d_out_ptr: int,
+                       stream_ptr: int = 0):
+    """nsfps_gather_rows_device."""
+    _ok(lib().nsfps_gather_rows_device(ctypes.byref(desc), _ptr(d_table_ptr), _ptr(d_idx_ptr),
+                                       _ptr(d_out_ptr), _ptr(stream_ptr)),
+        "nsfps_gather_rows_device")
+
+
+def gather_rows_grad_workspace(desc: RowsDesc) -> int:
+    """nsfps_gather_rows_grad_workspace: bytes of scratch."""
+    n = ctypes.c_uint64(0)
+    _ok(lib().nsfps_gather_rows_grad_workspace(ctypes.byref(desc), ctypes.byref(n)),
+        "nsfps_gather_rows_grad_workspace")
+    return n.value
+
+
+def gather_rows_grad_device(desc: RowsDesc, d_dout_ptr: int, d_idx_ptr: int, d_dtable_ptr: int,
+                            d_work_ptr: int, work_bytes: int, stream_ptr: int = 0):
+    """nsfps_gather_rows_grad_device."""
+    _ok(lib().nsfps_gather_rows_grad_device(ctypes.byref(desc), _ptr(d_dout_ptr), _ptr(d_idx_ptr),
+                                            _ptr(d_dtable_ptr), _ptr(d_work_ptr),
+                                            ctypes.c_uint64(work_bytes), _ptr(stream_ptr)),
+        "nsfps_gather_rows_grad_device")
+
+
+def select_blocks_workspace(desc: SelectDesc) -> int:
+    """nsfps_select_blocks_workspace: bytes of scratch."""
+    n = ctypes.c_uint64(0)
+    _ok(lib().nsfps_select_blocks_workspace(ctypes.byref(desc), ctypes.byref(n)),
+        "nsfps_select_blocks_workspace")
+    return n.value
+
+
+def select_blocks_device(desc: SelectDesc, d_xyz_ptr: int, d_lengths_ptr: int,
+                         d_centers_ptr: int, d_blocks_ptr: int, d_d2_ptr: int, d_work_ptr: int,
+                         work_bytes: int, stream_ptr: int = 0):
+    """nsfps_select_blocks_device (d_lengths_ptr, d_d2_ptr: 0 for NULL)."""
+    _ok(lib().nsfps_select_blocks_device(ctypes.byref(desc), _ptr(d_xyz_ptr), _ptr(d_lengths_ptr),
+                                         _ptr(d_centers_ptr), _ptr(d_blocks_ptr), _ptr(d_d2_ptr),
+                                         _ptr(d_work_ptr), ctypes.c_uint64(work_bytes),
+                                         _ptr(stream_ptr)),
+        "nsfps_select_blocks_device")
+
+
+def block_attention_workspace(desc: AttentionDesc, backward: bool) -> int:
+    """nsfps_block_attention_workspace: bytes of scratch."""
+    n = ctypes.c_uint64(0)
+    _ok(lib().nsfps_block_attention_workspace(ctypes.byref(desc),
+                                              ctypes.c_int(1 if backward else 0),
+                                              ctypes.byref(n)),
+        "nsfps_block_attention_workspace")
+    return n.value
+
+
+def block_attention_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int, lengths: int,
+                           out: int, lse: int, work: int, work_bytes: int, stream_ptr: int = 0):
+    """nsfps_block_attention_device on device addresses (lengths, lse: 0 for
+    NULL)."""
+    _ok(lib().nsfps_block_attention_device(
+        ctypes.byref(desc), *map(_ptr, (q, k, v, blocks, lengths, out, lse, work)),
+        ctypes.c_uint64(work_bytes), _ptr(stream_ptr)), "nsfps_block_attention_device")
+
+
+def block_attention_grad_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int,
+                                lengths: int, out: int, lse: int, dout: int, dq: int, dk: int,
+                                dv: int, work: int, work_bytes: int, stream_ptr: int = 0):
+    """nsfps_block_attention_grad_device on device addresses."""
+    _ok(lib().nsfps_block_attention_grad_device(
+        ctypes.byref(desc),
+        *map(_ptr, (q, k, v, blocks, lengths, out, lse, dout, dq, dk, dv, work)),
+        ctypes.c_uint64(work_bytes), _ptr(stream_ptr)), "nsfps_block_attention_grad_device")

@@ -8,8 +8,10 @@ follow farthest point sampling.
 * ``gather_points(points, idx)``: the coordinates of the indexed points.
 * ``group_points(points, centers, idx)``: those of ``idx`` (M, nsample)
   minus their centre, shape (M, nsample, 3).
+* ``gather_rows(table, idx, scale)``: the feature rows that indices name,
+  with their gradient.
 
-Each takes one cloud (N, 3) or a batch (B, N, 3) with matching (B, M, ...)
+The first three take coordinates.  Each takes one cloud (N, 3) or a batch (B, N, 3) with matching (B, M, ...)
 centres / indices, runs on PyTorch's current stream through the C ABI
 (``nsfps_ball_query_device`` and friends) and returns CUDA tensors.  The
 distance test is the sampler's: d2 = (dx*dx + dy*dy) + dz*dz, fp32 rounded
@@ -19,7 +21,7 @@ from __future__ import annotations
 
 from . import capi
 
-__all__ = ["ball_query", "gather_points", "group_points"]
+__all__ = ["ball_query", "gather_points", "group_points", "gather_rows"]
 
 
 def _cloud_batch(t, name):
@@ -103,3 +105,115 @@ def group_points(points, centers, idx):
         capi.group_points_device(pts.data_ptr(), _offsets(B, N), ctr.data_ptr(), _offsets(B, M),
                                  S, ix.data_ptr(), out.data_ptr(), stream.cuda_stream)
     return out[0] if single else out
+
+
+def _dtype_code(t, name, allowed):
+    import torch
+    code = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(t.dtype)
+    if code is None or code not in allowed:
+        names = {capi.F32: "float32", capi.F16: "float16", capi.BF16: "bfloat16"}
+        raise TypeError(f"{name} must be " + " or ".join(names[a] for a in allowed))
+    return code
+
+
+def _scratch(nbytes, device):
+    """Scratch of one call, from PyTorch's allocator on the current stream."""
+    import torch
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _rows_desc(B, N, C, P, scale, code, batch_stride=0, row_stride=0):
+    return capi.RowsDesc(B, N, C, P, batch_stride, row_stride, scale, code)
+
+
+def _gather_rows_forward(table, idx, scale):
+    import torch
+    single = table.dim() == 2
+    B, N, C = (1, *table.shape) if single else table.shape
+    if (C > 1 and table.stride(-1) != 1) or C == 0:
+        table = table.contiguous()
+    idx = idx.contiguous()
+    out = torch.empty((*idx.shape, C), dtype=table.dtype, device=table.device)
+    P = idx.numel() // B if B else 0
+    desc = _rows_desc(B, N, C, P, scale, _dtype_code(table, "table", (0, 1, 2)),
+                      0 if single else table.stride(0), table.stride(-2))
+    with torch.cuda.device(table.device):
+        stream = torch.cuda.current_stream(table.device)
+        capi.gather_rows_device(desc, table.data_ptr(), idx.data_ptr(), out.data_ptr(),
+                                stream.cuda_stream)
+    return out
+
+
+def _gather_rows_backward(dout, idx, shape, scale):
+    import torch
+    B, N, C = (1, *shape) if len(shape) == 2 else shape
+    dout, idx = dout.contiguous(), idx.contiguous()
+    grad = torch.empty(shape, dtype=dout.dtype, device=dout.device)
+    P = idx.numel() // B if B else 0
+    desc = _rows_desc(B, N, C, P, scale, _dtype_code(dout, "grad", (0, 1, 2)))
+    with torch.cuda.device(dout.device):
+        stream = torch.cuda.current_stream(dout.device)
+        work = _scratch(capi.gather_rows_grad_workspace(desc), dout.device)
+        capi.gather_rows_grad_device(desc, dout.data_ptr(), idx.data_ptr(), grad.data_ptr(),
+                                     work.data_ptr(), work.numel(), stream.cuda_stream)
+    return grad
+
+
+_gather_rows_function = None
+
+
+def _gather_rows_autograd():
+    """The autograd node, made at its first use (the module itself does not
+    need PyTorch)."""
+    global _gather_rows_function
+    if _gather_rows_function is None:
+        import torch
+        from torch.autograd.function import once_differentiable
+
+        class GatherRows(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, table, idx, scale):
+                ctx.save_for_backward(idx)
+                ctx.shape, ctx.scale = table.shape, scale
+                return _gather_rows_forward(table, idx, scale)
+
+            @staticmethod
+            @once_differentiable
+            def backward(ctx, dout):
+                idx, = ctx.saved_tensors
+                return _gather_rows_backward(dout, idx, ctx.shape, ctx.scale), None, None
+
+        _gather_rows_function = GatherRows
+    return _gather_rows_function
+
+
+def gather_rows(table, idx, scale: float = 1.0):
+    """``scale * table[idx]``: the feature rows that ``idx`` names, with a
+    gradient for ``table``.
+
+    table  (N, C), or (B, N, C) for B clouds: float32, float16 or bfloat16
+    idx    int64: any shape for (N, C); (B, ...) for (B, N, C)
+
+    Returns idx.shape + (C,) in the table's type (the product in float32,
+    rounded once).  A negative index stands for no row: zeros, and no gradient.
+    An index of N or more is never read: its row is NaN, and its gradient goes
+    nowhere.  The gradient adds a row's entries in float32 in index order, so
+    it is the same every time.  Runs on PyTorch's current stream without
+    waiting for it.
+    """
+    import torch
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise TypeError("table must be a CUDA tensor")
+    if not isinstance(idx, torch.Tensor) or not idx.is_cuda or idx.dtype != torch.int64:
+        raise TypeError("idx must be an int64 CUDA tensor")
+    _dtype_code(table, "table", (capi.F32, capi.F16, capi.BF16))
+    if table.dim() not in (2, 3):
+        raise ValueError("table: expected shape (N, C) or (B, N, C)")
+    if table.dim() == 3 and (idx.dim() < 1 or idx.shape[0] != table.shape[0]):
+        raise ValueError("idx must have shape (B, ...) for a (B, N, C) table")
+    if table.device != idx.device:
+        raise ValueError("table and idx must be on the same device")
+    scale = float(scale)
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _gather_rows_autograd().apply(table, idx, scale)
+    return _gather_rows_forward(table, idx, scale)

@@ -1,0 +1,316 @@
+"""Attention over listed blocks and its gradients against 64-bit formulas,
+with tolerances that count the roundings of the definition."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+U32 = 2.0 ** -24
+
+
+def _normal(shape, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=g).to(dtype)
+
+
+def _lists(B, M, nb, top, seed):
+    """Distinct blocks per query in no order, -1 behind the last block."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    order = torch.rand(B, M, nb, device="cuda", generator=g).argsort(2)[..., :top]
+    return torch.nn.functional.pad(order, (0, top - order.shape[2]), value=-1)
+
+
+def _seen(blocks, block, N, lengths, B):
+    """(B, M, N): whether a query reads a key."""
+    nb = (N + block - 1) // block
+    member = torch.zeros(*blocks.shape[:2], nb + 1, dtype=torch.bool, device="cuda")
+    member.scatter_(2, torch.where((blocks < 0) | (blocks >= nb), nb, blocks), True)
+    seen = member[..., :nb].repeat_interleave(block, dim=2)[..., :N]
+    if lengths is not None:
+        seen = seen & (torch.arange(N, device="cuda") < lengths[:, None])[:, None, :]
+    return seen
+
+
+class Exact:
+    """out, dq, dk, dv in 64 bits, and how far the operator may be off.
+
+    The operator works in fp32 and rounds, besides its outputs, the weights p
+    (for p v and p^T dout) and ds (for ds k and ds^T q) to the type, half a
+    step u each (at least half a step of the smallest numbers); its delta comes
+    from the rounded out.  An fp32 score is off by at most (D + 4) U32 of the
+    sum of its terms' magnitudes, which p takes on as a relative error."""
+
+    def __init__(self, q, k, v, blocks, block, lengths=None, scale=None, dout=None):
+        dtype, (B, M, H, D), (N, G) = q.dtype, q.shape, k.shape[1:3]
+        scale = 1 / math.sqrt(D) if scale is None else scale
+        u = torch.finfo(dtype).eps / 2
+        tiny = torch.finfo(dtype).smallest_normal * u
+        seen = _seen(blocks, block, N, lengths, B)[:, None]             # B 1 M N
+        valid = torch.ones(B, N, dtype=torch.bool, device="cuda")
+        if lengths is not None:
+            valid = torch.arange(N, device="cuda") < lengths[:, None]
+        clean = [torch.where(valid[..., None, None], t.double(), 0.0) for t in (k, v)]
+        kh, vh = (t.repeat_interleave(H // G, dim=2).transpose(1, 2) for t in clean)
+        qh = q.double().transpose(1, 2)
+        s = (qh @ kh.transpose(2, 3) * scale).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, dim=-1).nan_to_num(0.0)
+        off_s = (qh.abs() @ kh.abs().transpose(2, 3)) * abs(scale) * (D + 4) * U32
+        off_s = torch.where(seen, off_s, 0.0).amax(-1, keepdim=True)
+        rel = 2 * off_s + (64 + seen.sum(-1, keepdim=True)) * U32        # of p, in fp32
+        out = p @ vh
+        mag = (p * (u + rel) + tiny) @ vh.abs() * 1.01
+        self.out, self.out_off = out.transpose(1, 2), (mag + u * out.abs() + tiny).transpose(1, 2)
+        if dout is None:
+            return
+        do = dout.double().transpose(1, 2)
+        dp = do @ vh.transpose(2, 3)
+        delta = (p * dp).sum(-1, keepdim=True)
+        ds = p * (dp - delta) * scale
+        off_delta = (do.abs() * (mag + u * out.abs() + tiny)).sum(-1, keepdim=True)
+        off_dp = (do.abs() @ vh.abs().transpose(2, 3)) * (D + 4) * U32
+        off_ds = (abs(scale) * p * (off_delta + off_dp + (dp.abs() + delta.abs()) * rel) * 1.01 +
+                  u * ds.abs() * 1.01 + tiny)
+        off_ds = torch.where(seen, off_ds, 0.0)
+        n = (64 + M * H // G + N) * U32                                  # fp32 sums
+
+        def heads(t):  # B H N D -> B N G D, query heads of a key head summed
+            return t.reshape(B, G, H // G, N, D).sum(2).transpose(1, 2)
+
+        dq = ds @ kh
+        self.dq = dq.transpose(1, 2)
+        self.dq_off = (off_ds @ kh.abs() + u * dq.abs() + n * (ds.abs() @ kh.abs()) +
+                       tiny).transpose(1, 2)
+        off_p = torch.where(seen, p * (u + rel) * 1.01 + tiny, 0.0)
+        self.dk = heads(ds.transpose(2, 3) @ qh)
+        self.dk_off = (heads(off_ds.transpose(2, 3) @ qh.abs() +
+                             n * (ds.abs().transpose(2, 3) @ qh.abs())) + u * self.dk.abs() + tiny)
+        self.dv = heads(p.transpose(2, 3) @ do)
+        self.dv_off = (heads(off_p.transpose(2, 3) @ do.abs() +
+                             n * (p.transpose(2, 3) @ do.abs())) + u * self.dv.abs() + tiny)
+
+
+def _check(q, k, v, blocks, block, lengths=None, scale=None, train=True):
+    from ns_fps_b200 import attention
+    dout = _normal(q.shape, q.dtype, 99) if train else None
+    ref = Exact(q, k, v, blocks, block, lengths, scale, dout)
+    out = attention.block_attention(q, k, v, blocks, block, lengths=lengths, scale=scale)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    assert bool(((out.double() - ref.out).abs() <= ref.out_off).all())
+    if not train:
+        return out
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    again = attention.block_attention(*leaves, blocks, block, lengths=lengths, scale=scale)
+    assert torch.equal(again.detach(), out)
+    grads = torch.autograd.grad(again, leaves, dout)
+    for name, g, t in zip(("dq", "dk", "dv"), grads, (q, k, v)):
+        assert g.shape == t.shape and g.dtype == t.dtype
+        off = (g.double() - getattr(ref, name)).abs()
+        assert bool((off <= getattr(ref, name + "_off")).all()), name
+    return out
+
+
+CASES = [  # B, M, N, H, G, D, block, top
+    (1, 1, 1, 1, 1, 8, 16, 1),
+    (1, 1, 1000, 8, 8, 64, 64, 16),
+    (1, 3, 40, 2, 1, 16, 16, 64),
+    (2, 37, 333, 4, 2, 40, 16, 5),
+    (1, 130, 513, 6, 2, 72, 32, 9),
+    (3, 65, 200, 3, 1, 128, 128, 2),
+    (1, 20, 4500, 16, 1, 64, 64, 64),
+    (1, 300, 2100, 2, 2, 64, 32, 16),
+    (1, 500, 96, 4, 4, 32, 16, 6),
+    (2, 257, 1030, 8, 2, 128, 64, 8),
+    (1, 64, 700, 48, 2, 24, 128, 5),
+    (1, 1000, 3000, 1, 1, 112, 32, 24),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", CASES)
+def test_matches_the_formulas(case, dtype):
+    B, M, N, H, G, D, block, top = case
+    q, k, v = _normal((B, M, H, D), dtype, 1), _normal((B, N, G, D), dtype, 2), \
+        _normal((B, N, G, D), dtype, 3)
+    _check(q, k, v, _lists(B, M, (N + block - 1) // block, top, 4), block)
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_padded_clouds_and_lists_that_name_nothing(block):
+    """Lengths of 0, 1, inside a block and behind the end; entries that repeat,
+    are negative or too large; queries without a key; NaN and infinities in
+    what is padding."""
+    B, M, N, H, G, D, top = 5, 90, 390, 4, 2, 64, 6
+    dtype = torch.bfloat16
+    q, k, v = _normal((B, M, H, D), dtype, 1), _normal((B, N, G, D), dtype, 2), \
+        _normal((B, N, G, D), dtype, 3)
+    lengths = torch.tensor([N, 0, 1, 200, 139], dtype=torch.int32, device="cuda")
+    pad = torch.arange(N, device="cuda")[None, :] >= lengths[:, None]
+    k[pad], v[pad] = math.nan, math.inf
+    nb = (N + block - 1) // block
+    blocks = _lists(B, M, nb, top, 4)
+    blocks[:, ::7, 3] = blocks[:, ::7, 0]
+    blocks[:, 1::7, :2] = -5
+    blocks[:, 2::7, 1] = nb
+    blocks[:, 3::7, 2] = 2 ** 40
+    blocks[:, 4::7] = -1
+    blocks[:, 5::7] = 0
+    out = _check(q, k, v, blocks, block, lengths)
+    assert not out[1].any() and not out[:, 4::7].any()
+
+
+def test_every_query_lists_the_same_block():
+    q, k, v = _normal((1, 5000, 2, 64), torch.bfloat16, 1), \
+        _normal((1, 100, 1, 64), torch.bfloat16, 2), _normal((1, 100, 1, 64), torch.bfloat16, 3)
+    blocks = torch.full((1, 5000, 3), 1, dtype=torch.int64, device="cuda")
+    _check(q, k, v, blocks, 16)
+
+
+@pytest.mark.parametrize("scale", [0.0, 4.0, -0.3])
+def test_scales(scale):
+    """Uniform weights, weights of nearly one key, and a negative scale."""
+    q, k, v = _normal((1, 60, 2, 48), torch.float16, 1), _normal((1, 500, 2, 48), torch.float16, 2), \
+        _normal((1, 500, 2, 48), torch.float16, 3)
+    _check(q, k, v, _lists(1, 60, 32, 7, 4), 16, scale=scale)
+
+
+def test_single_cloud_views_and_unaligned_inputs():
+    from ns_fps_b200 import attention
+    packed = _normal((2, 300, 3, 4, 64), torch.bfloat16, 1)
+    q, k, v = packed[:, :70, 0], packed[:, :, 1], packed[:, :, 2]
+    blocks = _lists(2, 70, 10, 4, 2)
+    out = _check(q, k, v, blocks, 32)
+    one = attention.block_attention(q[1], k[1], v[1], blocks[1], 32)
+    assert torch.equal(one, out[1])
+    wide = _normal((2, 300, 4, 67), torch.bfloat16, 5)
+    _check(wide[:, :70, :, 3:], wide[..., 1:65], wide[..., 2:66], blocks, 32)
+    _check(k.transpose(1, 2).contiguous().transpose(1, 2)[:, :70], k, v, blocks, 32)
+    _check(k[:1, :70].expand(2, 70, 4, 64), k[:1].expand(2, 300, 4, 64), v, blocks, 32)
+
+
+def test_empty_sizes():
+    from ns_fps_b200 import attention
+    for B, M, N in [(0, 3, 4), (2, 0, 40), (2, 3, 0)]:
+        leaves = [torch.zeros(B, n, 2, 16, device="cuda", dtype=torch.float16, requires_grad=True)
+                  for n in (M, N, N)]
+        blocks = torch.zeros(B, M, 2, dtype=torch.int64, device="cuda")
+        out = attention.block_attention(*leaves, blocks, 16)
+        assert out.shape == (B, M, 2, 16) and not out.any()
+        for g, t in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), leaves):
+            assert g.shape == t.shape and not g.any()
+
+
+def test_gradient_matches_differences():
+    """Differences of the 64-bit formula along a direction against the
+    operator's gradient."""
+    from ns_fps_b200 import attention
+    x = [_normal(s, torch.float16, i) for i, s in enumerate([(1, 30, 2, 32), (1, 90, 1, 32),
+                                                            (1, 90, 1, 32)])]
+    d = [_normal(t.shape, torch.float64, 10 + i) for i, t in enumerate(x)]
+    blocks, w = _lists(1, 30, 6, 3, 7), _normal(x[0].shape, torch.float16, 8)
+    leaves = [t.detach().requires_grad_() for t in x]
+    grads = torch.autograd.grad(attention.block_attention(*leaves, blocks, 16), leaves, w)
+    got = sum(float((g.double() * y).sum()) for g, y in zip(grads, d))
+    h = 1e-4
+
+    def value(s):
+        q, k, v = (t.double() + s * h * y for t, y in zip(x, d))
+        kh, vh = (t.expand(1, 90, 2, 32).transpose(1, 2) for t in (k, v))
+        a = q.transpose(1, 2) @ kh.transpose(2, 3) / math.sqrt(32)
+        a = a.masked_fill(~_seen(blocks, 16, 90, None, 1)[:, None], -math.inf)
+        return float(((torch.softmax(a, -1) @ vh).transpose(1, 2) * w.double()).sum())
+
+    ref = Exact(*x, blocks, 16, None, None, w)
+    bound = sum(float((getattr(ref, n + "_off") * y.abs()).sum())
+                for n, y in zip(("dq", "dk", "dv"), d))
+    # the difference itself is off by a third derivative times h^2 / 6
+    assert abs((value(1) - value(-1)) / (2 * h) - got) <= bound + 1e-3
+
+
+def test_same_bits_again_on_another_stream_and_in_graphs():
+    from ns_fps_b200 import attention
+    q, k, v = _normal((2, 400, 4, 64), torch.bfloat16, 1), _normal((2, 1500, 2, 64), torch.bfloat16, 2), \
+        _normal((2, 1500, 2, 64), torch.bfloat16, 3)
+    blocks, dout = _lists(2, 400, 47, 9, 4), _normal(q.shape, torch.bfloat16, 5)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = attention.block_attention(*leaves, blocks, 32)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = step()
+        graphs.append((graph, kept))
+    for graph, _ in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in (step(), other, graphs[0][1], graphs[1][1]):
+        for a, b in zip(first, got):
+            assert torch.equal(a, b)
+
+
+def test_sampler_to_attention_together():
+    """The run a point network makes: samples, their features, nearby blocks,
+    attention, and the gradient back into the features."""
+    import numpy as np
+
+    from ns_fps_b200 import attention, group, synthetic, torch_fps
+    cloud = synthetic.cluster_cloud(5000, seed=5)
+    cloud = cloud[np.lexsort(cloud.T)]
+    pts = torch.from_numpy(np.ascontiguousarray(cloud)).cuda()
+    H, D, block = 2, 32, 32
+    feats = _normal((5000, H * D), torch.bfloat16, 1).requires_grad_()
+    s = torch_fps.fps(pts, 256)
+    q = group.gather_rows(feats, s).view(-1, H, D)
+    blocks, d2 = attention.select_blocks(pts, group.gather_points(pts, s), block, 6)
+    assert bool((d2[:, 0] == 0).all())  # a sample lies in a box
+    kv = feats.view(-1, H, D)
+    out = attention.block_attention(q, kv, kv, blocks, block)
+    dout = _normal(out.shape, torch.bfloat16, 2)
+    grad, = torch.autograd.grad(out, feats, dout)
+    x = feats.detach().view(1, -1, H, D)
+    ref = Exact(x[:, s], x, x, blocks[None], block, None, None, dout[None])
+    assert bool(((out[None].double() - ref.out).abs() <= ref.out_off).all())
+    total, off = ref.dk + ref.dv, ref.dk_off + ref.dv_off
+    total[:, s] += ref.dq
+    off[:, s] += ref.dq_off
+    # PyTorch adds the three gradients in bf16: two more roundings
+    size = ref.dk.abs() + ref.dv.abs() + off
+    size[:, s] += ref.dq.abs()
+    err = (grad.view(1, -1, H, D).double() - total).abs()
+    assert bool((err <= off + 2 * 2.0 ** -8 * size * 1.01).all())
+
+
+def test_refusals():
+    from ns_fps_b200 import attention
+    q, k = _normal((1, 5, 4, 64), torch.bfloat16, 1), _normal((1, 50, 2, 64), torch.bfloat16, 2)
+    blocks = _lists(1, 5, 4, 2, 3)
+    one = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for args, error in [
+            ((q.float(), k.float(), k.float(), blocks, 16), TypeError),
+            ((q, k.half(), k.half(), blocks, 16), TypeError),
+            ((q, k, k[:, :40], blocks, 16), ValueError),
+            ((q, k, k, blocks.int(), 16), TypeError),
+            ((q, k, k, blocks, 20), ValueError),
+            ((q, k, k, blocks[:, :3], 16), ValueError),
+            ((q, k, k, blocks[..., :0], 16), ValueError),
+            ((q, k, k, blocks.repeat(1, 1, 40), 16), ValueError),
+            ((q[:, :, :3], k, k, blocks, 16), ValueError),
+            ((q[..., :60], k[..., :60], k[..., :60], blocks, 16), ValueError),
+            ((q[0], k, k, blocks, 16), ValueError),
+            ((q, k, k, blocks, 16, one.repeat(2)), ValueError),
+            ((q, k, k, blocks, 16, one.long()), TypeError),
+            ((q, k, k, blocks, 16, None, math.inf), RuntimeError)]:
+        with pytest.raises(error):
+            attention.block_attention(*args)
