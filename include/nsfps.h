@@ -334,7 +334,8 @@ NSFPS_API int nsfps_select_blocks_device(const nsfps_select_desc *desc, const fl
  * (batch x queries x heads fp32: log of the softmax sum, -inf without a key;
  * may be NULL) are dense.  head_dim: a multiple of 8 up to 128; block: 16, 32,
  * 64 or 128; top: 1..NSFPS_MAX_TOP; heads a multiple of kv_heads, at most 256.
- * batch * queries * top and batch * keys below 2^30. */
+ * batch below 2^27, batch * queries * top and batch * keys below 2^30, queries *
+ * top * heads / kv_heads below 2^31. */
 typedef struct nsfps_attention_desc {
   uint64_t batch, queries, keys;
   uint32_t heads, kv_heads, head_dim, block, top;

@@ -1,5 +1,23 @@
 // nsfps_attention.cu -- attention over the blocks of keys chosen for each
 // query, and its gradient.
+//
+// A query reads few keys, and neighbouring queries read the same ones, so the
+// work is turned round: the keys are cut into spans of kSpan consecutive keys,
+// and every (query, span) pair that shares a key is sorted by span.  A CTA
+// takes a run of pairs of one span, gathers their query rows into matrix
+// tiles, and meets the span's keys once for all of them (mma.sync on 16-bit
+// operands, fp32 accumulators).  Each pair leaves a partial result in fp32
+// (its normalised output and log-sum-exp; in the gradient its share of dq),
+// and a last kernel joins the partials of a query.  No atomics: every partial
+// has one writer, and the sort is stable, so dk and dv add up in one order.
+//
+// What bounds it: per pair and head the tile products cost 4 * D * keys
+// operations against 8 * D bytes of partials (written and read), so the
+// partials and the softmax, not the matrix unit, set the pace; wide spans make
+// the pairs fewer.
+//
+// A handful of queries does not fill tiles and would wait for the sort; they
+// take a direct path, which splits each query's own keys over CTAs.
 #include <algorithm>
 #include <cmath>
 
@@ -9,189 +27,955 @@ namespace nsfps {
 namespace {
 
 constexpr uint32_t kFullMask = 0xffffffffu;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
-  const void *q, *k, *v, *dout;
-  const void *out_in;
-  void *out, *dq, *dk, *dv;
+  const char *q, *k, *v, *dout, *out_in;
+  char *out, *dq, *dk, *dv;
   float *lse;              // forward: may be null
   const float *lse_in;
   const int64_t *blocks;
   const int32_t *lengths;  // or null
-  uint32_t B, M, N, H, G, D, block_log2, top, nb;
-  int64_t qs[3], ks[3], vs[3];
+  uint32_t B, M, N, H, G, R, D;  // R = H / G query heads per key head
+  uint32_t block_log2, top, nb;
+  int64_t qs[3], ks[3], vs[3];   // element strides: batch, row, head
   float scale;
+  // plan of the (query, span) pairs
+  uint32_t nsb;            // spans per cloud
+  const uint32_t *vals;    // sorted pairs: query * top + leading slot
+  const uint32_t *mask;    // per query slot: blocks of the span that are listed
+  const unsigned long long *lead;  // per query: bit s = slot s leads a pair
+  const uint32_t *start;   // first pair of each span (B * nsb + 1)
+  const uint32_t *tile_off;  // first tile of each span (B * nsb + 1)
+  const uint2 *tiles;      // (span, tile within the span)
+  // partials of key heads g0 .. g0 + gc - 1
+  uint32_t g0, gc;
+  float *part;             // [pair][gc * R][D]
+  float *part_lse;         // [pair][gc * R], base 2
+  float *delta;            // [query][H]
+  float *part_kv;          // [tile][gc][2][span][D]
+  uint32_t splits;         // direct path: partials per query
 };
 
 __device__ __forceinline__ uint32_t cloud_length(const int32_t *lengths, uint32_t b, uint32_t n) {
   return lengths ? (uint32_t)min(max(lengths[b], 0), (int)n) : n;
 }
 
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o);
-  return x;
+// ------------------------------------------------------------ matrix tiles
+
+template <class T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
+                                                        uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4],
+                                                 uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One warp per (b, m, h); lane l holds elements l, l + 32, ...
 template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&x);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 x = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&x);
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm2t(uint32_t (&r)[2], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(addr)
+               : "memory");
+}
+
+// 16-byte asynchronous copy; zeros where `some` is false (the source is then
+// not read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool some) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(some ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool some) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(some ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// Shared tiles of 16-bit rows of DP elements: byte offset of 16-byte chunk c
+// of row r.  The chunks of a row are permuted by the row, so that the eight
+// rows of a matrix load fall into different banks.
+template <int DP>
+__device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
+  if (DP == 32) return r * 64u + ((c ^ ((r >> 1) & 3u)) << 4);
+  return r * (DP * 2u) + ((c ^ (r & 7u)) << 4);
+}
+
+// ------------------------------------------------------------- the plan
+
+// One warp per query: which slots lead a pair, and the blocks of each pair.
+// A pair's leading slot is the first slot that lists a block of its span; a
+// repeated block sets the same bit again.  The sort key is the span and the
+// 64-key chunks of it that are read, so that the rows of a tile read alike.
 __global__ void __launch_bounds__(256)
-attend_forward(const AttnArgs a) {
+plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
+           uint32_t *__restrict__ vals, uint32_t *__restrict__ mask,
+           unsigned long long *__restrict__ lead) {
   const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
-  if (w >= (uint64_t)a.B * a.M * a.H) return;
-  const uint32_t h = w % a.H;
-  const uint64_t bm = w / a.H;
-  const uint32_t m = bm % a.M, b = bm / a.M, g = h / (a.H / a.G);
-  const T *q = (const T *)a.q + b * a.qs[0] + m * a.qs[1] + h * a.qs[2];
-  const T *k = (const T *)a.k + b * a.ks[0] + g * a.ks[2];
-  const T *v = (const T *)a.v + b * a.vs[0] + g * a.vs[2];
-  const int64_t *list = a.blocks + bm * a.top;
+  const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (bm >= a.B * a.M) return;
+  const uint32_t b = bm / a.M;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
-  float qf[4], acc[4] = {};
+  const uint32_t live = (uint32_t)(((uint64_t)len + (1u << a.block_log2) - 1u) >> a.block_log2);
+  const uint32_t in_log2 = span_log2 - a.block_log2;  // blocks per span, log2
+  const uint32_t none = 0xffffffffu;
+  uint32_t sb[2], bit[2], m[2] = {0u, 0u};
+  bool first[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) qf[i] = lane + 32 * i < a.D ? to_f32(q[lane + 32 * i]) * a.scale : 0.f;
-  float mx = -INFINITY, sum = 0.f;
-  for (uint32_t s = 0; s < a.top; ++s) {
-    const int64_t j = list[s];
-    bool use = j >= 0 && j < (int64_t)a.nb;
-    for (uint32_t e = 0; e < s; ++e) use = use && list[e] != j;
-    if (!use) continue;
-    const uint32_t t0 = (uint32_t)j << a.block_log2;
-    const uint32_t t1 = (uint32_t)min((uint64_t)len, ((uint64_t)j + 1) << a.block_log2);
-    for (uint32_t t = t0; t < t1; ++t) {
-      float d = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.D) d += qf[i] * to_f32(k[(int64_t)t * a.ks[1] + lane + 32 * i]);
-      d = warp_sum(d);
-      const float nm = fmaxf(mx, d), c = expf(mx - nm), p = expf(d - nm);
-      mx = nm;
-      sum = sum * c + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.D)
-          acc[i] = acc[i] * c + p * to_f32(v[(int64_t)t * a.vs[1] + lane + 32 * i]);
-    }
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t s = lane + 32u * i;
+    const int64_t j = s < a.top ? a.blocks[(uint64_t)bm * a.top + s] : -1;
+    const bool use = j >= 0 && j < (int64_t)live;
+    sb[i] = use ? (uint32_t)j >> in_log2 : none;
+    bit[i] = use ? 1u << ((uint32_t)j & ((1u << in_log2) - 1u)) : 0u;
+    first[i] = use;
   }
-  T *o = (T *)a.out + w * a.D;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < a.D) o[lane + 32 * i] = from_f32<T>(sum > 0.f ? acc[i] / sum : 0.f);
-  if (a.lse && lane == 0) a.lse[w] = sum > 0.f ? mx + logf(sum) : -INFINITY;
-}
-
-template <class T>
-__device__ __forceinline__ float row_dot(const T *x, const T *y, uint32_t D, uint32_t lane) {
-  float d = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < D) d += to_f32(x[lane + 32 * i]) * to_f32(y[lane + 32 * i]);
-  return warp_sum(d);
-}
-
-template <class T>
-__global__ void __launch_bounds__(256)
-attend_dq(const AttnArgs a, float *delta) {
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
-  if (w >= (uint64_t)a.B * a.M * a.H) return;
-  const uint32_t h = w % a.H;
-  const uint64_t bm = w / a.H;
-  const uint32_t m = bm % a.M, b = bm / a.M, g = h / (a.H / a.G);
-  const T *q = (const T *)a.q + b * a.qs[0] + m * a.qs[1] + h * a.qs[2];
-  const T *k = (const T *)a.k + b * a.ks[0] + g * a.ks[2];
-  const T *v = (const T *)a.v + b * a.vs[0] + g * a.vs[2];
-  const T *dout = (const T *)a.dout + w * a.D, *out = (const T *)a.out_in + w * a.D;
-  const int64_t *list = a.blocks + bm * a.top;
-  const uint32_t len = cloud_length(a.lengths, b, a.N);
-  const float dl = row_dot(dout, out, a.D, lane), lse = a.lse_in[w];
-  if (lane == 0) delta[w] = dl;
-  float acc[4] = {};
   for (uint32_t s = 0; s < a.top; ++s) {
-    const int64_t j = list[s];
-    bool use = j >= 0 && j < (int64_t)a.nb;
-    for (uint32_t e = 0; e < s; ++e) use = use && list[e] != j;
-    if (!use) continue;
-    const uint32_t t0 = (uint32_t)j << a.block_log2;
-    const uint32_t t1 = (uint32_t)min((uint64_t)len, ((uint64_t)j + 1) << a.block_log2);
-    for (uint32_t t = t0; t < t1; ++t) {
-      const T *kt = k + (int64_t)t * a.ks[1];
-      const float p = expf(row_dot(q, kt, a.D, lane) * a.scale - lse);
-      const float ds = p * (row_dot(dout, v + (int64_t)t * a.vs[1], a.D, lane) - dl) * a.scale;
+    const uint32_t osb = __shfl_sync(kFullMask, s < 32u ? sb[0] : sb[1], s & 31u);
+    const uint32_t obit = __shfl_sync(kFullMask, s < 32u ? bit[0] : bit[1], s & 31u);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.D) acc[i] += ds * to_f32(kt[lane + 32 * i]);
-    }
+    for (int i = 0; i < 2; ++i)
+      if (osb == sb[i]) {
+        m[i] |= obit;
+        if (s < lane + 32u * i) first[i] = false;
+      }
   }
-  T *o = (T *)a.dq + w * a.D;
+  const uint32_t l0 = __ballot_sync(kFullMask, first[0]), l1 = __ballot_sync(kFullMask, first[1]);
+  if (lane == 0) lead[bm] = l0 | ((unsigned long long)l1 << 32);
+  const uint32_t chunks = 1u << (span_log2 - 6u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < a.D) o[lane + 32 * i] = from_f32<T>(acc[i]);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t s = lane + 32u * i;
+    if (s >= a.top) continue;
+    const uint64_t p = (uint64_t)bm * a.top + s;
+    uint32_t read = 0;
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const uint32_t lo = (c << 6) >> a.block_log2;
+      const uint32_t n = a.block_log2 >= 6u ? 1u : 64u >> a.block_log2;
+      read |= ((m[i] >> lo) & ((1u << n) - 1u)) ? 1u << c : 0u;
+    }
+    keys[p] = first[i] ? ((b * a.nsb + sb[i]) << chunks) | read : (a.B * a.nsb) << chunks;
+    vals[p] = (uint32_t)p;
+    mask[p] = m[i];
+  }
 }
 
-// (block of keys, query slot) pairs for the sort; `none` for a slot that
-// counts for nothing.
+// Per span: its first pair, and its tiles of tile_rows rows (at least
+// `least`).
 __global__ void __launch_bounds__(256)
-pair_keys(const AttnArgs a, uint32_t none, uint32_t *__restrict__ keys,
-          uint32_t *__restrict__ vals) {
-  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
-  if (p >= a.B * a.M * a.top) return;
-  const uint32_t bm = p / a.top, s = p - bm * a.top, b = bm / a.M;
-  const int64_t *list = a.blocks + (uint64_t)bm * a.top;
-  const int64_t j = list[s];
-  bool use = j >= 0 && j < (int64_t)a.nb;
-  for (uint32_t e = 0; e < s; ++e) use = use && list[e] != j;
-  keys[p] = use ? b * a.nb + (uint32_t)j : none;
-  vals[p] = p;
+plan_spans(const uint32_t *__restrict__ keys, uint32_t n, uint32_t spans, uint32_t shift,
+           uint32_t R, uint32_t tile_rows, uint32_t least, uint32_t *__restrict__ start,
+           uint32_t *__restrict__ count) {
+  const uint32_t s = blockIdx.x * 256u + threadIdx.x;
+  if (s > spans) return;
+  const uint32_t b = lower_bound(keys, n, s << shift);
+  start[s] = b;
+  uint32_t tiles = 0;
+  if (s < spans) {
+    const uint32_t e = lower_bound(keys, n, (s + 1u) << shift);
+    tiles = max(least, (uint32_t)(((uint64_t)(e - b) * R + tile_rows - 1u) / tile_rows));
+  }
+  count[s] = tiles;
 }
 
+// One warp per span: lists its tiles.
 __global__ void __launch_bounds__(256)
-pair_starts(const uint32_t *__restrict__ keys, uint32_t n, uint32_t groups,
-            uint32_t *__restrict__ start) {
-  const uint32_t r = blockIdx.x * 256u + threadIdx.x;
-  if (r <= groups) start[r] = lower_bound(keys, n, r);
+plan_tiles(const uint32_t *__restrict__ tile_off, uint32_t spans, uint2 *__restrict__ tiles) {
+  const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (s >= spans) return;
+  const uint32_t b = tile_off[s], e = tile_off[s + 1];
+  for (uint32_t i = b + (threadIdx.x & 31u); i < e; i += 32u) tiles[i] = make_uint2(s, i - b);
 }
 
-// One warp per (b, key, kv head): every query that chose the key's block, in
-// ascending order.
-template <class T>
-__global__ void __launch_bounds__(256)
-attend_dkv(const AttnArgs a, const float *delta, const uint32_t *vals, const uint32_t *start) {
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
-  if (w >= (uint64_t)a.B * a.N * a.G) return;
-  const uint32_t g = w % a.G;
-  const uint64_t bt = w / a.G;
-  const uint32_t t = bt % a.N, b = bt / a.N, r = a.H / a.G;
-  const T *kt = (const T *)a.k + b * a.ks[0] + t * a.ks[1] + g * a.ks[2];
-  const T *vt = (const T *)a.v + b * a.vs[0] + t * a.vs[1] + g * a.vs[2];
-  float dk[4] = {}, dv[4] = {};
-  const uint32_t j = b * a.nb + (t >> a.block_log2);
-  if (t < cloud_length(a.lengths, b, a.N))
-    for (uint32_t e = start[j]; e < start[j + 1]; ++e) {
-      const uint32_t bm = vals[e] / a.top, m = bm % a.M;
-      for (uint32_t h = g * r; h < (g + 1) * r; ++h) {
-        const uint64_t row = (uint64_t)bm * a.H + h;
-        const T *q = (const T *)a.q + b * a.qs[0] + m * a.qs[1] + h * a.qs[2];
-        const T *dout = (const T *)a.dout + row * a.D;
-        const float p = expf(row_dot(q, kt, a.D, lane) * a.scale - a.lse_in[row]);
-        const float ds = p * (row_dot(dout, vt, a.D, lane) - delta[row]) * a.scale;
+// -------------------------------------------------------------- forward
+
+constexpr uint32_t kSpanLog2 = 8;      // keys per span of the forward pass
+constexpr uint32_t kTileRows = 128;    // query rows per CTA: 8 warps of 16
+
+// Blocks (as bits of a pair's mask) of the 64-key chunk c of a span.
+__device__ __forceinline__ uint32_t chunk_blocks(uint32_t c, uint32_t block_log2) {
+  const uint32_t n = block_log2 >= 6u ? 1u : 64u >> block_log2;
+  return ((1u << n) - 1u) << ((c << 6) >> block_log2);
+}
+
+// Copies keys [key0, key0 + ROWS) of one head into a shared tile; zeros behind
+// the cloud's end and behind the head's elements.
+template <int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void load_keys(uint32_t dst, const char *src, int64_t row_stride,
+                                          uint32_t key0, uint32_t len, uint32_t D, uint32_t tid) {
+  constexpr uint32_t kChunks = DP / 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (lane + 32 * i < a.D) {
-            dk[i] += ds * to_f32(q[lane + 32 * i]);
-            dv[i] += p * to_f32(dout[lane + 32 * i]);
-          }
+  for (uint32_t i = tid; i < ROWS * kChunks; i += THREADS) {
+    const uint32_t r = i / kChunks, c = i % kChunks;
+    const bool some = key0 + r < len && c * 8u < D;
+    copy16(dst + tile_off<DP>(r, c), some ? src + ((int64_t)(key0 + r) * row_stride + c * 8) * 2 : src,
+           some);
+  }
+}
+
+// The A fragments (16 rows x DP) of two query rows per lane, straight from
+// memory.
+template <int DP>
+__device__ __forceinline__ void load_rows(uint32_t (&f)[DP / 16][4], const char *r0,
+                                          const char *r1, uint32_t D, uint32_t t) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t d = kk * 16 + h * 8 + 2 * t;
+      const bool in = d < D;
+      f[kk][2 * h] = r0 && in ? *reinterpret_cast<const uint32_t *>(r0 + 2 * d) : 0u;
+      f[kk][2 * h + 1] = r1 && in ? *reinterpret_cast<const uint32_t *>(r1 + 2 * d) : 0u;
+    }
+}
+
+// Running softmax state and output of 16 rows (two per lane).
+template <class T, int DP>
+struct RowsState {
+  float o[DP / 8][4];
+  float mx[2], sum[2];  // base-2 maximum; this lane's share of the sum
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    mx[0] = mx[1] = -INFINITY;
+    sum[0] = sum[1] = 0.f;
+  }
+
+  // 16 * KP keys at rows key_row.. of the tiles sk, sv.  sel(kp) tells whether
+  // any row reads keys 16 kp .. 16 kp + 15; rows(kp, h) whether row h of this
+  // lane does; key_at(kp) is their first key (for the cloud's end).  The
+  // weights are rounded to T for the product with v: half a step of T each,
+  // as the output's own rounding.
+  template <int KP, class Sel, class Row>
+  __device__ __forceinline__ void add(const uint32_t (&qf)[DP / 16][4], uint32_t sk, uint32_t sv,
+                                      uint32_t key_row, uint32_t key0, uint32_t len, float c2,
+                                      uint32_t lane, Sel sel, Row row) {
+    const uint32_t t = lane & 3u;
+    float s[2 * KP][4];
+    float nm[2] = {mx[0], mx[1]};
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[2 * kp][i] = s[2 * kp + 1][i] = 0.f;
+      if (!sel(kp)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[2 * kp][i] = s[2 * kp + 1][i] = -INFINITY;
+        continue;
+      }
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t b[4];
+        ldsm4(b, sk + tile_off<DP>(key_row + kp * 16 + (lane & 7u) + ((lane >> 4) << 3),
+                                   kk * 2 + ((lane >> 3) & 1u)));
+        mma16816<T>(s[2 * kp], qf[kk], b[0], b[1]);
+        mma16816<T>(s[2 * kp + 1], qf[kk], b[2], b[3]);
+      }
+      const bool r0 = row(kp, 0), r1 = row(kp, 1);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = (i < 2 ? r0 : r1) && key0 + kp * 16 + n * 8 + 2 * t + (i & 1) < len;
+          float &x = s[2 * kp + n][i];
+          x = in ? x * c2 : -INFINITY;
+          nm[i >> 1] = fmaxf(nm[i >> 1], x);
+        }
+    }
+    float base[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      nm[h] = fmaxf(nm[h], __shfl_xor_sync(kFullMask, nm[h], 1));
+      nm[h] = fmaxf(nm[h], __shfl_xor_sync(kFullMask, nm[h], 2));
+      base[h] = nm[h] == -INFINITY ? 0.f : nm[h];  // no key yet: exp2(-inf) = 0
+      const float c = exp2_fast(mx[h] - base[h]);
+      mx[h] = nm[h];
+      sum[h] *= c;
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= c, o[j][2 * h + 1] *= c;
+    }
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      if (!sel(kp)) continue;
+      uint32_t a[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float *x = s[2 * kp + n];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = exp2_fast(x[i] - base[i >> 1]);
+        sum[0] += x[0] + x[1];
+        sum[1] += x[2] + x[3];
+        a[2 * n] = pack2<T>(x[0], x[1]);
+        a[2 * n + 1] = pack2<T>(x[2], x[3]);
+      }
+#pragma unroll
+      for (int jj = 0; jj < DP / 16; ++jj) {
+        uint32_t b[4];
+        ldsm4t(b, sv + tile_off<DP>(key_row + kp * 16 + (lane & 15u), jj * 2 + (lane >> 4)));
+        mma16816<T>(o[2 * jj], a, b[0], b[1]);
+        mma16816<T>(o[2 * jj + 1], a, b[2], b[3]);
       }
     }
+  }
+
+  __device__ __forceinline__ void finish() {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < a.D) {
-      ((T *)a.dk)[w * a.D + lane + 32 * i] = from_f32<T>(dk[i]);
-      ((T *)a.dv)[w * a.D + lane + 32 * i] = from_f32<T>(dv[i]);
+    for (int h = 0; h < 2; ++h) {
+      sum[h] += __shfl_xor_sync(kFullMask, sum[h], 1);
+      sum[h] += __shfl_xor_sync(kFullMask, sum[h], 2);
     }
+  }
+};
+
+// One tile of pairs of one span and key head.
+template <class T, int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
+attend_tiles(const AttnArgs a) {
+  extern __shared__ __align__(128) char smem[];
+  __shared__ uint32_t s_any[8];
+  const uint32_t spans = a.B * a.nsb;
+  if (blockIdx.x >= a.tile_off[spans]) return;
+  const uint2 tile = a.tiles[blockIdx.x];
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
+  const uint32_t gi = blockIdx.y, g = a.g0 + gi;
+  const uint32_t e0 = a.start[tile.x], rows = (a.start[tile.x + 1] - e0) * a.R;
+  const uint32_t len = cloud_length(a.lengths, b, a.N);
+  const uint32_t key0 = sb << kSpanLog2;
+
+  // this lane's two rows
+  uint32_t pair[2], head[2], mask[2];
+  const char *qrow[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t r = tile.y * kTileRows + warp * 16u + (lane >> 2) + 8u * h;
+    pair[h] = 0xffffffffu;
+    head[h] = mask[h] = 0u;
+    qrow[h] = nullptr;
+    if (r < rows) {
+      const uint32_t e = r / a.R;
+      head[h] = r - e * a.R;
+      pair[h] = a.vals[e0 + e];
+      mask[h] = a.mask[pair[h]];
+      const uint32_t m = pair[h] / a.top - b * a.M;
+      qrow[h] = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
+                           (int64_t)(g * a.R + head[h]) * a.qs[2]);
+    }
+  }
+  const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
+  if (lane == 0) s_any[warp] = warp_any;
+  uint32_t qf[DP / 16][4];
+  load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
+  __syncthreads();
+  uint32_t any = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) any |= s_any[w];
+  uint32_t todo = 0;  // chunks that some row of the tile reads
+#pragma unroll
+  for (uint32_t c = 0; c < (1u << (kSpanLog2 - 6u)); ++c)
+    if ((any & chunk_blocks(c, a.block_log2)) && key0 + c * 64u < len) todo |= 1u << c;
+
+  const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+  const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+  constexpr uint32_t kTile = 64u * DP * 2u;
+  const uint32_t base = smem_u32(smem);
+  auto fetch = [&](uint32_t c, uint32_t buf) {
+    const uint32_t at = base + buf * 2u * kTile;
+    load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
+    load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
+    copy_commit();
+  };
+  RowsState<T, DP> st;
+  st.clear();
+  const float c2 = a.scale * kLog2e;
+  uint32_t buf = 0;
+  if (todo) fetch(__ffs(todo) - 1, 0);
+  while (todo) {
+    const uint32_t c = __ffs(todo) - 1;
+    todo &= todo - 1u;
+    if (todo) {
+      fetch(__ffs(todo) - 1, buf ^ 1u);
+      copy_wait<1>();
+    } else {
+      copy_wait<0>();
+    }
+    __syncthreads();
+    if (warp_any & chunk_blocks(c, a.block_log2)) {
+      const uint32_t at = base + buf * 2u * kTile;
+      auto bit = [&](int kp) { return (c * 64u + kp * 16u) >> a.block_log2; };
+      st.template add<4>(
+          qf, at, at + kTile, 0u, key0 + c * 64u, len, c2, lane,
+          [&](int kp) { return (warp_any >> bit(kp)) & 1u; },
+          [&](int kp, int h) { return (mask[h] >> bit(kp)) & 1u; });
+    }
+    __syncthreads();
+    buf ^= 1u;
+  }
+  st.finish();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (pair[h] == 0xffffffffu) continue;
+    const uint64_t row = (uint64_t)pair[h] * (a.gc * a.R) + gi * a.R + head[h];
+    const float inv = st.sum[h] > 0.f ? 1.f / st.sum[h] : 0.f;
+    float *o = a.part + row * a.D;
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+      if (j * 8u < a.D)
+        *reinterpret_cast<float2 *>(o + j * 8 + 2 * (lane & 3u)) =
+            make_float2(st.o[j][2 * h] * inv, st.o[j][2 * h + 1] * inv);
+    if ((lane & 3u) == 0)
+      a.part_lse[row] = st.sum[h] > 0.f ? st.mx[h] + log2f(st.sum[h]) : -INFINITY;
+  }
 }
+
+// Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse).
+// LANES = D / 4 lanes per row (rounded up to a power of two), four elements
+// each.  The partials of a row are those of its leading slots, or (direct)
+// of its splits.
+template <class T, bool DIRECT>
+__global__ void __launch_bounds__(256)
+attend_join(const AttnArgs a, const int lanes_log2) {
+  const uint32_t sub = threadIdx.x & ((1u << lanes_log2) - 1u);
+  const uint32_t hc = a.gc * a.R;
+  const uint64_t row = (uint64_t)blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (row >= (uint64_t)a.B * a.M * hc) return;
+  const uint32_t bm = (uint32_t)(row / hc), hh = (uint32_t)(row - (uint64_t)bm * hc);
+  const unsigned long long lead =
+      DIRECT ? (a.splits >= 64u ? ~0ull : (1ull << a.splits) - 1ull) : a.lead[bm];
+  auto at = [&](uint32_t s) {
+    return DIRECT ? row * a.splits + s : ((uint64_t)bm * a.top + s) * hc + hh;
+  };
+  float mx = -INFINITY;
+  for (unsigned long long l = lead; l; l &= l - 1)
+    mx = fmaxf(mx, a.part_lse[at(__ffsll(l) - 1)]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+  if (mx != -INFINITY)
+    for (unsigned long long l = lead; l; l &= l - 1) {
+      const uint64_t p = at(__ffsll(l) - 1);
+      const float w = exp2_fast(a.part_lse[p] - mx);
+      total += w;
+      if (4u * sub < a.D && w > 0.f) {
+        const float4 x = *reinterpret_cast<const float4 *>(a.part + p * a.D + 4 * sub);
+        acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+      }
+    }
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  const uint64_t out_row = (uint64_t)bm * a.H + a.g0 * a.R + hh;
+  if (4u * sub < a.D)
+    *reinterpret_cast<uint2 *>(a.out + (out_row * a.D + 4 * sub) * 2) =
+        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  if (a.lse && sub == 0) a.lse[out_row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
+}
+
+// Direct path: a CTA takes kDirectKeys of one query's listed keys and one key
+// head; each warp a run of 16-key slices, joined through shared memory.
+constexpr uint32_t kDirectKeys = 128;
+constexpr uint32_t kDirectWarps = 4;
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kDirectWarps * 32)
+attend_direct(const AttnArgs a) {
+  extern __shared__ __align__(128) char smem[];
+  constexpr uint32_t kSlices = kDirectKeys / 16 / kDirectWarps;  // per warp
+  constexpr uint32_t kTile = 16u * kSlices * DP * 2u;
+  __shared__ float s_stat[kDirectWarps][2][16];
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t split = blockIdx.x, bm = blockIdx.y, g = blockIdx.z;
+  const uint32_t b = bm / a.M, m = bm - b * a.M;
+  const uint32_t len = cloud_length(a.lengths, b, a.N);
+  const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+  const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+  const uint32_t sk = smem_u32(smem) + warp * 2u * kTile, sv = sk + kTile;
+  const int64_t *list = a.blocks + (uint64_t)bm * a.top;
+
+  uint32_t key[kSlices];
+  bool use[kSlices];
+  bool some = false;
+#pragma unroll
+  for (uint32_t i = 0; i < kSlices; ++i) {
+    const uint32_t at = split * kDirectKeys + (warp * kSlices + i) * 16u;  // of the listed keys
+    const uint32_t s = at >> a.block_log2;
+    use[i] = false;
+    key[i] = 0;
+    if (s < a.top) {
+      const int64_t j = list[s];
+      // an entry that an earlier slot holds already counts for nothing
+      bool again = false;
+      if (lane < s) again = list[lane] == j;
+      if (lane + 32u < s) again = again || list[lane + 32u] == j;
+      again = __any_sync(kFullMask, again);
+      if (!again && j >= 0 && j < (int64_t)a.nb) {
+        key[i] = ((uint32_t)j << a.block_log2) + (at & ((1u << a.block_log2) - 1u));
+        use[i] = key[i] < len;
+      }
+    }
+    some = some || use[i];
+    if (use[i]) {
+      load_keys<DP, 16, 32>(sk + i * 16u * DP * 2u, kh, a.ks[1], key[i], len, a.D, lane);
+      load_keys<DP, 16, 32>(sv + i * 16u * DP * 2u, vh, a.vs[1], key[i], len, a.D, lane);
+    }
+  }
+  copy_commit();
+  copy_wait<0>();
+  __syncwarp();
+  const float c2 = a.scale * kLog2e;
+  const uint32_t t = lane & 3u;
+  float *s_o = reinterpret_cast<float *>(smem);  // [warp][16][DP], over the tiles
+  for (uint32_t h0 = 0; h0 < a.R; h0 += 16u) {
+    const char *qrow[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t hh = h0 + (lane >> 2) + 8u * h;
+      qrow[h] = hh < a.R ? a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
+                                      (int64_t)(g * a.R + hh) * a.qs[2])
+                         : nullptr;
+    }
+    RowsState<T, DP> st;
+    st.clear();
+    if (some) {
+      uint32_t qf[DP / 16][4];
+      load_rows<DP>(qf, qrow[0], qrow[1], a.D, t);
+#pragma unroll
+      for (uint32_t i = 0; i < kSlices; ++i)
+        if (use[i])
+          st.template add<1>(qf, sk, sv, i * 16u, key[i], len, c2, lane,
+                             [](int) { return true; }, [](int, int) { return true; });
+    }
+    st.finish();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t == 0) {
+        s_stat[warp][0][(lane >> 2) + 8 * h] = st.mx[h];
+        s_stat[warp][1][(lane >> 2) + 8 * h] = st.sum[h];
+      }
+    if (a.R > 16u) {
+      // the tiles are needed again: the joint buffer lies behind them
+      s_o = reinterpret_cast<float *>(smem + kDirectWarps * 2u * kTile);
+    }
+    __syncthreads();  // statistics written, and every warp is done with its tiles
+    // rows of this m-tile that exist, scaled to the common maximum
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r = (lane >> 2) + 8u * h;
+      if (h0 + r >= a.R) continue;
+      float mx = -INFINITY;
+      for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
+      const float c = st.mx[h] == -INFINITY ? 0.f : exp2_fast(st.mx[h] - mx);
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+        *reinterpret_cast<float2 *>(s_o + (warp * 16u + r) * DP + j * 8 + 2 * t) =
+            make_float2(st.o[j][2 * h] * c, st.o[j][2 * h + 1] * c);
+    }
+    __syncthreads();
+    const uint32_t live = min(16u, a.R - h0);
+    for (uint32_t i = tid; i < live * (DP / 4); i += kDirectWarps * 32) {
+      const uint32_t r = i / (DP / 4), d = (i % (DP / 4)) * 4;
+      if (d >= a.D) continue;
+      float mx = -INFINITY, sum = 0.f;
+      for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t w = 0; w < kDirectWarps; ++w) {
+        if (s_stat[w][0][r] == -INFINITY) continue;
+        sum += s_stat[w][1][r] * exp2_fast(s_stat[w][0][r] - mx);
+        const float4 y = *reinterpret_cast<const float4 *>(s_o + (w * 16u + r) * DP + d);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const uint64_t row = (uint64_t)bm * a.H + g * a.R + h0 + r;
+      if (a.splits == 1u) {
+        *reinterpret_cast<uint2 *>(a.out + (row * a.D + d) * 2) =
+            make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+        if (a.lse && d == 0) a.lse[row] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+      } else {
+        *reinterpret_cast<float4 *>(a.part + (row * a.splits + split) * a.D + d) =
+            make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        if (d == 0) a.part_lse[row * a.splits + split] = sum > 0.f ? mx + log2f(sum) : -INFINITY;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------- gradient
+
+// delta = sum_d dout * out per row; 8 lanes per row, 8 elements per step.
+template <class T>
+__global__ void __launch_bounds__(256)
+grad_delta(const AttnArgs a) {
+  const uint64_t row = (uint64_t)blockIdx.x * 32u + (threadIdx.x >> 3);
+  const uint32_t sub = threadIdx.x & 7u;
+  float s = 0.f;
+  if (row < (uint64_t)a.B * a.M * a.H)
+    for (uint32_t d = sub * 8; d < a.D; d += 64) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(a.dout + (row * a.D + d) * 2);
+      const uint4 y = *reinterpret_cast<const uint4 *>(a.out_in + (row * a.D + d) * 2);
+      const T *xe = reinterpret_cast<const T *>(&x), *ye = reinterpret_cast<const T *>(&y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += to_f32(xe[i]) * to_f32(ye[i]);
+    }
+#pragma unroll
+  for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+  if (sub == 0 && row < (uint64_t)a.B * a.M * a.H) a.delta[row] = s;
+}
+
+constexpr uint32_t kGradRows = 32;     // query rows per step
+constexpr uint32_t kGradItem = 512;    // query rows per CTA
+
+template <int DP, int SPAN>
+constexpr uint32_t grad_smem() {
+  return 2u * SPAN * DP * 2u + 2u * 2u * kGradRows * DP * 2u + SPAN * kGradRows * 2u +
+         2u * kGradRows * 16u;
+}
+
+// Byte offset of 16-byte chunk c (8 rows) of key r in the ds tile
+// [key][kGradRows].
+__device__ __forceinline__ uint32_t ds_off(uint32_t r, uint32_t c) {
+  return r * (kGradRows * 2u) + ((c ^ ((r >> 1) & 3u)) << 4);
+}
+
+// One item: up to kGradItem rows of one span and key head.  Warp w owns keys
+// 16 w .. 16 w + 15 of the span and keeps their dk and dv in registers; per
+// step of 32 rows it forms s^T = k q^T and dp^T = v dout^T, from them p^T and
+// ds^T (whose accumulator layout is the A operand of the next products), adds
+// p^T dout and ds^T q, and puts ds into shared memory, from which all warps
+// make the rows' share of dq = ds k.
+template <class T, int DP, int SPAN>
+__global__ void __launch_bounds__(SPAN * 2, DP <= 64 && SPAN == 128 ? 2 : 1)
+attend_grad(const AttnArgs a) {
+  extern __shared__ __align__(128) char smem[];
+  constexpr uint32_t kThreads = SPAN * 2, kWarps = SPAN / 16, kChunks = DP / 8;
+  const uint32_t spans = a.B * a.nsb;
+  if (blockIdx.x >= a.tile_off[spans]) return;
+  const uint2 tile = a.tiles[blockIdx.x];
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, t = lane & 3u;
+  const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
+  const uint32_t gi = blockIdx.y, g = a.g0 + gi;
+  const uint32_t e0 = a.start[tile.x], all_rows = (a.start[tile.x + 1] - e0) * a.R;
+  const uint32_t row0 = tile.y * kGradItem;
+  const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
+  const uint32_t len = cloud_length(a.lengths, b, a.N);
+  const uint32_t key0 = sb * SPAN;
+  const uint32_t steps = (rows + kGradRows - 1u) / kGradRows;
+
+  const uint32_t sk = smem_u32(smem), sv = sk + SPAN * DP * 2u;
+  const uint32_t sq = sv + SPAN * DP * 2u;              // [2][q, dout][32][DP]
+  constexpr uint32_t kRowTile = kGradRows * DP * 2u;
+  const uint32_t sds = sq + 4u * kRowTile;
+  char *info = smem + (2u * SPAN * DP * 2u + 4u * kRowTile + SPAN * kGradRows * 2u);
+  // [2][lse, delta, mask, partial row][32]
+  const float *s_lse = reinterpret_cast<const float *>(info);
+  const float *s_delta = s_lse + kGradRows;
+  const uint32_t *s_mask = reinterpret_cast<const uint32_t *>(info) + 2 * kGradRows;
+  uint32_t *s_row = reinterpret_cast<uint32_t *>(info) + 3 * kGradRows;
+  constexpr uint32_t kInfo = 4 * kGradRows;  // words per buffer
+
+  float dk[DP / 8][4], dv[DP / 8][4];
+#pragma unroll
+  for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dk[j][i] = dv[j][i] = 0.f;
+
+  if (steps) {
+    const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+    const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+    load_keys<DP, SPAN, kThreads>(sk, kh, a.ks[1], key0, len, a.D, tid);
+    load_keys<DP, SPAN, kThreads>(sv, vh, a.vs[1], key0, len, a.D, tid);
+  }
+  // Rows of step i into buffer i & 1: 8 threads per row while DP = 64.
+  auto fetch = [&](uint32_t i) {
+    const uint32_t buf = i & 1u, at = sq + buf * 2u * kRowTile;
+    for (uint32_t x = tid; x < kGradRows * kChunks; x += kThreads) {
+      const uint32_t r = x / kChunks, c = x % kChunks, rr = i * kGradRows + r;
+      const bool some = rr < rows && c * 8u < a.D;
+      const char *qp = a.q, *op = a.dout;
+      if (some) {
+        const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
+        const uint32_t bm = a.vals[e0 + e] / a.top, m = bm - b * a.M, h = g * a.R + hh;
+        qp = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2] + c * 8);
+        op = a.dout + 2 * (((uint64_t)bm * a.H + h) * a.D + c * 8);
+      }
+      copy16(at + tile_off<DP>(r, c), qp, some);
+      copy16(at + kRowTile + tile_off<DP>(r, c), op, some);
+    }
+    if (tid < kGradRows) {
+      const uint32_t rr = i * kGradRows + tid;
+      const bool some = rr < rows;
+      const uint32_t w = smem_u32(info) + 4u * (buf * kInfo + tid);
+      const float *lp = a.lse_in, *dp = a.delta;
+      const uint32_t *mp = a.mask;
+      uint32_t prow = 0xffffffffu;
+      if (some) {
+        const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
+        const uint32_t p = a.vals[e0 + e];
+        const uint64_t row = (uint64_t)(p / a.top) * a.H + g * a.R + hh;
+        lp += row;
+        dp += row;
+        mp += p;
+        prow = p * (a.gc * a.R) + gi * a.R + hh;
+      }
+      copy4(w, lp, some);
+      copy4(w + 4u * kGradRows, dp, some);
+      copy4(w + 8u * kGradRows, mp, some);
+      s_row[buf * kInfo + tid] = prow;
+    }
+    copy_commit();
+  };
+  if (steps) fetch(0);
+  const float c2 = a.scale * kLog2e;
+  const uint32_t my_bit = (warp * 16u) >> a.block_log2;
+  const bool my_keys = key0 + warp * 16u < len;
+  const bool in0 = key0 + warp * 16u + (lane >> 2) < len;
+  const bool in1 = key0 + warp * 16u + (lane >> 2) + 8u < len;
+  for (uint32_t i = 0; i < steps; ++i) {
+    const uint32_t buf = i & 1u, tq = sq + buf * 2u * kRowTile, to = tq + kRowTile;
+    if (i + 1u < steps) {
+      fetch(i + 1u);
+      copy_wait<1>();
+    } else {
+      copy_wait<0>();
+    }
+    __syncthreads();
+    const uint32_t mask = s_mask[buf * kInfo + lane];
+    const uint32_t any = __reduce_or_sync(kFullMask, mask);
+    const uint32_t mine = __ballot_sync(kFullMask, (mask >> my_bit) & 1u);  // rows that read my keys
+    if (mine && my_keys) {
+      float s[4][4], dp[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t ka[4], va[4];
+        const uint32_t ao = tile_off<DP>(warp * 16u + (lane & 15u), kk * 2 + (lane >> 4));
+        ldsm4(ka, sk + ao);
+        ldsm4(va, sv + ao);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t x[4];
+          const uint32_t bo = tile_off<DP>(n * 16 + (lane & 7u) + ((lane >> 4) << 3),
+                                           kk * 2 + ((lane >> 3) & 1u));
+          ldsm4(x, tq + bo);
+          mma16816<T>(s[2 * n], ka, x[0], x[1]);
+          mma16816<T>(s[2 * n + 1], ka, x[2], x[3]);
+          ldsm4(x, to + bo);
+          mma16816<T>(dp[2 * n], va, x[0], x[1]);
+          mma16816<T>(dp[2 * n + 1], va, x[2], x[3]);
+        }
+      }
+      uint32_t pa[2][4], da[2][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t r = n * 8 + 2 * t;
+        const float2 lse = *reinterpret_cast<const float2 *>(s_lse + buf * kInfo + r);
+        const float2 del = *reinterpret_cast<const float2 *>(s_delta + buf * kInfo + r);
+        const bool r0 = (mine >> r) & 1u, r1 = (mine >> (r + 1u)) & 1u;
+        float p[4], ds[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const bool in = (x & 1 ? r1 : r0) && (x < 2 ? in0 : in1);
+          const float l = x & 1 ? lse.y : lse.x;
+          p[x] = in ? exp2_fast(fmaf(s[n][x], c2, -l * kLog2e)) : 0.f;
+          ds[x] = p[x] * (dp[n][x] - (x & 1 ? del.y : del.x));
+        }
+        pa[n >> 1][(n & 1) * 2] = pack2<T>(p[0], p[1]);
+        pa[n >> 1][(n & 1) * 2 + 1] = pack2<T>(p[2], p[3]);
+        const uint32_t d0 = pack2<T>(ds[0], ds[1]), d1 = pack2<T>(ds[2], ds[3]);
+        da[n >> 1][(n & 1) * 2] = d0;
+        da[n >> 1][(n & 1) * 2 + 1] = d1;
+        const uint32_t kr = warp * 16u + (lane >> 2);
+        *reinterpret_cast<uint32_t *>(smem + (sds - sk) + ds_off(kr, n) + 4u * t) = d0;
+        *reinterpret_cast<uint32_t *>(smem + (sds - sk) + ds_off(kr + 8u, n) + 4u * t) = d1;
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int jj = 0; jj < DP / 16; ++jj) {
+          uint32_t x[4];
+          const uint32_t bo = tile_off<DP>(kk * 16 + (lane & 15u), jj * 2 + (lane >> 4));
+          ldsm4t(x, to + bo);
+          mma16816<T>(dv[2 * jj], pa[kk], x[0], x[1]);
+          mma16816<T>(dv[2 * jj + 1], pa[kk], x[2], x[3]);
+          ldsm4t(x, tq + bo);
+          mma16816<T>(dk[2 * jj], da[kk], x[0], x[1]);
+          mma16816<T>(dk[2 * jj + 1], da[kk], x[2], x[3]);
+        }
+    }
+    __syncthreads();
+    // dq of the 32 rows: kUnits tiles of 16 rows x 8 kPer columns
+    constexpr uint32_t kPer = (2 * kChunks) / kWarps > 0 ? (2 * kChunks) / kWarps : 1;
+    constexpr uint32_t kUnits = 2 * kChunks / kPer;
+    if (warp < kUnits) {
+      const uint32_t rt = warp & 1u, j0 = (warp >> 1) * kPer;
+      float acc[kPer][4];
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
+      for (uint32_t ks = 0; ks < kWarps; ++ks) {
+        if (!((any >> ((ks * 16u) >> a.block_log2)) & 1u) || key0 + ks * 16u >= len) continue;
+        uint32_t x[4];
+        ldsm4t(x, sds + ds_off(ks * 16u + (lane & 7u) + ((lane >> 4) << 3),
+                               rt * 2u + ((lane >> 3) & 1u)));
+        if constexpr (kPer == 1) {
+          uint32_t y[2];
+          ldsm2t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0));
+          mma16816<T>(acc[0], x, y[0], y[1]);
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < kPer / 2; ++j) {
+            uint32_t y[4];
+            ldsm4t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0 + 2 * j + (lane >> 4)));
+            mma16816<T>(acc[2 * j], x, y[0], y[1]);
+            mma16816<T>(acc[2 * j + 1], x, y[2], y[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t prow = s_row[buf * kInfo + rt * 16u + (lane >> 2) + 8u * h];
+        if (prow == 0xffffffffu) continue;
+        float *o = a.part + (uint64_t)prow * a.D;
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; ++j)
+          if ((j0 + j) * 8u < a.D)
+            *reinterpret_cast<float2 *>(o + (j0 + j) * 8u + 2u * t) =
+                make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+      }
+    }
+    __syncthreads();
+  }
+  // the span's dk and dv, or this item's share of them
+  const bool whole = all_rows <= kGradItem;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t r = warp * 16u + (lane >> 2) + 8u * h;
+    if (key0 + r >= a.N) continue;
+    if (whole) {
+      const uint64_t row = ((uint64_t)b * a.N + key0 + r) * a.G + g;
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+        if (j * 8u < a.D) {
+          const uint64_t o = 2 * (row * a.D + j * 8 + 2 * t);
+          *reinterpret_cast<uint32_t *>(a.dk + o) =
+              pack2<T>(dk[j][2 * h] * a.scale, dk[j][2 * h + 1] * a.scale);
+          *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(dv[j][2 * h], dv[j][2 * h + 1]);
+        }
+    } else {
+      float *o = a.part_kv + (((uint64_t)blockIdx.x * a.gc + gi) * 2 * SPAN + r) * a.D;
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+        if (j * 8u < a.D) {
+          *reinterpret_cast<float2 *>(o + j * 8 + 2 * t) = make_float2(dk[j][2 * h], dk[j][2 * h + 1]);
+          *reinterpret_cast<float2 *>(o + (uint64_t)SPAN * a.D + j * 8 + 2 * t) =
+              make_float2(dv[j][2 * h], dv[j][2 * h + 1]);
+        }
+    }
+  }
+}
+
+// dk and dv of the spans that several items share, their shares in order.
+template <class T>
+__global__ void __launch_bounds__(256)
+grad_join_keys(const AttnArgs a, uint32_t span) {
+  const uint32_t s = blockIdx.x, gi = blockIdx.y, g = a.g0 + gi;
+  const uint32_t i0 = a.tile_off[s], i1 = a.tile_off[s + 1];
+  if (i1 - i0 < 2u) return;
+  const uint32_t b = s / a.nsb, key0 = (s - b * a.nsb) * span;
+  const uint32_t keys = min(span, a.N - key0);
+  for (uint32_t x = blockIdx.z * 256u + threadIdx.x; x < keys * a.D / 2u; x += 256u * gridDim.z) {
+    const uint32_t r = x / (a.D / 2u), d = (x - r * (a.D / 2u)) * 2u;
+    float2 k = make_float2(0.f, 0.f), v = k;
+    for (uint32_t i = i0; i < i1; ++i) {
+      const float *o = a.part_kv + (((uint64_t)i * a.gc + gi) * 2 * span + r) * a.D + d;
+      const float2 y = *reinterpret_cast<const float2 *>(o);
+      const float2 z = *reinterpret_cast<const float2 *>(o + (uint64_t)span * a.D);
+      k.x += y.x; k.y += y.y; v.x += z.x; v.y += z.y;
+    }
+    const uint64_t o = 2 * ((((uint64_t)b * a.N + key0 + r) * a.G + g) * a.D + d);
+    *reinterpret_cast<uint32_t *>(a.dk + o) = pack2<T>(k.x * a.scale, k.y * a.scale);
+    *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(v.x, v.y);
+  }
+}
+
+// dq of a query: the shares of its pairs, slots in order.
+template <class T>
+__global__ void __launch_bounds__(256)
+grad_join_queries(const AttnArgs a, const int lanes_log2) {
+  const uint32_t sub = threadIdx.x & ((1u << lanes_log2) - 1u);
+  const uint32_t hc = a.gc * a.R;
+  const uint64_t row = (uint64_t)blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (row >= (uint64_t)a.B * a.M * hc || 4u * sub >= a.D) return;
+  const uint32_t bm = (uint32_t)(row / hc), hh = (uint32_t)(row - (uint64_t)bm * hc);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (unsigned long long l = a.lead[bm]; l; l &= l - 1) {
+    const uint64_t p = ((uint64_t)bm * a.top + __ffsll(l) - 1) * hc + hh;
+    const float4 x = *reinterpret_cast<const float4 *>(a.part + p * a.D + 4 * sub);
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  }
+  const uint64_t out_row = (uint64_t)bm * a.H + a.g0 * a.R + hh;
+  *reinterpret_cast<uint2 *>(a.dq + (out_row * a.D + 4 * sub) * 2) =
+      make_uint2(pack2<T>(acc.x * a.scale, acc.y * a.scale),
+                 pack2<T>(acc.z * a.scale, acc.w * a.scale));
+}
+
+// ------------------------------------------------------------- host side
 
 int check_attention(const nsfps_attention_desc *d) {
   if (!d) return set_error(NSFPS_ERR_ARG, "desc is NULL");
@@ -208,10 +992,12 @@ int check_attention(const nsfps_attention_desc *d) {
     return set_error(NSFPS_ERR_ARG, "top must be in 1..%u", NSFPS_MAX_TOP);
   if (!std::isfinite(d->scale)) return set_error(NSFPS_ERR_ARG, "scale must be finite");
   const uint64_t lim = 1ull << 30;
-  if (d->batch >= lim || d->queries >= lim || d->keys >= lim || d->batch * d->keys >= lim ||
-      d->batch * d->queries >= lim || d->batch * d->queries * d->top >= lim)
+  if (d->batch >= lim / 8 || d->queries >= lim || d->keys >= lim || d->batch * d->keys >= lim ||
+      d->batch * d->queries >= lim || d->batch * d->queries * d->top >= lim ||
+      d->queries * d->top * (d->heads / d->kv_heads) >= 2 * lim)
     return set_error(NSFPS_ERR_UNSUPPORTED,
-                     "batch * queries * top and batch * keys must be below 2^30");
+                     "batch must be below 2^27, batch * queries * top and batch * keys below "
+                     "2^30, queries * top * heads / kv_heads below 2^31");
   for (int i = 0; i < 3; ++i)
     if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->q_stride[i] % 8 ||
         d->k_stride[i] % 8 || d->v_stride[i] % 8)
@@ -219,36 +1005,247 @@ int check_attention(const nsfps_attention_desc *d) {
   return NSFPS_OK;
 }
 
-struct AttnWork {
+uint32_t log2_of(uint32_t block) { return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; }
+
+int padded_dim(uint32_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// Keys per span of the gradient: as many as the warps' dk and dv fit in
+// registers for.
+constexpr uint32_t kGradSpanLog2 = 7;
+
+// Partials of a pass stay below this, by taking the key heads, then the clouds
+// of a call, in turns.
+constexpr uint64_t kMaxPartBytes = 1ull << 30;
+
+// How a call is cut up, and its scratch.
+struct AttnPlan {
+  bool direct;
+  uint32_t bc;             // clouds per turn
+  uint32_t gc;             // key heads per turn
+  uint32_t span_log2, tile_rows, least, splits;
+  uint64_t pairs, spans, max_tiles;  // of one turn
   SortScratch sort;
-  uint32_t *start;
-  float *delta;
+  uint32_t *mask, *start, *tile_off, *scan;
+  unsigned long long *lead;
+  uint2 *tiles;
+  float *part, *part_lse, *delta, *part_kv;
   uint64_t bytes;
 };
 
-AttnWork carve_attention(const nsfps_attention_desc &d, bool backward, void *base) {
-  AttnWork w{};
+// Forward calls whose queries would not fill the machine's tiles go the direct
+// way: it reads each query's keys once per query instead of once per tile.
+bool takes_direct(const nsfps_attention_desc &d) {
+  return d.batch * d.queries * d.kv_heads <= 512 && d.batch * d.queries <= 65535;
+}
+
+AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base) {
+  AttnPlan w{};
   WorkCarver c(base);
+  const uint64_t R = d.heads / d.kv_heads;
+  w.direct = !backward && takes_direct(d);
+  w.bc = (uint32_t)d.batch;
+  w.gc = d.kv_heads;
+  if (w.direct) {
+    w.splits = (uint32_t)ceil_div((uint64_t)d.top * d.block, kDirectKeys);
+    if (w.splits > 1) {
+      const uint64_t rows = d.batch * d.queries * d.heads * w.splits;
+      w.part = c.take<float>(rows * d.head_dim);
+      w.part_lse = c.take<float>(rows);
+    }
+    w.bytes = c.off + 256;
+    return w;
+  }
+  w.span_log2 = backward ? kGradSpanLog2 : kSpanLog2;
+  w.tile_rows = backward ? kGradItem : kTileRows;
+  w.least = backward ? 1 : 0;
+  const uint64_t span = 1ull << w.span_log2, nsb = ceil_div(d.keys, span);
+  auto part_bytes = [&](uint64_t clouds, uint64_t heads) {
+    const uint64_t pairs = clouds * d.queries * d.top, spans = clouds * nsb;
+    uint64_t b = pairs * R * heads * (d.head_dim + 1) * 4;
+    if (backward)
+      b += (pairs * R / w.tile_rows + spans) * heads * 2 * span * d.head_dim * 4;
+    return b;
+  };
+  while (w.gc > 1 && part_bytes(w.bc, w.gc) > kMaxPartBytes) w.gc = (w.gc + 1) / 2;
+  while (w.bc > 1 && part_bytes(w.bc, w.gc) > kMaxPartBytes) w.bc = (w.bc + 1) / 2;
+  w.pairs = w.bc * d.queries * d.top;
+  w.spans = w.bc * nsb;
+  w.max_tiles = w.pairs * R / w.tile_rows + w.spans;
+  w.sort.carve(c, (uint32_t)w.pairs);
+  w.mask = c.take<uint32_t>(w.pairs);
+  w.lead = c.take<unsigned long long>(w.bc * d.queries);
+  w.start = c.take<uint32_t>(w.spans + 1);
+  w.tile_off = c.take<uint32_t>(w.spans + 1);
+  w.scan = c.take<uint32_t>(ceil_div(w.spans + 1, 4096) + 2);
+  w.tiles = c.take<uint2>(w.max_tiles);
+  w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
-    w.sort.carve(c, (uint32_t)(d.batch * d.queries * d.top));
-    w.start = c.take<uint32_t>(d.batch * ceil_div(d.keys, d.block) + 1);
-    w.delta = c.take<float>(d.batch * d.queries * d.heads);
+    w.delta = c.take<float>(w.bc * d.queries * d.heads);
+    w.part_kv = c.take<float>(w.max_tiles * w.gc * 2 * span * d.head_dim);
+  } else {
+    w.part_lse = c.take<float>(w.pairs * R * w.gc);
   }
   w.bytes = c.off + 256;
   return w;
 }
 
 AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k, const void *v,
-                     const int64_t *blocks, const int32_t *lengths) {
+                     const int64_t *blocks, const int32_t *lengths, const AttnPlan &w) {
   AttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.blocks = blocks; a.lengths = lengths;
+  a.q = (const char *)q; a.k = (const char *)k; a.v = (const char *)v;
+  a.blocks = blocks; a.lengths = lengths;
   a.B = (uint32_t)d.batch; a.M = (uint32_t)d.queries; a.N = (uint32_t)d.keys;
-  a.H = d.heads; a.G = d.kv_heads; a.D = d.head_dim; a.top = d.top;
-  a.block_log2 = d.block == 16 ? 4 : d.block == 32 ? 5 : d.block == 64 ? 6 : 7;
+  a.H = d.heads; a.G = d.kv_heads; a.R = d.heads / d.kv_heads; a.D = d.head_dim; a.top = d.top;
+  a.block_log2 = log2_of(d.block);
   a.nb = (uint32_t)ceil_div(d.keys, d.block);
   for (int i = 0; i < 3; ++i) a.qs[i] = d.q_stride[i], a.ks[i] = d.k_stride[i], a.vs[i] = d.v_stride[i];
   a.scale = d.scale;
+  a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
+  a.mask = w.mask; a.lead = w.lead; a.start = w.start; a.tile_off = w.tile_off;
+  a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
+  a.part_kv = w.part_kv; a.splits = w.splits; a.gc = w.gc;
   return a;
+}
+
+// The turn that starts with cloud b0.
+AttnArgs turn_args(const AttnArgs &all, uint32_t b0, uint32_t bc) {
+  AttnArgs a = all;
+  a.B = std::min(bc, all.B - b0);
+  const uint64_t rows = (uint64_t)b0 * a.M;
+  a.q += 2 * (int64_t)b0 * a.qs[0];
+  a.k += 2 * (int64_t)b0 * a.ks[0];
+  a.v += 2 * (int64_t)b0 * a.vs[0];
+  a.blocks += rows * a.top;
+  if (a.lengths) a.lengths += b0;
+  const uint64_t ro = 2 * rows * a.H * a.D, ko = 2 * (uint64_t)b0 * a.N * a.G * a.D;
+  if (a.out) a.out += ro;
+  if (a.lse) a.lse += rows * a.H;
+  if (a.dout) a.dout += ro, a.out_in += ro, a.dq += ro, a.lse_in += rows * a.H;
+  if (a.dk) a.dk += ko, a.dv += ko;
+  return a;
+}
+
+// Sorts a turn's pairs by span and lists its tiles.
+cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
+  const uint32_t n = a.B * a.M * a.top, spans = a.B * a.nsb, shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
+  uint32_t *keys = w.sort.keys0, *vals = w.sort.vals0, launches = 0;
+  cudaError_t err;
+  if (n) {
+    plan_pairs<<<(uint32_t)ceil_div(a.B * a.M, 8), 256, 0, st>>>(a, w.span_log2, keys, vals, w.mask,
+                                                                 w.lead);
+    if ((err = cudaGetLastError())) return err;
+    if ((err = run_sort_pairs(&keys, &vals, w.sort.keys1, w.sort.vals1, n, spans << shift,
+                              w.sort.hist, w.sort.partial, st, launches)))
+      return err;
+  }
+  a.vals = vals;
+  plan_spans<<<(uint32_t)ceil_div((uint64_t)spans + 1, 256), 256, 0, st>>>(
+      keys, n, spans, shift, a.R, w.tile_rows, w.least, w.start, w.tile_off);
+  if ((err = cudaGetLastError())) return err;
+  if ((err = run_exclusive_scan(w.tile_off, w.tile_off, spans + 1, w.scan, st, launches)))
+    return err;
+  if (spans) plan_tiles<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(w.tile_off, spans, w.tiles);
+  return cudaGetLastError();
+}
+
+// Lanes (log2) of 4 elements for a row of D.
+int row_lanes_log2(uint32_t D) {
+  int l = 1;
+  while ((4u << l) < D) ++l;
+  return l;
+}
+
+template <class K>
+cudaError_t opt_in(K kernel, uint32_t smem) {
+  return smem <= 48u << 10 ? cudaSuccess
+                           : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  (int)smem);
+}
+
+template <class T, int DP>
+cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
+  cudaError_t err;
+  const int lanes = row_lanes_log2(all.D);
+  if (w.direct) {
+    AttnArgs a = all;
+    const uint32_t smem = kDirectKeys * DP * 4u + (a.R > 16 ? kDirectWarps * 16 * DP * 4u : 0u);
+    if ((err = opt_in(attend_direct<T, DP>, smem))) return err;
+    attend_direct<T, DP><<<dim3(w.splits, a.B * a.M, a.G), kDirectWarps * 32, smem, st>>>(a);
+    if ((err = cudaGetLastError())) return err;
+    if (w.splits > 1) {
+      const uint64_t rows = (uint64_t)a.B * a.M * a.H;
+      attend_join<T, true><<<(uint32_t)ceil_div(rows, 256 >> lanes), 256, 0, st>>>(a, lanes);
+    }
+    return cudaGetLastError();
+  }
+  const uint32_t smem = 4u * 64u * DP * 2u;
+  if ((err = opt_in(attend_tiles<T, DP>, smem))) return err;
+  for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
+    AttnArgs a = turn_args(all, b0, w.bc);
+    if ((err = run_plan(a, w, st))) return err;
+    const uint64_t tiles = (uint64_t)a.B * a.M * a.top * a.R / w.tile_rows + (uint64_t)a.B * a.nsb;
+    for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
+      a.gc = std::min(w.gc, a.G - a.g0);
+      if (tiles) attend_tiles<T, DP><<<dim3((uint32_t)tiles, a.gc), 256, smem, st>>>(a);
+      if ((err = cudaGetLastError())) return err;
+      const uint64_t rows = (uint64_t)a.B * a.M * a.gc * a.R;
+      attend_join<T, false><<<(uint32_t)ceil_div(rows, 256 >> lanes), 256, 0, st>>>(a, lanes);
+      if ((err = cudaGetLastError())) return err;
+    }
+  }
+  return cudaSuccess;
+}
+
+template <class T, int DP, int SPAN>
+cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
+  cudaError_t err;
+  const int lanes = row_lanes_log2(all.D);
+  const uint32_t smem = grad_smem<DP, SPAN>();
+  if ((err = opt_in(attend_grad<T, DP, SPAN>, smem))) return err;
+  for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
+    AttnArgs a = turn_args(all, b0, w.bc);
+    const uint64_t nq = (uint64_t)a.B * a.M;
+    if ((err = run_plan(a, w, st))) return err;
+    if (nq) {
+      grad_delta<T><<<(uint32_t)ceil_div(nq * a.H, 32), 256, 0, st>>>(a);
+      if ((err = cudaGetLastError())) return err;
+    }
+    const uint32_t spans = a.B * a.nsb;
+    const uint64_t tiles = nq * a.top * a.R / w.tile_rows + spans;
+    for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
+      a.gc = std::min(w.gc, a.G - a.g0);
+      if (tiles) attend_grad<T, DP, SPAN><<<dim3((uint32_t)tiles, a.gc), SPAN * 2, smem, st>>>(a);
+      if ((err = cudaGetLastError())) return err;
+      if (nq * a.top * a.R > w.tile_rows && spans) {
+        grad_join_keys<T><<<dim3(spans, a.gc, 4), 256, 0, st>>>(a, SPAN);
+        if ((err = cudaGetLastError())) return err;
+      }
+      if (nq) {
+        grad_join_queries<T><<<(uint32_t)ceil_div(nq * a.gc * a.R, 256 >> lanes), 256, 0, st>>>(
+            a, lanes);
+        if ((err = cudaGetLastError())) return err;
+      }
+    }
+  }
+  return cudaSuccess;
+}
+
+template <class T>
+cudaError_t forward_of(const AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
+  switch (padded_dim(a.D)) {
+    case 32: return launch_forward<T, 32>(a, w, st);
+    case 64: return launch_forward<T, 64>(a, w, st);
+    default: return launch_forward<T, 128>(a, w, st);
+  }
+}
+
+template <class T>
+cudaError_t backward_of(const AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
+  switch (padded_dim(a.D)) {
+    case 32: return launch_backward<T, 32, 128>(a, w, st);
+    case 64: return launch_backward<T, 64, 128>(a, w, st);
+    default: return launch_backward<T, 128, 128>(a, w, st);
+  }
 }
 
 int check_work(const void *d_work, uint64_t have, uint64_t need) {
@@ -273,7 +1270,7 @@ int nsfps_block_attention_workspace(const nsfps_attention_desc *desc, int backwa
   int rc = check_attention(desc);
   if (rc) return rc;
   if (!bytes) return set_error(NSFPS_ERR_ARG, "bytes is NULL");
-  *bytes = carve_attention(*desc, backward != 0, nullptr).bytes;
+  *bytes = plan_attention(*desc, backward != 0, nullptr).bytes;
   return NSFPS_OK;
 }
 
@@ -292,17 +1289,15 @@ int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d
     return set_error(NSFPS_ERR_ARG, "q, k, v and out must be 16-byte aligned");
   if ((uint64_t)d_blocks % 8 || ((uint64_t)d_lse | (uint64_t)d_lengths) % 4)
     return set_error(NSFPS_ERR_ARG, "a pointer is not aligned to its elements");
-  const AttnWork w = carve_attention(d, false, d_work);
+  const AttnPlan w = plan_attention(d, false, d_work);
   rc = check_work(d_work, work_bytes, w.bytes);
   if (rc) return rc;
-  AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths);
-  a.out = d_out;
+  AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths, w);
+  a.out = (char *)d_out;
   a.lse = d_lse;
   cudaStream_t st = (cudaStream_t)stream;
-  const uint32_t grid = (uint32_t)ceil_div(d.batch * d.queries * d.heads, 8);
-  if (d.dtype == NSFPS_F16) attend_forward<__half><<<grid, 256, 0, st>>>(a);
-  else attend_forward<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  NSFPS_FEATURE_CUDA(cudaGetLastError());
+  NSFPS_FEATURE_CUDA(d.dtype == NSFPS_F16 ? forward_of<__half>(a, w, st)
+                                          : forward_of<__nv_bfloat16>(a, w, st));
   return NSFPS_OK;
 }
 
@@ -326,37 +1321,15 @@ int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const vo
     return set_error(NSFPS_ERR_ARG, "q, k, v, out and the gradients must be 16-byte aligned");
   if ((uint64_t)d_blocks % 8 || ((uint64_t)d_lse | (uint64_t)d_lengths) % 4)
     return set_error(NSFPS_ERR_ARG, "a pointer is not aligned to its elements");
-  const AttnWork w = carve_attention(d, true, d_work);
+  const AttnPlan w = plan_attention(d, true, d_work);
   rc = check_work(d_work, work_bytes, w.bytes);
   if (rc) return rc;
-  AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths);
-  a.out_in = d_out; a.lse_in = d_lse; a.dout = d_dout;
-  a.dq = d_dq; a.dk = d_dk; a.dv = d_dv;
+  AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths, w);
+  a.out_in = (const char *)d_out; a.lse_in = d_lse; a.dout = (const char *)d_dout;
+  a.dq = (char *)d_dq; a.dk = (char *)d_dk; a.dv = (char *)d_dv;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool half = d.dtype == NSFPS_F16;
-  if (nq) {
-    const uint32_t grid = (uint32_t)ceil_div(nq * d.heads, 8);
-    if (half) attend_dq<__half><<<grid, 256, 0, st>>>(a, w.delta);
-    else attend_dq<__nv_bfloat16><<<grid, 256, 0, st>>>(a, w.delta);
-    NSFPS_FEATURE_CUDA(cudaGetLastError());
-  }
-  if (nk) {
-    const uint32_t n = (uint32_t)(nq * d.top), groups = a.B * a.nb;
-    uint32_t *keys = w.sort.keys0, *vals = w.sort.vals0, launches = 0;
-    if (n) {
-      pair_keys<<<(uint32_t)ceil_div(n, 256), 256, 0, st>>>(a, groups, keys, vals);
-      NSFPS_FEATURE_CUDA(cudaGetLastError());
-      NSFPS_FEATURE_CUDA(run_sort_pairs(&keys, &vals, w.sort.keys1, w.sort.vals1, n, groups,
-                                        w.sort.hist, w.sort.partial, st, launches));
-    }
-    pair_starts<<<(uint32_t)ceil_div((uint64_t)groups + 1, 256), 256, 0, st>>>(keys, n, groups,
-                                                                              w.start);
-    NSFPS_FEATURE_CUDA(cudaGetLastError());
-    const uint32_t grid = (uint32_t)ceil_div(nk * d.kv_heads, 8);
-    if (half) attend_dkv<__half><<<grid, 256, 0, st>>>(a, w.delta, vals, w.start);
-    else attend_dkv<__nv_bfloat16><<<grid, 256, 0, st>>>(a, w.delta, vals, w.start);
-    NSFPS_FEATURE_CUDA(cudaGetLastError());
-  }
+  NSFPS_FEATURE_CUDA(d.dtype == NSFPS_F16 ? backward_of<__half>(a, w, st)
+                                          : backward_of<__nv_bfloat16>(a, w, st));
   return NSFPS_OK;
 }
 
