@@ -21,10 +21,12 @@ With the sampler and the grouping operators:
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 
 from . import capi
-from .group import _cloud_batch, _dtype_code, _scratch
+from .group import _cloud_batch, _dtype_code, _on
 
 __all__ = ["select_blocks", "block_attention"]
 
@@ -54,6 +56,12 @@ def _check_lengths(lengths, B, device):
     return lengths.data_ptr(), lengths
 
 
+@functools.lru_cache(maxsize=256)
+def _select_desc(B, N, M, block, top):
+    desc = capi.SelectDesc(B, N, M, block, top)
+    return desc, capi.select_blocks_workspace(desc)
+
+
 def select_blocks(points, centers, block: int, top: int, lengths=None):
     """The ``top`` blocks nearest to each centre.
 
@@ -81,15 +89,13 @@ def select_blocks(points, centers, block: int, top: int, lengths=None):
     _check_block(block, top)
     B, N, M = int(pts.shape[0]), int(pts.shape[1]), int(ctr.shape[1])
     len_ptr, _len = _check_lengths(lengths, B, pts.device)
-    blocks = torch.empty((B, M, top), dtype=torch.int64, device=pts.device)
-    d2 = torch.empty((B, M, top), dtype=torch.float32, device=pts.device)
-    desc = capi.SelectDesc(B, N, M, block, top)
-    with torch.cuda.device(pts.device):
-        stream = torch.cuda.current_stream(pts.device)
-        work = _scratch(capi.select_blocks_workspace(desc), pts.device)
+    blocks = pts.new_empty((B, M, top), dtype=torch.int64)
+    d2 = pts.new_empty((B, M, top))
+    desc, need = _select_desc(B, N, M, block, top)
+    with _on(pts) as stream:
+        work = pts.new_empty(need, dtype=torch.uint8)
         capi.select_blocks_device(desc, pts.data_ptr(), len_ptr, ctr.data_ptr(),
-                                  blocks.data_ptr(), d2.data_ptr(), work.data_ptr(),
-                                  work.numel(), stream.cuda_stream)
+                                  blocks.data_ptr(), d2.data_ptr(), work.data_ptr(), need, stream)
     return (blocks[0], d2[0]) if single else (blocks, d2)
 
 
@@ -104,32 +110,38 @@ def _rows16(t):
 
 def _strides(t):
     """Strides of batch, row and head; an axis of one entry is never stepped."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])])
 
 
-def _desc(q, k, v, blocks, block, scale):
-    B, M, H, D = q.shape
-    three = capi.ctypes.c_int64 * 3
-    return capi.AttentionDesc(B, M, k.shape[1], H, k.shape[2], D, block, blocks.shape[2],
-                              _dtype_code(q, "q", (capi.F16, capi.BF16)),
-                              three(*_strides(q)), three(*_strides(k)), three(*_strides(v)),
-                              scale, 0)
+@functools.lru_cache(maxsize=256)
+def _make_desc(q_shape, k_shape, top, q_strides, k_strides, v_strides, code, block, scale,
+               backward):
+    B, M, H, D = q_shape
+    three = ctypes.c_int64 * 3
+    desc = capi.AttentionDesc(B, M, k_shape[1], H, k_shape[2], D, block, top, code,
+                              three(*q_strides), three(*k_strides), three(*v_strides), scale, 0)
+    return desc, capi.block_attention_workspace(desc, backward)
+
+
+def _desc(q, k, v, blocks, block, scale, backward):
+    """The call's descriptor and its scratch bytes."""
+    return _make_desc(q.shape, k.shape, blocks.shape[2], _strides(q), _strides(k), _strides(v),
+                      _dtype_code(q, "q", (capi.F16, capi.BF16)), block, scale, backward)
 
 
 def _forward(q, k, v, blocks, block, lengths, scale, want_lse):
     import torch
     q, k, v, blocks = _rows16(q), _rows16(k), _rows16(v), blocks.contiguous()
     len_ptr, _len = _check_lengths(lengths, q.shape[0], q.device)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    desc = _desc(q, k, v, blocks, block, scale)
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream(q.device)
-        work = _scratch(capi.block_attention_workspace(desc, False), q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if want_lse else None
+    desc, need = _desc(q, k, v, blocks, block, scale, False)
+    with _on(q) as stream:
+        work = q.new_empty(need, dtype=torch.uint8)
         capi.block_attention_device(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                     blocks.data_ptr(), len_ptr, out.data_ptr(),
-                                    lse.data_ptr() if want_lse else 0, work.data_ptr(),
-                                    work.numel(), stream.cuda_stream)
+                                    lse.data_ptr() if want_lse else 0, work.data_ptr(), need,
+                                    stream)
     return out, lse
 
 
@@ -138,15 +150,14 @@ def _backward(q, k, v, blocks, block, lengths, scale, out, lse, dout):
     q, k, v, dout, blocks = _rows16(q), _rows16(k), _rows16(v), dout.contiguous(), blocks.contiguous()
     dout = _rows16(dout)
     len_ptr, _len = _check_lengths(lengths, q.shape[0], q.device)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    desc = _desc(q, k, v, blocks, block, scale)
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream(q.device)
-        work = _scratch(capi.block_attention_workspace(desc, True), q.device)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    desc, need = _desc(q, k, v, blocks, block, scale, True)
+    with _on(q) as stream:
+        work = q.new_empty(need, dtype=torch.uint8)
         capi.block_attention_grad_device(
             desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), len_ptr,
             out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), work.data_ptr(), work.numel(), stream.cuda_stream)
+            dv.data_ptr(), work.data_ptr(), need, stream)
     return dq, dk, dv
 
 

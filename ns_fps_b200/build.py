@@ -26,7 +26,8 @@ MODULE = os.path.join(HERE, "yuezu_fps_module" + EXT)
 CU_SOURCES = ["nsfps_setup.cu", "nsfps_loop.cu", "nsfps_rounds.cu", "nsfps_static.cu",
               "nsfps_group.cu", "nsfps_rows.cu", "nsfps_select.cu", "nsfps_attention.cu",
               "nsfps_capi.cu"]
-HEADERS = ["nsfps_internal.cuh", "nsfps_kernels.h", "nsfps_device.cuh", "nsfps_feature.cuh"]
+HEADERS = ["nsfps_internal.cuh", "nsfps_kernels.h", "nsfps_device.cuh", "nsfps_feature.cuh",
+           "nsfps_sort.cuh"]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 NVCC_FLAGS = [

@@ -307,83 +307,96 @@ class AttentionDesc(ctypes.Structure):
                 ("reserved", ctypes.c_uint32)]
 
 
-def _ok(rc, name):
+def _feature_functions():
+    """The feature entries by name, their argument types set once: addresses
+    and sizes then pass as plain integers."""
+    p, u = ctypes.c_void_p, ctypes.c_uint64
+    types = {
+        "nsfps_gather_rows_device": [p] * 5,
+        "nsfps_gather_rows_grad_workspace": [p, p],
+        "nsfps_gather_rows_grad_device": [p] * 5 + [u, p],
+        "nsfps_select_blocks_workspace": [p, p],
+        "nsfps_select_blocks_device": [p] * 7 + [u, p],
+        "nsfps_block_attention_workspace": [p, ctypes.c_int, p],
+        "nsfps_block_attention_device": [p] * 9 + [u, p],
+        "nsfps_block_attention_grad_device": [p] * 13 + [u, p],
+    }
+    # a second handle of the library: other callers of lib() set no types
+    handle = ctypes.CDLL(lib()._name)
+    found = {}
+    for name, args in types.items():
+        f = getattr(handle, name)
+        f.argtypes, f.restype = args, ctypes.c_int
+        found[name] = f
+    return found
+
+
+_feature = None
+
+
+def _call(name, *args):
+    global _feature
+    if _feature is None:
+        _feature = _feature_functions()
+    rc = _feature[name](*args)
     if rc != OK:
         raise RuntimeError(f"{name} rc={rc}: {last_error()}")
 
 
-def _ptr(p):
-    return ctypes.c_void_p(p or None)
+def _bytes(name, *args):
+    n = ctypes.c_uint64(0)
+    _call(name, *args, ctypes.addressof(n))
+    return n.value
 
 
 def gather_rows_device(desc: RowsDesc, d_table_ptr: int, d_idx_ptr: int, d_out_ptr: int,
                        stream_ptr: int = 0):
     """nsfps_gather_rows_device."""
-    _ok(lib().nsfps_gather_rows_device(ctypes.byref(desc), _ptr(d_table_ptr), _ptr(d_idx_ptr),
-                                       _ptr(d_out_ptr), _ptr(stream_ptr)),
-        "nsfps_gather_rows_device")
+    _call("nsfps_gather_rows_device", ctypes.addressof(desc), d_table_ptr, d_idx_ptr, d_out_ptr,
+          stream_ptr)
 
 
 def gather_rows_grad_workspace(desc: RowsDesc) -> int:
     """nsfps_gather_rows_grad_workspace: bytes of scratch."""
-    n = ctypes.c_uint64(0)
-    _ok(lib().nsfps_gather_rows_grad_workspace(ctypes.byref(desc), ctypes.byref(n)),
-        "nsfps_gather_rows_grad_workspace")
-    return n.value
+    return _bytes("nsfps_gather_rows_grad_workspace", ctypes.addressof(desc))
 
 
 def gather_rows_grad_device(desc: RowsDesc, d_dout_ptr: int, d_idx_ptr: int, d_dtable_ptr: int,
                             d_work_ptr: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_gather_rows_grad_device."""
-    _ok(lib().nsfps_gather_rows_grad_device(ctypes.byref(desc), _ptr(d_dout_ptr), _ptr(d_idx_ptr),
-                                            _ptr(d_dtable_ptr), _ptr(d_work_ptr),
-                                            ctypes.c_uint64(work_bytes), _ptr(stream_ptr)),
-        "nsfps_gather_rows_grad_device")
+    _call("nsfps_gather_rows_grad_device", ctypes.addressof(desc), d_dout_ptr, d_idx_ptr,
+          d_dtable_ptr, d_work_ptr, work_bytes, stream_ptr)
 
 
 def select_blocks_workspace(desc: SelectDesc) -> int:
     """nsfps_select_blocks_workspace: bytes of scratch."""
-    n = ctypes.c_uint64(0)
-    _ok(lib().nsfps_select_blocks_workspace(ctypes.byref(desc), ctypes.byref(n)),
-        "nsfps_select_blocks_workspace")
-    return n.value
+    return _bytes("nsfps_select_blocks_workspace", ctypes.addressof(desc))
 
 
 def select_blocks_device(desc: SelectDesc, d_xyz_ptr: int, d_lengths_ptr: int,
                          d_centers_ptr: int, d_blocks_ptr: int, d_d2_ptr: int, d_work_ptr: int,
                          work_bytes: int, stream_ptr: int = 0):
     """nsfps_select_blocks_device (d_lengths_ptr, d_d2_ptr: 0 for NULL)."""
-    _ok(lib().nsfps_select_blocks_device(ctypes.byref(desc), _ptr(d_xyz_ptr), _ptr(d_lengths_ptr),
-                                         _ptr(d_centers_ptr), _ptr(d_blocks_ptr), _ptr(d_d2_ptr),
-                                         _ptr(d_work_ptr), ctypes.c_uint64(work_bytes),
-                                         _ptr(stream_ptr)),
-        "nsfps_select_blocks_device")
+    _call("nsfps_select_blocks_device", ctypes.addressof(desc), d_xyz_ptr, d_lengths_ptr,
+          d_centers_ptr, d_blocks_ptr, d_d2_ptr, d_work_ptr, work_bytes, stream_ptr)
 
 
 def block_attention_workspace(desc: AttentionDesc, backward: bool) -> int:
     """nsfps_block_attention_workspace: bytes of scratch."""
-    n = ctypes.c_uint64(0)
-    _ok(lib().nsfps_block_attention_workspace(ctypes.byref(desc),
-                                              ctypes.c_int(1 if backward else 0),
-                                              ctypes.byref(n)),
-        "nsfps_block_attention_workspace")
-    return n.value
+    return _bytes("nsfps_block_attention_workspace", ctypes.addressof(desc), 1 if backward else 0)
 
 
 def block_attention_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int, lengths: int,
                            out: int, lse: int, work: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_block_attention_device on device addresses (lengths, lse: 0 for
     NULL)."""
-    _ok(lib().nsfps_block_attention_device(
-        ctypes.byref(desc), *map(_ptr, (q, k, v, blocks, lengths, out, lse, work)),
-        ctypes.c_uint64(work_bytes), _ptr(stream_ptr)), "nsfps_block_attention_device")
+    _call("nsfps_block_attention_device", ctypes.addressof(desc), q, k, v, blocks, lengths, out,
+          lse, work, work_bytes, stream_ptr)
 
 
 def block_attention_grad_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int,
                                 lengths: int, out: int, lse: int, dout: int, dq: int, dk: int,
                                 dv: int, work: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_block_attention_grad_device on device addresses."""
-    _ok(lib().nsfps_block_attention_grad_device(
-        ctypes.byref(desc),
-        *map(_ptr, (q, k, v, blocks, lengths, out, lse, dout, dq, dk, dv, work)),
-        ctypes.c_uint64(work_bytes), _ptr(stream_ptr)), "nsfps_block_attention_grad_device")
+    _call("nsfps_block_attention_grad_device", ctypes.addressof(desc), q, k, v, blocks, lengths,
+          out, lse, dout, dq, dk, dv, work, work_bytes, stream_ptr)

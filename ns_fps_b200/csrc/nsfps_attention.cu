@@ -22,6 +22,7 @@
 #include <cmath>
 
 #include "nsfps_feature.cuh"
+#include "nsfps_sort.cuh"
 
 namespace nsfps {
 namespace {
@@ -46,9 +47,9 @@ struct AttnArgs {
   const uint32_t *vals;    // sorted pairs: query * top + leading slot
   const uint32_t *mask;    // per query slot: blocks of the span that are listed
   const unsigned long long *lead;  // per query: bit s = slot s leads a pair
-  const uint32_t *start;   // first pair of each span (B * nsb + 1)
-  const uint32_t *tile_off;  // first tile of each span (B * nsb + 1)
+  const uint4 *span;       // per span: first pair, end, first tile, tiles
   const uint2 *tiles;      // (span, tile within the span)
+  const uint32_t *tile_count;
   // partials of key heads g0 .. g0 + gc - 1
   uint32_t g0, gc;
   float *part;             // [pair][gc * R][D]
@@ -163,9 +164,10 @@ __device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
 // 64-key chunks of it that are read, so that the rows of a tile read alike.
 __global__ void __launch_bounds__(256)
 plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
-           uint32_t *__restrict__ vals, uint32_t *__restrict__ mask,
-           unsigned long long *__restrict__ lead) {
+           uint32_t *__restrict__ mask,
+           unsigned long long *__restrict__ lead, uint32_t *__restrict__ tile_count) {
   const uint32_t lane = threadIdx.x & 31u;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *tile_count = 0;  // for plan_spans
   const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (bm >= a.B * a.M) return;
   const uint32_t b = bm / a.M;
@@ -209,36 +211,37 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
       read |= ((m[i] >> lo) & ((1u << n) - 1u)) ? 1u << c : 0u;
     }
     keys[p] = first[i] ? ((b * a.nsb + sb[i]) << chunks) | read : (a.B * a.nsb) << chunks;
-    vals[p] = (uint32_t)p;
     mask[p] = m[i];
   }
 }
 
-// Per span: its first pair, and its tiles of tile_rows rows (at least
-// `least`).
-__global__ void __launch_bounds__(256)
-plan_spans(const uint32_t *__restrict__ keys, uint32_t n, uint32_t spans, uint32_t shift,
-           uint32_t R, uint32_t tile_rows, uint32_t least, uint32_t *__restrict__ start,
-           uint32_t *__restrict__ count) {
-  const uint32_t s = blockIdx.x * 256u + threadIdx.x;
-  if (s > spans) return;
-  const uint32_t b = lower_bound(keys, n, s << shift);
-  start[s] = b;
-  uint32_t tiles = 0;
-  if (s < spans) {
-    const uint32_t e = lower_bound(keys, n, (s + 1u) << shift);
-    tiles = max(least, (uint32_t)(((uint64_t)(e - b) * R + tile_rows - 1u) / tile_rows));
-  }
-  count[s] = tiles;
-}
+// Keys of the sort: one per query slot, in slot order.
+struct PairKeys {
+  const uint32_t *keys;
+  static constexpr bool kFirst = true;
+  __device__ __forceinline__ uint32_t count(uint32_t n) const { return n; }
+  __device__ __forceinline__ uint32_t key(uint32_t i) const { return keys[i]; }
+  __device__ __forceinline__ uint32_t value(uint32_t i) const { return i; }
+};
 
-// One warp per span: lists its tiles.
+// One warp per span: its pairs, and its tiles of tile_rows rows (at least
+// `least`), which it lists at a place it takes from a counter.  The places
+// differ from run to run; no result depends on them.
 __global__ void __launch_bounds__(256)
-plan_tiles(const uint32_t *__restrict__ tile_off, uint32_t spans, uint2 *__restrict__ tiles) {
-  const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5);
+plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, uint32_t tile_rows,
+           uint32_t least, uint4 *__restrict__ span, uint2 *__restrict__ tiles,
+           uint32_t *__restrict__ tile_count) {
+  const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
   if (s >= spans) return;
-  const uint32_t b = tile_off[s], e = tile_off[s + 1];
-  for (uint32_t i = b + (threadIdx.x & 31u); i < e; i += 32u) tiles[i] = make_uint2(s, i - b);
+  const uint32_t n = *list.kept;
+  const uint32_t b = warp_lower_bound(list.keys, n, s << shift);
+  const uint32_t e = b + warp_lower_bound(list.keys + b, n - b, (s + 1u) << shift);
+  const uint32_t count = max(least, (uint32_t)(((uint64_t)(e - b) * R + tile_rows - 1u) / tile_rows));
+  uint32_t first = 0;
+  if (lane == 0 && count) first = atomicAdd(tile_count, count);
+  first = __shfl_sync(kFullMask, first, 0);
+  if (lane == 0) span[s] = make_uint4(b, e, first, count);
+  for (uint32_t i = lane; i < count; i += 32u) tiles[first + i] = make_uint2(s, i);
 }
 
 // -------------------------------------------------------------- forward
@@ -388,13 +391,13 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
 attend_tiles(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t s_any[8];
-  const uint32_t spans = a.B * a.nsb;
-  if (blockIdx.x >= a.tile_off[spans]) return;
+  if (blockIdx.x >= *a.tile_count) return;
   const uint2 tile = a.tiles[blockIdx.x];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
   const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint32_t e0 = a.start[tile.x], rows = (a.start[tile.x + 1] - e0) * a.R;
+  const uint4 span = a.span[tile.x];
+  const uint32_t e0 = span.x, rows = (span.y - e0) * a.R;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
   const uint32_t key0 = sb << kSpanLog2;
 
@@ -700,13 +703,13 @@ __global__ void __launch_bounds__(SPAN * 2, DP <= 64 && SPAN == 128 ? 2 : 1)
 attend_grad(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   constexpr uint32_t kThreads = SPAN * 2, kWarps = SPAN / 16, kChunks = DP / 8;
-  const uint32_t spans = a.B * a.nsb;
-  if (blockIdx.x >= a.tile_off[spans]) return;
+  if (blockIdx.x >= *a.tile_count) return;
   const uint2 tile = a.tiles[blockIdx.x];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, t = lane & 3u;
   const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
   const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint32_t e0 = a.start[tile.x], all_rows = (a.start[tile.x + 1] - e0) * a.R;
+  const uint4 span = a.span[tile.x];
+  const uint32_t e0 = span.x, all_rows = (span.y - e0) * a.R;
   const uint32_t row0 = tile.y * kGradItem;
   const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
@@ -935,8 +938,9 @@ template <class T>
 __global__ void __launch_bounds__(256)
 grad_join_keys(const AttnArgs a, uint32_t span) {
   const uint32_t s = blockIdx.x, gi = blockIdx.y, g = a.g0 + gi;
-  const uint32_t i0 = a.tile_off[s], i1 = a.tile_off[s + 1];
-  if (i1 - i0 < 2u) return;
+  const uint4 sp = a.span[s];
+  const uint32_t i0 = sp.z, i1 = sp.z + sp.w;
+  if (sp.w < 2u) return;
   const uint32_t b = s / a.nsb, key0 = (s - b * a.nsb) * span;
   const uint32_t keys = min(span, a.N - key0);
   for (uint32_t x = blockIdx.z * 256u + threadIdx.x; x < keys * a.D / 2u; x += 256u * gridDim.z) {
@@ -1025,7 +1029,8 @@ struct AttnPlan {
   uint32_t span_log2, tile_rows, least, splits;
   uint64_t pairs, spans, max_tiles;  // of one turn
   SortScratch sort;
-  uint32_t *mask, *start, *tile_off, *scan;
+  uint32_t *mask, *tile_count;
+  uint4 *span;
   unsigned long long *lead;
   uint2 *tiles;
   float *part, *part_lse, *delta, *part_kv;
@@ -1074,9 +1079,8 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.sort.carve(c, (uint32_t)w.pairs);
   w.mask = c.take<uint32_t>(w.pairs);
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
-  w.start = c.take<uint32_t>(w.spans + 1);
-  w.tile_off = c.take<uint32_t>(w.spans + 1);
-  w.scan = c.take<uint32_t>(ceil_div(w.spans + 1, 4096) + 2);
+  w.span = c.take<uint4>(w.spans);
+  w.tile_count = c.take<uint32_t>(1);
   w.tiles = c.take<uint2>(w.max_tiles);
   w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
@@ -1101,7 +1105,7 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   for (int i = 0; i < 3; ++i) a.qs[i] = d.q_stride[i], a.ks[i] = d.k_stride[i], a.vs[i] = d.v_stride[i];
   a.scale = d.scale;
   a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
-  a.mask = w.mask; a.lead = w.lead; a.start = w.start; a.tile_off = w.tile_off;
+  a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
   a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
   a.part_kv = w.part_kv; a.splits = w.splits; a.gc = w.gc;
   return a;
@@ -1127,24 +1131,27 @@ AttnArgs turn_args(const AttnArgs &all, uint32_t b0, uint32_t bc) {
 
 // Sorts a turn's pairs by span and lists its tiles.
 cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
-  const uint32_t n = a.B * a.M * a.top, spans = a.B * a.nsb, shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
-  uint32_t *keys = w.sort.keys0, *vals = w.sort.vals0, launches = 0;
+  const uint32_t n = a.B * a.M * a.top, spans = a.B * a.nsb;
+  const uint32_t shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
+  SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
-  if (n) {
-    plan_pairs<<<(uint32_t)ceil_div(a.B * a.M, 8), 256, 0, st>>>(a, w.span_log2, keys, vals, w.mask,
-                                                                 w.lead);
+  if (n && spans) {
+    plan_pairs<<<(uint32_t)ceil_div(a.B * a.M, 8), 256, 0, st>>>(a, w.span_log2, w.sort.keys0,
+                                                                 w.mask, w.lead, w.tile_count);
     if ((err = cudaGetLastError())) return err;
-    if ((err = run_sort_pairs(&keys, &vals, w.sort.keys1, w.sort.vals1, n, spans << shift,
-                              w.sort.hist, w.sort.partial, st, launches)))
+    if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
+  } else {  // no pair, or no key to form one with
+    if ((err = cudaMemsetAsync(w.sort.kept, 0, 4, st))) return err;
+    if ((err = cudaMemsetAsync(w.tile_count, 0, 4, st))) return err;
+    if (a.B * a.M &&
+        (err = cudaMemsetAsync(w.lead, 0, sizeof(*w.lead) * (uint64_t)a.B * a.M, st)))
       return err;
   }
-  a.vals = vals;
-  plan_spans<<<(uint32_t)ceil_div((uint64_t)spans + 1, 256), 256, 0, st>>>(
-      keys, n, spans, shift, a.R, w.tile_rows, w.least, w.start, w.tile_off);
-  if ((err = cudaGetLastError())) return err;
-  if ((err = run_exclusive_scan(w.tile_off, w.tile_off, spans + 1, w.scan, st, launches)))
-    return err;
-  if (spans) plan_tiles<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(w.tile_off, spans, w.tiles);
+  a.vals = list.vals;
+  if (spans)
+    plan_spans<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(list, spans, shift, a.R, w.tile_rows,
+                                                             w.least, w.span, w.tiles,
+                                                             w.tile_count);
   return cudaGetLastError();
 }
 

@@ -42,20 +42,6 @@ inline int sm_count() {
   return sms;
 }
 
-// Scratch of run_sort_pairs over n pairs (its second buffers included).
-struct SortScratch {
-  uint32_t *keys0, *vals0, *keys1, *vals1, *hist, *partial;
-  void carve(WorkCarver &w, uint32_t n) {
-    const uint64_t h = 256ull * radix_tiles(n) + 1;
-    keys0 = w.take<uint32_t>(n);
-    vals0 = w.take<uint32_t>(n);
-    keys1 = w.take<uint32_t>(n);
-    vals1 = w.take<uint32_t>(n);
-    hist = w.take<uint32_t>(h);
-    partial = w.take<uint32_t>(h / 4096 + 3);
-  }
-};
-
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -68,18 +54,6 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
-}
-
-// First position in the ascending keys[0 .. n) whose key is >= v.
-__device__ __forceinline__ uint32_t lower_bound(const uint32_t *__restrict__ keys, uint32_t n,
-                                                uint32_t v) {
-  uint32_t lo = 0, hi = n;
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (keys[mid] < v) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
 }
 
 }  // namespace nsfps

@@ -4,13 +4,16 @@
 // the row and the output move once.
 //
 // Gradient: dtable[n] = scale * sum of dout[p] over idx[p] == n.  The entries
-// (n, p) are sorted by n with the engine's stable radix sort, so each row's
-// entries are consecutive and ascending in p, and every row is written once
-// by one owner: no atomics, the same bits every time.
+// are sorted by index, stably, so a row's entries are consecutive and ascending
+// in p, and every row is written once by one owner: no atomics, the same bits
+// every time.  In a batch the index alone is the key: positions ascend with the
+// batch entry, so the entries of (n, b) are consecutive too, and the sort needs
+// the bits of N and not those of B * N.
 #include <algorithm>
 #include <cmath>
 
 #include "nsfps_feature.cuh"
+#include "nsfps_sort.cuh"
 
 namespace nsfps {
 namespace {
@@ -94,30 +97,35 @@ gather_rows_kernel(const RowsArgs a, const int lanes_log2) {
   }
 }
 
-// Sort keys: the table row over all batch entries; `none` (batch * rows) for
-// entries without a row, which sort behind every row.
+// Sort keys: the indices; `rows` for an entry without a row, which is dropped.
+struct IndexKeys {
+  const int64_t *idx;
+  uint32_t rows;
+  static constexpr bool kFirst = true;
+  __device__ __forceinline__ uint32_t count(uint32_t n) const { return n; }
+  __device__ __forceinline__ uint32_t key(uint32_t i) const {
+    const int64_t v = idx[i];
+    return v >= 0 && v < (int64_t)rows ? (uint32_t)v : rows;
+  }
+  __device__ __forceinline__ uint32_t value(uint32_t i) const { return i; }
+};
+
+// Where each table row's entries lie in the sorted list: its first and last
+// entry write their ends (rows without an entry keep the zeros written before).
 __global__ void __launch_bounds__(256)
-rows_keys(const int64_t *__restrict__ idx, uint32_t total, uint32_t count, uint32_t rows,
-          uint32_t none, uint32_t *__restrict__ keys, uint32_t *__restrict__ vals) {
-  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
-  if (p >= total) return;
-  const int64_t i = idx[p];
-  keys[p] = (i >= 0 && i < (int64_t)rows) ? (p / count) * rows + (uint32_t)i : none;
-  vals[p] = p;
+rows_runs(const SortedList list, uint32_t count, uint32_t rows, uint2 *__restrict__ run) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, n = *list.kept;
+  if (i >= n) return;
+  const uint32_t key = list.keys[i], b = list.vals[i] / count;
+  const uint32_t row = b * rows + key;
+  if (i == 0 || list.keys[i - 1] != key || list.vals[i - 1] / count != b) run[row].x = i;
+  if (i + 1 == n || list.keys[i + 1] != key || list.vals[i + 1] / count != b) run[row].y = i + 1;
 }
 
-// start[r] = first sorted entry of row r; start[rows] = entries with a row.
-__global__ void __launch_bounds__(256)
-rows_starts(const uint32_t *__restrict__ keys, uint32_t n, uint32_t rows,
-            uint32_t *__restrict__ start) {
-  const uint32_t r = blockIdx.x * 256u + threadIdx.x;
-  if (r <= rows) start[r] = lower_bound(keys, n, r);
-}
-
-// A row with more entries than this is summed in tiles of the sorted list by
-// rows_hot_tiles / rows_hot_join: one warp's serial walk would otherwise hold
-// up the launch (a row that every entry names).
-constexpr uint32_t kHotTile = 256;
+// A row with more entries than a tile is summed tile by tile (rows_hot_tiles,
+// rows_hot_join): one warp's serial walk would hold up the launch.  64 entries
+// are 16 steps of four loads.
+constexpr uint32_t kHotTile = 64;
 
 template <class T, int VB>
 __device__ __forceinline__ void add_entries(const char *__restrict__ dout,
@@ -153,48 +161,144 @@ __device__ __forceinline__ void store_row(char *out, uint64_t r, uint32_t vecs, 
   *reinterpret_cast<typename VecOf<VB>::type *>(out + (r * vecs + j) * VB) = y.v;
 }
 
+// Rows that a group of lanes sums side by side, two entries of each at a time:
+// eight loads in flight behind the run -> entry -> row chain.
+constexpr int kSumFlight = 4;
+
 // LANES lanes per table row.
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
 rows_sum(const char *__restrict__ dout, const uint32_t *__restrict__ vals,
-         const uint32_t *__restrict__ start, uint32_t rows, uint32_t vecs, float scale,
+         const uint2 *__restrict__ run, uint32_t rows, uint32_t vecs, float scale,
          char *__restrict__ out, const int lanes_log2) {
-  const uint32_t lanes = 1u << lanes_log2;
-  const uint32_t r = blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  if (r >= rows) return;
-  const uint32_t b = start[r], e = start[r + 1];
-  if (e - b > kHotTile) return;
+  constexpr int E = Pack<T, VB>::E;
+  using V = typename VecOf<VB>::type;
+  const uint32_t lanes = 1u << lanes_log2, per_block = 256u >> lanes_log2;
+  const uint32_t first = blockIdx.x * (per_block * kSumFlight) + (threadIdx.x >> lanes_log2);
+  uint32_t b[kSumFlight], n[kSumFlight], most = 0;
+#pragma unroll
+  for (int u = 0; u < kSumFlight; ++u) {
+    const uint32_t r = first + u * per_block;
+    const uint2 x = r < rows ? run[r] : make_uint2(0u, 0u);
+    b[u] = x.x;
+    n[u] = x.y - x.x > kHotTile ? 0u : x.y - x.x;  // a hot row is written elsewhere
+    most = max(most, n[u]);
+  }
   for (uint32_t j = threadIdx.x & (lanes - 1u); j < vecs; j += lanes) {
-    float acc[Pack<T, VB>::E] = {};
-    add_entries<T, VB>(dout, vals, b, e, vecs, j, acc);
-    store_row<T, VB>(out, r, vecs, j, scale, acc);
+    float acc[kSumFlight][E] = {};
+    for (uint32_t i = 0; i < most; i += 2u) {
+      uint32_t v[kSumFlight][2];
+      Pack<T, VB> x[kSumFlight][2];
+#pragma unroll
+      for (int u = 0; u < kSumFlight; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[u][k] = i + k < n[u] ? vals[b[u] + i + k] : 0u;
+#pragma unroll
+      for (int u = 0; u < kSumFlight; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (i + k < n[u])
+            x[u][k].v = *reinterpret_cast<const V *>(dout + ((uint64_t)v[u][k] * vecs + j) * VB);
+#pragma unroll
+      for (int u = 0; u < kSumFlight; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (i + k < n[u])
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[u][e] += to_f32(x[u][k].e[e]);
+    }
+#pragma unroll
+    for (int u = 0; u < kSumFlight; ++u) {
+      const uint32_t r = first + u * per_block;
+      if (r < rows && (n[u] || run[r].x == run[r].y))
+        store_row<T, VB>(out, r, vecs, j, scale, acc[u]);
+    }
   }
 }
 
-// Tile t: sorted entries [t * kHotTile, ...).  It meets at most two hot rows,
+// Tiles of the sorted list, one warp each.  A tile meets at most two hot rows,
 // that of its first entry and that of its last (any row between them is
 // shorter than the tile); slot 0 / 1 of part[] takes their sums over the tile.
+struct TileRow {
+  uint32_t row, lo, hi;  // table row (all ones: none), its entries
+};
+
+__device__ __forceinline__ TileRow row_of_entry(const SortedList &list, const uint2 *run,
+                                                uint32_t i, uint32_t count, uint32_t rows) {
+  TileRow t;
+  t.row = list.vals[i] / count * rows + list.keys[i];
+  const uint2 x = run[t.row];
+  t.lo = x.x;
+  t.hi = x.y;
+  if (t.hi - t.lo <= kHotTile) t.row = 0xffffffffu;
+  return t;
+}
+
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
-rows_hot_tiles(const char *__restrict__ dout, const uint32_t *__restrict__ keys,
-               const uint32_t *__restrict__ vals, const uint32_t *__restrict__ start,
-               uint32_t n, uint32_t none, uint32_t vecs, float *__restrict__ part) {
+rows_hot_tiles(const char *__restrict__ dout, const SortedList list,
+               const uint2 *__restrict__ run, uint32_t count, uint32_t rows, uint32_t vecs,
+               float *__restrict__ part) {
+  constexpr int E = Pack<T, VB>::E;
+  const uint32_t t = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+  const uint32_t n = *list.kept, b = t * kHotTile, e = min(n, b + kHotTile);
+  if (b >= n) return;
+  const TileRow first = row_of_entry(list, run, b, count, rows);
+  const TileRow last = row_of_entry(list, run, e - 1u, count, rows);
+  for (int s = 0; s < 2; ++s) {
+    const TileRow r = s ? last : first;
+    if (r.row == 0xffffffffu || (s && last.row == first.row)) continue;
+    for (uint32_t j = lane; j < vecs; j += 32u) {
+      float acc[E] = {};
+      add_entries<T, VB>(dout, list.vals, max(b, r.lo), min(e, r.hi), vecs, j, acc);
+      float *o = part + ((uint64_t)(2u * t + s) * vecs + j) * E;
+#pragma unroll
+      for (int k = 0; k < E; ++k) o[k] = acc[k];
+    }
+  }
+}
+
+// The hot row that starts in a tile (at most one: it reaches the tile's end)
+// adds its tile sums in order: eight warps a share each, then the shares.
+template <class T, int VB>
+__global__ void __launch_bounds__(256)
+rows_hot_join(const SortedList list, const uint2 *__restrict__ run, uint32_t count,
+              uint32_t rows, uint32_t vecs, float scale, const float *__restrict__ part,
+              char *__restrict__ out) {
   constexpr int E = Pack<T, VB>::E;
   __shared__ float s_acc[8][32][E];
-  const uint32_t b = blockIdx.x * kHotTile, e = min(n, b + kHotTile);
-  const uint32_t r0 = keys[b], r1 = keys[e - 1];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  for (int s = 0; s < 2; ++s) {
-    const uint32_t r = s ? r1 : r0;
-    if (r == none || (s && r1 == r0)) continue;
-    const uint32_t rb = start[r], re = start[r + 1];
-    if (re - rb <= kHotTile) continue;
-    const uint32_t lo = max(b, rb), hi = min(e, re);
-    const uint32_t per = (hi - lo + 7u) / 8u;
-    const uint32_t wb = min(hi, lo + warp * per), we = min(hi, wb + per);
+  __shared__ TileRow s_row[8];
+  __shared__ uint32_t s_slot[8];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = *list.kept;
+  if (blockIdx.x * 8u * kHotTile >= n) return;
+  {
+    const uint32_t t = blockIdx.x * 8u + warp, b = t * kHotTile, e = min(n, b + kHotTile);
+    TileRow r{0xffffffffu, 0u, 0u};
+    uint32_t slot = 0;
+    if (b < n) {
+      r = row_of_entry(list, run, e - 1u, count, rows);
+      if (r.row != 0xffffffffu && r.lo < b) r.row = 0xffffffffu;
+      slot = 2u * t + (r.lo == b ? 0u : 1u);
+    }
+    if (lane == 0) s_row[warp] = r, s_slot[warp] = slot;
+  }
+  __syncthreads();
+  for (uint32_t i = 0; i < 8u; ++i) {
+    const TileRow r = s_row[i];
+    if (r.row == 0xffffffffu) continue;
+    const uint32_t t = blockIdx.x * 8u + i, last = (r.hi - 1u) / kHotTile;  // tiles t .. last
+    const uint32_t per = (last - t + 8u) / 8u;
+    const uint32_t wb = min(last + 1u, t + warp * per), we = min(last + 1u, wb + per);
     for (uint32_t j0 = 0; j0 < vecs; j0 += 32u) {
       float acc[E] = {};
-      if (j0 + lane < vecs) add_entries<T, VB>(dout, vals, wb, we, vecs, j0 + lane, acc);
+      if (j0 + lane < vecs)
+#pragma unroll 4
+        for (uint32_t x = wb; x < we; ++x) {
+          const uint32_t slot = x == t ? s_slot[i] : 2u * x;
+          const float *o = part + ((uint64_t)slot * vecs + j0 + lane) * E;
+#pragma unroll
+          for (int k = 0; k < E; ++k) acc[k] += o[k];
+        }
 #pragma unroll
       for (int k = 0; k < E; ++k) s_acc[warp][lane][k] = acc[k];
       __syncthreads();
@@ -202,52 +306,10 @@ rows_hot_tiles(const char *__restrict__ dout, const uint32_t *__restrict__ keys,
         for (int w = 1; w < 8; ++w)
 #pragma unroll
           for (int k = 0; k < E; ++k) acc[k] += s_acc[w][lane][k];
-        float *o = part + ((uint64_t)(2u * blockIdx.x + s) * vecs + j0 + lane) * E;
-#pragma unroll
-        for (int k = 0; k < E; ++k) o[k] = acc[k];
+        store_row<T, VB>(out, r.row, vecs, j0 + lane, scale, acc);
       }
       __syncthreads();
     }
-  }
-}
-
-// The tile in which a hot row starts adds that row's tile sums in order.
-template <class T, int VB>
-__global__ void __launch_bounds__(256)
-rows_hot_join(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ start, uint32_t n,
-              uint32_t none, uint32_t vecs, float scale, const float *__restrict__ part,
-              char *__restrict__ out) {
-  constexpr int E = Pack<T, VB>::E;
-  __shared__ float s_acc[8][32][E];
-  const uint32_t t = blockIdx.x, b = t * kHotTile, e = min(n, b + kHotTile);
-  const uint32_t r = keys[e - 1];
-  if (r == none) return;
-  const uint32_t rb = start[r], re = start[r + 1];
-  if (re - rb <= kHotTile || rb < b) return;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t last = (re - 1u) / kHotTile;         // tiles t .. last
-  const uint32_t s0 = keys[b] == r ? 0u : 1u;         // its slot in tile t
-  const uint32_t per = (last - t + 8u) / 8u;
-  const uint32_t wb = t + warp * per, we = min(last + 1u, wb + per);
-  for (uint32_t j0 = 0; j0 < vecs; j0 += 32u) {
-    float acc[E] = {};
-    if (j0 + lane < vecs)
-      for (uint32_t i = wb; i < we; ++i) {
-        const uint32_t slot = 2u * i + (i == t ? s0 : 0u);
-        const float *o = part + ((uint64_t)slot * vecs + j0 + lane) * E;
-#pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] += o[k];
-      }
-#pragma unroll
-    for (int k = 0; k < E; ++k) s_acc[warp][lane][k] = acc[k];
-    __syncthreads();
-    if (warp == 0 && j0 + lane < vecs) {
-      for (int w = 1; w < 8; ++w)
-#pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] += s_acc[w][lane][k];
-      store_row<T, VB>(out, r, vecs, j0 + lane, scale, acc);
-    }
-    __syncthreads();
   }
 }
 
@@ -280,7 +342,7 @@ int check_rows(const nsfps_rows_desc *d) {
 
 struct RowsGradWork {
   SortScratch sort;
-  uint32_t *start;
+  uint2 *run;
   float *part;
   uint64_t bytes;
 };
@@ -290,7 +352,7 @@ RowsGradWork carve_rows_grad(const nsfps_rows_desc &d, void *base) {
   WorkCarver c(base);
   const uint32_t n = (uint32_t)(d.batch * d.count);
   w.sort.carve(c, n);
-  w.start = c.take<uint32_t>(d.batch * d.rows + 1);
+  w.run = c.take<uint2>(d.batch * d.rows);
   w.part = c.take<float>(2 * ceil_div(n, kHotTile) * d.width);
   w.bytes = c.off;
   return w;
@@ -333,20 +395,21 @@ struct LaunchGather {
 struct LaunchRowsSum {
   const char *dout;
   char *out;
-  const uint32_t *keys, *vals, *start;
+  SortedList list;
+  const uint2 *run;
   float *part;
-  uint32_t n, rows, vecs;
+  uint32_t n, count, all_rows, rows, vecs;
   float scale;
   int lanes_log2;
   cudaStream_t st;
   template <class T, int VB>
   cudaError_t operator()() const {
-    rows_sum<T, VB><<<(uint32_t)ceil_div(rows, 256u >> lanes_log2), 256, 0, st>>>(
-        dout, vals, start, rows, vecs, scale, out, lanes_log2);
+    rows_sum<T, VB><<<(uint32_t)ceil_div(all_rows, (256u >> lanes_log2) * kSumFlight), 256, 0,
+                      st>>>(dout, list.vals, run, all_rows, vecs, scale, out, lanes_log2);
     if (n > kHotTile) {  // fewer entries make no hot row
-      const uint32_t tiles = (uint32_t)ceil_div(n, kHotTile);
-      rows_hot_tiles<T, VB><<<tiles, 256, 0, st>>>(dout, keys, vals, start, n, rows, vecs, part);
-      rows_hot_join<T, VB><<<tiles, 256, 0, st>>>(keys, start, n, rows, vecs, scale, part, out);
+      const uint32_t grid = (uint32_t)ceil_div(n, 8u * kHotTile);
+      rows_hot_tiles<T, VB><<<grid, 256, 0, st>>>(dout, list, run, count, rows, vecs, part);
+      rows_hot_join<T, VB><<<grid, 256, 0, st>>>(list, run, count, rows, vecs, scale, part, out);
     }
     return cudaGetLastError();
   }
@@ -425,21 +488,20 @@ int nsfps_gather_rows_grad_device(const nsfps_rows_desc *desc, const void *d_dou
   if (work_bytes < w.bytes)
     return set_error(NSFPS_ERR_ARG, "d_work holds %llu bytes, %llu are needed",
                      (unsigned long long)work_bytes, (unsigned long long)w.bytes);
-  rows_keys<<<(uint32_t)ceil_div(n, 256), 256, 0, st>>>(d_idx, n, (uint32_t)d.count,
-                                                        (uint32_t)d.rows, rows, w.sort.keys0,
-                                                        w.sort.vals0);
-  NSFPS_FEATURE_CUDA(cudaGetLastError());
-  uint32_t *keys = w.sort.keys0, *vals = w.sort.vals0, launches = 0;
-  NSFPS_FEATURE_CUDA(run_sort_pairs(&keys, &vals, w.sort.keys1, w.sort.vals1, n, rows,
-                                    w.sort.hist, w.sort.partial, st, launches));
-  rows_starts<<<(uint32_t)ceil_div((uint64_t)rows + 1, 256), 256, 0, st>>>(keys, n, rows, w.start);
+  SortedList list;
+  NSFPS_FEATURE_CUDA(run_sort(IndexKeys{d_idx, (uint32_t)d.rows}, n, (uint32_t)d.rows, w.sort,
+                              &list, st));
+  NSFPS_FEATURE_CUDA(cudaMemsetAsync(w.run, 0, (uint64_t)rows * sizeof(uint2), st));
+  rows_runs<<<(uint32_t)ceil_div(n, 256), 256, 0, st>>>(list, (uint32_t)d.count, (uint32_t)d.rows,
+                                                        w.run);
   NSFPS_FEATURE_CUDA(cudaGetLastError());
   const int vb = vec_bytes((uint64_t)d_dout | (uint64_t)d_dtable | d.width * elem, elem);
   const uint32_t vecs = (uint32_t)(d.width * elem / vb);
   NSFPS_FEATURE_CUDA(with_vec(
       d.dtype, vb,
-      LaunchRowsSum{(const char *)d_dout, (char *)d_dtable, keys, vals, w.start, w.part, n, rows,
-                    vecs, d.scale, lanes_log2_for(vecs), st}));
+      LaunchRowsSum{(const char *)d_dout, (char *)d_dtable, list, w.run, w.part, n,
+                    (uint32_t)d.count, rows, (uint32_t)d.rows, vecs, d.scale,
+                    lanes_log2_for(vecs), st}));
   return NSFPS_OK;
 }
 

@@ -19,6 +19,8 @@ per operation without multiply-add contraction, hit iff d2 < radius * radius.
 """
 from __future__ import annotations
 
+import functools
+
 from . import capi
 
 __all__ = ["ball_query", "gather_points", "group_points", "gather_rows"]
@@ -107,40 +109,70 @@ def group_points(points, centers, idx):
     return out[0] if single else out
 
 
+_FLOATS = (capi.F32, capi.F16, capi.BF16)
+_codes = {}
+
+
 def _dtype_code(t, name, allowed):
-    import torch
-    code = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}.get(t.dtype)
-    if code is None or code not in allowed:
+    """The C code of t's type."""
+    if not _codes:
+        import torch
+        _codes.update({torch.float32: capi.F32, torch.float16: capi.F16,
+                       torch.bfloat16: capi.BF16})
+    code = _codes.get(t.dtype)
+    if code not in allowed:
         names = {capi.F32: "float32", capi.F16: "float16", capi.BF16: "bfloat16"}
         raise TypeError(f"{name} must be " + " or ".join(names[a] for a in allowed))
     return code
 
 
-def _scratch(nbytes, device):
-    """Scratch of one call, from PyTorch's allocator on the current stream."""
-    import torch
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+class _on:
+    """The current stream of a tensor's device, with that device current.  (The
+    switch is skipped where it is current already: it costs a small call more
+    than its kernels.)"""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, t):
+        self.device = t.device
+
+    def __enter__(self):
+        import torch
+        self.guard = None
+        if torch.cuda.current_device() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
-def _rows_desc(B, N, C, P, scale, code, batch_stride=0, row_stride=0):
+@functools.lru_cache(maxsize=256)
+def _rows_desc(B, N, C, P, batch_stride, row_stride, scale, code):
     return capi.RowsDesc(B, N, C, P, batch_stride, row_stride, scale, code)
 
 
+@functools.lru_cache(maxsize=256)
+def _rows_grad_desc(B, N, C, P, scale, code):
+    desc = capi.RowsDesc(B, N, C, P, 0, 0, scale, code)
+    return desc, capi.gather_rows_grad_workspace(desc)
+
+
 def _gather_rows_forward(table, idx, scale):
-    import torch
-    single = table.dim() == 2
-    B, N, C = (1, *table.shape) if single else table.shape
+    shape = table.shape
+    B, N, C = (1, *shape) if len(shape) == 2 else shape
     if (C > 1 and table.stride(-1) != 1) or C == 0:
         table = table.contiguous()
     idx = idx.contiguous()
-    out = torch.empty((*idx.shape, C), dtype=table.dtype, device=table.device)
-    P = idx.numel() // B if B else 0
-    desc = _rows_desc(B, N, C, P, scale, _dtype_code(table, "table", (0, 1, 2)),
-                      0 if single else table.stride(0), table.stride(-2))
-    with torch.cuda.device(table.device):
-        stream = torch.cuda.current_stream(table.device)
-        capi.gather_rows_device(desc, table.data_ptr(), idx.data_ptr(), out.data_ptr(),
-                                stream.cuda_stream)
+    out = table.new_empty((*idx.shape, C))
+    strides = table.stride()
+    desc = _rows_desc(B, N, C, idx.numel() // B if B else 0,
+                      strides[0] if len(shape) == 3 else 0, strides[-2], scale,
+                      _dtype_code(table, "table", _FLOATS))
+    with _on(table) as stream:
+        capi.gather_rows_device(desc, table.data_ptr(), idx.data_ptr(), out.data_ptr(), stream)
     return out
 
 
@@ -148,14 +180,13 @@ def _gather_rows_backward(dout, idx, shape, scale):
     import torch
     B, N, C = (1, *shape) if len(shape) == 2 else shape
     dout, idx = dout.contiguous(), idx.contiguous()
-    grad = torch.empty(shape, dtype=dout.dtype, device=dout.device)
-    P = idx.numel() // B if B else 0
-    desc = _rows_desc(B, N, C, P, scale, _dtype_code(dout, "grad", (0, 1, 2)))
-    with torch.cuda.device(dout.device):
-        stream = torch.cuda.current_stream(dout.device)
-        work = _scratch(capi.gather_rows_grad_workspace(desc), dout.device)
+    grad = dout.new_empty(shape)
+    desc, need = _rows_grad_desc(B, N, C, idx.numel() // B if B else 0, scale,
+                                 _dtype_code(dout, "grad", _FLOATS))
+    with _on(dout) as stream:
+        work = dout.new_empty(need, dtype=torch.uint8)
         capi.gather_rows_grad_device(desc, dout.data_ptr(), idx.data_ptr(), grad.data_ptr(),
-                                     work.data_ptr(), work.numel(), stream.cuda_stream)
+                                     work.data_ptr(), need, stream)
     return grad
 
 
@@ -206,7 +237,7 @@ def gather_rows(table, idx, scale: float = 1.0):
         raise TypeError("table must be a CUDA tensor")
     if not isinstance(idx, torch.Tensor) or not idx.is_cuda or idx.dtype != torch.int64:
         raise TypeError("idx must be an int64 CUDA tensor")
-    _dtype_code(table, "table", (capi.F32, capi.F16, capi.BF16))
+    _dtype_code(table, "table", _FLOATS)
     if table.dim() not in (2, 3):
         raise ValueError("table: expected shape (N, C) or (B, N, C)")
     if table.dim() == 3 and (idx.dim() < 1 or idx.shape[0] != table.shape[0]):
