@@ -291,7 +291,8 @@ NSFPS_API int nsfps_gather_rows_device(const nsfps_rows_desc *desc, const void *
  * width; the strides of `desc` are not used):
  *   dtable[b][n][:] = scale * sum over p with idx[b][p] == n of dout[b][p][:]
  * summed in fp32 in a fixed order of p and rounded once; rows that no index
- * names are written as zeros.  batch * count and batch * rows below 2^31. */
+ * names are written as zeros.  batch * count and batch * rows below 2^31, width
+ * below 2^20. */
 NSFPS_API int nsfps_gather_rows_grad_workspace(const nsfps_rows_desc *desc, uint64_t *bytes);
 NSFPS_API int nsfps_gather_rows_grad_device(const nsfps_rows_desc *desc, const void *d_dout,
                                             const int64_t *d_idx, void *d_dtable, void *d_work,

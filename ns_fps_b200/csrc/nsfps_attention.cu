@@ -47,8 +47,9 @@ struct AttnArgs {
   const uint32_t *vals;    // sorted pairs: query * top + leading slot
   const uint32_t *mask;    // per query slot: blocks of the span that are listed
   const unsigned long long *lead;  // per query: bit s = slot s leads a pair
+  const uint32_t *skeys;   // their sort keys: span, then the chunks read
   const uint4 *span;       // per span: first pair, end, first tile, tiles
-  const uint2 *tiles;      // (span, tile within the span)
+  const uint4 *tiles;      // (span, tile within the span, first pair, pairs of the span)
   const uint32_t *tile_count;
   // partials of key heads g0 .. g0 + gc - 1
   uint32_t g0, gc;
@@ -229,7 +230,7 @@ struct PairKeys {
 // differ from run to run; no result depends on them.
 __global__ void __launch_bounds__(256)
 plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, uint32_t tile_rows,
-           uint32_t least, uint4 *__restrict__ span, uint2 *__restrict__ tiles,
+           uint32_t least, uint4 *__restrict__ span, uint4 *__restrict__ tiles,
            uint32_t *__restrict__ tile_count) {
   const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
   if (s >= spans) return;
@@ -241,7 +242,7 @@ plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, ui
   if (lane == 0 && count) first = atomicAdd(tile_count, count);
   first = __shfl_sync(kFullMask, first, 0);
   if (lane == 0) span[s] = make_uint4(b, e, first, count);
-  for (uint32_t i = lane; i < count; i += 32u) tiles[first + i] = make_uint2(s, i);
+  for (uint32_t i = lane; i < count; i += 32u) tiles[first + i] = make_uint4(s, i, b, e - b);
 }
 
 // -------------------------------------------------------------- forward
@@ -385,6 +386,9 @@ struct RowsState {
   }
 };
 
+// Key chunks in shared memory: two being loaded behind the one in use.
+constexpr uint32_t kStages = 3;
+
 // One tile of pairs of one span and key head.
 template <class T, int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
@@ -392,14 +396,49 @@ attend_tiles(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t s_any[8];
   if (blockIdx.x >= *a.tile_count) return;
-  const uint2 tile = a.tiles[blockIdx.x];
+  const uint4 tile = a.tiles[blockIdx.x];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
   const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint4 span = a.span[tile.x];
-  const uint32_t e0 = span.x, rows = (span.y - e0) * a.R;
+  const uint32_t e0 = tile.z, rows = tile.w * a.R;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
   const uint32_t key0 = sb << kSpanLog2;
+
+
+  // the span's chunks that some row of the tile reads: the rows are sorted by
+  // them, and the keys tell before the rows themselves are known
+  constexpr uint32_t kChunkBits = 1u << (kSpanLog2 - 6u);
+  {
+    const uint32_t r = tile.y * kTileRows + tid;
+    uint32_t read = 0;
+    if (tid < kTileRows && r < rows)
+      read = a.skeys[e0 + r / a.R] & ((1u << kChunkBits) - 1u);
+    read = __reduce_or_sync(kFullMask, read);
+    if (lane == 0) s_any[warp] = read;
+  }
+  __syncthreads();
+  uint32_t todo = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) todo |= s_any[w];
+  const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+  const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+  constexpr uint32_t kTile = 64u * DP * 2u;
+  const uint32_t base = smem_u32(smem);
+  // chunk c into stage `buf`; one group per call, empty or not
+  auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
+    if (some) {
+      const uint32_t at = base + buf * 2u * kTile;
+      load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
+      load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
+    }
+    copy_commit();
+  };
+  uint32_t ahead = todo;  // chunks not yet asked for
+#pragma unroll
+  for (uint32_t i = 0; i + 1u < kStages; ++i) {
+    fetch(__ffs(ahead) - 1, i, ahead != 0);
+    ahead &= ahead - 1u;
+  }
 
   // this lane's two rows
   uint32_t pair[2], head[2], mask[2];
@@ -420,44 +459,19 @@ attend_tiles(const AttnArgs a) {
                            (int64_t)(g * a.R + head[h]) * a.qs[2]);
     }
   }
-  const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
-  if (lane == 0) s_any[warp] = warp_any;
   uint32_t qf[DP / 16][4];
   load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
-  __syncthreads();
-  uint32_t any = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) any |= s_any[w];
-  uint32_t todo = 0;  // chunks that some row of the tile reads
-#pragma unroll
-  for (uint32_t c = 0; c < (1u << (kSpanLog2 - 6u)); ++c)
-    if ((any & chunk_blocks(c, a.block_log2)) && key0 + c * 64u < len) todo |= 1u << c;
-
-  const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
-  const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-  constexpr uint32_t kTile = 64u * DP * 2u;
-  const uint32_t base = smem_u32(smem);
-  auto fetch = [&](uint32_t c, uint32_t buf) {
-    const uint32_t at = base + buf * 2u * kTile;
-    load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
-    load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
-    copy_commit();
-  };
+  const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
   RowsState<T, DP> st;
   st.clear();
   const float c2 = a.scale * kLog2e;
-  uint32_t buf = 0;
-  if (todo) fetch(__ffs(todo) - 1, 0);
-  while (todo) {
+  for (uint32_t buf = 0; todo; buf = buf + 1u == kStages ? 0u : buf + 1u) {
     const uint32_t c = __ffs(todo) - 1;
     todo &= todo - 1u;
-    if (todo) {
-      fetch(__ffs(todo) - 1, buf ^ 1u);
-      copy_wait<1>();
-    } else {
-      copy_wait<0>();
-    }
-    __syncthreads();
+    copy_wait<kStages - 2>();
+    __syncthreads();  // chunk c is here, and the stage before it is free
+    fetch(__ffs(ahead) - 1, buf ? buf - 1u : kStages - 1u, ahead != 0);
+    ahead &= ahead - 1u;
     if (warp_any & chunk_blocks(c, a.block_log2)) {
       const uint32_t at = base + buf * 2u * kTile;
       auto bit = [&](int kp) { return (c * 64u + kp * 16u) >> a.block_log2; };
@@ -466,8 +480,6 @@ attend_tiles(const AttnArgs a) {
           [&](int kp) { return (warp_any >> bit(kp)) & 1u; },
           [&](int kp, int h) { return (mask[h] >> bit(kp)) & 1u; });
     }
-    __syncthreads();
-    buf ^= 1u;
   }
   st.finish();
 #pragma unroll
@@ -486,49 +498,129 @@ attend_tiles(const AttnArgs a) {
   }
 }
 
-// Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse).
-// LANES = D / 4 lanes per row (rounded up to a power of two), four elements
-// each.  The partials of a row are those of its leading slots, or (direct)
-// of its splits.
-template <class T, bool DIRECT>
+// Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
+// its leading slots.  LANES = D / 4 lanes per row (rounded up to a power of
+// two), four elements each; the lanes hold the slots' weights, and the partial
+// rows are read four at a time.
+template <class T, int LANES>
 __global__ void __launch_bounds__(256)
-attend_join(const AttnArgs a, const int lanes_log2) {
-  const uint32_t sub = threadIdx.x & ((1u << lanes_log2) - 1u);
+attend_join(const AttnArgs a) {
+  constexpr int kHeld = 64 / LANES;  // slots per lane
+  const uint32_t sub = threadIdx.x & (LANES - 1u);
   const uint32_t hc = a.gc * a.R;
-  const uint64_t row = (uint64_t)blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  if (row >= (uint64_t)a.B * a.M * hc) return;
-  const uint32_t bm = (uint32_t)(row / hc), hh = (uint32_t)(row - (uint64_t)bm * hc);
-  const unsigned long long lead =
-      DIRECT ? (a.splits >= 64u ? ~0ull : (1ull << a.splits) - 1ull) : a.lead[bm];
-  auto at = [&](uint32_t s) {
-    return DIRECT ? row * a.splits + s : ((uint64_t)bm * a.top + s) * hc + hh;
-  };
-  float mx = -INFINITY;
-  for (unsigned long long l = lead; l; l &= l - 1)
-    mx = fmaxf(mx, a.part_lse[at(__ffsll(l) - 1)]);
+  const uint64_t row = (uint64_t)blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
+  const bool live = row < (uint64_t)a.B * a.M * hc;
+  const uint32_t bm = live ? (uint32_t)(row / hc) : 0u;
+  const uint32_t hh = live ? (uint32_t)(row - (uint64_t)bm * hc) : 0u;
+  unsigned long long lead = live ? a.lead[bm] : 0ull;
+  const uint64_t first = (uint64_t)bm * a.top * hc + hh;  // partial of slot 0
+  float w[kHeld], mx = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const uint32_t s = sub + i * LANES;
+    w[i] = (lead >> s) & 1ull ? a.part_lse[first + (uint64_t)s * hc] : -INFINITY;
+    mx = fmaxf(mx, w[i]);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
+  const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    w[i] = exp2_fast(w[i] - base);
+    total += w[i];
+  }
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) total += __shfl_xor_sync(kFullMask, total, o);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float total = 0.f;
-  if (mx != -INFINITY)
-    for (unsigned long long l = lead; l; l &= l - 1) {
-      const uint64_t p = at(__ffsll(l) - 1);
-      const float w = exp2_fast(a.part_lse[p] - mx);
-      total += w;
-      if (4u * sub < a.D && w > 0.f) {
-        const float4 x = *reinterpret_cast<const float4 *>(a.part + p * a.D + 4 * sub);
-        acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+  const bool mine = 4u * sub < a.D;
+  uint32_t most = __popcll(lead);  // the same number of steps for the warp's rows
+#pragma unroll
+  for (int o = 16; o >= LANES; o >>= 1) most = max(most, __shfl_xor_sync(kFullMask, most, o));
+  for (uint32_t i = 0; i < most; i += 4u) {
+    float4 x[4];
+    float c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool some = lead != 0ull;
+      const uint32_t s = some ? __ffsll(lead) - 1 : 0u;
+      lead &= lead - 1ull;
+      c[u] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        const float y = __shfl_sync(kFullMask, w[k], s & (LANES - 1u), LANES);
+        if (s / LANES == k) c[u] = y;
       }
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (some && mine)
+        x[u] = *reinterpret_cast<const float4 *>(a.part + (first + (uint64_t)s * hc) * a.D + 4 * sub);
+      if (!some) c[u] = 0.f;
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc.x += c[u] * x[u].x; acc.y += c[u] * x[u].y;
+      acc.z += c[u] * x[u].z; acc.w += c[u] * x[u].w;
+    }
+  }
+  if (!live) return;
   const float inv = total > 0.f ? 1.f / total : 0.f;
   const uint64_t out_row = (uint64_t)bm * a.H + a.g0 * a.R + hh;
-  if (4u * sub < a.D)
+  if (mine)
     *reinterpret_cast<uint2 *>(a.out + (out_row * a.D + 4 * sub) * 2) =
         make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
   if (a.lse && sub == 0) a.lse[out_row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
 }
 
+// The same for the direct path, one CTA per row: groups of LANES lanes take
+// the splits in turns, and their sums meet in shared memory.
+template <class T, int LANES>
+__global__ void __launch_bounds__(256)
+attend_join_direct(const AttnArgs a) {
+  constexpr uint32_t kGroups = 256 / LANES;
+  __shared__ float s_mx[8];
+  __shared__ float4 s_acc[kGroups][LANES];
+  __shared__ float s_total[kGroups];
+  const uint32_t tid = threadIdx.x, sub = tid & (LANES - 1u), grp = tid / LANES;
+  const uint64_t row = blockIdx.x, first = row * a.splits;
+  float mx = -INFINITY;
+  for (uint32_t s = tid; s < a.splits; s += 256u) mx = fmaxf(mx, a.part_lse[first + s]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
+  if ((tid & 31u) == 0) s_mx[tid >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, s_mx[w]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+#pragma unroll 4
+  for (uint32_t s = grp; s < a.splits; s += kGroups) {
+    const float w = exp2_fast(a.part_lse[first + s] - base);
+    total += w;
+    if (4u * sub < a.D) {
+      const float4 x = *reinterpret_cast<const float4 *>(a.part + (first + s) * a.D + 4 * sub);
+      acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+    }
+  }
+  s_acc[grp][sub] = acc;
+  if (sub == 0) s_total[grp] = total;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (uint32_t g = 1; g < kGroups; ++g) {
+    const float4 x = s_acc[g][sub];
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    total += s_total[g];
+  }
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  if (4u * sub < a.D)
+    *reinterpret_cast<uint2 *>(a.out + (row * a.D + 4 * sub) * 2) =
+        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  if (a.lse && sub == 0) a.lse[row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
+}
+
 // Direct path: a CTA takes kDirectKeys of one query's listed keys and one key
 // head; each warp a run of 16-key slices, joined through shared memory.
-constexpr uint32_t kDirectKeys = 128;
+constexpr uint32_t kDirectKeys = 64;
 constexpr uint32_t kDirectWarps = 4;
 
 template <class T, int DP>
@@ -683,7 +775,7 @@ constexpr uint32_t kGradItem = 512;    // query rows per CTA
 template <int DP, int SPAN>
 constexpr uint32_t grad_smem() {
   return 2u * SPAN * DP * 2u + 2u * 2u * kGradRows * DP * 2u + SPAN * kGradRows * 2u +
-         2u * kGradRows * 16u;
+         2u * kGradRows * 16u + kGradItem * 4u;
 }
 
 // Byte offset of 16-byte chunk c (8 rows) of key r in the ds tile
@@ -704,12 +796,11 @@ attend_grad(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   constexpr uint32_t kThreads = SPAN * 2, kWarps = SPAN / 16, kChunks = DP / 8;
   if (blockIdx.x >= *a.tile_count) return;
-  const uint2 tile = a.tiles[blockIdx.x];
+  const uint4 tile = a.tiles[blockIdx.x];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, t = lane & 3u;
   const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
   const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint4 span = a.span[tile.x];
-  const uint32_t e0 = span.x, all_rows = (span.y - e0) * a.R;
+  const uint32_t e0 = tile.z, all_rows = tile.w * a.R;
   const uint32_t row0 = tile.y * kGradItem;
   const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
@@ -727,6 +818,7 @@ attend_grad(const AttnArgs a) {
   const uint32_t *s_mask = reinterpret_cast<const uint32_t *>(info) + 2 * kGradRows;
   uint32_t *s_row = reinterpret_cast<uint32_t *>(info) + 3 * kGradRows;
   constexpr uint32_t kInfo = 4 * kGradRows;  // words per buffer
+  uint32_t *s_pair = reinterpret_cast<uint32_t *>(info) + 2 * kInfo;  // [kGradItem]
 
   float dk[DP / 8][4], dv[DP / 8][4];
 #pragma unroll
@@ -740,6 +832,9 @@ attend_grad(const AttnArgs a) {
     load_keys<DP, SPAN, kThreads>(sk, kh, a.ks[1], key0, len, a.D, tid);
     load_keys<DP, SPAN, kThreads>(sv, vh, a.vs[1], key0, len, a.D, tid);
   }
+  // the item's pairs: the address of a row is then one multiplication away
+  for (uint32_t r = tid; r < rows; r += kThreads) s_pair[r] = a.vals[e0 + (row0 + r) / a.R];
+  __syncthreads();
   // Rows of step i into buffer i & 1: 8 threads per row while DP = 64.
   auto fetch = [&](uint32_t i) {
     const uint32_t buf = i & 1u, at = sq + buf * 2u * kRowTile;
@@ -749,7 +844,7 @@ attend_grad(const AttnArgs a) {
       const char *qp = a.q, *op = a.dout;
       if (some) {
         const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
-        const uint32_t bm = a.vals[e0 + e] / a.top, m = bm - b * a.M, h = g * a.R + hh;
+        const uint32_t bm = s_pair[rr] / a.top, m = bm - b * a.M, h = g * a.R + hh;
         qp = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2] + c * 8);
         op = a.dout + 2 * (((uint64_t)bm * a.H + h) * a.D + c * 8);
       }
@@ -765,7 +860,7 @@ attend_grad(const AttnArgs a) {
       uint32_t prow = 0xffffffffu;
       if (some) {
         const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
-        const uint32_t p = a.vals[e0 + e];
+        const uint32_t p = s_pair[rr];
         const uint64_t row = (uint64_t)(p / a.top) * a.H + g * a.R + hh;
         lp += row;
         dp += row;
@@ -1032,7 +1127,7 @@ struct AttnPlan {
   uint32_t *mask, *tile_count;
   uint4 *span;
   unsigned long long *lead;
-  uint2 *tiles;
+  uint4 *tiles;
   float *part, *part_lse, *delta, *part_kv;
   uint64_t bytes;
 };
@@ -1081,7 +1176,7 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
   w.span = c.take<uint4>(w.spans);
   w.tile_count = c.take<uint32_t>(1);
-  w.tiles = c.take<uint2>(w.max_tiles);
+  w.tiles = c.take<uint4>(w.max_tiles);
   w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
     w.delta = c.take<float>(w.bc * d.queries * d.heads);
@@ -1148,6 +1243,7 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
       return err;
   }
   a.vals = list.vals;
+  a.skeys = list.keys;
   if (spans)
     plan_spans<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(list, spans, shift, a.R, w.tile_rows,
                                                              w.least, w.span, w.tiles,
@@ -1162,9 +1258,10 @@ int row_lanes_log2(uint32_t D) {
   return l;
 }
 
+// More than 48 KB a CTA, static shared memory included, has to be asked for.
 template <class K>
 cudaError_t opt_in(K kernel, uint32_t smem) {
-  return smem <= 48u << 10 ? cudaSuccess
+  return smem <= 40u << 10 ? cudaSuccess
                            : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   (int)smem);
 }
@@ -1172,7 +1269,6 @@ cudaError_t opt_in(K kernel, uint32_t smem) {
 template <class T, int DP>
 cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
   cudaError_t err;
-  const int lanes = row_lanes_log2(all.D);
   if (w.direct) {
     AttnArgs a = all;
     const uint32_t smem = kDirectKeys * DP * 4u + (a.R > 16 ? kDirectWarps * 16 * DP * 4u : 0u);
@@ -1181,11 +1277,11 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
     if ((err = cudaGetLastError())) return err;
     if (w.splits > 1) {
       const uint64_t rows = (uint64_t)a.B * a.M * a.H;
-      attend_join<T, true><<<(uint32_t)ceil_div(rows, 256 >> lanes), 256, 0, st>>>(a, lanes);
+      attend_join_direct<T, DP / 4><<<(uint32_t)rows, 256, 0, st>>>(a);
     }
     return cudaGetLastError();
   }
-  const uint32_t smem = 4u * 64u * DP * 2u;
+  const uint32_t smem = kStages * 2u * 64u * DP * 2u;
   if ((err = opt_in(attend_tiles<T, DP>, smem))) return err;
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
@@ -1196,7 +1292,7 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
       if (tiles) attend_tiles<T, DP><<<dim3((uint32_t)tiles, a.gc), 256, smem, st>>>(a);
       if ((err = cudaGetLastError())) return err;
       const uint64_t rows = (uint64_t)a.B * a.M * a.gc * a.R;
-      attend_join<T, false><<<(uint32_t)ceil_div(rows, 256 >> lanes), 256, 0, st>>>(a, lanes);
+      attend_join<T, DP / 4><<<(uint32_t)ceil_div(rows, 1024 / DP), 256, 0, st>>>(a);
       if ((err = cudaGetLastError())) return err;
     }
   }

@@ -92,7 +92,8 @@ gather_rows_kernel(const RowsArgs a, const int lanes_log2) {
           x[u].e[e] = from_f32<T>(to_f32(x[u].e[e]) * a.scale);
       }
       const uint64_t p = first + u * per_block;
-      *reinterpret_cast<typename VecOf<VB>::type *>(a.out + (p * a.vecs + j) * VB) = x[u].v;
+      // written once and not read here: kept out of the way of the table's rows
+      __stcs(reinterpret_cast<typename VecOf<VB>::type *>(a.out + (p * a.vecs + j) * VB), x[u].v);
     }
   }
 }
@@ -110,46 +111,20 @@ struct IndexKeys {
   __device__ __forceinline__ uint32_t value(uint32_t i) const { return i; }
 };
 
-// Where each table row's entries lie in the sorted list: its first and last
-// entry write their ends (rows without an entry keep the zeros written before).
-__global__ void __launch_bounds__(256)
-rows_runs(const SortedList list, uint32_t count, uint32_t rows, uint2 *__restrict__ run) {
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x, n = *list.kept;
-  if (i >= n) return;
-  const uint32_t key = list.keys[i], b = list.vals[i] / count;
-  const uint32_t row = b * rows + key;
-  if (i == 0 || list.keys[i - 1] != key || list.vals[i - 1] / count != b) run[row].x = i;
-  if (i + 1 == n || list.keys[i + 1] != key || list.vals[i + 1] / count != b) run[row].y = i + 1;
-}
+// The sum walks the sorted list in tiles of kWalk entries, one group of lanes
+// each: whatever the rows' lengths, a group has the same work, and its loads
+// depend on the list alone, eight in flight (one group per table row waited for
+// run -> entry -> row: 123 us for 2^20 entries of 192 bytes).  A row inside the
+// tile is written by it.  Of a row that the tile's border cuts, the tile leaves
+// a partial sum: slot 0 for a row that began before the tile, slot 1 for one
+// that begins in it and goes on.  rows_join adds those in order.
+constexpr uint32_t kWalk = 32;
+constexpr int kWalkFlight = 8;
 
-// A row with more entries than a tile is summed tile by tile (rows_hot_tiles,
-// rows_hot_join): one warp's serial walk would hold up the launch.  64 entries
-// are 16 steps of four loads.
-constexpr uint32_t kHotTile = 64;
-
-template <class T, int VB>
-__device__ __forceinline__ void add_entries(const char *__restrict__ dout,
-                                            const uint32_t *__restrict__ vals, uint32_t b,
-                                            uint32_t e, uint32_t vecs, uint32_t j,
-                                            float (&acc)[Pack<T, VB>::E]) {
-  using V = typename VecOf<VB>::type;
-  uint32_t i = b;
-  for (; i + 4u <= e; i += 4u) {
-    Pack<T, VB> x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      x[u].v = *reinterpret_cast<const V *>(dout + ((uint64_t)vals[i + u] * vecs + j) * VB);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int k = 0; k < Pack<T, VB>::E; ++k) acc[k] += to_f32(x[u].e[k]);
-  }
-  for (; i < e; ++i) {
-    Pack<T, VB> x;
-    x.v = *reinterpret_cast<const V *>(dout + ((uint64_t)vals[i] * vecs + j) * VB);
-#pragma unroll
-    for (int k = 0; k < Pack<T, VB>::E; ++k) acc[k] += to_f32(x.e[k]);
-  }
+// Table row of a sorted entry.
+__device__ __forceinline__ uint32_t entry_row(const SortedList &list, uint32_t i, uint32_t count,
+                                              uint32_t rows) {
+  return list.vals[i] / count * rows + list.keys[i];
 }
 
 template <class T, int VB>
@@ -161,156 +136,183 @@ __device__ __forceinline__ void store_row(char *out, uint64_t r, uint32_t vecs, 
   *reinterpret_cast<typename VecOf<VB>::type *>(out + (r * vecs + j) * VB) = y.v;
 }
 
-// Rows that a group of lanes sums side by side, two entries of each at a time:
-// eight loads in flight behind the run -> entry -> row chain.
-constexpr int kSumFlight = 4;
-
-// LANES lanes per table row.
-template <class T, int VB>
-__global__ void __launch_bounds__(256)
-rows_sum(const char *__restrict__ dout, const uint32_t *__restrict__ vals,
-         const uint2 *__restrict__ run, uint32_t rows, uint32_t vecs, float scale,
-         char *__restrict__ out, const int lanes_log2) {
-  constexpr int E = Pack<T, VB>::E;
-  using V = typename VecOf<VB>::type;
-  const uint32_t lanes = 1u << lanes_log2, per_block = 256u >> lanes_log2;
-  const uint32_t first = blockIdx.x * (per_block * kSumFlight) + (threadIdx.x >> lanes_log2);
-  uint32_t b[kSumFlight], n[kSumFlight], most = 0;
-#pragma unroll
-  for (int u = 0; u < kSumFlight; ++u) {
-    const uint32_t r = first + u * per_block;
-    const uint2 x = r < rows ? run[r] : make_uint2(0u, 0u);
-    b[u] = x.x;
-    n[u] = x.y - x.x > kHotTile ? 0u : x.y - x.x;  // a hot row is written elsewhere
-    most = max(most, n[u]);
-  }
-  for (uint32_t j = threadIdx.x & (lanes - 1u); j < vecs; j += lanes) {
-    float acc[kSumFlight][E] = {};
-    for (uint32_t i = 0; i < most; i += 2u) {
-      uint32_t v[kSumFlight][2];
-      Pack<T, VB> x[kSumFlight][2];
-#pragma unroll
-      for (int u = 0; u < kSumFlight; ++u)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) v[u][k] = i + k < n[u] ? vals[b[u] + i + k] : 0u;
-#pragma unroll
-      for (int u = 0; u < kSumFlight; ++u)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (i + k < n[u])
-            x[u][k].v = *reinterpret_cast<const V *>(dout + ((uint64_t)v[u][k] * vecs + j) * VB);
-#pragma unroll
-      for (int u = 0; u < kSumFlight; ++u)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (i + k < n[u])
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[u][e] += to_f32(x[u][k].e[e]);
-    }
-#pragma unroll
-    for (int u = 0; u < kSumFlight; ++u) {
-      const uint32_t r = first + u * per_block;
-      if (r < rows && (n[u] || run[r].x == run[r].y))
-        store_row<T, VB>(out, r, vecs, j, scale, acc[u]);
-    }
-  }
-}
-
-// Tiles of the sorted list, one warp each.  A tile meets at most two hot rows,
-// that of its first entry and that of its last (any row between them is
-// shorter than the tile); slot 0 / 1 of part[] takes their sums over the tile.
-struct TileRow {
-  uint32_t row, lo, hi;  // table row (all ones: none), its entries
+struct WalkArgs {
+  const char *dout;
+  char *out;
+  SortedList list;
+  uint8_t *seen;    // per table row: some entry names it
+  float *part;      // [2 * tile + slot][width]
+  uint32_t count, rows, vecs;
+  float scale;
+  int lanes_log2;   // 4 or 5: 16 or 32 lanes per tile, one vector each
 };
 
-__device__ __forceinline__ TileRow row_of_entry(const SortedList &list, const uint2 *run,
-                                                uint32_t i, uint32_t count, uint32_t rows) {
-  TileRow t;
-  t.row = list.vals[i] / count * rows + list.keys[i];
-  const uint2 x = run[t.row];
-  t.lo = x.x;
-  t.hi = x.y;
-  if (t.hi - t.lo <= kHotTile) t.row = 0xffffffffu;
-  return t;
-}
-
+// grid.y: runs of 1 << lanes_log2 vectors of the rows.
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
-rows_hot_tiles(const char *__restrict__ dout, const SortedList list,
-               const uint2 *__restrict__ run, uint32_t count, uint32_t rows, uint32_t vecs,
-               float *__restrict__ part) {
+rows_walk(const WalkArgs a) {
   constexpr int E = Pack<T, VB>::E;
-  const uint32_t t = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
-  const uint32_t n = *list.kept, b = t * kHotTile, e = min(n, b + kHotTile);
-  if (b >= n) return;
-  const TileRow first = row_of_entry(list, run, b, count, rows);
-  const TileRow last = row_of_entry(list, run, e - 1u, count, rows);
-  for (int s = 0; s < 2; ++s) {
-    const TileRow r = s ? last : first;
-    if (r.row == 0xffffffffu || (s && last.row == first.row)) continue;
-    for (uint32_t j = lane; j < vecs; j += 32u) {
-      float acc[E] = {};
-      add_entries<T, VB>(dout, list.vals, max(b, r.lo), min(e, r.hi), vecs, j, acc);
-      float *o = part + ((uint64_t)(2u * t + s) * vecs + j) * E;
+  using V = typename VecOf<VB>::type;
+  const uint32_t lanes = 1u << a.lanes_log2, sub = threadIdx.x & (lanes - 1u);
+  const uint32_t tile = blockIdx.x * (256u >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const uint32_t n = *a.list.kept, b = tile * kWalk;
+  const uint32_t warp_tile = blockIdx.x * (256u >> a.lanes_log2) +
+                             ((threadIdx.x & ~31u) >> a.lanes_log2);
+  if (warp_tile * kWalk >= n) return;  // the whole warp
+  const uint32_t m = b < n ? min(kWalk, n - b) : 0u;
+  const uint32_t j = blockIdx.y * lanes + sub;
+  const bool mine = j < a.vecs;
+  // the tile's entries over its lanes: two per lane of 16, one per lane of 32
+  uint32_t val[2], row[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t e = sub + i * lanes;
+    val[i] = row[i] = 0xffffffffu;
+    if (e < m) {
+      val[i] = a.list.vals[b + e];
+      row[i] = val[i] / a.count * a.rows + a.list.keys[b + e];
+    }
+  }
+  const uint32_t before = m && b ? entry_row(a.list, b - 1u, a.count, a.rows) : 0xffffffffu;
+  const uint32_t after = b + m < n && m ? entry_row(a.list, b + m, a.count, a.rows) : 0xffffffffu;
+  uint32_t cur = __shfl_sync(0xffffffffu, row[0], 0, (int)lanes);
+  bool begun = m && cur == before;  // the current row began in an earlier tile
+  float acc[E] = {};
+  auto flush = [&](bool goes_on) {
+    if (!mine) return;
+    if (begun || goes_on) {
+      float *o = a.part + ((uint64_t)(2u * tile + (begun ? 0u : 1u)) * a.vecs + j) * E;
 #pragma unroll
       for (int k = 0; k < E; ++k) o[k] = acc[k];
+    } else {
+      store_row<T, VB>(a.out, cur, a.vecs, j, a.scale, acc);
+    }
+    if (j == 0 && !begun) a.seen[cur] = 1;
+  };
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWalk; i += kWalkFlight) {
+    uint32_t r[kWalkFlight];
+    Pack<T, VB> x[kWalkFlight];
+#pragma unroll
+    for (int u = 0; u < kWalkFlight; ++u) {
+      const uint32_t e = i + u;
+      const uint32_t v0 = __shfl_sync(0xffffffffu, val[0], e & (lanes - 1u), (int)lanes);
+      const uint32_t v1 = __shfl_sync(0xffffffffu, val[1], e & (lanes - 1u), (int)lanes);
+      const uint32_t r0 = __shfl_sync(0xffffffffu, row[0], e & (lanes - 1u), (int)lanes);
+      const uint32_t r1 = __shfl_sync(0xffffffffu, row[1], e & (lanes - 1u), (int)lanes);
+      const uint32_t v = e < lanes ? v0 : v1;
+      r[u] = e < lanes ? r0 : r1;
+      if (e < m && mine)
+        x[u].v = __ldcs(reinterpret_cast<const V *>(a.dout + ((uint64_t)v * a.vecs + j) * VB));
+    }
+#pragma unroll
+    for (int u = 0; u < kWalkFlight; ++u) {
+      if (i + u >= m) continue;
+      if (r[u] != cur) {
+        flush(false);
+        cur = r[u];
+        begun = false;
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] = 0.f;
+      }
+      if (mine)
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] += to_f32(x[u].e[k]);
     }
   }
+  if (m) flush(cur == after);
 }
 
-// The hot row that starts in a tile (at most one: it reaches the tile's end)
-// adds its tile sums in order: eight warps a share each, then the shares.
+// One warp per tile: the row that begins in it and goes on.  A long chain of
+// tiles (a row that thousands of entries name) is shared by the CTA's warps.
+constexpr uint32_t kLongChain = 32;
+
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
-rows_hot_join(const SortedList list, const uint2 *__restrict__ run, uint32_t count,
-              uint32_t rows, uint32_t vecs, float scale, const float *__restrict__ part,
-              char *__restrict__ out) {
+rows_join(const WalkArgs a) {
   constexpr int E = Pack<T, VB>::E;
   __shared__ float s_acc[8][32][E];
-  __shared__ TileRow s_row[8];
-  __shared__ uint32_t s_slot[8];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = *list.kept;
-  if (blockIdx.x * 8u * kHotTile >= n) return;
-  {
-    const uint32_t t = blockIdx.x * 8u + warp, b = t * kHotTile, e = min(n, b + kHotTile);
-    TileRow r{0xffffffffu, 0u, 0u};
-    uint32_t slot = 0;
-    if (b < n) {
-      r = row_of_entry(list, run, e - 1u, count, rows);
-      if (r.row != 0xffffffffu && r.lo < b) r.row = 0xffffffffu;
-      slot = 2u * t + (r.lo == b ? 0u : 1u);
-    }
-    if (lane == 0) s_row[warp] = r, s_slot[warp] = slot;
-  }
-  __syncthreads();
-  for (uint32_t i = 0; i < 8u; ++i) {
-    const TileRow r = s_row[i];
-    if (r.row == 0xffffffffu) continue;
-    const uint32_t t = blockIdx.x * 8u + i, last = (r.hi - 1u) / kHotTile;  // tiles t .. last
-    const uint32_t per = (last - t + 8u) / 8u;
-    const uint32_t wb = min(last + 1u, t + warp * per), we = min(last + 1u, wb + per);
-    for (uint32_t j0 = 0; j0 < vecs; j0 += 32u) {
-      float acc[E] = {};
-      if (j0 + lane < vecs)
-#pragma unroll 4
-        for (uint32_t x = wb; x < we; ++x) {
-          const uint32_t slot = x == t ? s_slot[i] : 2u * x;
-          const float *o = part + ((uint64_t)slot * vecs + j0 + lane) * E;
-#pragma unroll
-          for (int k = 0; k < E; ++k) acc[k] += o[k];
+  __shared__ uint32_t s_row[8], s_len[8];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t n = *a.list.kept, t = blockIdx.x * 8u + warp, e = (t + 1u) * kWalk;
+  if (blockIdx.x * 8u * kWalk >= n) return;
+  uint32_t row = 0xffffffffu, len = 0;  // tiles behind t that the row reaches
+  if (e < n) {
+    const uint32_t r = entry_row(a.list, e - 1u, a.count, a.rows);
+    const uint32_t head = t ? entry_row(a.list, t * kWalk - 1u, a.count, a.rows) : 0xffffffffu;
+    if (r == entry_row(a.list, e, a.count, a.rows) && r != head) {
+      row = r;
+      // tile t + 1 + i holds a part while its first entry is the row's
+      for (;; len += 32u) {
+        const uint64_t first = ((uint64_t)t + 1u + len + lane) * kWalk;
+        const bool in = first < n && entry_row(a.list, (uint32_t)first, a.count, a.rows) == r;
+        const uint32_t out = ~__ballot_sync(0xffffffffu, in);
+        if (out) {
+          len += __ffs(out) - 1;
+          break;
         }
+      }
+    }
+  }
+  if (row != 0xffffffffu && len <= kLongChain) {
+    for (uint32_t j = lane; j < a.vecs; j += 32u) {
+      float acc[E];
+      const float *o = a.part + ((uint64_t)(2u * t + 1u) * a.vecs + j) * E;
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc[k] = o[k];
+#pragma unroll 4
+      for (uint32_t i = 1; i <= len; ++i)
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] += (o + (uint64_t)(2u * i - 1u) * a.vecs * E)[k];
+      store_row<T, VB>(a.out, row, a.vecs, j, a.scale, acc);
+    }
+    row = 0xffffffffu;
+  }
+  if (lane == 0) s_row[warp] = row, s_len[warp] = len;
+  __syncthreads();
+  for (uint32_t c = 0; c < 8u; ++c) {
+    if (s_row[c] == 0xffffffffu) continue;
+    const uint32_t tc = blockIdx.x * 8u + c, per = (s_len[c] + 7u) / 8u;
+    const uint32_t i0 = 1u + warp * per, i1 = min(s_len[c] + 1u, i0 + per);
+    for (uint32_t j0 = 0; j0 < a.vecs; j0 += 32u) {
+      const uint32_t j = j0 + lane;
+      float acc[E] = {};
+      if (j < a.vecs) {
+        const float *o = a.part + ((uint64_t)(2u * tc + 1u) * a.vecs + j) * E;
+        if (warp == 0)
+#pragma unroll
+          for (int k = 0; k < E; ++k) acc[k] = o[k];
+#pragma unroll 8
+        for (uint32_t i = i0; i < i1; ++i)
+#pragma unroll
+          for (int k = 0; k < E; ++k) acc[k] += (o + (uint64_t)(2u * i - 1u) * a.vecs * E)[k];
+      }
 #pragma unroll
       for (int k = 0; k < E; ++k) s_acc[warp][lane][k] = acc[k];
       __syncthreads();
-      if (warp == 0 && j0 + lane < vecs) {
+      if (warp == 0 && j < a.vecs) {
         for (int w = 1; w < 8; ++w)
 #pragma unroll
           for (int k = 0; k < E; ++k) acc[k] += s_acc[w][lane][k];
-        store_row<T, VB>(out, r.row, vecs, j0 + lane, scale, acc);
+        store_row<T, VB>(a.out, s_row[c], a.vecs, j, a.scale, acc);
       }
       __syncthreads();
     }
   }
+}
+
+// Zeros for the rows that no entry names.
+template <class T, int VB>
+__global__ void __launch_bounds__(256)
+rows_unseen(const uint8_t *__restrict__ seen, uint32_t rows, uint32_t vecs,
+            char *__restrict__ out, const int lanes_log2) {
+  using V = typename VecOf<VB>::type;
+  const uint32_t lanes = 1u << lanes_log2;
+  const uint32_t r = blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (r >= rows || seen[r]) return;
+  const V zero = {};
+  for (uint32_t j = threadIdx.x & (lanes - 1u); j < vecs; j += lanes)
+    *reinterpret_cast<V *>(out + ((uint64_t)r * vecs + j) * VB) = zero;
 }
 
 // Widest vector (up to 16 bytes) that divides every one of the given byte
@@ -332,17 +334,17 @@ int check_rows(const nsfps_rows_desc *d) {
   if (d->dtype != NSFPS_F32 && d->dtype != NSFPS_F16 && d->dtype != NSFPS_BF16)
     return set_error(NSFPS_ERR_ARG, "dtype must be float32, float16 or bfloat16");
   const uint64_t lim = 1ull << 31;
-  if (d->batch >= lim || d->rows >= lim || d->count >= lim || d->width >= (1ull << 24) ||
+  if (d->batch >= lim || d->rows >= lim || d->count >= lim || d->width >= (1ull << 20) ||
       d->batch * d->rows >= lim || d->batch * d->count >= lim)
     return set_error(NSFPS_ERR_UNSUPPORTED,
-                     "batch * rows and batch * count must be below 2^31, width below 2^24");
+                     "batch * rows and batch * count must be below 2^31, width below 2^20");
   if (!std::isfinite(d->scale)) return set_error(NSFPS_ERR_ARG, "scale must be finite");
   return NSFPS_OK;
 }
 
 struct RowsGradWork {
   SortScratch sort;
-  uint2 *run;
+  uint8_t *seen;
   float *part;
   uint64_t bytes;
 };
@@ -352,8 +354,8 @@ RowsGradWork carve_rows_grad(const nsfps_rows_desc &d, void *base) {
   WorkCarver c(base);
   const uint32_t n = (uint32_t)(d.batch * d.count);
   w.sort.carve(c, n);
-  w.run = c.take<uint2>(d.batch * d.rows);
-  w.part = c.take<float>(2 * ceil_div(n, kHotTile) * d.width);
+  w.seen = c.take<uint8_t>(d.batch * d.rows);
+  w.part = c.take<float>(2 * ceil_div(n, kWalk) * d.width);
   w.bytes = c.off;
   return w;
 }
@@ -392,25 +394,19 @@ struct LaunchGather {
   }
 };
 
-struct LaunchRowsSum {
-  const char *dout;
-  char *out;
-  SortedList list;
-  const uint2 *run;
-  float *part;
-  uint32_t n, count, all_rows, rows, vecs;
-  float scale;
-  int lanes_log2;
+struct LaunchWalk {
+  WalkArgs a;
+  uint32_t n, all_rows;
   cudaStream_t st;
   template <class T, int VB>
   cudaError_t operator()() const {
-    rows_sum<T, VB><<<(uint32_t)ceil_div(all_rows, (256u >> lanes_log2) * kSumFlight), 256, 0,
-                      st>>>(dout, list.vals, run, all_rows, vecs, scale, out, lanes_log2);
-    if (n > kHotTile) {  // fewer entries make no hot row
-      const uint32_t grid = (uint32_t)ceil_div(n, 8u * kHotTile);
-      rows_hot_tiles<T, VB><<<grid, 256, 0, st>>>(dout, list, run, count, rows, vecs, part);
-      rows_hot_join<T, VB><<<grid, 256, 0, st>>>(list, run, count, rows, vecs, scale, part, out);
-    }
+    const uint32_t tiles = (uint32_t)ceil_div(n, kWalk);
+    rows_walk<T, VB><<<dim3((uint32_t)ceil_div(tiles, 256u >> a.lanes_log2),
+                            (uint32_t)ceil_div(a.vecs, 1u << a.lanes_log2)), 256, 0, st>>>(a);
+    if (n > kWalk) rows_join<T, VB><<<(uint32_t)ceil_div(tiles, 8), 256, 0, st>>>(a);
+    const int l = lanes_log2_for(a.vecs);
+    rows_unseen<T, VB><<<(uint32_t)ceil_div(all_rows, 256u >> l), 256, 0, st>>>(
+        a.seen, all_rows, a.vecs, a.out, l);
     return cudaGetLastError();
   }
 };
@@ -491,17 +487,20 @@ int nsfps_gather_rows_grad_device(const nsfps_rows_desc *desc, const void *d_dou
   SortedList list;
   NSFPS_FEATURE_CUDA(run_sort(IndexKeys{d_idx, (uint32_t)d.rows}, n, (uint32_t)d.rows, w.sort,
                               &list, st));
-  NSFPS_FEATURE_CUDA(cudaMemsetAsync(w.run, 0, (uint64_t)rows * sizeof(uint2), st));
-  rows_runs<<<(uint32_t)ceil_div(n, 256), 256, 0, st>>>(list, (uint32_t)d.count, (uint32_t)d.rows,
-                                                        w.run);
-  NSFPS_FEATURE_CUDA(cudaGetLastError());
+  NSFPS_FEATURE_CUDA(cudaMemsetAsync(w.seen, 0, rows, st));
   const int vb = vec_bytes((uint64_t)d_dout | (uint64_t)d_dtable | d.width * elem, elem);
-  const uint32_t vecs = (uint32_t)(d.width * elem / vb);
-  NSFPS_FEATURE_CUDA(with_vec(
-      d.dtype, vb,
-      LaunchRowsSum{(const char *)d_dout, (char *)d_dtable, list, w.run, w.part, n,
-                    (uint32_t)d.count, rows, (uint32_t)d.rows, vecs, d.scale,
-                    lanes_log2_for(vecs), st}));
+  WalkArgs a{};
+  a.dout = (const char *)d_dout;
+  a.out = (char *)d_dtable;
+  a.list = list;
+  a.seen = w.seen;
+  a.part = w.part;
+  a.count = (uint32_t)d.count;
+  a.rows = (uint32_t)d.rows;
+  a.vecs = (uint32_t)(d.width * elem / vb);
+  a.scale = d.scale;
+  a.lanes_log2 = a.vecs <= 16 ? 4 : 5;
+  NSFPS_FEATURE_CUDA(with_vec(d.dtype, vb, LaunchWalk{a, n, rows, st}));
   return NSFPS_OK;
 }
 

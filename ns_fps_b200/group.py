@@ -131,18 +131,18 @@ class _on:
     switch is skipped where it is current already: it costs a small call more
     than its kernels.)"""
 
-    __slots__ = ("device", "guard")
+    __slots__ = ("index", "guard")
 
     def __init__(self, t):
-        self.device = t.device
+        self.index = t.get_device()
 
     def __enter__(self):
         import torch
         self.guard = None
-        if torch.cuda.current_device() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
+        if torch._C._cuda_getDevice() != self.index:
+            self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
