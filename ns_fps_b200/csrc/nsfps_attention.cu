@@ -159,14 +159,22 @@ __device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
 
 // ------------------------------------------------------------- the plan
 
+// Blocks (as bits of a pair's mask) of the 64-key chunk c of a span.
+__device__ __forceinline__ uint32_t chunk_blocks(uint32_t c, uint32_t block_log2) {
+  const uint32_t n = block_log2 >= 6u ? 1u : 64u >> block_log2;
+  return ((1u << n) - 1u) << ((c << 6) >> block_log2);
+}
+
 // One warp per query: which slots lead a pair, and the blocks of each pair.
 // A pair's leading slot is the first slot that lists a block of its span; a
-// repeated block sets the same bit again.  The sort key is the span and the
-// 64-key chunks of it that are read, so that the rows of a tile read alike.
+// repeated block sets the same bit again.  The sort key is the span and, as
+// its place in a Gray code, the set of 64-key chunks that are read: neighbours
+// in that order differ in few chunks, so the rows of a tile read alike.
+template <int SLOTS>  // 32-slot parts of a list
 __global__ void __launch_bounds__(256)
 plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
-           uint32_t *__restrict__ mask,
-           unsigned long long *__restrict__ lead, uint32_t *__restrict__ tile_count) {
+           uint32_t *__restrict__ mask, unsigned long long *__restrict__ lead,
+           uint32_t *__restrict__ tile_count) {
   const uint32_t lane = threadIdx.x & 31u;
   if (blockIdx.x == 0 && threadIdx.x == 0) *tile_count = 0;  // for plan_spans
   const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
@@ -176,44 +184,51 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
   const uint32_t live = (uint32_t)(((uint64_t)len + (1u << a.block_log2) - 1u) >> a.block_log2);
   const uint32_t in_log2 = span_log2 - a.block_log2;  // blocks per span, log2
   const uint32_t none = 0xffffffffu;
-  uint32_t sb[2], bit[2], m[2] = {0u, 0u};
-  bool first[2];
+  uint32_t sb[SLOTS], bit[SLOTS], m[SLOTS], lead_of[SLOTS];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < SLOTS; ++i) {
     const uint32_t s = lane + 32u * i;
     const int64_t j = s < a.top ? a.blocks[(uint64_t)bm * a.top + s] : -1;
     const bool use = j >= 0 && j < (int64_t)live;
     sb[i] = use ? (uint32_t)j >> in_log2 : none;
     bit[i] = use ? 1u << ((uint32_t)j & ((1u << in_log2) - 1u)) : 0u;
-    first[i] = use;
+    m[i] = 0u;
+    lead_of[i] = none;
   }
-  for (uint32_t s = 0; s < a.top; ++s) {
-    const uint32_t osb = __shfl_sync(kFullMask, s < 32u ? sb[0] : sb[1], s & 31u);
-    const uint32_t obit = __shfl_sync(kFullMask, s < 32u ? bit[0] : bit[1], s & 31u);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (osb == sb[i]) {
-        m[i] |= obit;
-        if (s < lane + 32u * i) first[i] = false;
-      }
+  for (int part = SLOTS - 1; part >= 0; --part) {
+    const uint32_t n = min(32u, a.top > 32u * part ? a.top - 32u * part : 0u);
+#pragma unroll 4
+    for (uint32_t s = n; s-- > 0u;) {  // downwards: the last match is the first slot
+      const uint32_t osb = __shfl_sync(kFullMask, sb[part], s);
+      const uint32_t obit = __shfl_sync(kFullMask, bit[part], s);
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+        if (osb == sb[i]) {
+          m[i] |= obit;
+          lead_of[i] = s + 32u * part;
+        }
+    }
   }
-  const uint32_t l0 = __ballot_sync(kFullMask, first[0]), l1 = __ballot_sync(kFullMask, first[1]);
-  if (lane == 0) lead[bm] = l0 | ((unsigned long long)l1 << 32);
+  unsigned long long leaders = 0;
   const uint32_t chunks = 1u << (span_log2 - 6u);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < SLOTS; ++i) {
     const uint32_t s = lane + 32u * i;
+    const bool first = sb[i] != none && lead_of[i] == s;
+    leaders |= (unsigned long long)__ballot_sync(kFullMask, first) << (32 * i);
     if (s >= a.top) continue;
-    const uint64_t p = (uint64_t)bm * a.top + s;
     uint32_t read = 0;
-    for (uint32_t c = 0; c < chunks; ++c) {
-      const uint32_t lo = (c << 6) >> a.block_log2;
-      const uint32_t n = a.block_log2 >= 6u ? 1u : 64u >> a.block_log2;
-      read |= ((m[i] >> lo) & ((1u << n) - 1u)) ? 1u << c : 0u;
-    }
-    keys[p] = first[i] ? ((b * a.nsb + sb[i]) << chunks) | read : (a.B * a.nsb) << chunks;
+    for (uint32_t c = 0; c < chunks; ++c)
+      read |= (m[i] & chunk_blocks(c, a.block_log2)) ? 1u << c : 0u;
+    uint32_t rank = read;  // the inverse of r ^ (r >> 1), over up to 4 bits
+    rank ^= rank >> 1;
+    rank ^= rank >> 2;
+    const uint64_t p = (uint64_t)bm * a.top + s;
+    keys[p] = first ? ((b * a.nsb + sb[i]) << chunks) | rank : (a.B * a.nsb) << chunks;
     mask[p] = m[i];
   }
+  if (lane == 0) lead[bm] = leaders;
 }
 
 // Keys of the sort: one per query slot, in slot order.
@@ -250,12 +265,6 @@ plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, ui
 constexpr uint32_t kSpanLog2 = 8;      // keys per span of the forward pass
 constexpr uint32_t kTileRows = 128;    // query rows per CTA: 8 warps of 16
 
-// Blocks (as bits of a pair's mask) of the 64-key chunk c of a span.
-__device__ __forceinline__ uint32_t chunk_blocks(uint32_t c, uint32_t block_log2) {
-  const uint32_t n = block_log2 >= 6u ? 1u : 64u >> block_log2;
-  return ((1u << n) - 1u) << ((c << 6) >> block_log2);
-}
-
 // Copies keys [key0, key0 + ROWS) of one head into a shared tile; zeros behind
 // the cloud's end and behind the head's elements.
 template <int DP, int ROWS, int THREADS>
@@ -287,11 +296,31 @@ __device__ __forceinline__ void load_rows(uint32_t (&f)[DP / 16][4], const char 
     }
 }
 
+// What turns a raw score into base-2 exponents: exp2(s * c2).  The factor is
+// kept positive, so that the maximum of the raw scores is that of the scaled
+// ones: a negative scale flips the signs of q, a scale of zero makes q zero.
+struct ScoreScale {
+  float c2;
+  uint32_t flip, keep;  // on two packed elements of q
+  __device__ __forceinline__ explicit ScoreScale(float scale) {
+    c2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
+    flip = scale < 0.f ? 0x80008000u : 0u;
+    keep = scale == 0.f ? 0u : 0xffffffffu;
+  }
+  template <int N>
+  __device__ __forceinline__ void apply(uint32_t (&f)[N][4]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[i][j] = (f[i][j] & keep) ^ flip;
+  }
+};
+
 // Running softmax state and output of 16 rows (two per lane).
 template <class T, int DP>
 struct RowsState {
   float o[DP / 8][4];
-  float mx[2], sum[2];  // base-2 maximum; this lane's share of the sum
+  float mx[2], sum[2];  // maximum of the raw scores; this lane's share of the sum
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int j = 0; j < DP / 8; ++j)
@@ -301,27 +330,25 @@ struct RowsState {
     sum[0] = sum[1] = 0.f;
   }
 
-  // 16 * KP keys at rows key_row.. of the tiles sk, sv.  sel(kp) tells whether
-  // any row reads keys 16 kp .. 16 kp + 15; rows(kp, h) whether row h of this
-  // lane does; key_at(kp) is their first key (for the cloud's end).  The
-  // weights are rounded to T for the product with v: half a step of T each,
-  // as the output's own rounding.
-  template <int KP, class Sel, class Row>
+  // 16 * KP keys at rows key_row.. of the tiles sk, sv; key0 is the first.
+  // For its 16 keys kp: sel(kp) tells whether any row of the warp reads them,
+  // all(kp) whether every one does, row(kp, h) whether row h of this lane
+  // does.  Instructions per score, not the matrix products, are what this
+  // costs, so the masks are looked at only where a warp's rows differ or the
+  // cloud ends.  The weights are rounded to T for the product with v: half a
+  // step of T each, as the output's own rounding.
+  template <int KP, class Sel, class All, class Row>
   __device__ __forceinline__ void add(const uint32_t (&qf)[DP / 16][4], uint32_t sk, uint32_t sv,
                                       uint32_t key_row, uint32_t key0, uint32_t len, float c2,
-                                      uint32_t lane, Sel sel, Row row) {
+                                      uint32_t lane, Sel sel, All all, Row row) {
     const uint32_t t = lane & 3u;
     float s[2 * KP][4];
     float nm[2] = {mx[0], mx[1]};
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
+      if (!sel(kp)) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[2 * kp][i] = s[2 * kp + 1][i] = 0.f;
-      if (!sel(kp)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[2 * kp][i] = s[2 * kp + 1][i] = -INFINITY;
-        continue;
-      }
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         uint32_t b[4];
@@ -330,28 +357,38 @@ struct RowsState {
         mma16816<T>(s[2 * kp], qf[kk], b[0], b[1]);
         mma16816<T>(s[2 * kp + 1], qf[kk], b[2], b[3]);
       }
-      const bool r0 = row(kp, 0), r1 = row(kp, 1);
+      if (!all(kp) || key0 + kp * 16 + 16u > len) {
+        const bool r0 = row(kp, 0), r1 = row(kp, 1);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = (i < 2 ? r0 : r1) && key0 + kp * 16 + n * 8 + 2 * t + (i & 1) < len;
+            s[2 * kp + n][i] = in ? s[2 * kp + n][i] : -INFINITY;
+          }
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = (i < 2 ? r0 : r1) && key0 + kp * 16 + n * 8 + 2 * t + (i & 1) < len;
-          float &x = s[2 * kp + n][i];
-          x = in ? x * c2 : -INFINITY;
-          nm[i >> 1] = fmaxf(nm[i >> 1], x);
-        }
+        for (int h = 0; h < 2; ++h)
+          nm[h] = fmaxf(nm[h], fmaxf(s[2 * kp + n][2 * h], s[2 * kp + n][2 * h + 1]));
     }
     float base[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       nm[h] = fmaxf(nm[h], __shfl_xor_sync(kFullMask, nm[h], 1));
       nm[h] = fmaxf(nm[h], __shfl_xor_sync(kFullMask, nm[h], 2));
-      base[h] = nm[h] == -INFINITY ? 0.f : nm[h];  // no key yet: exp2(-inf) = 0
-      const float c = exp2_fast(mx[h] - base[h]);
-      mx[h] = nm[h];
-      sum[h] *= c;
+      base[h] = nm[h] == -INFINITY ? 0.f : nm[h] * c2;  // no key yet: exp2(-inf) = 0
+    }
+    if (__any_sync(kFullMask, nm[0] > mx[0] || nm[1] > mx[1])) {
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= c, o[j][2 * h + 1] *= c;
+      for (int h = 0; h < 2; ++h) {
+        const float c = exp2_fast(fmaf(mx[h], c2, -base[h]));
+        mx[h] = nm[h];
+        sum[h] *= c;
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= c, o[j][2 * h + 1] *= c;
+      }
     }
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
@@ -361,7 +398,7 @@ struct RowsState {
       for (int n = 0; n < 2; ++n) {
         float *x = s[2 * kp + n];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = exp2_fast(x[i] - base[i >> 1]);
+        for (int i = 0; i < 4; ++i) x[i] = exp2_fast(fmaf(x[i], c2, -base[i >> 1]));
         sum[0] += x[0] + x[1];
         sum[1] += x[2] + x[3];
         a[2 * n] = pack2<T>(x[0], x[1]);
@@ -377,11 +414,13 @@ struct RowsState {
     }
   }
 
-  __device__ __forceinline__ void finish() {
+  // Sums over the lanes of a row, and the maximum in base 2.
+  __device__ __forceinline__ void finish(float c2) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       sum[h] += __shfl_xor_sync(kFullMask, sum[h], 1);
       sum[h] += __shfl_xor_sync(kFullMask, sum[h], 2);
+      mx[h] *= c2;
     }
   }
 };
@@ -389,185 +428,179 @@ struct RowsState {
 // Key chunks in shared memory: two being loaded behind the one in use.
 constexpr uint32_t kStages = 3;
 
-// One tile of pairs of one span and key head.
+// Tiles of pairs of one span and key head, CTAs taking them in turns.
 template <class T, int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
 attend_tiles(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t s_any[8];
-  if (blockIdx.x >= *a.tile_count) return;
-  const uint4 tile = a.tiles[blockIdx.x];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
-  const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint32_t e0 = tile.z, rows = tile.w * a.R;
-  const uint32_t len = cloud_length(a.lengths, b, a.N);
-  const uint32_t key0 = sb << kSpanLog2;
-
-
-  // the span's chunks that some row of the tile reads: the rows are sorted by
-  // them, and the keys tell before the rows themselves are known
-  constexpr uint32_t kChunkBits = 1u << (kSpanLog2 - 6u);
-  {
-    const uint32_t r = tile.y * kTileRows + tid;
-    uint32_t read = 0;
-    if (tid < kTileRows && r < rows)
-      read = a.skeys[e0 + r / a.R] & ((1u << kChunkBits) - 1u);
-    read = __reduce_or_sync(kFullMask, read);
-    if (lane == 0) s_any[warp] = read;
-  }
-  __syncthreads();
-  uint32_t todo = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) todo |= s_any[w];
-  const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
-  const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-  constexpr uint32_t kTile = 64u * DP * 2u;
   const uint32_t base = smem_u32(smem);
-  // chunk c into stage `buf`; one group per call, empty or not
-  auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
-    if (some) {
-      const uint32_t at = base + buf * 2u * kTile;
-      load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
-      load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
-    }
-    copy_commit();
-  };
-  uint32_t ahead = todo;  // chunks not yet asked for
-#pragma unroll
-  for (uint32_t i = 0; i + 1u < kStages; ++i) {
-    fetch(__ffs(ahead) - 1, i, ahead != 0);
-    ahead &= ahead - 1u;
-  }
+  constexpr uint32_t kTile = 64u * DP * 2u;
+  constexpr uint32_t kChunkBits = 1u << (kSpanLog2 - 6u);
+  const ScoreScale sc(a.scale);
+  const uint32_t work = *a.tile_count * a.gc;
+  for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const uint32_t gi = w % a.gc, g = a.g0 + gi;
+    const uint4 tile = a.tiles[w / a.gc];
+    const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
+    const uint32_t e0 = tile.z, rows = tile.w * a.R;
+    const uint32_t len = cloud_length(a.lengths, b, a.N);
+    const uint32_t key0 = sb << kSpanLog2;
 
-  // this lane's two rows
-  uint32_t pair[2], head[2], mask[2];
-  const char *qrow[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t r = tile.y * kTileRows + warp * 16u + (lane >> 2) + 8u * h;
-    pair[h] = 0xffffffffu;
-    head[h] = mask[h] = 0u;
-    qrow[h] = nullptr;
-    if (r < rows) {
-      const uint32_t e = r / a.R;
-      head[h] = r - e * a.R;
-      pair[h] = a.vals[e0 + e];
-      mask[h] = a.mask[pair[h]];
-      const uint32_t m = pair[h] / a.top - b * a.M;
-      qrow[h] = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
-                           (int64_t)(g * a.R + head[h]) * a.qs[2]);
+    // the span's chunks that some row of the tile reads: the sort keys tell
+    // before the rows themselves are known
+    {
+      const uint32_t r = tile.y * kTileRows + tid;
+      uint32_t read = 0;
+      if (tid < kTileRows && r < rows) {
+        read = a.skeys[e0 + r / a.R] & ((1u << kChunkBits) - 1u);
+        read ^= read >> 1;  // from the place in the Gray code
+      }
+      read = __reduce_or_sync(kFullMask, read);
+      if (lane == 0) s_any[warp] = read;
     }
-  }
-  uint32_t qf[DP / 16][4];
-  load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
-  const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
-  RowsState<T, DP> st;
-  st.clear();
-  const float c2 = a.scale * kLog2e;
-  for (uint32_t buf = 0; todo; buf = buf + 1u == kStages ? 0u : buf + 1u) {
-    const uint32_t c = __ffs(todo) - 1;
-    todo &= todo - 1u;
-    copy_wait<kStages - 2>();
-    __syncthreads();  // chunk c is here, and the stage before it is free
-    fetch(__ffs(ahead) - 1, buf ? buf - 1u : kStages - 1u, ahead != 0);
-    ahead &= ahead - 1u;
-    if (warp_any & chunk_blocks(c, a.block_log2)) {
-      const uint32_t at = base + buf * 2u * kTile;
-      auto bit = [&](int kp) { return (c * 64u + kp * 16u) >> a.block_log2; };
-      st.template add<4>(
-          qf, at, at + kTile, 0u, key0 + c * 64u, len, c2, lane,
-          [&](int kp) { return (warp_any >> bit(kp)) & 1u; },
-          [&](int kp, int h) { return (mask[h] >> bit(kp)) & 1u; });
+    __syncthreads();
+    uint32_t todo = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) todo |= s_any[i];
+    const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+    const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+    // chunk c into stage `buf`; one group per call, empty or not
+    auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
+      if (some) {
+        const uint32_t at = base + buf * 2u * kTile;
+        load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
+        load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
+      }
+      copy_commit();
+    };
+    uint32_t ahead = todo;  // chunks not yet asked for
+#pragma unroll
+    for (uint32_t i = 0; i + 1u < kStages; ++i) {
+      fetch(__ffs(ahead) - 1, i, ahead != 0);
+      ahead &= ahead - 1u;
     }
-  }
-  st.finish();
+
+    // this lane's two rows
+    uint32_t pair[2], head[2], mask[2];
+    const char *qrow[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (pair[h] == 0xffffffffu) continue;
-    const uint64_t row = (uint64_t)pair[h] * (a.gc * a.R) + gi * a.R + head[h];
-    const float inv = st.sum[h] > 0.f ? 1.f / st.sum[h] : 0.f;
-    float *o = a.part + row * a.D;
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r = tile.y * kTileRows + warp * 16u + (lane >> 2) + 8u * h;
+      pair[h] = 0xffffffffu;
+      head[h] = mask[h] = 0u;
+      qrow[h] = nullptr;
+      if (r < rows) {
+        const uint32_t e = r / a.R;
+        head[h] = r - e * a.R;
+        pair[h] = a.vals[e0 + e];
+        mask[h] = a.mask[pair[h]];
+        const uint32_t m = pair[h] / a.top - b * a.M;
+        qrow[h] = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
+                             (int64_t)(g * a.R + head[h]) * a.qs[2]);
+      }
+    }
+    uint32_t qf[DP / 16][4];
+    load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
+    sc.apply(qf);
+    const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
+    const uint32_t warp_all = __reduce_and_sync(
+        kFullMask, (qrow[0] ? mask[0] : ~0u) & (qrow[1] ? mask[1] : ~0u));
+    RowsState<T, DP> st;
+    st.clear();
+    for (uint32_t buf = 0; todo; buf = buf + 1u == kStages ? 0u : buf + 1u) {
+      const uint32_t c = __ffs(todo) - 1;
+      todo &= todo - 1u;
+      copy_wait<kStages - 2>();
+      __syncthreads();  // chunk c is here, and the stage before it is free
+      fetch(__ffs(ahead) - 1, buf ? buf - 1u : kStages - 1u, ahead != 0);
+      ahead &= ahead - 1u;
+      if (warp_any & chunk_blocks(c, a.block_log2)) {
+        const uint32_t at = base + buf * 2u * kTile;
+        auto bit = [&](int kp) { return (c * 64u + kp * 16u) >> a.block_log2; };
+        st.template add<4>(
+            qf, at, at + kTile, 0u, key0 + c * 64u, len, sc.c2, lane,
+            [&](int kp) { return (warp_any >> bit(kp)) & 1u; },
+            [&](int kp) { return (warp_all >> bit(kp)) & 1u; },
+            [&](int kp, int h) { return (mask[h] >> bit(kp)) & 1u; });
+      }
+    }
+    st.finish(sc.c2);
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j)
-      if (j * 8u < a.D)
-        *reinterpret_cast<float2 *>(o + j * 8 + 2 * (lane & 3u)) =
-            make_float2(st.o[j][2 * h] * inv, st.o[j][2 * h + 1] * inv);
-    if ((lane & 3u) == 0)
-      a.part_lse[row] = st.sum[h] > 0.f ? st.mx[h] + log2f(st.sum[h]) : -INFINITY;
+    for (int h = 0; h < 2; ++h) {
+      if (pair[h] == 0xffffffffu) continue;
+      const uint64_t row = (uint64_t)pair[h] * (a.gc * a.R) + gi * a.R + head[h];
+      const float inv = st.sum[h] > 0.f ? 1.f / st.sum[h] : 0.f;
+      float *o = a.part + row * a.D;
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+        if (j * 8u < a.D)
+          *reinterpret_cast<float2 *>(o + j * 8 + 2 * (lane & 3u)) =
+              make_float2(st.o[j][2 * h] * inv, st.o[j][2 * h + 1] * inv);
+      if ((lane & 3u) == 0)
+        a.part_lse[row] = st.sum[h] > 0.f ? st.mx[h] + log2f(st.sum[h]) : -INFINITY;
+    }
+    __syncthreads();  // every warp is done with the stages and s_any
   }
 }
 
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
-// its leading slots.  LANES = D / 4 lanes per row (rounded up to a power of
-// two), four elements each; the lanes hold the slots' weights, and the partial
-// rows are read four at a time.
-template <class T, int LANES>
+// its leading slots.  A warp takes 128 consecutive elements of a query's heads,
+// four per lane: the slots are the same for all lanes, and what a slot's
+// partial holds of them is consecutive too.
+template <class T>
 __global__ void __launch_bounds__(256)
-attend_join(const AttnArgs a) {
-  constexpr int kHeld = 64 / LANES;  // slots per lane
-  const uint32_t sub = threadIdx.x & (LANES - 1u);
-  const uint32_t hc = a.gc * a.R;
-  const uint64_t row = (uint64_t)blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
-  const bool live = row < (uint64_t)a.B * a.M * hc;
-  const uint32_t bm = live ? (uint32_t)(row / hc) : 0u;
-  const uint32_t hh = live ? (uint32_t)(row - (uint64_t)bm * hc) : 0u;
-  unsigned long long lead = live ? a.lead[bm] : 0ull;
-  const uint64_t first = (uint64_t)bm * a.top * hc + hh;  // partial of slot 0
-  float w[kHeld], mx = -INFINITY, total = 0.f;
+attend_join(const AttnArgs a, uint32_t parts) {
+  const uint32_t lane = threadIdx.x & 31u, hc = a.gc * a.R;
+  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
+  const uint32_t bm = (uint32_t)(w / parts);
+  if (bm >= a.B * a.M) return;
+  const uint32_t d = (uint32_t)(w - (uint64_t)bm * parts) * 128u + lane * 4u;
+  if (d >= hc * a.D) return;
+  const uint32_t hh = d / a.D;
+  const unsigned long long lead = a.lead[bm];
+  const float *lse = a.part_lse + (uint64_t)bm * a.top * hc + hh;
+  const float *part = a.part + (uint64_t)bm * a.top * hc * a.D + d;
+  const uint64_t step = (uint64_t)hc * a.D;
+  float mx = -INFINITY;
+  for (unsigned long long l = lead; l;) {
+    float x[4];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const uint32_t s = sub + i * LANES;
-    w[i] = (lead >> s) & 1ull ? a.part_lse[first + (uint64_t)s * hc] : -INFINITY;
-    mx = fmaxf(mx, w[i]);
+    for (int u = 0; u < 4; ++u) {
+      x[u] = l ? lse[(uint64_t)(__ffsll(l) - 1) * hc] : -INFINITY;
+      l &= l - 1ull;
+    }
+    mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   }
-#pragma unroll
-  for (int o = LANES / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
   const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    w[i] = exp2_fast(w[i] - base);
-    total += w[i];
-  }
-#pragma unroll
-  for (int o = LANES / 2; o; o >>= 1) total += __shfl_xor_sync(kFullMask, total, o);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const bool mine = 4u * sub < a.D;
-  uint32_t most = __popcll(lead);  // the same number of steps for the warp's rows
-#pragma unroll
-  for (int o = 16; o >= LANES; o >>= 1) most = max(most, __shfl_xor_sync(kFullMask, most, o));
-  for (uint32_t i = 0; i < most; i += 4u) {
-    float4 x[4];
+  float total = 0.f;
+  for (unsigned long long l = lead; l;) {
     float c[4];
+    float4 x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const bool some = lead != 0ull;
-      const uint32_t s = some ? __ffsll(lead) - 1 : 0u;
-      lead &= lead - 1ull;
-      c[u] = 0.f;
-#pragma unroll
-      for (int k = 0; k < kHeld; ++k) {
-        const float y = __shfl_sync(kFullMask, w[k], s & (LANES - 1u), LANES);
-        if (s / LANES == k) c[u] = y;
-      }
-      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (some && mine)
-        x[u] = *reinterpret_cast<const float4 *>(a.part + (first + (uint64_t)s * hc) * a.D + 4 * sub);
-      if (!some) c[u] = 0.f;
+      const uint32_t s = l ? __ffsll(l) - 1 : 0u;
+      c[u] = l ? lse[(uint64_t)s * hc] : -INFINITY;
+      x[u] = l ? __ldcs(reinterpret_cast<const float4 *>(part + s * step))
+               : make_float4(0.f, 0.f, 0.f, 0.f);
+      l &= l - 1ull;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      acc.x += c[u] * x[u].x; acc.y += c[u] * x[u].y;
-      acc.z += c[u] * x[u].z; acc.w += c[u] * x[u].w;
+      const float y = exp2_fast(c[u] - base);
+      total += y;
+      acc.x += y * x[u].x; acc.y += y * x[u].y; acc.z += y * x[u].z; acc.w += y * x[u].w;
     }
   }
-  if (!live) return;
   const float inv = total > 0.f ? 1.f / total : 0.f;
-  const uint64_t out_row = (uint64_t)bm * a.H + a.g0 * a.R + hh;
-  if (mine)
-    *reinterpret_cast<uint2 *>(a.out + (out_row * a.D + 4 * sub) * 2) =
-        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-  if (a.lse && sub == 0) a.lse[out_row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
+  const uint64_t out = ((uint64_t)bm * a.H + a.g0 * a.R) * a.D + d;
+  *reinterpret_cast<uint2 *>(a.out + out * 2) =
+      make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  if (a.lse && d == hh * a.D)
+    a.lse[(uint64_t)bm * a.H + a.g0 * a.R + hh] =
+        total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
 }
 
 // The same for the direct path, one CTA per row: groups of LANES lanes take
@@ -669,7 +702,7 @@ attend_direct(const AttnArgs a) {
   copy_commit();
   copy_wait<0>();
   __syncwarp();
-  const float c2 = a.scale * kLog2e;
+  const ScoreScale sc(a.scale);
   const uint32_t t = lane & 3u;
   float *s_o = reinterpret_cast<float *>(smem);  // [warp][16][DP], over the tiles
   for (uint32_t h0 = 0; h0 < a.R; h0 += 16u) {
@@ -686,13 +719,15 @@ attend_direct(const AttnArgs a) {
     if (some) {
       uint32_t qf[DP / 16][4];
       load_rows<DP>(qf, qrow[0], qrow[1], a.D, t);
+      sc.apply(qf);
 #pragma unroll
       for (uint32_t i = 0; i < kSlices; ++i)
         if (use[i])
-          st.template add<1>(qf, sk, sv, i * 16u, key[i], len, c2, lane,
-                             [](int) { return true; }, [](int, int) { return true; });
+          st.template add<1>(qf, sk, sv, i * 16u, key[i], len, sc.c2, lane,
+                             [](int) { return true; }, [](int) { return true; },
+                             [](int, int) { return true; });
     }
-    st.finish();
+    st.finish(sc.c2);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       if (t == 0) {
@@ -775,7 +810,7 @@ constexpr uint32_t kGradItem = 512;    // query rows per CTA
 template <int DP, int SPAN>
 constexpr uint32_t grad_smem() {
   return 2u * SPAN * DP * 2u + 2u * 2u * kGradRows * DP * 2u + SPAN * kGradRows * 2u +
-         2u * kGradRows * 16u + kGradItem * 4u;
+         2u * kGradRows * 16u + kGradItem * 16u;
 }
 
 // Byte offset of 16-byte chunk c (8 rows) of key r in the ds tile
@@ -784,247 +819,274 @@ __device__ __forceinline__ uint32_t ds_off(uint32_t r, uint32_t c) {
   return r * (kGradRows * 2u) + ((c ^ ((r >> 1) & 3u)) << 4);
 }
 
-// One item: up to kGradItem rows of one span and key head.  Warp w owns keys
-// 16 w .. 16 w + 15 of the span and keeps their dk and dv in registers; per
-// step of 32 rows it forms s^T = k q^T and dp^T = v dout^T, from them p^T and
-// ds^T (whose accumulator layout is the A operand of the next products), adds
-// p^T dout and ds^T q, and puts ds into shared memory, from which all warps
-// make the rows' share of dq = ds k.
+// What a step needs to know of a query row.
+struct GradRow {
+  int64_t q;      // byte offset of the row of q
+  uint32_t row;   // (query, head) over the turn
+  uint32_t pair;
+};
+
+// Items of up to kGradItem rows of one span and key head, CTAs taking them in
+// turns.  Warp w owns keys 16 w .. 16 w + 15 of the span and keeps their dk and
+// dv in registers; per step of 32 rows it forms s^T = k q^T and dp^T = v
+// dout^T, from them p^T and ds^T (whose accumulator layout is the A operand of
+// the next products), adds p^T dout and ds^T q, and puts ds into shared memory,
+// from which all warps make the rows' share of dq = ds k.
 template <class T, int DP, int SPAN>
 __global__ void __launch_bounds__(SPAN * 2, DP <= 64 && SPAN == 128 ? 2 : 1)
 attend_grad(const AttnArgs a) {
   extern __shared__ __align__(128) char smem[];
   constexpr uint32_t kThreads = SPAN * 2, kWarps = SPAN / 16, kChunks = DP / 8;
-  if (blockIdx.x >= *a.tile_count) return;
-  const uint4 tile = a.tiles[blockIdx.x];
+  constexpr uint32_t kRowTile = kGradRows * DP * 2u;
+  constexpr uint32_t kDsAt = 2u * SPAN * DP * 2u + 4u * kRowTile;
+  constexpr uint32_t kInfoAt = kDsAt + SPAN * kGradRows * 2u;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, t = lane & 3u;
-  const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
-  const uint32_t gi = blockIdx.y, g = a.g0 + gi;
-  const uint32_t e0 = tile.z, all_rows = tile.w * a.R;
-  const uint32_t row0 = tile.y * kGradItem;
-  const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
-  const uint32_t len = cloud_length(a.lengths, b, a.N);
-  const uint32_t key0 = sb * SPAN;
-  const uint32_t steps = (rows + kGradRows - 1u) / kGradRows;
-
   const uint32_t sk = smem_u32(smem), sv = sk + SPAN * DP * 2u;
   const uint32_t sq = sv + SPAN * DP * 2u;              // [2][q, dout][32][DP]
-  constexpr uint32_t kRowTile = kGradRows * DP * 2u;
-  const uint32_t sds = sq + 4u * kRowTile;
-  char *info = smem + (2u * SPAN * DP * 2u + 4u * kRowTile + SPAN * kGradRows * 2u);
-  // [2][lse, delta, mask, partial row][32]
-  const float *s_lse = reinterpret_cast<const float *>(info);
-  const float *s_delta = s_lse + kGradRows;
-  const uint32_t *s_mask = reinterpret_cast<const uint32_t *>(info) + 2 * kGradRows;
-  uint32_t *s_row = reinterpret_cast<uint32_t *>(info) + 3 * kGradRows;
-  constexpr uint32_t kInfo = 4 * kGradRows;  // words per buffer
-  uint32_t *s_pair = reinterpret_cast<uint32_t *>(info) + 2 * kInfo;  // [kGradItem]
-
-  float dk[DP / 8][4], dv[DP / 8][4];
-#pragma unroll
-  for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dk[j][i] = dv[j][i] = 0.f;
-
-  if (steps) {
-    const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
-    const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-    load_keys<DP, SPAN, kThreads>(sk, kh, a.ks[1], key0, len, a.D, tid);
-    load_keys<DP, SPAN, kThreads>(sv, vh, a.vs[1], key0, len, a.D, tid);
-  }
-  // the item's pairs: the address of a row is then one multiplication away
-  for (uint32_t r = tid; r < rows; r += kThreads) s_pair[r] = a.vals[e0 + (row0 + r) / a.R];
-  __syncthreads();
-  // Rows of step i into buffer i & 1: 8 threads per row while DP = 64.
-  auto fetch = [&](uint32_t i) {
-    const uint32_t buf = i & 1u, at = sq + buf * 2u * kRowTile;
-    for (uint32_t x = tid; x < kGradRows * kChunks; x += kThreads) {
-      const uint32_t r = x / kChunks, c = x % kChunks, rr = i * kGradRows + r;
-      const bool some = rr < rows && c * 8u < a.D;
-      const char *qp = a.q, *op = a.dout;
-      if (some) {
-        const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
-        const uint32_t bm = s_pair[rr] / a.top, m = bm - b * a.M, h = g * a.R + hh;
-        qp = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2] + c * 8);
-        op = a.dout + 2 * (((uint64_t)bm * a.H + h) * a.D + c * 8);
-      }
-      copy16(at + tile_off<DP>(r, c), qp, some);
-      copy16(at + kRowTile + tile_off<DP>(r, c), op, some);
-    }
-    if (tid < kGradRows) {
-      const uint32_t rr = i * kGradRows + tid;
-      const bool some = rr < rows;
-      const uint32_t w = smem_u32(info) + 4u * (buf * kInfo + tid);
-      const float *lp = a.lse_in, *dp = a.delta;
-      const uint32_t *mp = a.mask;
-      uint32_t prow = 0xffffffffu;
-      if (some) {
-        const uint32_t e = (row0 + rr) / a.R, hh = row0 + rr - e * a.R;
-        const uint32_t p = s_pair[rr];
-        const uint64_t row = (uint64_t)(p / a.top) * a.H + g * a.R + hh;
-        lp += row;
-        dp += row;
-        mp += p;
-        prow = p * (a.gc * a.R) + gi * a.R + hh;
-      }
-      copy4(w, lp, some);
-      copy4(w + 4u * kGradRows, dp, some);
-      copy4(w + 8u * kGradRows, mp, some);
-      s_row[buf * kInfo + tid] = prow;
-    }
-    copy_commit();
-  };
-  if (steps) fetch(0);
+  const uint32_t sds = sk + kDsAt;
+  // [2]: (lse, delta) of 32 rows, their masks, their partial rows
+  const char *info = smem + kInfoAt;
+  constexpr uint32_t kInfo = 16u * kGradRows;  // bytes per buffer
+  GradRow *s_rows = reinterpret_cast<GradRow *>(smem + kInfoAt + 2u * kInfo);  // [kGradItem]
   const float c2 = a.scale * kLog2e;
-  const uint32_t my_bit = (warp * 16u) >> a.block_log2;
-  const bool my_keys = key0 + warp * 16u < len;
-  const bool in0 = key0 + warp * 16u + (lane >> 2) < len;
-  const bool in1 = key0 + warp * 16u + (lane >> 2) + 8u < len;
-  for (uint32_t i = 0; i < steps; ++i) {
-    const uint32_t buf = i & 1u, tq = sq + buf * 2u * kRowTile, to = tq + kRowTile;
-    if (i + 1u < steps) {
-      fetch(i + 1u);
-      copy_wait<1>();
-    } else {
-      copy_wait<0>();
+  const uint32_t work = *a.tile_count * a.gc;
+  for (uint32_t item = blockIdx.x; item < work; item += gridDim.x) {
+    const uint32_t gi = item % a.gc, g = a.g0 + gi, place = item / a.gc;
+    const uint4 tile = a.tiles[place];
+    const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
+    const uint32_t e0 = tile.z, all_rows = tile.w * a.R;
+    const uint32_t row0 = tile.y * kGradItem;
+    const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
+    const uint32_t len = cloud_length(a.lengths, b, a.N);
+    const uint32_t key0 = sb * SPAN;
+    const uint32_t steps = (rows + kGradRows - 1u) / kGradRows;
+
+    float dk[DP / 8][4], dv[DP / 8][4];
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dk[j][i] = dv[j][i] = 0.f;
+
+    if (steps) {
+      const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+      const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+      load_keys<DP, SPAN, kThreads>(sk, kh, a.ks[1], key0, len, a.D, tid);
+      load_keys<DP, SPAN, kThreads>(sv, vh, a.vs[1], key0, len, a.D, tid);
+    }
+    // the item's rows, once: a step's addresses are then one shared load away
+    for (uint32_t r = tid; r < rows; r += kThreads) {
+      const uint32_t e = (row0 + r) / a.R, h = g * a.R + row0 + r - e * a.R;
+      GradRow x;
+      x.pair = a.vals[e0 + e];
+      const uint32_t bm = x.pair / a.top, m = bm - b * a.M;
+      x.q = 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2]);
+      x.row = bm * a.H + h;
+      s_rows[r] = x;
     }
     __syncthreads();
-    const uint32_t mask = s_mask[buf * kInfo + lane];
-    const uint32_t any = __reduce_or_sync(kFullMask, mask);
-    const uint32_t mine = __ballot_sync(kFullMask, (mask >> my_bit) & 1u);  // rows that read my keys
-    if (mine && my_keys) {
-      float s[4][4], dp[4][4];
+    // Rows of step i into buffer i & 1, 16 bytes of a row per thread and turn.
+    auto fetch = [&](uint32_t i) {
+      const uint32_t buf = i & 1u, at = sq + buf * 2u * kRowTile;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        uint32_t ka[4], va[4];
-        const uint32_t ao = tile_off<DP>(warp * 16u + (lane & 15u), kk * 2 + (lane >> 4));
-        ldsm4(ka, sk + ao);
-        ldsm4(va, sv + ao);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          uint32_t x[4];
-          const uint32_t bo = tile_off<DP>(n * 16 + (lane & 7u) + ((lane >> 4) << 3),
-                                           kk * 2 + ((lane >> 3) & 1u));
-          ldsm4(x, tq + bo);
-          mma16816<T>(s[2 * n], ka, x[0], x[1]);
-          mma16816<T>(s[2 * n + 1], ka, x[2], x[3]);
-          ldsm4(x, to + bo);
-          mma16816<T>(dp[2 * n], va, x[0], x[1]);
-          mma16816<T>(dp[2 * n + 1], va, x[2], x[3]);
+      for (uint32_t x = tid; x < kGradRows * kChunks; x += kThreads) {
+        const uint32_t r = x / kChunks, c = x % kChunks, rr = i * kGradRows + r;
+        const bool some = rr < rows && c * 8u < a.D;
+        const char *qp = a.q, *op = a.dout;
+        if (some) {
+          const GradRow y = s_rows[rr];
+          qp += y.q + c * 16u;
+          op += ((uint64_t)y.row * a.D + c * 8u) * 2u;
         }
+        copy16(at + tile_off<DP>(r, c), qp, some);
+        copy16(at + kRowTile + tile_off<DP>(r, c), op, some);
       }
-      uint32_t pa[2][4], da[2][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint32_t r = n * 8 + 2 * t;
-        const float2 lse = *reinterpret_cast<const float2 *>(s_lse + buf * kInfo + r);
-        const float2 del = *reinterpret_cast<const float2 *>(s_delta + buf * kInfo + r);
-        const bool r0 = (mine >> r) & 1u, r1 = (mine >> (r + 1u)) & 1u;
-        float p[4], ds[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const bool in = (x & 1 ? r1 : r0) && (x < 2 ? in0 : in1);
-          const float l = x & 1 ? lse.y : lse.x;
-          p[x] = in ? exp2_fast(fmaf(s[n][x], c2, -l * kLog2e)) : 0.f;
-          ds[x] = p[x] * (dp[n][x] - (x & 1 ? del.y : del.x));
+      if (tid < kGradRows) {
+        const uint32_t rr = i * kGradRows + tid;
+        const bool some = rr < rows;
+        const uint32_t w = sk + kInfoAt + buf * kInfo;
+        const float *lp = a.lse_in, *dp = a.delta;
+        const uint32_t *mp = a.mask;
+        uint32_t prow = 0xffffffffu;
+        if (some) {
+          const GradRow y = s_rows[rr];
+          lp += y.row;
+          dp += y.row;
+          mp += y.pair;
+          prow = y.pair * (a.gc * a.R) + gi * a.R + (y.row - (y.pair / a.top) * a.H - g * a.R);
         }
-        pa[n >> 1][(n & 1) * 2] = pack2<T>(p[0], p[1]);
-        pa[n >> 1][(n & 1) * 2 + 1] = pack2<T>(p[2], p[3]);
-        const uint32_t d0 = pack2<T>(ds[0], ds[1]), d1 = pack2<T>(ds[2], ds[3]);
-        da[n >> 1][(n & 1) * 2] = d0;
-        da[n >> 1][(n & 1) * 2 + 1] = d1;
-        const uint32_t kr = warp * 16u + (lane >> 2);
-        *reinterpret_cast<uint32_t *>(smem + (sds - sk) + ds_off(kr, n) + 4u * t) = d0;
-        *reinterpret_cast<uint32_t *>(smem + (sds - sk) + ds_off(kr + 8u, n) + 4u * t) = d1;
+        copy4(w + 8u * tid, lp, some);
+        copy4(w + 8u * tid + 4u, dp, some);
+        copy4(w + 8u * kGradRows + 4u * tid, mp, some);
+        reinterpret_cast<uint32_t *>(smem + kInfoAt + buf * kInfo)[3 * kGradRows + tid] = prow;
       }
+      copy_commit();
+    };
+    if (steps) fetch(0);
+    const uint32_t my_bit = (warp * 16u) >> a.block_log2, my_key = key0 + warp * 16u;
+    const bool in0 = my_key + (lane >> 2) < len, in1 = my_key + (lane >> 2) + 8u < len;
+    for (uint32_t i = 0; i < steps; ++i) {
+      const uint32_t buf = i & 1u, tq = sq + buf * 2u * kRowTile, to = tq + kRowTile;
+      const char *inf = info + buf * kInfo;
+      if (i + 1u < steps) {
+        fetch(i + 1u);
+        copy_wait<1>();
+      } else {
+        copy_wait<0>();
+      }
+      __syncthreads();
+      const uint32_t mask = reinterpret_cast<const uint32_t *>(inf)[2 * kGradRows + lane];
+      const uint32_t any = __reduce_or_sync(kFullMask, mask);
+      const uint32_t mine = __ballot_sync(kFullMask, (mask >> my_bit) & 1u);  // rows reading my keys
+      if (mine && my_key < len) {
+        float s[4][4], dp[4][4];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int jj = 0; jj < DP / 16; ++jj) {
-          uint32_t x[4];
-          const uint32_t bo = tile_off<DP>(kk * 16 + (lane & 15u), jj * 2 + (lane >> 4));
-          ldsm4t(x, to + bo);
-          mma16816<T>(dv[2 * jj], pa[kk], x[0], x[1]);
-          mma16816<T>(dv[2 * jj + 1], pa[kk], x[2], x[3]);
-          ldsm4t(x, tq + bo);
-          mma16816<T>(dk[2 * jj], da[kk], x[0], x[1]);
-          mma16816<T>(dk[2 * jj + 1], da[kk], x[2], x[3]);
-        }
-    }
-    __syncthreads();
-    // dq of the 32 rows: kUnits tiles of 16 rows x 8 kPer columns
-    constexpr uint32_t kPer = (2 * kChunks) / kWarps > 0 ? (2 * kChunks) / kWarps : 1;
-    constexpr uint32_t kUnits = 2 * kChunks / kPer;
-    if (warp < kUnits) {
-      const uint32_t rt = warp & 1u, j0 = (warp >> 1) * kPer;
-      float acc[kPer][4];
+          for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
 #pragma unroll
-      for (uint32_t j = 0; j < kPer; ++j)
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          uint32_t ka[4], va[4];
+          const uint32_t ao = tile_off<DP>(warp * 16u + (lane & 15u), kk * 2 + (lane >> 4));
+          ldsm4(ka, sk + ao);
+          ldsm4(va, sv + ao);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
-      for (uint32_t ks = 0; ks < kWarps; ++ks) {
-        if (!((any >> ((ks * 16u) >> a.block_log2)) & 1u) || key0 + ks * 16u >= len) continue;
-        uint32_t x[4];
-        ldsm4t(x, sds + ds_off(ks * 16u + (lane & 7u) + ((lane >> 4) << 3),
-                               rt * 2u + ((lane >> 3) & 1u)));
-        if constexpr (kPer == 1) {
-          uint32_t y[2];
-          ldsm2t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0));
-          mma16816<T>(acc[0], x, y[0], y[1]);
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < kPer / 2; ++j) {
-            uint32_t y[4];
-            ldsm4t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0 + 2 * j + (lane >> 4)));
-            mma16816<T>(acc[2 * j], x, y[0], y[1]);
-            mma16816<T>(acc[2 * j + 1], x, y[2], y[3]);
+          for (int n = 0; n < 2; ++n) {
+            uint32_t x[4];
+            const uint32_t bo = tile_off<DP>(n * 16 + (lane & 7u) + ((lane >> 4) << 3),
+                                             kk * 2 + ((lane >> 3) & 1u));
+            ldsm4(x, tq + bo);
+            mma16816<T>(s[2 * n], ka, x[0], x[1]);
+            mma16816<T>(s[2 * n + 1], ka, x[2], x[3]);
+            ldsm4(x, to + bo);
+            mma16816<T>(dp[2 * n], va, x[0], x[1]);
+            mma16816<T>(dp[2 * n + 1], va, x[2], x[3]);
           }
         }
-      }
+        uint32_t pa[2][4], da[2][4];
+        // p = exp(scale s - lse) and ds = p (dp - delta) of row pair n * 8 + 2 t
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t prow = s_row[buf * kInfo + rt * 16u + (lane >> 2) + 8u * h];
-        if (prow == 0xffffffffu) continue;
-        float *o = a.part + (uint64_t)prow * a.D;
+        for (int n = 0; n < 4; ++n) {
+          const float4 y = reinterpret_cast<const float4 *>(inf)[n * 4 + t];  // two rows
+          const float l0 = y.x * kLog2e, l1 = y.z * kLog2e;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[n][x] = exp2_fast(fmaf(s[n][x], c2, x & 1 ? -l1 : -l0));
+            dp[n][x] -= x & 1 ? y.w : y.y;
+          }
+        }
+        if (mine != kFullMask || my_key + 16u > len) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t two = mine >> (n * 8 + 2 * t);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              s[n][x] = ((two >> (x & 1)) & 1u) && (x < 2 ? in0 : in1) ? s[n][x] : 0.f;
+          }
+        }
+        char *ds = smem + kDsAt;
+        const uint32_t kr = warp * 16u + (lane >> 2);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float *p = s[n], *e = dp[n];
+          pa[n >> 1][(n & 1) * 2] = pack2<T>(p[0], p[1]);
+          pa[n >> 1][(n & 1) * 2 + 1] = pack2<T>(p[2], p[3]);
+          const uint32_t d0 = pack2<T>(p[0] * e[0], p[1] * e[1]);
+          const uint32_t d1 = pack2<T>(p[2] * e[2], p[3] * e[3]);
+          da[n >> 1][(n & 1) * 2] = d0;
+          da[n >> 1][(n & 1) * 2 + 1] = d1;
+          *reinterpret_cast<uint32_t *>(ds + ds_off(kr, n) + 4u * t) = d0;
+          *reinterpret_cast<uint32_t *>(ds + ds_off(kr + 8u, n) + 4u * t) = d1;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int jj = 0; jj < DP / 16; ++jj) {
+            uint32_t x[4];
+            const uint32_t bo = tile_off<DP>(kk * 16 + (lane & 15u), jj * 2 + (lane >> 4));
+            ldsm4t(x, to + bo);
+            mma16816<T>(dv[2 * jj], pa[kk], x[0], x[1]);
+            mma16816<T>(dv[2 * jj + 1], pa[kk], x[2], x[3]);
+            ldsm4t(x, tq + bo);
+            mma16816<T>(dk[2 * jj], da[kk], x[0], x[1]);
+            mma16816<T>(dk[2 * jj + 1], da[kk], x[2], x[3]);
+          }
+      }
+      __syncthreads();
+      // dq of the 32 rows: kUnits tiles of 16 rows x 8 kPer columns
+      constexpr uint32_t kPer = (2 * kChunks) / kWarps > 0 ? (2 * kChunks) / kWarps : 1;
+      constexpr uint32_t kUnits = 2 * kChunks / kPer;
+      if (warp < kUnits) {
+        const uint32_t rt = warp & 1u, j0 = (warp >> 1) * kPer;
+        float acc[kPer][4];
 #pragma unroll
         for (uint32_t j = 0; j < kPer; ++j)
-          if ((j0 + j) * 8u < a.D)
-            *reinterpret_cast<float2 *>(o + (j0 + j) * 8u + 2u * t) =
-                make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
+#pragma unroll
+        for (uint32_t ks = 0; ks < kWarps; ++ks) {
+          if (!((any >> ((ks * 16u) >> a.block_log2)) & 1u) || key0 + ks * 16u >= len) continue;
+          uint32_t x[4];
+          ldsm4t(x, sds + ds_off(ks * 16u + (lane & 7u) + ((lane >> 4) << 3),
+                                 rt * 2u + ((lane >> 3) & 1u)));
+          if constexpr (kPer == 1) {
+            uint32_t y[2];
+            ldsm2t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0));
+            mma16816<T>(acc[0], x, y[0], y[1]);
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kPer / 2; ++j) {
+              uint32_t y[4];
+              ldsm4t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0 + 2 * j + (lane >> 4)));
+              mma16816<T>(acc[2 * j], x, y[0], y[1]);
+              mma16816<T>(acc[2 * j + 1], x, y[2], y[3]);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t prow = reinterpret_cast<const uint32_t *>(
+              inf)[3 * kGradRows + rt * 16u + (lane >> 2) + 8u * h];
+          if (prow == 0xffffffffu) continue;
+          float *o = a.part + (uint64_t)prow * a.D;
+#pragma unroll
+          for (uint32_t j = 0; j < kPer; ++j)
+            if ((j0 + j) * 8u < a.D)
+              *reinterpret_cast<float2 *>(o + (j0 + j) * 8u + 2u * t) =
+                  make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+        }
+      }
+      __syncthreads();
+    }
+    // the span's dk and dv, or this item's share of them
+    const bool whole = all_rows <= kGradItem;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r = warp * 16u + (lane >> 2) + 8u * h;
+      if (key0 + r >= a.N) continue;
+      if (whole) {
+        const uint64_t row = ((uint64_t)b * a.N + key0 + r) * a.G + g;
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j)
+          if (j * 8u < a.D) {
+            const uint64_t o = 2 * (row * a.D + j * 8 + 2 * t);
+            *reinterpret_cast<uint32_t *>(a.dk + o) =
+                pack2<T>(dk[j][2 * h] * a.scale, dk[j][2 * h + 1] * a.scale);
+            *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(dv[j][2 * h], dv[j][2 * h + 1]);
+          }
+      } else {
+        float *o = a.part_kv + (((uint64_t)place * a.gc + gi) * 2 * SPAN + r) * a.D;
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j)
+          if (j * 8u < a.D) {
+            *reinterpret_cast<float2 *>(o + j * 8 + 2 * t) =
+                make_float2(dk[j][2 * h], dk[j][2 * h + 1]);
+            *reinterpret_cast<float2 *>(o + (uint64_t)SPAN * a.D + j * 8 + 2 * t) =
+                make_float2(dv[j][2 * h], dv[j][2 * h + 1]);
+          }
       }
     }
-    __syncthreads();
-  }
-  // the span's dk and dv, or this item's share of them
-  const bool whole = all_rows <= kGradItem;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t r = warp * 16u + (lane >> 2) + 8u * h;
-    if (key0 + r >= a.N) continue;
-    if (whole) {
-      const uint64_t row = ((uint64_t)b * a.N + key0 + r) * a.G + g;
-#pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
-        if (j * 8u < a.D) {
-          const uint64_t o = 2 * (row * a.D + j * 8 + 2 * t);
-          *reinterpret_cast<uint32_t *>(a.dk + o) =
-              pack2<T>(dk[j][2 * h] * a.scale, dk[j][2 * h + 1] * a.scale);
-          *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(dv[j][2 * h], dv[j][2 * h + 1]);
-        }
-    } else {
-      float *o = a.part_kv + (((uint64_t)blockIdx.x * a.gc + gi) * 2 * SPAN + r) * a.D;
-#pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
-        if (j * 8u < a.D) {
-          *reinterpret_cast<float2 *>(o + j * 8 + 2 * t) = make_float2(dk[j][2 * h], dk[j][2 * h + 1]);
-          *reinterpret_cast<float2 *>(o + (uint64_t)SPAN * a.D + j * 8 + 2 * t) =
-              make_float2(dv[j][2 * h], dv[j][2 * h + 1]);
-        }
-    }
+    // (the last step's barrier, or none of the shared tiles used: the next
+    // item may load)
   }
 }
 
@@ -1053,23 +1115,35 @@ grad_join_keys(const AttnArgs a, uint32_t span) {
   }
 }
 
-// dq of a query: the shares of its pairs, slots in order.
+// dq of a query: the shares of its pairs, slots in order; lanes as in
+// attend_join.
 template <class T>
 __global__ void __launch_bounds__(256)
-grad_join_queries(const AttnArgs a, const int lanes_log2) {
-  const uint32_t sub = threadIdx.x & ((1u << lanes_log2) - 1u);
-  const uint32_t hc = a.gc * a.R;
-  const uint64_t row = (uint64_t)blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  if (row >= (uint64_t)a.B * a.M * hc || 4u * sub >= a.D) return;
-  const uint32_t bm = (uint32_t)(row / hc), hh = (uint32_t)(row - (uint64_t)bm * hc);
+grad_join_queries(const AttnArgs a, uint32_t parts) {
+  const uint32_t lane = threadIdx.x & 31u, hc = a.gc * a.R;
+  const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
+  const uint32_t bm = (uint32_t)(w / parts);
+  if (bm >= a.B * a.M) return;
+  const uint32_t d = (uint32_t)(w - (uint64_t)bm * parts) * 128u + lane * 4u;
+  if (d >= hc * a.D) return;
+  const float *part = a.part + (uint64_t)bm * a.top * hc * a.D + d;
+  const uint64_t step = (uint64_t)hc * a.D;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (unsigned long long l = a.lead[bm]; l; l &= l - 1) {
-    const uint64_t p = ((uint64_t)bm * a.top + __ffsll(l) - 1) * hc + hh;
-    const float4 x = *reinterpret_cast<const float4 *>(a.part + p * a.D + 4 * sub);
-    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  for (unsigned long long l = a.lead[bm]; l;) {
+    float4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      x[u] = l ? __ldcs(reinterpret_cast<const float4 *>(part + (uint64_t)(__ffsll(l) - 1) * step))
+               : make_float4(0.f, 0.f, 0.f, 0.f);
+      l &= l - 1ull;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      acc.x += x[u].x; acc.y += x[u].y; acc.z += x[u].z; acc.w += x[u].w;
+    }
   }
-  const uint64_t out_row = (uint64_t)bm * a.H + a.g0 * a.R + hh;
-  *reinterpret_cast<uint2 *>(a.dq + (out_row * a.D + 4 * sub) * 2) =
+  const uint64_t out = ((uint64_t)bm * a.H + a.g0 * a.R) * a.D + d;
+  *reinterpret_cast<uint2 *>(a.dq + out * 2) =
       make_uint2(pack2<T>(acc.x * a.scale, acc.y * a.scale),
                  pack2<T>(acc.z * a.scale, acc.w * a.scale));
 }
@@ -1231,8 +1305,13 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
   if (n && spans) {
-    plan_pairs<<<(uint32_t)ceil_div(a.B * a.M, 8), 256, 0, st>>>(a, w.span_log2, w.sort.keys0,
-                                                                 w.mask, w.lead, w.tile_count);
+    const uint32_t grid = (uint32_t)ceil_div(a.B * a.M, 8);
+    if (a.top <= 32)
+      plan_pairs<1><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
+                                          w.tile_count);
+    else
+      plan_pairs<2><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
+                                          w.tile_count);
     if ((err = cudaGetLastError())) return err;
     if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
   } else {  // no pair, or no key to form one with
@@ -1249,13 +1328,6 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
                                                              w.least, w.span, w.tiles,
                                                              w.tile_count);
   return cudaGetLastError();
-}
-
-// Lanes (log2) of 4 elements for a row of D.
-int row_lanes_log2(uint32_t D) {
-  int l = 1;
-  while ((4u << l) < D) ++l;
-  return l;
 }
 
 // More than 48 KB a CTA, static shared memory included, has to be asked for.
@@ -1283,16 +1355,19 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
   }
   const uint32_t smem = kStages * 2u * 64u * DP * 2u;
   if ((err = opt_in(attend_tiles<T, DP>, smem))) return err;
+  const uint64_t resident = (uint64_t)sm_count() * (DP <= 64 ? 2 : 1);
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
     if ((err = run_plan(a, w, st))) return err;
     const uint64_t tiles = (uint64_t)a.B * a.M * a.top * a.R / w.tile_rows + (uint64_t)a.B * a.nsb;
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
-      if (tiles) attend_tiles<T, DP><<<dim3((uint32_t)tiles, a.gc), 256, smem, st>>>(a);
+      if (tiles)
+        attend_tiles<T, DP><<<(uint32_t)std::min(tiles * a.gc, resident), 256, smem, st>>>(a);
       if ((err = cudaGetLastError())) return err;
-      const uint64_t rows = (uint64_t)a.B * a.M * a.gc * a.R;
-      attend_join<T, DP / 4><<<(uint32_t)ceil_div(rows, 1024 / DP), 256, 0, st>>>(a);
+      const uint64_t rows = (uint64_t)a.B * a.M;
+      const uint32_t parts = (uint32_t)ceil_div((uint64_t)a.gc * a.R * a.D, 128);
+      attend_join<T><<<(uint32_t)ceil_div(rows * parts, 8), 256, 0, st>>>(a, parts);
       if ((err = cudaGetLastError())) return err;
     }
   }
@@ -1302,9 +1377,9 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
 template <class T, int DP, int SPAN>
 cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
   cudaError_t err;
-  const int lanes = row_lanes_log2(all.D);
   const uint32_t smem = grad_smem<DP, SPAN>();
   if ((err = opt_in(attend_grad<T, DP, SPAN>, smem))) return err;
+  const uint64_t resident = (uint64_t)sm_count() * (DP <= 64 && SPAN == 128 ? 2 : 1);
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
     const uint64_t nq = (uint64_t)a.B * a.M;
@@ -1317,15 +1392,16 @@ cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t
     const uint64_t tiles = nq * a.top * a.R / w.tile_rows + spans;
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
-      if (tiles) attend_grad<T, DP, SPAN><<<dim3((uint32_t)tiles, a.gc), SPAN * 2, smem, st>>>(a);
+      if (tiles)
+        attend_grad<T, DP, SPAN><<<(uint32_t)std::min(tiles * a.gc, resident), SPAN * 2, smem, st>>>(a);
       if ((err = cudaGetLastError())) return err;
       if (nq * a.top * a.R > w.tile_rows && spans) {
         grad_join_keys<T><<<dim3(spans, a.gc, 4), 256, 0, st>>>(a, SPAN);
         if ((err = cudaGetLastError())) return err;
       }
       if (nq) {
-        grad_join_queries<T><<<(uint32_t)ceil_div(nq * a.gc * a.R, 256 >> lanes), 256, 0, st>>>(
-            a, lanes);
+        const uint32_t parts = (uint32_t)ceil_div((uint64_t)a.gc * a.R * a.D, 128);
+        grad_join_queries<T><<<(uint32_t)ceil_div(nq * parts, 8), 256, 0, st>>>(a, parts);
         if ((err = cudaGetLastError())) return err;
       }
     }
