@@ -27,7 +27,7 @@ CU_SOURCES = ["nsfps_setup.cu", "nsfps_loop.cu", "nsfps_rounds.cu", "nsfps_stati
               "nsfps_group.cu", "nsfps_rows.cu", "nsfps_select.cu", "nsfps_attention.cu",
               "nsfps_capi.cu"]
 HEADERS = ["nsfps_internal.cuh", "nsfps_kernels.h", "nsfps_device.cuh", "nsfps_feature.cuh",
-           "nsfps_sort.cuh"]
+           "nsfps_sort.cuh", "nsfps_tmem.cuh"]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 NVCC_FLAGS = [

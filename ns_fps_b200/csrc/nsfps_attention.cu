@@ -23,6 +23,7 @@
 
 #include "nsfps_feature.cuh"
 #include "nsfps_sort.cuh"
+#include "nsfps_tmem.cuh"
 
 namespace nsfps {
 namespace {
@@ -263,7 +264,7 @@ plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, ui
 // -------------------------------------------------------------- forward
 
 constexpr uint32_t kSpanLog2 = 8;      // keys per span of the forward pass
-constexpr uint32_t kTileRows = 128;    // query rows per CTA: 8 warps of 16
+constexpr uint32_t kTileRows = 128;    // query rows per tile
 
 // Copies keys [key0, key0 + ROWS) of one head into a shared tile; zeros behind
 // the cloud's end and behind the head's elements.
@@ -425,20 +426,73 @@ struct RowsState {
   }
 };
 
-// Key chunks in shared memory: two being loaded behind the one in use.
-constexpr uint32_t kStages = 3;
+// A tile of 128 rows against one span: thread r owns row r.  Per 64-key chunk
+// that some row reads: s = q k^T (128 x 64) by the tensor core into tensor
+// memory, the thread takes its row's scores out, makes the weights, puts them
+// back as 16-bit values over the scores, and o += p v takes them from there.
+// Nothing but the operands' tiles passes through shared memory.  The softmax
+// (one exp2 per score, 16 per cycle and SM) bounds it; while one CTA waits for
+// its products or its loads, the others of the SM compute.
+constexpr uint32_t kTileThreads = 128;
 
-// Tiles of pairs of one span and key head, CTAs taking them in turns.
+// The reference maximum moves only when a row's maximum outgrows it by this
+// much (in base 2): weights up to 2^8 sum exactly as well, and the output in
+// tensor memory is rescaled about once per tile instead of once per chunk.
+constexpr float kLazy = 8.f;
+
+template <int DP>  // 64 or 128
+struct TileShape {
+  static constexpr uint32_t kQ = kTileRows * DP * 2u, kChunk = 64u * DP * 2u;
+  static constexpr uint32_t kSmem = kQ + 4u * kChunk + 1024u;  // two chunks of k and v
+  static constexpr uint32_t kTmem = DP == 64 ? 128u : 256u;    // scores, then output
+  static constexpr uint32_t kCtas = DP == 64 ? 4 : 2;          // per SM
+};
+
+// ROWS rows of DP elements into shared tiles of 64 columns each; src(r) gives
+// the row (null: zeros).
+template <int DP, uint32_t ROWS, uint32_t THREADS, class Src>
+__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t D, uint32_t tid, const char *any,
+                                          Src src) {
+  constexpr uint32_t kChunks = DP / 8;
+#pragma unroll
+  for (uint32_t i = 0; i < ROWS * kChunks / THREADS; ++i) {
+    const uint32_t x = tid + i * THREADS, r = x / kChunks, c = x % kChunks;
+    const char *p = src(r);
+    const bool some = p && c * 8u < D;
+    copy16(dst + (c >> 3) * (ROWS * 128u) + swizzled(r, c & 7u), some ? p + c * 16u : any, some);
+  }
+}
+
 template <class T, int DP>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kTileThreads, TileShape<DP>::kCtas)
 attend_tiles(const AttnArgs a) {
-  extern __shared__ __align__(128) char smem[];
-  __shared__ uint32_t s_any[8];
+  using Shape = TileShape<DP>;
+  extern __shared__ char smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2];
+  __shared__ uint32_t s_tmem, s_any[4];
+  __shared__ const char *s_q[kTileRows];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t base = smem_u32(smem);
-  constexpr uint32_t kTile = 64u * DP * 2u;
+  const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the swizzle's pattern
+  const uint32_t sk = sq + Shape::kQ, sv = sk + 2u * Shape::kChunk;
+  const uint32_t bar_s = smem_u32(&s_bar[0]), bar_o = smem_u32(&s_bar[1]);
   constexpr uint32_t kChunkBits = 1u << (kSpanLog2 - 6u);
-  const ScoreScale sc(a.scale);
+  if (warp == 0) tmem_alloc<Shape::kTmem>(smem_u32(&s_tmem));
+  if (tid == 0) {
+    bar_init(bar_s);
+    bar_init(bar_o);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tm = s_tmem, tm_s = tm, tm_o = tm + 64u;
+  const uint32_t my = (warp * 32u) << 16;  // this warp's lanes
+  constexpr uint32_t kScores = mma_desc<T>(128, 64, false, false);
+  constexpr uint32_t kOutput = mma_desc<T>(128, DP, false, true);
+  const float c2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+  const float sign = a.scale == 0.f ? 0.f : a.scale < 0.f ? -1.f : 1.f;
+  uint32_t phase = 0;     // of both barriers: each completes once per chunk
+  bool failed = false;
   const uint32_t work = *a.tile_count * a.gc;
   for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
     const uint32_t gi = w % a.gc, g = a.g0 + gi;
@@ -447,102 +501,188 @@ attend_tiles(const AttnArgs a) {
     const uint32_t e0 = tile.z, rows = tile.w * a.R;
     const uint32_t len = cloud_length(a.lengths, b, a.N);
     const uint32_t key0 = sb << kSpanLog2;
-
-    // the span's chunks that some row of the tile reads: the sort keys tell
-    // before the rows themselves are known
-    {
-      const uint32_t r = tile.y * kTileRows + tid;
-      uint32_t read = 0;
-      if (tid < kTileRows && r < rows) {
-        read = a.skeys[e0 + r / a.R] & ((1u << kChunkBits) - 1u);
-        read ^= read >> 1;  // from the place in the Gray code
-      }
-      read = __reduce_or_sync(kFullMask, read);
-      if (lane == 0) s_any[warp] = read;
+    // this thread's row, and the chunks that any row reads
+    const uint32_t r = tile.y * kTileRows + tid;
+    uint32_t pair = 0xffffffffu, mask = 0u, read = 0u, head = 0u;
+    const char *q = nullptr;
+    if (r < rows) {
+      const uint32_t e = r / a.R;
+      head = r - e * a.R;
+      pair = a.vals[e0 + e];
+      read = a.skeys[e0 + e] & ((1u << kChunkBits) - 1u);
+      read ^= read >> 1;  // from the place in the Gray code
+      mask = a.mask[pair];
+      const uint32_t m = pair / a.top - b * a.M;
+      q = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
+                     (int64_t)(g * a.R + head) * a.qs[2]);
     }
+    const uint32_t warp_read = __reduce_or_sync(kFullMask, read);
+    if (lane == 0) s_any[warp] = warp_read;
+    s_q[tid] = q;
     __syncthreads();
-    uint32_t todo = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) todo |= s_any[i];
+    uint32_t todo = s_any[0] | s_any[1] | s_any[2] | s_any[3];
     const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
     const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-    // chunk c into stage `buf`; one group per call, empty or not
     auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
       if (some) {
-        const uint32_t at = base + buf * 2u * kTile;
-        load_keys<DP, 64, 256>(at, kh, a.ks[1], key0 + c * 64u, len, a.D, tid);
-        load_keys<DP, 64, 256>(at + kTile, vh, a.vs[1], key0 + c * 64u, len, a.D, tid);
+        const uint32_t key = key0 + c * 64u;
+        load_tile<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid, kh, [&](uint32_t x) {
+          return key + x < len ? kh + (int64_t)(key + x) * a.ks[1] * 2 : nullptr;
+        });
+        load_tile<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid, vh, [&](uint32_t x) {
+          return key + x < len ? vh + (int64_t)(key + x) * a.vs[1] * 2 : nullptr;
+        });
       }
       copy_commit();
     };
-    uint32_t ahead = todo;  // chunks not yet asked for
+    uint32_t ahead = todo;
+    load_tile<DP, kTileRows, kTileThreads>(sq, a.D, tid, a.q, [&](uint32_t x) { return s_q[x]; });
 #pragma unroll
-    for (uint32_t i = 0; i + 1u < kStages; ++i) {
+    for (uint32_t i = 0; i < 2u; ++i) {  // (q goes with the first chunk)
       fetch(__ffs(ahead) - 1, i, ahead != 0);
       ahead &= ahead - 1u;
     }
-
-    // this lane's two rows
-    uint32_t pair[2], head[2], mask[2];
-    const char *qrow[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t r = tile.y * kTileRows + warp * 16u + (lane >> 2) + 8u * h;
-      pair[h] = 0xffffffffu;
-      head[h] = mask[h] = 0u;
-      qrow[h] = nullptr;
-      if (r < rows) {
-        const uint32_t e = r / a.R;
-        head[h] = r - e * a.R;
-        pair[h] = a.vals[e0 + e];
-        mask[h] = a.mask[pair[h]];
-        const uint32_t m = pair[h] / a.top - b * a.M;
-        qrow[h] = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
-                             (int64_t)(g * a.R + head[h]) * a.qs[2]);
-      }
-    }
-    uint32_t qf[DP / 16][4];
-    load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
-    sc.apply(qf);
-    const uint32_t warp_any = __reduce_or_sync(kFullMask, mask[0] | mask[1]);
-    const uint32_t warp_all = __reduce_and_sync(
-        kFullMask, (qrow[0] ? mask[0] : ~0u) & (qrow[1] ? mask[1] : ~0u));
-    RowsState<T, DP> st;
-    st.clear();
-    for (uint32_t buf = 0; todo; buf = buf + 1u == kStages ? 0u : buf + 1u) {
-      const uint32_t c = __ffs(todo) - 1;
+    const uint32_t warp_any = __reduce_or_sync(kFullMask, mask);
+    const uint32_t warp_all = __reduce_and_sync(kFullMask, q ? mask : ~0u);
+    float ref = -INFINITY, sum = 0.f;  // reference maximum of the signed raw scores
+    for (uint32_t i = 0; todo; ++i) {
+      const uint32_t c = __ffs(todo) - 1, buf = i & 1u;
       todo &= todo - 1u;
-      copy_wait<kStages - 2>();
-      __syncthreads();  // chunk c is here, and the stage before it is free
-      fetch(__ffs(ahead) - 1, buf ? buf - 1u : kStages - 1u, ahead != 0);
-      ahead &= ahead - 1u;
-      if (warp_any & chunk_blocks(c, a.block_log2)) {
-        const uint32_t at = base + buf * 2u * kTile;
-        auto bit = [&](int kp) { return (c * 64u + kp * 16u) >> a.block_log2; };
-        st.template add<4>(
-            qf, at, at + kTile, 0u, key0 + c * 64u, len, sc.c2, lane,
-            [&](int kp) { return (warp_any >> bit(kp)) & 1u; },
-            [&](int kp) { return (warp_all >> bit(kp)) & 1u; },
-            [&](int kp, int h) { return (mask[h] >> bit(kp)) & 1u; });
+      if (i) {
+        // the chunk before is used up: its buffers take the next but one
+        if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
+        __syncwarp();
+        tmem_after_sync();
+        fetch(__ffs(ahead) - 1, buf ^ 1u, ahead != 0);
+        ahead &= ahead - 1u;
       }
-    }
-    st.finish(sc.c2);
+      copy_wait<1>();
+      smem_to_mma();
+      tmem_before_sync();
+      __syncthreads();
+      if (tid == 0) {
+        tmem_after_sync();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (pair[h] == 0xffffffffu) continue;
-      const uint64_t row = (uint64_t)pair[h] * (a.gc * a.R) + gi * a.R + head[h];
-      const float inv = st.sum[h] > 0.f ? 1.f / st.sum[h] : 0.f;
-      float *o = a.part + row * a.D;
+        for (uint32_t kk = 0; kk < DP / 16; ++kk)
+          mma_ss(tm_s, tile_desc(sq + (kk >> 2) * (kTileRows * 128u) + (kk & 3u) * 32u, 16u),
+                 tile_desc(sk + buf * Shape::kChunk + (kk >> 2) * (64u * 128u) + (kk & 3u) * 32u, 16u),
+                 kScores, kk != 0u);
+        mma_commit(bar_s);
+      }
+      __syncwarp();
+      if (!failed) failed = !bar_wait(bar_s, phase);
+      __syncwarp();
+      tmem_after_sync();
+      uint32_t s[2][32];
+      tmem_ld32(s[0], tm_s + my);
+      tmem_ld32(s[1], tm_s + my + 32u);
+      tmem_ld_wait();
+      // scores that the row does not read are -inf; 16 keys that no row of the
+      // warp reads are not looked at
+      float mx = -INFINITY;
+      auto bit = [&](uint32_t x) { return (c * 64u + x * 16u) >> a.block_log2; };
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
-        if (j * 8u < a.D)
-          *reinterpret_cast<float2 *>(o + j * 8 + 2 * (lane & 3u)) =
-              make_float2(st.o[j][2 * h] * inv, st.o[j][2 * h + 1] * inv);
-      if ((lane & 3u) == 0)
-        a.part_lse[row] = st.sum[h] > 0.f ? st.mx[h] + log2f(st.sum[h]) : -INFINITY;
+      for (uint32_t x = 0; x < 4u; ++x) {
+        if (!((warp_any >> bit(x)) & 1u)) continue;
+        uint32_t *v = &s[x >> 1][(x & 1u) * 16u];
+        const uint32_t key = key0 + c * 64u + x * 16u;
+        if (!((warp_all >> bit(x)) & 1u) || key + 16u > len) {
+          const uint32_t n = (mask >> bit(x)) & 1u && key < len ? len - key : 0u;
+#pragma unroll
+          for (uint32_t y = 0; y < 16u; ++y)
+            v[y] = y < n ? __float_as_uint(__uint_as_float(v[y]) * sign) : 0xff800000u;
+        } else if (sign != 1.f) {
+#pragma unroll
+          for (uint32_t y = 0; y < 16u; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * sign);
+        }
+#pragma unroll
+        for (uint32_t y = 0; y < 16u; ++y) mx = fmaxf(mx, __uint_as_float(v[y]));
+      }
+      // (no key yet: the reference stays -inf and the weights come out 0)
+      const bool grow = mx * c2 > ref * c2 + kLazy || (ref == -INFINITY && mx != -INFINITY);
+      const float next = grow ? mx : ref;
+      const float base = next == -INFINITY ? 0.f : next * c2;
+      if (i && __any_sync(kFullMask, grow)) {
+        const float f = exp2_fast(fmaf(ref, c2, -base));  // 0 while ref is -inf
+        sum *= f;
+#pragma unroll
+        for (uint32_t j = 0; j < DP / 32; ++j) {
+          uint32_t o[32];
+          tmem_ld32(o, tm_o + my + j * 32u);
+          tmem_ld_wait();
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+          tmem_st32(tm_o + my + j * 32u, o);
+        }
+      }
+      ref = next;
+      // weights, rounded to T for the product with v: half a step of T each,
+      // like the output's own rounding
+      uint32_t p[32];
+#pragma unroll
+      for (uint32_t x = 0; x < 4u; ++x) {
+        const uint32_t *v = &s[x >> 1][(x & 1u) * 16u];
+        if ((warp_any >> bit(x)) & 1u) {
+#pragma unroll
+          for (uint32_t y = 0; y < 16u; y += 2) {
+            const float e0_ = exp2_fast(fmaf(__uint_as_float(v[y]), c2, -base));
+            const float e1_ = exp2_fast(fmaf(__uint_as_float(v[y + 1]), c2, -base));
+            sum += e0_ + e1_;
+            p[x * 8u + y / 2u] = pack2<T>(e0_, e1_);
+          }
+        } else {
+#pragma unroll
+          for (uint32_t y = 0; y < 8u; ++y) p[x * 8u + y] = 0u;
+        }
+      }
+      tmem_st32(tm_s + my, p);
+      tmem_st_wait();
+      tmem_before_sync();
+      __syncthreads();
+      if (tid == 0) {
+        tmem_after_sync();
+#pragma unroll
+        for (uint32_t kk = 0; kk < 4u; ++kk)
+          mma_ts(tm_o, tm_s + kk * 8u, tile_desc(sv + buf * Shape::kChunk + kk * 2048u, 64u * 128u),
+                 kOutput, i != 0u || kk != 0u);
+        mma_commit(bar_o);
+      }
+      __syncwarp();
+      phase ^= 1u;
     }
-    __syncthreads();  // every warp is done with the stages and s_any
+    if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
+    __syncwarp();
+    tmem_after_sync();
+    const uint64_t row = (uint64_t)pair * (a.gc * a.R) + gi * a.R + head;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (uint32_t j = 0; j < DP / 32; ++j) {
+      uint32_t o[32];
+      tmem_ld32(o, tm_o + my + j * 32u);
+      tmem_ld_wait();
+      if (r < rows)
+#pragma unroll
+        for (uint32_t y = 0; y < 32u; y += 8u)
+          if (j * 32u + y < a.D) {
+            float f[8];
+#pragma unroll
+            for (uint32_t z = 0; z < 8u; ++z) f[z] = __uint_as_float(o[y + z]) * inv;
+            // 32 bytes: a whole sector per thread
+            asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                         ::"l"(a.part + row * a.D + j * 32u + y), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+                         "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                         : "memory");
+          }
+      __syncwarp();
+    }
+    if (r < rows)  // (a wait that ran out shows as NaN)
+      a.part_lse[row] = failed ? __int_as_float(0x7fc00000)
+                        : sum > 0.f ? fmaf(ref, c2, log2f(sum)) : -INFINITY;
+    tmem_before_sync();
+    __syncthreads();  // every thread is done with the tiles and the output
+    tmem_after_sync();
   }
+  if (warp == 0) tmem_free<Shape::kTmem>(tm);
 }
 
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
@@ -1353,9 +1493,10 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
     }
     return cudaGetLastError();
   }
-  const uint32_t smem = kStages * 2u * 64u * DP * 2u;
-  if ((err = opt_in(attend_tiles<T, DP>, smem))) return err;
-  const uint64_t resident = (uint64_t)sm_count() * (DP <= 64 ? 2 : 1);
+  constexpr int TP = DP < 64 ? 64 : DP;  // the tiles' rows are 64 or 128 elements
+  const uint32_t smem = TileShape<TP>::kSmem;
+  if ((err = opt_in(attend_tiles<T, TP>, smem))) return err;
+  const uint64_t resident = (uint64_t)sm_count() * TileShape<TP>::kCtas;
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
     if ((err = run_plan(a, w, st))) return err;
@@ -1363,7 +1504,8 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
       if (tiles)
-        attend_tiles<T, DP><<<(uint32_t)std::min(tiles * a.gc, resident), 256, smem, st>>>(a);
+        attend_tiles<T, TP><<<(uint32_t)std::min(tiles * a.gc, resident), kTileThreads, smem, st>>>(
+            a);
       if ((err = cudaGetLastError())) return err;
       const uint64_t rows = (uint64_t)a.B * a.M;
       const uint32_t parts = (uint32_t)ceil_div((uint64_t)a.gc * a.R * a.D, 128);
