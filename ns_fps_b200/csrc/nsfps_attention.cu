@@ -114,23 +114,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void ldsm2t(uint32_t (&r)[2], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1])
-               : "r"(addr)
-               : "memory");
-}
 
 // 16-byte asynchronous copy; zeros where `some` is false (the source is then
 // not read).
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(some ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool some) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
-               "r"(some ? 4 : 0)
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -463,6 +452,16 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t D, uint32_t tid
   }
 }
 
+// Eight accumulators times f: 32 bytes, a whole sector per thread.
+__device__ __forceinline__ void store8(float *to, const uint32_t *x, float f) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(x[i]) * f;
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "f"(y[0]), "f"(y[1]),
+               "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
+               : "memory");
+}
+
 template <class T, int DP>
 __global__ void __launch_bounds__(kTileThreads, TileShape<DP>::kCtas)
 attend_tiles(const AttnArgs a) {
@@ -618,24 +617,24 @@ attend_tiles(const AttnArgs a) {
       ref = next;
       // weights, rounded to T for the product with v: half a step of T each,
       // like the output's own rounding
-      uint32_t p[32];
 #pragma unroll
       for (uint32_t x = 0; x < 4u; ++x) {
         const uint32_t *v = &s[x >> 1][(x & 1u) * 16u];
+        uint32_t *p = &s[0][x * 8u];  // the packed weights move up over the scores
         if ((warp_any >> bit(x)) & 1u) {
 #pragma unroll
           for (uint32_t y = 0; y < 16u; y += 2) {
-            const float e0_ = exp2_fast(fmaf(__uint_as_float(v[y]), c2, -base));
-            const float e1_ = exp2_fast(fmaf(__uint_as_float(v[y + 1]), c2, -base));
-            sum += e0_ + e1_;
-            p[x * 8u + y / 2u] = pack2<T>(e0_, e1_);
+            const float f0 = exp2_fast(fmaf(__uint_as_float(v[y]), c2, -base));
+            const float f1 = exp2_fast(fmaf(__uint_as_float(v[y + 1]), c2, -base));
+            sum += f0 + f1;
+            p[y / 2u] = pack2<T>(f0, f1);
           }
         } else {
 #pragma unroll
-          for (uint32_t y = 0; y < 8u; ++y) p[x * 8u + y] = 0u;
+          for (uint32_t y = 0; y < 8u; ++y) p[y] = 0u;
         }
       }
-      tmem_st32(tm_s + my, p);
+      tmem_st32(tm_s + my, s[0]);
       tmem_st_wait();
       tmem_before_sync();
       __syncthreads();
@@ -663,16 +662,7 @@ attend_tiles(const AttnArgs a) {
       if (r < rows)
 #pragma unroll
         for (uint32_t y = 0; y < 32u; y += 8u)
-          if (j * 32u + y < a.D) {
-            float f[8];
-#pragma unroll
-            for (uint32_t z = 0; z < 8u; ++z) f[z] = __uint_as_float(o[y + z]) * inv;
-            // 32 bytes: a whole sector per thread
-            asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                         ::"l"(a.part + row * a.D + j * 32u + y), "f"(f[0]), "f"(f[1]), "f"(f[2]),
-                         "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
-                         : "memory");
-          }
+          if (j * 32u + y < a.D) store8(a.part + row * a.D + j * 32u + y, &o[y], inv);
       __syncwarp();
     }
     if (r < rows)  // (a wait that ran out shows as NaN)
@@ -944,20 +934,9 @@ grad_delta(const AttnArgs a) {
   if (sub == 0 && row < (uint64_t)a.B * a.M * a.H) a.delta[row] = s;
 }
 
-constexpr uint32_t kGradRows = 32;     // query rows per step
-constexpr uint32_t kGradItem = 512;    // query rows per CTA
-
-template <int DP, int SPAN>
-constexpr uint32_t grad_smem() {
-  return 2u * SPAN * DP * 2u + 2u * 2u * kGradRows * DP * 2u + SPAN * kGradRows * 2u +
-         2u * kGradRows * 16u + kGradItem * 16u;
-}
-
-// Byte offset of 16-byte chunk c (8 rows) of key r in the ds tile
-// [key][kGradRows].
-__device__ __forceinline__ uint32_t ds_off(uint32_t r, uint32_t c) {
-  return r * (kGradRows * 2u) + ((c ^ ((r >> 1) & 3u)) << 4);
-}
+constexpr uint32_t kGradRows = 128;    // query rows per step
+constexpr uint32_t kGradItem = 512;    // query rows per item
+constexpr uint32_t kGradThreads = 256;
 
 // What a step needs to know of a query row.
 struct GradRow {
@@ -966,29 +945,64 @@ struct GradRow {
   uint32_t pair;
 };
 
-// Items of up to kGradItem rows of one span and key head, CTAs taking them in
-// turns.  Warp w owns keys 16 w .. 16 w + 15 of the span and keeps their dk and
-// dv in registers; per step of 32 rows it forms s^T = k q^T and dp^T = v
-// dout^T, from them p^T and ds^T (whose accumulator layout is the A operand of
-// the next products), adds p^T dout and ds^T q, and puts ds into shared memory,
-// from which all warps make the rows' share of dq = ds k.
-template <class T, int DP, int SPAN>
-__global__ void __launch_bounds__(SPAN * 2, DP <= 64 && SPAN == 128 ? 2 : 1)
+template <int DP>  // 64 or 128
+struct GradShape {
+  static constexpr bool kTwo = DP == 64;  // room for the next step's rows
+  static constexpr uint32_t kTile = 128u * DP * 2u;  // 128 rows: k, v, q or dout
+  static constexpr uint32_t kDs = 128u * 128u * 2u;
+  static constexpr uint32_t kRowsAt = 2u * kTile, kDsAt = kRowsAt + (kTwo ? 4u : 2u) * kTile;
+  static constexpr uint32_t kInfoAt = kDsAt + kDs;
+  // per buffer: (lse, delta) of 128 rows; which rows read block j, j < 8
+  static constexpr uint32_t kInfo = 128u * 8u + 8u * 16u;
+  static constexpr uint32_t kListAt = kInfoAt + 2u * kInfo;
+  static constexpr uint32_t kSmem = kListAt + kGradItem * sizeof(GradRow) + 1024u;
+  // tensor memory columns: s^T, dp^T (then p^T), dv, dk, and dq where it fits
+  static constexpr uint32_t kDp = 128u, kDv = 256u, kDk = 256u + DP, kDq = kTwo ? 384u : 0u;
+};
+
+// Items of up to kGradItem rows of one span of 128 keys and key head, CTAs
+// taking them in turns; dk and dv of the item stay in tensor memory.  Per step
+// of 128 rows the tensor core forms s^T = k q^T and dp^T = v dout^T (keys over
+// the lanes, rows over the columns); each thread takes one key and 64 rows, and
+// puts p^T back into tensor memory and ds^T into shared memory, rows
+// consecutive.  That tile is dk's left operand as it lies (dk += ds^T q), and
+// dq's read down its rows (dq = ds k); dv += p^T dout takes p from tensor
+// memory.  p and ds are rounded to T for these products, half a step each.
+// The products' time is hidden behind nothing but each other, about a third of
+// a step; the two thirds are the 16,384 weights of a step and the rows' loads.
+template <class T, int DP>
+__global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
-  extern __shared__ __align__(128) char smem[];
-  constexpr uint32_t kThreads = SPAN * 2, kWarps = SPAN / 16, kChunks = DP / 8;
-  constexpr uint32_t kRowTile = kGradRows * DP * 2u;
-  constexpr uint32_t kDsAt = 2u * SPAN * DP * 2u + 4u * kRowTile;
-  constexpr uint32_t kInfoAt = kDsAt + SPAN * kGradRows * 2u;
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, t = lane & 3u;
-  const uint32_t sk = smem_u32(smem), sv = sk + SPAN * DP * 2u;
-  const uint32_t sq = sv + SPAN * DP * 2u;              // [2][q, dout][32][DP]
-  const uint32_t sds = sk + kDsAt;
-  // [2]: (lse, delta) of 32 rows, their masks, their partial rows
-  const char *info = smem + kInfoAt;
-  constexpr uint32_t kInfo = 16u * kGradRows;  // bytes per buffer
-  GradRow *s_rows = reinterpret_cast<GradRow *>(smem + kInfoAt + 2u * kInfo);  // [kGradItem]
+  using Shape = GradShape<DP>;
+  constexpr uint32_t kTile = Shape::kTile, kChunks = DP / 8;
+  extern __shared__ char smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2];
+  __shared__ uint32_t s_tmem;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  char *smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sk = base, sv = base + kTile, sds = base + Shape::kDsAt;
+  GradRow *s_rows = reinterpret_cast<GradRow *>(smem + Shape::kListAt);
+  const uint32_t bar_s = smem_u32(&s_bar[0]), bar_g = smem_u32(&s_bar[1]);
+  if (warp == 0) tmem_alloc<512>(smem_u32(&s_tmem));
+  if (tid == 0) {
+    bar_init(bar_s);
+    bar_init(bar_g);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
+  const uint32_t tm = s_tmem;
+  const uint32_t quad = warp & 3u, half = warp >> 2;  // lanes 32 quad.., columns 64 half..
+  const uint32_t my = (quad * 32u) << 16;
+  const uint32_t key_in = quad * 32u + lane;          // this thread's key in the span
+  constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
+  constexpr uint32_t kRowsBy = mma_desc<T>(128, DP, false, true);  // dv, dk
+  constexpr uint32_t kDqBy = mma_desc<T>(128, DP, true, true);
   const float c2 = a.scale * kLog2e;
+  uint32_t phase = 0;  // of both barriers: each completes once per step
+  bool failed = false;
   const uint32_t work = *a.tile_count * a.gc;
   for (uint32_t item = blockIdx.x; item < work; item += gridDim.x) {
     const uint32_t gi = item % a.gc, g = a.g0 + gi, place = item / a.gc;
@@ -998,23 +1012,20 @@ attend_grad(const AttnArgs a) {
     const uint32_t row0 = tile.y * kGradItem;
     const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
     const uint32_t len = cloud_length(a.lengths, b, a.N);
-    const uint32_t key0 = sb * SPAN;
+    const uint32_t key0 = sb * 128u;
     const uint32_t steps = (rows + kGradRows - 1u) / kGradRows;
-
-    float dk[DP / 8][4], dv[DP / 8][4];
-#pragma unroll
-    for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dk[j][i] = dv[j][i] = 0.f;
-
     if (steps) {
       const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
       const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-      load_keys<DP, SPAN, kThreads>(sk, kh, a.ks[1], key0, len, a.D, tid);
-      load_keys<DP, SPAN, kThreads>(sv, vh, a.vs[1], key0, len, a.D, tid);
+      load_tile<DP, 128, kGradThreads>(sk, a.D, tid, kh, [&](uint32_t x) {
+        return key0 + x < len ? kh + (int64_t)(key0 + x) * a.ks[1] * 2 : nullptr;
+      });
+      load_tile<DP, 128, kGradThreads>(sv, a.D, tid, vh, [&](uint32_t x) {
+        return key0 + x < len ? vh + (int64_t)(key0 + x) * a.vs[1] * 2 : nullptr;
+      });
     }
     // the item's rows, once: a step's addresses are then one shared load away
-    for (uint32_t r = tid; r < rows; r += kThreads) {
+    for (uint32_t r = tid; r < rows; r += kGradThreads) {
       const uint32_t e = (row0 + r) / a.R, h = g * a.R + row0 + r - e * a.R;
       GradRow x;
       x.pair = a.vals[e0 + e];
@@ -1024,210 +1035,218 @@ attend_grad(const AttnArgs a) {
       s_rows[r] = x;
     }
     __syncthreads();
-    // Rows of step i into buffer i & 1, 16 bytes of a row per thread and turn.
+    auto rows_at = [&](uint32_t i) { return base + Shape::kRowsAt + (Shape::kTwo ? (i & 1u) : 0u) * 2u * kTile; };
+    // q and dout of step i, and what the weights need of its rows
     auto fetch = [&](uint32_t i) {
-      const uint32_t buf = i & 1u, at = sq + buf * 2u * kRowTile;
+      const uint32_t at = rows_at(i);
 #pragma unroll
-      for (uint32_t x = tid; x < kGradRows * kChunks; x += kThreads) {
-        const uint32_t r = x / kChunks, c = x % kChunks, rr = i * kGradRows + r;
+      for (uint32_t y = 0; y < 128u * kChunks / kGradThreads; ++y) {
+        const uint32_t x = tid + y * kGradThreads, r = x / kChunks, c = x % kChunks;
+        const uint32_t rr = i * kGradRows + r;
         const bool some = rr < rows && c * 8u < a.D;
         const char *qp = a.q, *op = a.dout;
         if (some) {
-          const GradRow y = s_rows[rr];
-          qp += y.q + c * 16u;
-          op += ((uint64_t)y.row * a.D + c * 8u) * 2u;
+          const GradRow z = s_rows[rr];
+          qp += z.q + c * 16u;
+          op += ((uint64_t)z.row * a.D + c * 8u) * 2u;
         }
-        copy16(at + tile_off<DP>(r, c), qp, some);
-        copy16(at + kRowTile + tile_off<DP>(r, c), op, some);
-      }
-      if (tid < kGradRows) {
-        const uint32_t rr = i * kGradRows + tid;
-        const bool some = rr < rows;
-        const uint32_t w = sk + kInfoAt + buf * kInfo;
-        const float *lp = a.lse_in, *dp = a.delta;
-        const uint32_t *mp = a.mask;
-        uint32_t prow = 0xffffffffu;
-        if (some) {
-          const GradRow y = s_rows[rr];
-          lp += y.row;
-          dp += y.row;
-          mp += y.pair;
-          prow = y.pair * (a.gc * a.R) + gi * a.R + (y.row - (y.pair / a.top) * a.H - g * a.R);
-        }
-        copy4(w + 8u * tid, lp, some);
-        copy4(w + 8u * tid + 4u, dp, some);
-        copy4(w + 8u * kGradRows + 4u * tid, mp, some);
-        reinterpret_cast<uint32_t *>(smem + kInfoAt + buf * kInfo)[3 * kGradRows + tid] = prow;
+        const uint32_t to = at + (c >> 3) * 16384u + swizzled(r, c & 7u);
+        copy16(to, qp, some);
+        copy16(to + kTile, op, some);
       }
       copy_commit();
+      if (tid < kGradRows) {
+        char *info = smem + Shape::kInfoAt + (i & 1u) * Shape::kInfo;
+        const uint32_t rr = i * kGradRows + tid;
+        float2 y = make_float2(0.f, 0.f);
+        uint32_t mask = 0;
+        if (rr < rows) {
+          const GradRow z = s_rows[rr];
+          y = make_float2(a.lse_in[z.row] * kLog2e, a.delta[z.row]);
+          mask = a.mask[z.pair];
+        }
+        reinterpret_cast<float2 *>(info)[tid] = y;
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) {
+          const uint32_t bits = __ballot_sync(kFullMask, (mask >> j) & 1u);
+          if (lane == j) reinterpret_cast<uint32_t *>(info + 1024)[j * 4u + warp] = bits;
+        }
+      }
     };
-    if (steps) fetch(0);
-    const uint32_t my_bit = (warp * 16u) >> a.block_log2, my_key = key0 + warp * 16u;
-    const bool in0 = my_key + (lane >> 2) < len, in1 = my_key + (lane >> 2) + 8u < len;
+    // (one thread) s^T and dp^T of step i
+    auto scores = [&](uint32_t i) {
+      const uint32_t q = rows_at(i), o = q + kTile;
+#pragma unroll
+      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+        const uint32_t at = (kk >> 2) * 16384u + (kk & 3u) * 32u;
+        mma_ss(tm, tile_desc(sk + at, 16u), tile_desc(q + at, 16u), kScores, kk != 0u);
+      }
+#pragma unroll
+      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+        const uint32_t at = (kk >> 2) * 16384u + (kk & 3u) * 32u;
+        mma_ss(tm + Shape::kDp, tile_desc(sv + at, 16u), tile_desc(o + at, 16u), kScores, kk != 0u);
+      }
+      mma_commit(bar_s);
+    };
+    // all threads: the loads of step i are here, its products may start
+    auto start = [&](uint32_t i) {
+      copy_wait<0>();
+      smem_to_mma();
+      tmem_before_sync();
+      __syncthreads();
+      if (tid == 0) {
+        tmem_after_sync();
+        scores(i);
+      }
+      __syncwarp();
+    };
+    if (steps) {
+      fetch(0);
+      start(0);
+    }
+    const uint32_t block = key_in >> a.block_log2;
     for (uint32_t i = 0; i < steps; ++i) {
-      const uint32_t buf = i & 1u, tq = sq + buf * 2u * kRowTile, to = tq + kRowTile;
-      const char *inf = info + buf * kInfo;
-      if (i + 1u < steps) {
-        fetch(i + 1u);
-        copy_wait<1>();
-      } else {
-        copy_wait<0>();
+      if (Shape::kTwo && i + 1u < steps) fetch(i + 1u);
+      if (!failed) failed = !bar_wait(bar_s, phase);
+      __syncwarp();
+      tmem_after_sync();
+      const char *info = smem + Shape::kInfoAt + (i & 1u) * Shape::kInfo;
+      uint32_t s[2][32], d[2][32];
+      tmem_ld32(s[0], tm + my + half * 64u);
+      tmem_ld32(s[1], tm + my + half * 64u + 32u);
+      tmem_ld32(d[0], tm + Shape::kDp + my + half * 64u);
+      tmem_ld32(d[1], tm + Shape::kDp + my + half * 64u + 32u);
+      // which of the 64 rows read this key
+      uint2 bits = reinterpret_cast<const uint2 *>(info + 1024)[block * 2u + half];
+      if (key0 + key_in >= len) bits = make_uint2(0u, 0u);
+      tmem_ld_wait();
+      const bool full = __all_sync(kFullMask, (bits.x & bits.y) == kFullMask);
+#pragma unroll
+      for (uint32_t x = 0; x < 2u; ++x) {
+        const uint32_t in = x ? bits.y : bits.x;
+        const bool some = __any_sync(kFullMask, in != 0u);
+#pragma unroll
+        for (uint32_t y = 0; y < 32u; y += 2u) {
+          // (lse, delta) of two rows
+          const float4 z = reinterpret_cast<const float4 *>(info)[half * 32u + x * 16u + y / 2u];
+          float p0 = 0.f, p1 = 0.f;
+          if (some) {
+            p0 = exp2_fast(fmaf(__uint_as_float(s[x][y]), c2, -z.x));
+            p1 = exp2_fast(fmaf(__uint_as_float(s[x][y + 1]), c2, -z.z));
+            if (!full) {
+              p0 = (in >> y) & 1u ? p0 : 0.f;
+              p1 = (in >> (y + 1u)) & 1u ? p1 : 0.f;
+            }
+          }
+          const float d0 = p0 * (__uint_as_float(d[x][y]) - z.y);
+          const float d1 = p1 * (__uint_as_float(d[x][y + 1]) - z.w);
+          s[0][x * 16u + y / 2u] = pack2<T>(p0, p1);
+          d[0][x * 16u + y / 2u] = pack2<T>(d0, d1);
+        }
       }
+      // (over this thread's own dp: the other half's may not be read yet)
+      tmem_st32(tm + Shape::kDp + my + half * 64u, s[0]);
+#pragma unroll
+      for (uint32_t c = 0; c < 8u; ++c)
+        *reinterpret_cast<uint4 *>(smem + Shape::kDsAt + half * 16384u + swizzled(key_in, c)) =
+            make_uint4(d[0][4 * c], d[0][4 * c + 1], d[0][4 * c + 2], d[0][4 * c + 3]);
+      tmem_st_wait();
+      smem_to_mma();
+      tmem_before_sync();
       __syncthreads();
-      const uint32_t mask = reinterpret_cast<const uint32_t *>(inf)[2 * kGradRows + lane];
-      const uint32_t any = __reduce_or_sync(kFullMask, mask);
-      const uint32_t mine = __ballot_sync(kFullMask, (mask >> my_bit) & 1u);  // rows reading my keys
-      if (mine && my_key < len) {
-        float s[4][4], dp[4][4];
+      if (tid == 0) {
+        tmem_after_sync();
+        const uint32_t q = rows_at(i), o = q + kTile;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (uint32_t kk = 0; kk < 8u; ++kk)
+          mma_ts(tm + Shape::kDv, tm + Shape::kDp + (kk >> 2) * 64u + (kk & 3u) * 8u,
+                 tile_desc(o + kk * 2048u, 16384u), kRowsBy, i != 0u || kk != 0u);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[n][x] = dp[n][x] = 0.f;
+        for (uint32_t kk = 0; kk < 8u; ++kk)
+          mma_ss(tm + Shape::kDk, tile_desc(sds + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
+                 tile_desc(q + kk * 2048u, 16384u), kRowsBy, i != 0u || kk != 0u);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          uint32_t ka[4], va[4];
-          const uint32_t ao = tile_off<DP>(warp * 16u + (lane & 15u), kk * 2 + (lane >> 4));
-          ldsm4(ka, sk + ao);
-          ldsm4(va, sv + ao);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            uint32_t x[4];
-            const uint32_t bo = tile_off<DP>(n * 16 + (lane & 7u) + ((lane >> 4) << 3),
-                                             kk * 2 + ((lane >> 3) & 1u));
-            ldsm4(x, tq + bo);
-            mma16816<T>(s[2 * n], ka, x[0], x[1]);
-            mma16816<T>(s[2 * n + 1], ka, x[2], x[3]);
-            ldsm4(x, to + bo);
-            mma16816<T>(dp[2 * n], va, x[0], x[1]);
-            mma16816<T>(dp[2 * n + 1], va, x[2], x[3]);
-          }
-        }
-        uint32_t pa[2][4], da[2][4];
-        // p = exp(scale s - lse) and ds = p (dp - delta) of row pair n * 8 + 2 t
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float4 y = reinterpret_cast<const float4 *>(inf)[n * 4 + t];  // two rows
-          const float l0 = y.x * kLog2e, l1 = y.z * kLog2e;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[n][x] = exp2_fast(fmaf(s[n][x], c2, x & 1 ? -l1 : -l0));
-            dp[n][x] -= x & 1 ? y.w : y.y;
-          }
-        }
-        if (mine != kFullMask || my_key + 16u > len) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const uint32_t two = mine >> (n * 8 + 2 * t);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              s[n][x] = ((two >> (x & 1)) & 1u) && (x < 2 ? in0 : in1) ? s[n][x] : 0.f;
-          }
-        }
-        char *ds = smem + kDsAt;
-        const uint32_t kr = warp * 16u + (lane >> 2);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float *p = s[n], *e = dp[n];
-          pa[n >> 1][(n & 1) * 2] = pack2<T>(p[0], p[1]);
-          pa[n >> 1][(n & 1) * 2 + 1] = pack2<T>(p[2], p[3]);
-          const uint32_t d0 = pack2<T>(p[0] * e[0], p[1] * e[1]);
-          const uint32_t d1 = pack2<T>(p[2] * e[2], p[3] * e[3]);
-          da[n >> 1][(n & 1) * 2] = d0;
-          da[n >> 1][(n & 1) * 2 + 1] = d1;
-          *reinterpret_cast<uint32_t *>(ds + ds_off(kr, n) + 4u * t) = d0;
-          *reinterpret_cast<uint32_t *>(ds + ds_off(kr + 8u, n) + 4u * t) = d1;
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int jj = 0; jj < DP / 16; ++jj) {
-            uint32_t x[4];
-            const uint32_t bo = tile_off<DP>(kk * 16 + (lane & 15u), jj * 2 + (lane >> 4));
-            ldsm4t(x, to + bo);
-            mma16816<T>(dv[2 * jj], pa[kk], x[0], x[1]);
-            mma16816<T>(dv[2 * jj + 1], pa[kk], x[2], x[3]);
-            ldsm4t(x, tq + bo);
-            mma16816<T>(dk[2 * jj], da[kk], x[0], x[1]);
-            mma16816<T>(dk[2 * jj + 1], da[kk], x[2], x[3]);
-          }
+        for (uint32_t kk = 0; kk < 8u; ++kk)
+          mma_ss(tm + Shape::kDq, tile_desc(sds + kk * 2048u, 16384u),
+                 tile_desc(sk + kk * 2048u, 16384u), kDqBy, kk != 0u);
+        mma_commit(bar_g);
       }
-      __syncthreads();
-      // dq of the 32 rows: kUnits tiles of 16 rows x 8 kPer columns
-      constexpr uint32_t kPer = (2 * kChunks) / kWarps > 0 ? (2 * kChunks) / kWarps : 1;
-      constexpr uint32_t kUnits = 2 * kChunks / kPer;
-      if (warp < kUnits) {
-        const uint32_t rt = warp & 1u, j0 = (warp >> 1) * kPer;
-        float acc[kPer][4];
+      __syncwarp();
+      if (!failed) failed = !bar_wait(bar_g, phase);
+      __syncwarp();
+      tmem_after_sync();
+      phase ^= 1u;
+      // the next step's scores go before this step's dq is written out
+      if (Shape::kTwo && i + 1u < steps) start(i + 1u);
+      if (!Shape::kTwo && i + 1u < steps) fetch(i + 1u);
+      {
+        const uint32_t rr = i * kGradRows + key_in;  // lanes are rows here
+        const bool some = rr < rows;
+        uint64_t to = 0;
+        if (some) {
+          const GradRow z = s_rows[rr];
+          const uint32_t hh = z.row - (z.pair / a.top) * a.H - g * a.R;
+          to = ((uint64_t)z.pair * (a.gc * a.R) + gi * a.R + hh) * a.D;
+        }
 #pragma unroll
-        for (uint32_t j = 0; j < kPer; ++j)
+        for (uint32_t j = 0; j < DP / 64; ++j) {
+          uint32_t o[32];
+          const uint32_t col = half * (DP / 2) + j * 32u;
+          tmem_ld32(o, tm + Shape::kDq + my + col);
+          tmem_ld_wait();
+          if (some)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
+            for (uint32_t y = 0; y < 32u; y += 8u)
+              if (col + y < a.D) store8(a.part + to + col + y, &o[y], failed ? NAN : 1.f);
+          __syncwarp();
+        }
+      }
+      if (!Shape::kTwo && i + 1u < steps) start(i + 1u);
+    }
+    // the span's dk and dv, or this item's share of them: one key per lane,
+    // dv by the first four warps, dk by the others
+    if (steps) {
+      const bool some = key0 + key_in < a.N, whole = all_rows <= kGradItem;
+      const float f = (half && whole ? a.scale : 1.f) * (failed ? NAN : 1.f);
+      char *out = (half ? a.dk : a.dv) +
+                  2 * ((((uint64_t)b * a.N + key0 + key_in) * a.G + g) * a.D);
+      float *share = a.part_kv +
+                     ((((uint64_t)place * a.gc + gi) * 2 + (half ? 0u : 1u)) * 128u + key_in) * a.D;
 #pragma unroll
-        for (uint32_t ks = 0; ks < kWarps; ++ks) {
-          if (!((any >> ((ks * 16u) >> a.block_log2)) & 1u) || key0 + ks * 16u >= len) continue;
-          uint32_t x[4];
-          ldsm4t(x, sds + ds_off(ks * 16u + (lane & 7u) + ((lane >> 4) << 3),
-                                 rt * 2u + ((lane >> 3) & 1u)));
-          if constexpr (kPer == 1) {
-            uint32_t y[2];
-            ldsm2t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0));
-            mma16816<T>(acc[0], x, y[0], y[1]);
-          } else {
+      for (uint32_t j = 0; j < DP / 32; ++j) {
+        uint32_t o[32];
+        tmem_ld32(o, tm + (half ? Shape::kDk : Shape::kDv) + my + j * 32u);
+        tmem_ld_wait();
+        if (some) {
 #pragma unroll
-            for (uint32_t j = 0; j < kPer / 2; ++j) {
-              uint32_t y[4];
-              ldsm4t(y, sk + tile_off<DP>(ks * 16u + (lane & 15u), j0 + 2 * j + (lane >> 4)));
-              mma16816<T>(acc[2 * j], x, y[0], y[1]);
-              mma16816<T>(acc[2 * j + 1], x, y[2], y[3]);
+          for (uint32_t y = 0; y < 32u; y += 8u) {
+            if (j * 32u + y >= a.D) continue;
+            if (whole) {
+              uint32_t h[4];
+#pragma unroll
+              for (uint32_t z = 0; z < 4u; ++z)
+                h[z] = pack2<T>(__uint_as_float(o[y + 2 * z]) * f,
+                                __uint_as_float(o[y + 2 * z + 1]) * f);
+              *reinterpret_cast<uint4 *>(out + 2u * (j * 32u + y)) =
+                  make_uint4(h[0], h[1], h[2], h[3]);
+            } else {
+              store8(share + j * 32u + y, &o[y], f);
             }
           }
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t prow = reinterpret_cast<const uint32_t *>(
-              inf)[3 * kGradRows + rt * 16u + (lane >> 2) + 8u * h];
-          if (prow == 0xffffffffu) continue;
-          float *o = a.part + (uint64_t)prow * a.D;
-#pragma unroll
-          for (uint32_t j = 0; j < kPer; ++j)
-            if ((j0 + j) * 8u < a.D)
-              *reinterpret_cast<float2 *>(o + (j0 + j) * 8u + 2u * t) =
-                  make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-        }
+        __syncwarp();
       }
-      __syncthreads();
+    } else if (key0 + key_in < a.N) {  // a span that nobody reads
+      char *out = (half ? a.dk : a.dv) +
+                  2 * ((((uint64_t)b * a.N + key0 + key_in) * a.G + g) * a.D);
+      for (uint32_t j = 0; j < a.D; j += 8u)
+        *reinterpret_cast<uint4 *>(out + 2u * j) = make_uint4(0u, 0u, 0u, 0u);
     }
-    // the span's dk and dv, or this item's share of them
-    const bool whole = all_rows <= kGradItem;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t r = warp * 16u + (lane >> 2) + 8u * h;
-      if (key0 + r >= a.N) continue;
-      if (whole) {
-        const uint64_t row = ((uint64_t)b * a.N + key0 + r) * a.G + g;
-#pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
-          if (j * 8u < a.D) {
-            const uint64_t o = 2 * (row * a.D + j * 8 + 2 * t);
-            *reinterpret_cast<uint32_t *>(a.dk + o) =
-                pack2<T>(dk[j][2 * h] * a.scale, dk[j][2 * h + 1] * a.scale);
-            *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(dv[j][2 * h], dv[j][2 * h + 1]);
-          }
-      } else {
-        float *o = a.part_kv + (((uint64_t)place * a.gc + gi) * 2 * SPAN + r) * a.D;
-#pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
-          if (j * 8u < a.D) {
-            *reinterpret_cast<float2 *>(o + j * 8 + 2 * t) =
-                make_float2(dk[j][2 * h], dk[j][2 * h + 1]);
-            *reinterpret_cast<float2 *>(o + (uint64_t)SPAN * a.D + j * 8 + 2 * t) =
-                make_float2(dv[j][2 * h], dv[j][2 * h + 1]);
-          }
-      }
-    }
-    // (the last step's barrier, or none of the shared tiles used: the next
-    // item may load)
+    tmem_before_sync();
+    __syncthreads();  // the tiles, the rows and dk, dv are free for the next item
+    tmem_after_sync();
   }
+  if (warp == 0) tmem_free<512>(tm);
 }
 
 // dk and dv of the spans that several items share, their shares in order.
@@ -1322,9 +1341,8 @@ uint32_t log2_of(uint32_t block) { return block == 16 ? 4 : block == 32 ? 5 : bl
 
 int padded_dim(uint32_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// Keys per span of the gradient: as many as the warps' dk and dv fit in
-// registers for.
-constexpr uint32_t kGradSpanLog2 = 7;
+// Keys per span of the gradient.
+constexpr uint32_t kGradSpanLog2 = 7;  // one key per lane of tensor memory
 
 // Partials of a pass stay below this, by taking the key heads, then the clouds
 // of a call, in turns.
@@ -1516,12 +1534,12 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
   return cudaSuccess;
 }
 
-template <class T, int DP, int SPAN>
+template <class T, int DP>
 cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
   cudaError_t err;
-  const uint32_t smem = grad_smem<DP, SPAN>();
-  if ((err = opt_in(attend_grad<T, DP, SPAN>, smem))) return err;
-  const uint64_t resident = (uint64_t)sm_count() * (DP <= 64 && SPAN == 128 ? 2 : 1);
+  const uint32_t smem = GradShape<DP>::kSmem;
+  if ((err = opt_in(attend_grad<T, DP>, smem))) return err;
+  const uint64_t resident = (uint64_t)sm_count();
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
     const uint64_t nq = (uint64_t)a.B * a.M;
@@ -1535,10 +1553,11 @@ cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
       if (tiles)
-        attend_grad<T, DP, SPAN><<<(uint32_t)std::min(tiles * a.gc, resident), SPAN * 2, smem, st>>>(a);
+        attend_grad<T, DP><<<(uint32_t)std::min(tiles * a.gc, resident), kGradThreads, smem, st>>>(
+            a);
       if ((err = cudaGetLastError())) return err;
       if (nq * a.top * a.R > w.tile_rows && spans) {
-        grad_join_keys<T><<<dim3(spans, a.gc, 4), 256, 0, st>>>(a, SPAN);
+        grad_join_keys<T><<<dim3(spans, a.gc, 4), 256, 0, st>>>(a, 1u << kGradSpanLog2);
         if ((err = cudaGetLastError())) return err;
       }
       if (nq) {
@@ -1563,9 +1582,9 @@ cudaError_t forward_of(const AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
 template <class T>
 cudaError_t backward_of(const AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   switch (padded_dim(a.D)) {
-    case 32: return launch_backward<T, 32, 128>(a, w, st);
-    case 64: return launch_backward<T, 64, 128>(a, w, st);
-    default: return launch_backward<T, 128, 128>(a, w, st);
+    case 32:
+    case 64: return launch_backward<T, 64>(a, w, st);
+    default: return launch_backward<T, 128>(a, w, st);
   }
 }
 
