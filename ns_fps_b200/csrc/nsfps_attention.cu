@@ -134,6 +134,31 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two at once: one instruction each.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;"
+      : "=f"(d)
+      : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
@@ -585,38 +610,45 @@ attend_tiles(const AttnArgs a) {
         if (!((warp_any >> bit(x)) & 1u)) continue;
         uint32_t *v = &s[x >> 1][(x & 1u) * 16u];
         const uint32_t key = key0 + c * 64u + x * 16u;
-        if (!((warp_all >> bit(x)) & 1u) || key + 16u > len) {
-          const uint32_t n = (mask >> bit(x)) & 1u && key < len ? len - key : 0u;
-#pragma unroll
-          for (uint32_t y = 0; y < 16u; ++y)
-            v[y] = y < n ? __float_as_uint(__uint_as_float(v[y]) * sign) : 0xff800000u;
-        } else if (sign != 1.f) {
+        if (sign != 1.f) {
 #pragma unroll
           for (uint32_t y = 0; y < 16u; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * sign);
         }
+        if (!((warp_all >> bit(x)) & 1u) || key + 16u > len) {
+          const uint32_t n = (mask >> bit(x)) & 1u && key < len ? len - key : 0u;
 #pragma unroll
-        for (uint32_t y = 0; y < 16u; ++y) mx = fmaxf(mx, __uint_as_float(v[y]));
+          for (uint32_t y = 0; y < 16u; ++y) v[y] = y < n ? v[y] : 0xff800000u;
+        }
+        // a tree: a chain of maxima would wait for each
+        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
+        float m2 = max3(v[6], v[7], v[8]), m3 = max3(v[9], v[10], v[11]);
+        m0 = fmaxf(m0, max3(v[12], v[13], v[14]));
+        m1 = fmaxf(m1, __uint_as_float(v[15]));
+        mx = fmaxf(mx, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
       }
-      // (no key yet: the reference stays -inf and the weights come out 0)
-      const bool grow = mx * c2 > ref * c2 + kLazy || (ref == -INFINITY && mx != -INFINITY);
+      // A row whose first keys these are has nothing to rescale; without a key
+      // the reference stays -inf and the weights come out 0.
+      const bool grow = mx * c2 > ref * c2 + kLazy;
       const float next = grow ? mx : ref;
       const float base = next == -INFINITY ? 0.f : next * c2;
-      if (i && __any_sync(kFullMask, grow)) {
-        const float f = exp2_fast(fmaf(ref, c2, -base));  // 0 while ref is -inf
+      if (__any_sync(kFullMask, grow && ref != -INFINITY)) {
+        const float f = ref == -INFINITY ? 0.f : exp2_fast(fmaf(ref, c2, -base));
         sum *= f;
-#pragma unroll
-        for (uint32_t j = 0; j < DP / 32; ++j) {
-          uint32_t o[32];
-          tmem_ld32(o, tm_o + my + j * 32u);
+#pragma unroll 1
+        for (uint32_t j = 0; j < DP / 16; ++j) {
+          uint32_t o[16];
+          tmem_ld16(o, tm_o + my + j * 16u);
           tmem_ld_wait();
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-          tmem_st32(tm_o + my + j * 32u, o);
+          for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+          tmem_st16(tm_o + my + j * 16u, o);
         }
       }
       ref = next;
       // weights, rounded to T for the product with v: half a step of T each,
       // like the output's own rounding
+      float2 part[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+      const float2 scale2 = make_float2(c2, c2), base2 = make_float2(-base, -base);
 #pragma unroll
       for (uint32_t x = 0; x < 4u; ++x) {
         const uint32_t *v = &s[x >> 1][(x & 1u) * 16u];
@@ -624,16 +656,20 @@ attend_tiles(const AttnArgs a) {
         if ((warp_any >> bit(x)) & 1u) {
 #pragma unroll
           for (uint32_t y = 0; y < 16u; y += 2) {
-            const float f0 = exp2_fast(fmaf(__uint_as_float(v[y]), c2, -base));
-            const float f1 = exp2_fast(fmaf(__uint_as_float(v[y + 1]), c2, -base));
-            sum += f0 + f1;
-            p[y / 2u] = pack2<T>(f0, f1);
+            float2 f = fma2(make_float2(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), scale2,
+                            base2);
+            f.x = exp2_fast(f.x);
+            f.y = exp2_fast(f.y);
+            part[(y / 2u) & 3u] = add2(part[(y / 2u) & 3u], f);
+            p[y / 2u] = pack2<T>(f.x, f.y);
           }
         } else {
 #pragma unroll
           for (uint32_t y = 0; y < 8u; ++y) p[y] = 0u;
         }
       }
+      part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+      sum += part[0].x + part[0].y;
       tmem_st32(tm_s + my, s[0]);
       tmem_st_wait();
       tmem_before_sync();

@@ -88,7 +88,6 @@ __device__ __forceinline__ void smem_to_mma() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-#define NSFPS_R8(a, i) a[i], a[i + 1], a[i + 2], a[i + 3], a[i + 4], a[i + 5], a[i + 6], a[i + 7]
 #define NSFPS_OUT8(a, i)                                                                    \
   "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), \
       "=r"(a[i + 6]), "=r"(a[i + 7])
@@ -110,6 +109,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
       "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
       ::"r"(addr), NSFPS_IN8(r, 0), NSFPS_IN8(r, 8), NSFPS_IN8(r, 16), NSFPS_IN8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : NSFPS_OUT8(r, 0), NSFPS_OUT8(r, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16};" ::"r"(addr), NSFPS_IN8(r, 0), NSFPS_IN8(r, 8)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() {
