@@ -465,15 +465,35 @@ struct TileShape {
 // ROWS rows of DP elements into shared tiles of 64 columns each; src(r) gives
 // the row (null: zeros).
 template <int DP, uint32_t ROWS, uint32_t THREADS, class Src>
-__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t D, uint32_t tid, const char *any,
-                                          Src src) {
-  constexpr uint32_t kChunks = DP / 8;
+__device__ __forceinline__ void load_rows_by(uint32_t dst, uint32_t D, uint32_t tid,
+                                             const char *any, Src src) {
+  constexpr uint32_t kChunks = DP / 8, kStep = THREADS / kChunks;
+  const uint32_t c = tid % kChunks, r0 = tid / kChunks;
+  const uint32_t at = dst + (c >> 3) * (ROWS * 128u) + swizzled(r0, c & 7u);
+  const bool in = c * 8u < D;
 #pragma unroll
-  for (uint32_t i = 0; i < ROWS * kChunks / THREADS; ++i) {
-    const uint32_t x = tid + i * THREADS, r = x / kChunks, c = x % kChunks;
-    const char *p = src(r);
-    const bool some = p && c * 8u < D;
-    copy16(dst + (c >> 3) * (ROWS * 128u) + swizzled(r, c & 7u), some ? p + c * 16u : any, some);
+  for (uint32_t i = 0; i < ROWS / kStep; ++i) {  // (kStep is a multiple of 8 rows)
+    const char *p = src(r0 + i * kStep);
+    const bool some = p && in;
+    copy16(at + i * kStep * 128u, some ? p + c * 16u : any, some);
+  }
+}
+
+// The same for rows `stride` bytes apart, the first `live` of them; zeros
+// behind.
+template <int DP, uint32_t ROWS, uint32_t THREADS>
+__device__ __forceinline__ void load_strided(uint32_t dst, uint32_t D, uint32_t tid,
+                                             const char *first, int64_t stride, uint32_t live) {
+  constexpr uint32_t kChunks = DP / 8, kStep = THREADS / kChunks;
+  const uint32_t c = tid % kChunks, r0 = tid / kChunks;
+  const uint32_t at = dst + (c >> 3) * (ROWS * 128u) + swizzled(r0, c & 7u);
+  const char *p = first + (int64_t)r0 * stride + c * 16u;
+  const bool in = c * 8u < D;
+#pragma unroll
+  for (uint32_t i = 0; i < ROWS / kStep; ++i) {
+    const bool some = in && r0 + i * kStep < live;
+    copy16(at + i * kStep * 128u, some ? p : first, some);
+    p += (int64_t)kStep * stride;
   }
 }
 
@@ -518,28 +538,49 @@ attend_tiles(const AttnArgs a) {
   uint32_t phase = 0;     // of both barriers: each completes once per chunk
   bool failed = false;
   const uint32_t work = *a.tile_count * a.gc;
-  for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
+  // What this thread's row of a tile is: asked for one tile ahead, the tile
+  // itself two, as each waits for the one before.
+  struct Row {
+    uint32_t pair, head, read;
+    bool live;
+  };
+  auto row_of = [&](const uint4 &tile) {
+    Row x{0xffffffffu, 0u, 0u, false};
+    const uint32_t r = tile.y * kTileRows + tid;
+    x.live = r < tile.w * a.R;
+    if (x.live) {
+      const uint32_t e = r / a.R;
+      x.head = r - e * a.R;
+      x.pair = a.vals[tile.z + e];
+      x.read = a.skeys[tile.z + e];
+    }
+    return x;
+  };
+  const uint32_t step = gridDim.x;
+  uint4 tile = make_uint4(0u, 0u, 0u, 0u), tile_next = tile;
+  if (blockIdx.x < work) tile = a.tiles[blockIdx.x / a.gc];
+  if (blockIdx.x + step < work) tile_next = a.tiles[(blockIdx.x + step) / a.gc];
+  Row mine = row_of(tile);
+  for (uint32_t w = blockIdx.x; w < work; w += step) {
     const uint32_t gi = w % a.gc, g = a.g0 + gi;
-    const uint4 tile = a.tiles[w / a.gc];
     const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
-    const uint32_t e0 = tile.z, rows = tile.w * a.R;
     const uint32_t len = cloud_length(a.lengths, b, a.N);
     const uint32_t key0 = sb << kSpanLog2;
     // this thread's row, and the chunks that any row reads
-    const uint32_t r = tile.y * kTileRows + tid;
-    uint32_t pair = 0xffffffffu, mask = 0u, read = 0u, head = 0u;
+    const uint32_t pair = mine.pair, head = mine.head;
+    const bool live_row = mine.live;
+    uint32_t read = mine.read & ((1u << kChunkBits) - 1u), mask = 0u;
+    read ^= read >> 1;  // from the place in the Gray code
     const char *q = nullptr;
-    if (r < rows) {
-      const uint32_t e = r / a.R;
-      head = r - e * a.R;
-      pair = a.vals[e0 + e];
-      read = a.skeys[e0 + e] & ((1u << kChunkBits) - 1u);
-      read ^= read >> 1;  // from the place in the Gray code
+    if (live_row) {
       mask = a.mask[pair];
       const uint32_t m = pair / a.top - b * a.M;
       q = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
                      (int64_t)(g * a.R + head) * a.qs[2]);
     }
+    tile = tile_next;
+    mine = row_of(tile);
+    if (w + 2u * step < work) tile_next = a.tiles[(w + 2u * step) / a.gc];
     const uint32_t warp_read = __reduce_or_sync(kFullMask, read);
     if (lane == 0) s_any[warp] = warp_read;
     s_q[tid] = q;
@@ -549,18 +590,19 @@ attend_tiles(const AttnArgs a) {
     const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
     auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
       if (some) {
-        const uint32_t key = key0 + c * 64u;
-        load_tile<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid, kh, [&](uint32_t x) {
-          return key + x < len ? kh + (int64_t)(key + x) * a.ks[1] * 2 : nullptr;
-        });
-        load_tile<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid, vh, [&](uint32_t x) {
-          return key + x < len ? vh + (int64_t)(key + x) * a.vs[1] * 2 : nullptr;
-        });
+        const uint32_t key = key0 + c * 64u, live = key < len ? len - key : 0u;
+        const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
+        // (a chunk wholly behind the end reads nothing, but its address is formed)
+        load_strided<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid,
+                                           kh + (live ? (int64_t)key * ks : 0), ks, live);
+        load_strided<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid,
+                                           vh + (live ? (int64_t)key * vs : 0), vs, live);
       }
       copy_commit();
     };
     uint32_t ahead = todo;
-    load_tile<DP, kTileRows, kTileThreads>(sq, a.D, tid, a.q, [&](uint32_t x) { return s_q[x]; });
+    load_rows_by<DP, kTileRows, kTileThreads>(sq, a.D, tid, a.q,
+                                              [&](uint32_t x) { return s_q[x]; });
 #pragma unroll
     for (uint32_t i = 0; i < 2u; ++i) {  // (q goes with the first chunk)
       fetch(__ffs(ahead) - 1, i, ahead != 0);
@@ -695,13 +737,13 @@ attend_tiles(const AttnArgs a) {
       uint32_t o[32];
       tmem_ld32(o, tm_o + my + j * 32u);
       tmem_ld_wait();
-      if (r < rows)
+      if (live_row)
 #pragma unroll
         for (uint32_t y = 0; y < 32u; y += 8u)
           if (j * 32u + y < a.D) store8(a.part + row * a.D + j * 32u + y, &o[y], inv);
       __syncwarp();
     }
-    if (r < rows)  // (a wait that ran out shows as NaN)
+    if (live_row)  // (a wait that ran out shows as NaN)
       a.part_lse[row] = failed ? __int_as_float(0x7fc00000)
                         : sum > 0.f ? fmaf(ref, c2, log2f(sum)) : -INFINITY;
     tmem_before_sync();
@@ -1053,12 +1095,10 @@ attend_grad(const AttnArgs a) {
     if (steps) {
       const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
       const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-      load_tile<DP, 128, kGradThreads>(sk, a.D, tid, kh, [&](uint32_t x) {
-        return key0 + x < len ? kh + (int64_t)(key0 + x) * a.ks[1] * 2 : nullptr;
-      });
-      load_tile<DP, 128, kGradThreads>(sv, a.D, tid, vh, [&](uint32_t x) {
-        return key0 + x < len ? vh + (int64_t)(key0 + x) * a.vs[1] * 2 : nullptr;
-      });
+      // (a span with rows has a key below the cloud's end)
+      const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
+      load_strided<DP, 128, kGradThreads>(sk, a.D, tid, kh + (int64_t)key0 * ks, ks, len - key0);
+      load_strided<DP, 128, kGradThreads>(sv, a.D, tid, vh + (int64_t)key0 * vs, vs, len - key0);
     }
     // the item's rows, once: a step's addresses are then one shared load away
     for (uint32_t r = tid; r < rows; r += kGradThreads) {
