@@ -151,6 +151,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;"
@@ -1012,316 +1020,492 @@ grad_delta(const AttnArgs a) {
   if (sub == 0 && row < (uint64_t)a.B * a.M * a.H) a.delta[row] = s;
 }
 
-constexpr uint32_t kGradRows = 128;    // query rows per step
 constexpr uint32_t kGradItem = 512;    // query rows per item
-constexpr uint32_t kGradThreads = 256;
-
-// What a step needs to know of a query row.
-struct GradRow {
-  int64_t q;      // byte offset of the row of q
-  uint32_t row;   // (query, head) over the turn
-  uint32_t pair;
-};
+constexpr uint32_t kGradThreads = 512;
 
 template <int DP>  // 64 or 128
 struct GradShape {
-  static constexpr bool kTwo = DP == 64;  // room for the next step's rows
-  static constexpr uint32_t kTile = 128u * DP * 2u;  // 128 rows: k, v, q or dout
-  static constexpr uint32_t kDs = 128u * 128u * 2u;
-  static constexpr uint32_t kRowsAt = 2u * kTile, kDsAt = kRowsAt + (kTwo ? 4u : 2u) * kTile;
-  static constexpr uint32_t kInfoAt = kDsAt + kDs;
-  // per buffer: (lse, delta) of 128 rows; which rows read block j, j < 8
-  static constexpr uint32_t kInfo = 128u * 8u + 8u * 16u;
-  static constexpr uint32_t kListAt = kInfoAt + 2u * kInfo;
-  static constexpr uint32_t kSmem = kListAt + kGradItem * sizeof(GradRow) + 1024u;
-  // tensor memory columns: s^T, dp^T (then p^T), dv, dk, and dq where it fits
-  static constexpr uint32_t kDp = 128u, kDv = 256u, kDk = 256u + DP, kDq = kTwo ? 384u : 0u;
+  static constexpr uint32_t kRows = DP == 64 ? 128u : 64u;  // query rows per step
+  static constexpr uint32_t kStages = 3;                    // steps' rows in shared memory
+  static constexpr uint32_t kKv = DP == 64 ? 2u : 1u;       // items' keys in shared memory
+  static constexpr uint32_t kKeyTile = 128u * DP * 2u, kRowTile = kRows * DP * 2u;
+  static constexpr uint32_t kStage = 2u * kRowTile;         // q, dout
+  static constexpr uint32_t kRowsAt = kKv * 2u * kKeyTile, kDsAt = kRowsAt + kStages * kStage;
+  static constexpr uint32_t kInfoAt = kDsAt + 128u * kRows * 2u;
+  // per stage: (lse, delta) of the rows; which rows read block j, j < 8; the
+  // rows' places among the partials
+  static constexpr uint32_t kBitsAt = 1024u, kPlaceAt = 1152u, kInfo = 1664u;
+  // per stage, for the loads: where the rows of q and dout begin
+  static constexpr uint32_t kFromAt = kInfoAt + kStages * kInfo, kFrom = kRows * 16u;
+  static constexpr uint32_t kSmem = kFromAt + kStages * kFrom + 1024u;
+  // tensor memory columns: s^T, dp^T, dv, dk, dq, p^T
+  static constexpr uint32_t kDp = kRows, kDv = 2u * kRows, kDk = kDv + DP, kDq = 384u, kP = 448u;
+};
+
+// What the roles of the gradient kernel know of an item.
+struct GradItem {
+  uint32_t gi, g, place, b, key0, len, e0, row0, rows, all_rows, steps;
 };
 
 // Items of up to kGradItem rows of one span of 128 keys and key head, CTAs
 // taking them in turns; dk and dv of the item stay in tensor memory.  Per step
-// of 128 rows the tensor core forms s^T = k q^T and dp^T = v dout^T (keys over
-// the lanes, rows over the columns); each thread takes one key and 64 rows, and
+// of rows the tensor core forms s^T = k q^T and dp^T = v dout^T (keys over the
+// lanes, rows over the columns); a thread takes one key and half the rows, and
 // puts p^T back into tensor memory and ds^T into shared memory, rows
-// consecutive.  That tile is dk's left operand as it lies (dk += ds^T q), and
-// dq's read down its rows (dq = ds k); dv += p^T dout takes p from tensor
-// memory.  p and ds are rounded to T for these products, half a step each.
-// The products' time is hidden behind nothing but each other, about a third of
-// a step; the two thirds are the 16,384 weights of a step and the rows' loads.
+// consecutive.  That tile is dk's left operand as it lies (dk += ds^T q) and
+// an operand of dq read down its rows (dq = ds k, or with heads of 128
+// elements dq^T = k^T ds^T, so that 64 rows a step suffice); dv += p^T dout
+// takes p from tensor memory.  p and ds are rounded to T for these products,
+// half a step each.
+//
+// Done in turns by all warps, the stages of a step took 11,000 cycles, of
+// which the weights were 2,500.  So the warps have roles and meet at barriers:
+// eight make weights, three load a step's rows each (the loads of three steps
+// are in the air), four take dq, dk and dv out, and one thread issues the
+// products, the next step's scores before this step's gradients.
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
   using Shape = GradShape<DP>;
-  constexpr uint32_t kTile = Shape::kTile, kChunks = DP / 8;
+  constexpr uint32_t kRows = Shape::kRows, kStages = Shape::kStages, kChunks = DP / 8;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2];
+  __shared__ __align__(8) uint64_t s_bar[kStages * 2 + 4 + 6];
   __shared__ uint32_t s_tmem;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char *smem = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sk = base, sv = base + kTile, sds = base + Shape::kDsAt;
-  GradRow *s_rows = reinterpret_cast<GradRow *>(smem + Shape::kListAt);
-  const uint32_t bar_s = smem_u32(&s_bar[0]), bar_g = smem_u32(&s_bar[1]);
+  const uint32_t bars = smem_u32(s_bar);
+  auto full = [&](uint32_t st) { return bars + 8u * st; };                // rows loaded
+  auto empty = [&](uint32_t st) { return bars + 8u * (kStages + st); };   // and used up
+  // (of item k; in turns even where there is one buffer, as a loader may be
+  // three steps ahead and must not take one phase for another)
+  auto kv_full = [&](uint32_t k) { return bars + 8u * (2 * kStages + (k & 1u)); };
+  auto kv_empty = [&](uint32_t k) { return bars + 8u * (2 * kStages + 2 + (k & 1u)); };
+  constexpr uint32_t kRest = 8u * (2 * kStages + 4);
+  const uint32_t s_ready = bars + kRest, s_free = s_ready + 8u;   // scores made, taken out
+  const uint32_t p_ready = s_free + 8u, g_done = p_ready + 8u;    // weights there; products done
+  const uint32_t dq_free = g_done + 8u, acc_free = dq_free + 8u;  // dq, dk and dv taken out
   if (warp == 0) tmem_alloc<512>(smem_u32(&s_tmem));
   if (tid == 0) {
-    bar_init(bar_s);
-    bar_init(bar_g);
+    for (uint32_t i = 0; i < kStages; ++i) {
+      bar_init(full(i));
+      bar_init(empty(i), 5u);  // the products, and four warps' reading of the places
+    }
+    for (uint32_t i = 0; i < 2u; ++i) {
+      bar_init(kv_full(i), 4u);
+      bar_init(kv_empty(i));
+    }
+    bar_init(s_ready);
+    bar_init(s_free, 8u);
+    bar_init(p_ready, 8u);
+    bar_init(g_done);
+    bar_init(dq_free, 4u);
+    bar_init(acc_free, 4u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
   const uint32_t tm = s_tmem;
-  const uint32_t quad = warp & 3u, half = warp >> 2;  // lanes 32 quad.., columns 64 half..
-  const uint32_t my = (quad * 32u) << 16;
-  const uint32_t key_in = quad * 32u + lane;          // this thread's key in the span
-  constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
-  constexpr uint32_t kRowsBy = mma_desc<T>(128, DP, false, true);  // dv, dk
-  constexpr uint32_t kDqBy = mma_desc<T>(128, DP, true, true);
-  const float c2 = a.scale * kLog2e;
-  uint32_t phase = 0;  // of both barriers: each completes once per step
-  bool failed = false;
   const uint32_t work = *a.tile_count * a.gc;
-  for (uint32_t item = blockIdx.x; item < work; item += gridDim.x) {
-    const uint32_t gi = item % a.gc, g = a.g0 + gi, place = item / a.gc;
-    const uint4 tile = a.tiles[place];
-    const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
-    const uint32_t e0 = tile.z, all_rows = tile.w * a.R;
-    const uint32_t row0 = tile.y * kGradItem;
-    const uint32_t rows = all_rows > row0 ? min(all_rows - row0, kGradItem) : 0u;
-    const uint32_t len = cloud_length(a.lengths, b, a.N);
-    const uint32_t key0 = sb * 128u;
-    const uint32_t steps = (rows + kGradRows - 1u) / kGradRows;
-    if (steps) {
-      const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
-      const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-      // (a span with rows has a key below the cloud's end)
-      const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
-      load_strided<DP, 128, kGradThreads>(sk, a.D, tid, kh + (int64_t)key0 * ks, ks, len - key0);
-      load_strided<DP, 128, kGradThreads>(sv, a.D, tid, vh + (int64_t)key0 * vs, vs, len - key0);
+  // Every role walks the same items; the next one's tile is asked for ahead.
+  struct Items {
+    uint32_t w;
+    uint4 tile, next;
+  };
+  auto tile_at = [&](uint32_t w) {
+    return w < work ? a.tiles[w / a.gc] : make_uint4(0u, 0u, 0u, 0u);
+  };
+  auto items = [&]() {
+    return Items{blockIdx.x, tile_at(blockIdx.x), tile_at(blockIdx.x + gridDim.x)};
+  };
+  auto advance = [&](Items &x) {
+    x.w += gridDim.x;
+    x.tile = x.next;
+    x.next = tile_at(x.w + gridDim.x);
+  };
+  auto steps_of = [&](const uint4 &tile) {
+    const uint32_t all = tile.w * a.R, row0 = tile.y * kGradItem;
+    return all > row0 ? (min(all - row0, kGradItem) + kRows - 1u) / kRows : 0u;
+  };
+  auto item_of = [&](const Items &y) {
+    GradItem x;
+    x.gi = y.w % a.gc;
+    x.g = a.g0 + x.gi;
+    x.place = y.w / a.gc;
+    x.b = y.tile.x / a.nsb;
+    x.key0 = (y.tile.x - x.b * a.nsb) * 128u;
+    x.len = cloud_length(a.lengths, x.b, a.N);
+    x.e0 = y.tile.z;
+    x.all_rows = y.tile.w * a.R;
+    x.row0 = y.tile.y * kGradItem;
+    x.rows = x.all_rows > x.row0 ? min(x.all_rows - x.row0, kGradItem) : 0u;
+    x.steps = steps_of(y.tile);
+    return x;
+  };
+  bool failed = false;  // a wait of this thread ran out: go on without waiting
+  auto wait = [&](uint32_t bar, uint32_t phase) {
+    if (!failed) failed = !bar_wait(bar, phase);
+  };
+  // n counts the steps, k the items
+  // with steps.  Use u of a buffer or result waits for completion u - 1 of its
+  // release, whose parity is (u - 1) & 1.
+  if (warp < 8u) {
+    // ---- weights: lanes 32 quad.. of tensor memory, half the columns
+    const uint32_t quad = warp & 3u, half = warp >> 2, my = (quad * 32u) << 16;
+    constexpr uint32_t kCols = kRows / 2u;
+    const uint32_t key_in = quad * 32u + lane, block = key_in >> a.block_log2;
+    const float c2 = a.scale * kLog2e;
+    uint32_t n = 0;
+    for (Items y = items(); y.w < work; advance(y)) {
+      const GradItem it = item_of(y);
+      const bool key_live = it.key0 + key_in < it.len;
+      for (uint32_t i = 0; i < it.steps; ++i, ++n) {
+        const uint32_t st = n % kStages;
+        const char *info = smem + Shape::kInfoAt + st * Shape::kInfo;
+        wait(full(st), (n / kStages) & 1u);
+        wait(s_ready, n & 1u);
+        __syncwarp();
+        tmem_after_sync();
+        constexpr uint32_t kPieces = kCols / 16u;  // of 16 rows, the next in flight
+        uint32_t s[2][16], d[2][16];
+        tmem_ld16(s[0], tm + my + half * kCols);
+        tmem_ld16(d[0], tm + Shape::kDp + my + half * kCols);
+#pragma unroll
+        for (uint32_t x = 0; x < kPieces; ++x) {
+          const uint32_t col = half * kCols + x * 16u;
+          // which of the 16 rows read this key
+          uint32_t in = reinterpret_cast<const uint16_t *>(info + Shape::kBitsAt)[block * 8u + col / 16u];
+          if (!key_live) in = 0u;
+          tmem_ld_wait();
+          if (x + 1u < kPieces) {
+            tmem_ld16(s[(x + 1u) & 1u], tm + my + col + 16u);
+            tmem_ld16(d[(x + 1u) & 1u], tm + Shape::kDp + my + col + 16u);
+          } else {
+            tmem_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(s_free);
+          }
+          uint32_t *sx = s[x & 1u], *dx = d[x & 1u];
+          uint32_t p16[8], e16[8];
+          const bool all = __all_sync(kFullMask, in == 0xffffu);
+          if (__any_sync(kFullMask, in != 0u)) {
+#pragma unroll
+            for (uint32_t y = 0; y < 16u; y += 2u) {
+              // (lse, delta) of two rows
+              const float4 z = reinterpret_cast<const float4 *>(info)[col / 2u + y / 2u];
+              float2 p = fma2(make_float2(__uint_as_float(sx[y]), __uint_as_float(sx[y + 1])),
+                              make_float2(c2, c2), make_float2(-z.x, -z.z));
+              p.x = exp2_fast(p.x);
+              p.y = exp2_fast(p.y);
+              if (!all) {
+                p.x = (in >> y) & 1u ? p.x : 0.f;
+                p.y = (in >> (y + 1u)) & 1u ? p.y : 0.f;
+              }
+              const float2 e = mul2(p, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
+                                            make_float2(-z.y, -z.w)));
+              p16[y / 2u] = pack2<T>(p.x, p.y);
+              e16[y / 2u] = pack2<T>(e.x, e.y);
+            }
+          } else {
+#pragma unroll
+            for (uint32_t y = 0; y < 8u; ++y) p16[y] = e16[y] = 0u;
+          }
+          if (x == 0 && n) {  // the step before is done with p and ds
+            wait(g_done, (n - 1u) & 1u);
+            __syncwarp();
+            tmem_after_sync();
+          }
+          tmem_st8(tm + Shape::kP + my + col / 2u, p16);
+#pragma unroll
+          for (uint32_t c = 0; c < 2u; ++c)
+            *reinterpret_cast<uint4 *>(smem + Shape::kDsAt + (col / 64u) * 16384u +
+                                       swizzled(key_in, (col % 64u) / 8u + c)) =
+                make_uint4(e16[4 * c], e16[4 * c + 1], e16[4 * c + 2], e16[4 * c + 3]);
+        }
+        tmem_st_wait();
+        smem_to_mma();
+        tmem_before_sync();
+        __syncwarp();
+        if (lane == 0) bar_arrive(p_ready);
+      }
     }
-    // the item's rows, once: a step's addresses are then one shared load away
-    for (uint32_t r = tid; r < rows; r += kGradThreads) {
-      const uint32_t e = (row0 + r) / a.R, h = g * a.R + row0 + r - e * a.R;
-      GradRow x;
-      x.pair = a.vals[e0 + e];
-      const uint32_t bm = x.pair / a.top, m = bm - b * a.M;
-      x.q = 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2]);
-      x.row = bm * a.H + h;
-      s_rows[r] = x;
-    }
-    __syncthreads();
-    auto rows_at = [&](uint32_t i) { return base + Shape::kRowsAt + (Shape::kTwo ? (i & 1u) : 0u) * 2u * kTile; };
-    // q and dout of step i, and what the weights need of its rows
-    auto fetch = [&](uint32_t i) {
-      const uint32_t at = rows_at(i);
-#pragma unroll
-      for (uint32_t y = 0; y < 128u * kChunks / kGradThreads; ++y) {
-        const uint32_t x = tid + y * kGradThreads, r = x / kChunks, c = x % kChunks;
-        const uint32_t rr = i * kGradRows + r;
-        const bool some = rr < rows && c * 8u < a.D;
-        const char *qp = a.q, *op = a.dout;
-        if (some) {
-          const GradRow z = s_rows[rr];
-          qp += z.q + c * 16u;
-          op += ((uint64_t)z.row * a.D + c * 8u) * 2u;
-        }
-        const uint32_t to = at + (c >> 3) * 16384u + swizzled(r, c & 7u);
-        copy16(to, qp, some);
-        copy16(to + kTile, op, some);
+  } else if (warp < 12u) {
+    // ---- results: lanes 32 (warp - 8).. of tensor memory
+    const uint32_t at_lane = (warp & 3u) * 32u + lane, my = (at_lane & ~31u) << 16;
+    uint32_t n = 0;
+    // These warps also load the items' keys: item k's at the beginning, then
+    // one ahead where there are two buffers.
+    Items later = items();
+    uint32_t loaded = 0;
+    auto load_next = [&]() {  // the next item with steps, if any
+      for (; later.w < work; advance(later)) {
+        if (!steps_of(later.tile)) continue;
+        const GradItem x = item_of(later);
+        if (loaded >= Shape::kKv)
+          wait(kv_empty(loaded - Shape::kKv), ((loaded - Shape::kKv) >> 1) & 1u);
+        __syncwarp();
+        const uint32_t sk = base + (loaded % Shape::kKv) * 2u * Shape::kKeyTile;
+        const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
+        const char *kh = a.k + 2 * ((int64_t)x.b * a.ks[0] + (int64_t)x.g * a.ks[2]) + x.key0 * ks;
+        const char *vh = a.v + 2 * ((int64_t)x.b * a.vs[0] + (int64_t)x.g * a.vs[2]) + x.key0 * vs;
+        load_strided<DP, 128, 128>(sk, a.D, tid - 256u, kh, ks, x.len - x.key0);
+        load_strided<DP, 128, 128>(sk + Shape::kKeyTile, a.D, tid - 256u, vh, vs, x.len - x.key0);
+        copy_commit();
+        advance(later);
+        return true;
       }
-      copy_commit();
-      if (tid < kGradRows) {
-        char *info = smem + Shape::kInfoAt + (i & 1u) * Shape::kInfo;
-        const uint32_t rr = i * kGradRows + tid;
-        float2 y = make_float2(0.f, 0.f);
-        uint32_t mask = 0;
-        if (rr < rows) {
-          const GradRow z = s_rows[rr];
-          y = make_float2(a.lse_in[z.row] * kLog2e, a.delta[z.row]);
-          mask = a.mask[z.pair];
-        }
-        reinterpret_cast<float2 *>(info)[tid] = y;
-#pragma unroll
-        for (uint32_t j = 0; j < 8u; ++j) {
-          const uint32_t bits = __ballot_sync(kFullMask, (mask >> j) & 1u);
-          if (lane == j) reinterpret_cast<uint32_t *>(info + 1024)[j * 4u + warp] = bits;
-        }
-      }
+      return false;
     };
-    // (one thread) s^T and dp^T of step i
-    auto scores = [&](uint32_t i) {
-      const uint32_t q = rows_at(i), o = q + kTile;
-#pragma unroll
-      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t at = (kk >> 2) * 16384u + (kk & 3u) * 32u;
-        mma_ss(tm, tile_desc(sk + at, 16u), tile_desc(q + at, 16u), kScores, kk != 0u);
-      }
-#pragma unroll
-      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t at = (kk >> 2) * 16384u + (kk & 3u) * 32u;
-        mma_ss(tm + Shape::kDp, tile_desc(sv + at, 16u), tile_desc(o + at, 16u), kScores, kk != 0u);
-      }
-      mma_commit(bar_s);
-    };
-    // all threads: the loads of step i are here, its products may start
-    auto start = [&](uint32_t i) {
+    auto finish_load = [&]() {
       copy_wait<0>();
       smem_to_mma();
-      tmem_before_sync();
-      __syncthreads();
-      if (tid == 0) {
-        tmem_after_sync();
-        scores(i);
-      }
       __syncwarp();
+      if (lane == 0) bar_arrive(kv_full(loaded));
+      ++loaded;
     };
-    if (steps) {
-      fetch(0);
-      start(0);
-    }
-    const uint32_t block = key_in >> a.block_log2;
-    for (uint32_t i = 0; i < steps; ++i) {
-      if (Shape::kTwo && i + 1u < steps) fetch(i + 1u);
-      if (!failed) failed = !bar_wait(bar_s, phase);
-      __syncwarp();
-      tmem_after_sync();
-      const char *info = smem + Shape::kInfoAt + (i & 1u) * Shape::kInfo;
-      uint32_t s[2][32], d[2][32];
-      tmem_ld32(s[0], tm + my + half * 64u);
-      tmem_ld32(s[1], tm + my + half * 64u + 32u);
-      tmem_ld32(d[0], tm + Shape::kDp + my + half * 64u);
-      tmem_ld32(d[1], tm + Shape::kDp + my + half * 64u + 32u);
-      // which of the 64 rows read this key
-      uint2 bits = reinterpret_cast<const uint2 *>(info + 1024)[block * 2u + half];
-      if (key0 + key_in >= len) bits = make_uint2(0u, 0u);
-      tmem_ld_wait();
-      const bool full = __all_sync(kFullMask, (bits.x & bits.y) == kFullMask);
+    if (load_next()) finish_load();
+    for (Items y = items(); y.w < work; advance(y)) {
+      const GradItem it = item_of(y);
+      // (waited for here: the products of this item's last step come after the
+      // next item's scores)
+      if (it.steps && Shape::kKv == 2u && load_next()) finish_load();
+      const uint32_t key = it.key0 + at_lane;
+      const uint64_t key_row = ((uint64_t)it.b * a.N + key) * a.G + it.g;
+      for (uint32_t i = 0; i < it.steps; ++i, ++n) {
+        const uint32_t st = n % kStages;
+        const uint32_t *place = reinterpret_cast<const uint32_t *>(
+            smem + Shape::kInfoAt + st * Shape::kInfo + Shape::kPlaceAt);
+        wait(full(st), (n / kStages) & 1u);
+        wait(g_done, n & 1u);
+        __syncwarp();
+        tmem_after_sync();
+        uint32_t o[2][32];
+        tmem_ld32(o[0], tm + Shape::kDq + my);
+        tmem_ld32(o[1], tm + Shape::kDq + my + 32u);
+        tmem_ld_wait();
+        tmem_before_sync();
+        __syncwarp();
+        if (lane == 0) bar_arrive(dq_free);
+        const float f = failed ? NAN : 1.f;
+        if (DP == 64) {  // a lane has a row
+          const uint32_t to = place[at_lane];
+          __syncwarp();
+          if (lane == 0) bar_arrive(empty(st));
+          if (to != 0xffffffffu) {
+            float *p = a.part + (uint64_t)to * a.D;
 #pragma unroll
-      for (uint32_t x = 0; x < 2u; ++x) {
-        const uint32_t in = x ? bits.y : bits.x;
-        const bool some = __any_sync(kFullMask, in != 0u);
+            for (uint32_t y = 0; y < 64u; y += 8u)
+              if (y < a.D) store8(p + y, &o[y / 32u][y % 32u], f);
+          }
+        } else {         // a lane has one element of 64 rows
 #pragma unroll
-        for (uint32_t y = 0; y < 32u; y += 2u) {
-          // (lse, delta) of two rows
-          const float4 z = reinterpret_cast<const float4 *>(info)[half * 32u + x * 16u + y / 2u];
-          float p0 = 0.f, p1 = 0.f;
+          for (uint32_t y = 0; y < 64u; ++y) {
+            const uint32_t to = place[y];
+            if (to != 0xffffffffu && at_lane < a.D)
+              a.part[(uint64_t)to * a.D + at_lane] = __uint_as_float(o[y / 32u][y % 32u]) * f;
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(empty(st));
+        }
+      }
+      // the span's dk and dv, or this item's share of them: a lane has a key
+      const bool whole = it.all_rows <= kGradItem, some = key < a.N;
+      if (it.steps) {
+        const float f = failed ? NAN : 1.f;
+        float *share = a.part_kv + (((uint64_t)it.place * a.gc + it.gi) * 256u + at_lane) * a.D;
+#pragma unroll
+        for (uint32_t j = 0; j < DP / 16; ++j) {
+          const bool is_k = j >= DP / 32;
+          const uint32_t col = (j % (DP / 32)) * 32u;
+          uint32_t o[32];
+          tmem_ld32(o, tm + (is_k ? Shape::kDk : Shape::kDv) + my + col);
+          tmem_ld_wait();
+          if (j + 1u == DP / 16) {
+            tmem_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(acc_free);
+          }
+          const float g = is_k && whole ? f * a.scale : f;
           if (some) {
-            p0 = exp2_fast(fmaf(__uint_as_float(s[x][y]), c2, -z.x));
-            p1 = exp2_fast(fmaf(__uint_as_float(s[x][y + 1]), c2, -z.z));
-            if (!full) {
-              p0 = (in >> y) & 1u ? p0 : 0.f;
-              p1 = (in >> (y + 1u)) & 1u ? p1 : 0.f;
+#pragma unroll
+            for (uint32_t y = 0; y < 32u; y += 8u) {
+              if (col + y >= a.D) continue;
+              if (whole) {
+                uint32_t h[4];
+#pragma unroll
+                for (uint32_t z = 0; z < 4u; ++z)
+                  h[z] = pack2<T>(__uint_as_float(o[y + 2 * z]) * g,
+                                  __uint_as_float(o[y + 2 * z + 1]) * g);
+                *reinterpret_cast<uint4 *>((is_k ? a.dk : a.dv) + 2 * (key_row * a.D + col + y)) =
+                    make_uint4(h[0], h[1], h[2], h[3]);
+              } else {
+                store8(share + (is_k ? 0 : 128 * (uint64_t)a.D) + col + y, &o[y], g);
+              }
             }
           }
-          const float d0 = p0 * (__uint_as_float(d[x][y]) - z.y);
-          const float d1 = p1 * (__uint_as_float(d[x][y + 1]) - z.w);
-          s[0][x * 16u + y / 2u] = pack2<T>(p0, p1);
-          d[0][x * 16u + y / 2u] = pack2<T>(d0, d1);
-        }
-      }
-      // (over this thread's own dp: the other half's may not be read yet)
-      tmem_st32(tm + Shape::kDp + my + half * 64u, s[0]);
-#pragma unroll
-      for (uint32_t c = 0; c < 8u; ++c)
-        *reinterpret_cast<uint4 *>(smem + Shape::kDsAt + half * 16384u + swizzled(key_in, c)) =
-            make_uint4(d[0][4 * c], d[0][4 * c + 1], d[0][4 * c + 2], d[0][4 * c + 3]);
-      tmem_st_wait();
-      smem_to_mma();
-      tmem_before_sync();
-      __syncthreads();
-      if (tid == 0) {
-        tmem_after_sync();
-        const uint32_t q = rows_at(i), o = q + kTile;
-#pragma unroll
-        for (uint32_t kk = 0; kk < 8u; ++kk)
-          mma_ts(tm + Shape::kDv, tm + Shape::kDp + (kk >> 2) * 64u + (kk & 3u) * 8u,
-                 tile_desc(o + kk * 2048u, 16384u), kRowsBy, i != 0u || kk != 0u);
-#pragma unroll
-        for (uint32_t kk = 0; kk < 8u; ++kk)
-          mma_ss(tm + Shape::kDk, tile_desc(sds + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
-                 tile_desc(q + kk * 2048u, 16384u), kRowsBy, i != 0u || kk != 0u);
-#pragma unroll
-        for (uint32_t kk = 0; kk < 8u; ++kk)
-          mma_ss(tm + Shape::kDq, tile_desc(sds + kk * 2048u, 16384u),
-                 tile_desc(sk + kk * 2048u, 16384u), kDqBy, kk != 0u);
-        mma_commit(bar_g);
-      }
-      __syncwarp();
-      if (!failed) failed = !bar_wait(bar_g, phase);
-      __syncwarp();
-      tmem_after_sync();
-      phase ^= 1u;
-      // the next step's scores go before this step's dq is written out
-      if (Shape::kTwo && i + 1u < steps) start(i + 1u);
-      if (!Shape::kTwo && i + 1u < steps) fetch(i + 1u);
-      {
-        const uint32_t rr = i * kGradRows + key_in;  // lanes are rows here
-        const bool some = rr < rows;
-        uint64_t to = 0;
-        if (some) {
-          const GradRow z = s_rows[rr];
-          const uint32_t hh = z.row - (z.pair / a.top) * a.H - g * a.R;
-          to = ((uint64_t)z.pair * (a.gc * a.R) + gi * a.R + hh) * a.D;
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < DP / 64; ++j) {
-          uint32_t o[32];
-          const uint32_t col = half * (DP / 2) + j * 32u;
-          tmem_ld32(o, tm + Shape::kDq + my + col);
-          tmem_ld_wait();
-          if (some)
-#pragma unroll
-            for (uint32_t y = 0; y < 32u; y += 8u)
-              if (col + y < a.D) store8(a.part + to + col + y, &o[y], failed ? NAN : 1.f);
           __syncwarp();
         }
+        if (Shape::kKv == 1u && load_next()) finish_load();
+      } else if (some) {  // a span that nobody reads
+        for (uint32_t j = 0; j < a.D; j += 8u) {
+          *reinterpret_cast<uint4 *>(a.dk + 2 * (key_row * a.D + j)) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4 *>(a.dv + 2 * (key_row * a.D + j)) = make_uint4(0u, 0u, 0u, 0u);
+        }
       }
-      if (!Shape::kTwo && i + 1u < steps) start(i + 1u);
     }
-    // the span's dk and dv, or this item's share of them: one key per lane,
-    // dv by the first four warps, dk by the others
-    if (steps) {
-      const bool some = key0 + key_in < a.N, whole = all_rows <= kGradItem;
-      const float f = (half && whole ? a.scale : 1.f) * (failed ? NAN : 1.f);
-      char *out = (half ? a.dk : a.dv) +
-                  2 * ((((uint64_t)b * a.N + key0 + key_in) * a.G + g) * a.D);
-      float *share = a.part_kv +
-                     ((((uint64_t)place * a.gc + gi) * 2 + (half ? 0u : 1u)) * 128u + key_in) * a.D;
+  } else if (warp == 12u) {
+    // ---- products: one thread
+    if (lane == 0) {
+      constexpr uint32_t kScores = mma_desc<T>(128, kRows, false, false);
+      constexpr uint32_t kRowsBy = mma_desc<T>(128, DP, false, true);  // dv, dk
+      constexpr uint32_t kDqBy = mma_desc<T>(128, 64, true, true);
+      struct Walk {  // steps in order
+        Items y;
+        uint32_t i, steps, n, k;
+      };
+      auto settle = [&](Walk &x) {  // on the next item with steps
+        for (; x.y.w < work; advance(x.y))
+          if ((x.steps = steps_of(x.y.tile))) return;
+      };
+      auto next = [&](Walk &x) {
+        ++x.n;
+        if (++x.i < x.steps) return;
+        x.i = 0;
+        ++x.k;
+        advance(x.y);
+        settle(x);
+      };
+      const uint32_t sds = base + Shape::kDsAt;
+      auto keys_at = [&](uint32_t k) { return base + (k % Shape::kKv) * 2u * Shape::kKeyTile; };
+      auto rows_at = [&](uint32_t n) { return base + Shape::kRowsAt + (n % kStages) * Shape::kStage; };
+      auto scores = [&](Walk &x) {
+        wait(full(x.n % kStages), (x.n / kStages) & 1u);
+        if (x.i == 0) wait(kv_full(x.k), (x.k >> 1) & 1u);
+        if (x.n) wait(s_free, (x.n - 1u) & 1u);
+        tmem_after_sync();
+        const uint32_t sk = keys_at(x.k), sv = sk + Shape::kKeyTile;
+        const uint32_t q = rows_at(x.n), o = q + Shape::kRowTile;
 #pragma unroll
-      for (uint32_t j = 0; j < DP / 32; ++j) {
-        uint32_t o[32];
-        tmem_ld32(o, tm + (half ? Shape::kDk : Shape::kDv) + my + j * 32u);
-        tmem_ld_wait();
-        if (some) {
+        for (uint32_t kk = 0; kk < DP / 16; ++kk)
+          mma_ss(tm, tile_desc(sk + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
+                 tile_desc(q + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u, 16u), kScores, kk != 0u);
 #pragma unroll
-          for (uint32_t y = 0; y < 32u; y += 8u) {
-            if (j * 32u + y >= a.D) continue;
-            if (whole) {
-              uint32_t h[4];
+        for (uint32_t kk = 0; kk < DP / 16; ++kk)
+          mma_ss(tm + Shape::kDp, tile_desc(sv + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
+                 tile_desc(o + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u, 16u), kScores, kk != 0u);
+        mma_commit(s_ready);
+        next(x);
+      };
+      auto grads = [&](Walk &x) {
+        wait(p_ready, x.n & 1u);
+        if (x.n) wait(dq_free, (x.n - 1u) & 1u);
+        if (x.i == 0 && x.k) wait(acc_free, (x.k - 1u) & 1u);
+        tmem_after_sync();
+        const uint32_t sk = keys_at(x.k), q = rows_at(x.n), o = q + Shape::kRowTile;
 #pragma unroll
-              for (uint32_t z = 0; z < 4u; ++z)
-                h[z] = pack2<T>(__uint_as_float(o[y + 2 * z]) * f,
-                                __uint_as_float(o[y + 2 * z + 1]) * f);
-              *reinterpret_cast<uint4 *>(out + 2u * (j * 32u + y)) =
-                  make_uint4(h[0], h[1], h[2], h[3]);
-            } else {
-              store8(share + j * 32u + y, &o[y], f);
-            }
+        for (uint32_t kk = 0; kk < kRows / 16; ++kk)
+          mma_ts(tm + Shape::kDv, tm + Shape::kP + kk * 8u, tile_desc(o + kk * 2048u, kRows * 128u),
+                 kRowsBy, x.i != 0u || kk != 0u);
+#pragma unroll
+        for (uint32_t kk = 0; kk < kRows / 16; ++kk)
+          mma_ss(tm + Shape::kDk, tile_desc(sds + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
+                 tile_desc(q + kk * 2048u, kRows * 128u), kRowsBy, x.i != 0u || kk != 0u);
+#pragma unroll
+        for (uint32_t kk = 0; kk < 8u; ++kk) {
+          const uint64_t ds = tile_desc(sds + kk * 2048u, 16384u);
+          const uint64_t ky = tile_desc(sk + kk * 2048u, 16384u);
+          mma_ss(tm + Shape::kDq, DP == 64 ? ds : ky, DP == 64 ? ky : ds, kDqBy, kk != 0u);
+        }
+        mma_commit(g_done);
+        mma_commit(empty(x.n % kStages));
+        if (x.i + 1u == x.steps) mma_commit(kv_empty(x.k));
+        next(x);
+      };
+      Walk ahead{items(), 0u, 0u, 0u, 0u};
+      settle(ahead);
+      Walk now = ahead;
+      if (ahead.y.w < work) scores(ahead);
+      while (now.y.w < work) {
+        // (with one buffer of keys the next item's wait for this one's products)
+        const bool early = ahead.y.w < work && (Shape::kKv == 2u || ahead.i != 0u);
+        if (early) scores(ahead);
+        grads(now);
+        if (!early && ahead.y.w < work) scores(ahead);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- loads: steps n with n % 3 == stage
+    const uint32_t stage = warp - 13u;
+    char *info = smem + Shape::kInfoAt + stage * Shape::kInfo;
+    longlong2 *from = reinterpret_cast<longlong2 *>(smem + Shape::kFromAt + stage * Shape::kFrom);
+    const uint32_t at = base + Shape::kRowsAt + stage * Shape::kStage;
+    uint32_t n = 0;
+    for (Items y = items(); y.w < work; advance(y)) {
+      const GradItem it = item_of(y);
+      for (uint32_t i = 0; i < it.steps; ++i, ++n) {
+        if (n % kStages != stage) continue;
+        const uint32_t use = n / kStages;
+        // the rows: lane, lane + 32, ... (asked for before the stage is free);
+        // rows behind the last repeat it, and no weight of theirs is kept
+        constexpr uint32_t kHeld = kRows / 32u;
+        float lse[kHeld], delta[kHeld];
+        uint32_t mask[kHeld], place[kHeld];
+#pragma unroll
+        for (uint32_t j = 0; j < kHeld; ++j) {
+          const uint32_t r0 = i * kRows + j * 32u + lane, r = min(r0, it.rows - 1u);
+          const uint32_t e = (it.row0 + r) / a.R, head = it.row0 + r - e * a.R;
+          const uint32_t pair = a.vals[it.e0 + e];
+          const uint32_t bm = pair / a.top, m = bm - it.b * a.M, h = it.g * a.R + head;
+          const uint32_t row = bm * a.H + h;
+          lse[j] = a.lse_in[row] * kLog2e;
+          delta[j] = a.delta[row];
+          mask[j] = r0 < it.rows ? a.mask[pair] : 0u;
+          place[j] = r0 < it.rows ? pair * (a.gc * a.R) + it.gi * a.R + head : 0xffffffffu;
+          from[j * 32u + lane] = make_longlong2(
+              2 * ((int64_t)it.b * a.qs[0] + (int64_t)m * a.qs[1] + (int64_t)h * a.qs[2]),
+              2 * (int64_t)((uint64_t)row * a.D));
+        }
+        if (use) wait(empty(stage), (use - 1u) & 1u);
+        __syncwarp();
+        {
+          constexpr uint32_t kTogether = 32u / kChunks;  // rows per turn
+          const uint32_t c = lane % kChunks, r0 = lane / kChunks;
+          const bool in = c * 8u < a.D;
+          const char *q = a.q + (in ? c * 16u : 0u), *o = a.dout + (in ? c * 16u : 0u);
+          const uint32_t to = at + (c >> 3) * (kRows * 128u);
+#pragma unroll 8
+          for (uint32_t y = 0; y < kRows / kTogether; ++y) {
+            const uint32_t r = y * kTogether + r0;
+            const longlong2 x = from[r];
+            const uint32_t dst = to + swizzled(r, c & 7u);
+            copy16(dst, q + x.x, in);
+            copy16(dst + Shape::kRowTile, o + x.y, in);
           }
         }
+        copy_commit();
+#pragma unroll
+        for (uint32_t j = 0; j < kHeld; ++j) {
+          reinterpret_cast<float2 *>(info)[j * 32u + lane] = make_float2(lse[j], delta[j]);
+          reinterpret_cast<uint32_t *>(info + Shape::kPlaceAt)[j * 32u + lane] = place[j];
+#pragma unroll
+          for (uint32_t x = 0; x < 8u; ++x) {
+            const uint32_t bits = __ballot_sync(kFullMask, (mask[j] >> x) & 1u);
+            if (lane == x) reinterpret_cast<uint32_t *>(info + Shape::kBitsAt)[x * 4u + j] = bits;
+          }
+        }
+        copy_wait<0>();
+        smem_to_mma();
         __syncwarp();
+        if (lane == 0) bar_arrive(full(stage));
       }
-    } else if (key0 + key_in < a.N) {  // a span that nobody reads
-      char *out = (half ? a.dk : a.dv) +
-                  2 * ((((uint64_t)b * a.N + key0 + key_in) * a.G + g) * a.D);
-      for (uint32_t j = 0; j < a.D; j += 8u)
-        *reinterpret_cast<uint4 *>(out + 2u * j) = make_uint4(0u, 0u, 0u, 0u);
     }
-    tmem_before_sync();
-    __syncthreads();  // the tiles, the rows and dk, dv are free for the next item
-    tmem_after_sync();
   }
+  __syncwarp();
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
   if (warp == 0) tmem_free<512>(tm);
 }
 

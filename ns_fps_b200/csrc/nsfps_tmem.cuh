@@ -124,6 +124,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "%15,%16};" ::"r"(addr), NSFPS_IN8(r, 0), NSFPS_IN8(r, 8)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+               NSFPS_IN8(r, 0)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -131,22 +136,33 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void bar_init(uint32_t bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+// A barrier whose phase completes after `count` arrivals (a commit is one).
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count = 1u) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-// Waits for the phase of parity `phase`; false when it has not come after some
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Waits for the phase of parity `phase`; false when it has not come after two
 // seconds (a product that never ends), which no working call sees.
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.b32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(phase)
+      : "memory");
+  return done;
+}
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t phase) {
-  for (uint32_t i = 0; i < 1u << 22; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.b32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(bar), "r"(phase)
-        : "memory");
-    if (done) return true;
-  }
+  if (bar_try(bar, phase)) return true;
+  unsigned long long begin, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
+  do {
+    if (bar_try(bar, phase)) return true;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+  } while (now - begin < 2000000000ull);
   return false;
 }
 
