@@ -49,15 +49,16 @@ struct AttnArgs {
   const uint32_t *mask;    // per query slot: blocks of the span that are listed
   const unsigned long long *lead;  // per query: bit s = slot s leads a pair
   const uint32_t *skeys;   // their sort keys: span, then the chunks read
-  const uint4 *span;       // per span: first pair, end, first tile, tiles
-  const uint4 *tiles;      // (span, tile within the span, first pair, pairs of the span)
+  const uint4 *span;       // per span: first pair, end, first share, tiles
+  const uint4 *tiles;      // by cost: (span, tile within it, first pair, pairs of the span)
+  uint32_t tile_stride;    // places per cost class
   const uint32_t *tile_count;
   // partials of key heads g0 .. g0 + gc - 1
   uint32_t g0, gc;
   float *part;             // [pair][gc * R][D]
   float *part_lse;         // [pair][gc * R], base 2
   float *delta;            // [query][H]
-  float *part_kv;          // [tile][gc][2][span][D]
+  float *part_kv;          // [share][gc][2][span][D]
   uint32_t splits;         // direct path: partials per query
 };
 
@@ -182,6 +183,8 @@ __device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
 
 // ------------------------------------------------------------- the plan
 
+constexpr uint32_t kTileClasses = 5;  // of cost: 4 quarters .. 0
+
 // Blocks (as bits of a pair's mask) of the 64-key chunk c of a span.
 __device__ __forceinline__ uint32_t chunk_blocks(uint32_t c, uint32_t block_log2) {
   const uint32_t n = block_log2 >= 6u ? 1u : 64u >> block_log2;
@@ -199,7 +202,7 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
            uint32_t *__restrict__ mask, unsigned long long *__restrict__ lead,
            uint32_t *__restrict__ tile_count) {
   const uint32_t lane = threadIdx.x & 31u;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *tile_count = 0;  // for plan_spans
+  if (blockIdx.x == 0 && threadIdx.x <= kTileClasses) tile_count[threadIdx.x] = 0;  // for plan_spans
   const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (bm >= a.B * a.M) return;
   const uint32_t b = bm / a.M;
@@ -264,24 +267,62 @@ struct PairKeys {
 };
 
 // One warp per span: its pairs, and its tiles of tile_rows rows (at least
-// `least`), which it lists at a place it takes from a counter.  The places
-// differ from run to run; no result depends on them.
+// `least`), listed by cost.  CTAs take the tiles in turns, so with the dear
+// ones first the turns come out even (unsorted, the longest CTA of the
+// gradient had 1.4 times the mean).  A tile's place in its class comes from a
+// counter and differs from run to run; no result depends on it.  Spans of
+// several tiles get places for their tiles' shares of dk and dv, in order.
 __global__ void __launch_bounds__(256)
 plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, uint32_t tile_rows,
-           uint32_t least, uint4 *__restrict__ span, uint4 *__restrict__ tiles,
-           uint32_t *__restrict__ tile_count) {
+           uint32_t least, bool by_chunks, uint4 *__restrict__ span, uint4 *__restrict__ tiles,
+           uint32_t tile_stride, uint32_t *__restrict__ tile_count) {
   const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
   if (s >= spans) return;
   const uint32_t n = *list.kept;
   const uint32_t b = warp_lower_bound(list.keys, n, s << shift);
   const uint32_t e = b + warp_lower_bound(list.keys + b, n - b, (s + 1u) << shift);
-  const uint32_t count = max(least, (uint32_t)(((uint64_t)(e - b) * R + tile_rows - 1u) / tile_rows));
+  const uint32_t rows = (e - b) * R, count = max(least, (rows + tile_rows - 1u) / tile_rows);
   uint32_t first = 0;
-  if (lane == 0 && count) first = atomicAdd(tile_count, count);
+  if (lane == 0 && count > 1u) first = atomicAdd(tile_count + kTileClasses, count);
   first = __shfl_sync(kFullMask, first, 0);
   if (lane == 0) span[s] = make_uint4(b, e, first, count);
-  for (uint32_t i = lane; i < count; i += 32u) tiles[first + i] = make_uint4(s, i, b, e - b);
+  for (uint32_t i = lane; i < count; i += 32u) {
+    const uint32_t r0 = i * tile_rows, r1 = min(rows, r0 + tile_rows);
+    uint32_t cost = 0;  // 0 .. 4
+    if (by_chunks && r0 < r1) {
+      // the chunks between the Gray ranks of the first and the last row
+      const uint32_t low = (1u << shift) - 1u;
+      const uint32_t g0 = list.keys[b + r0 / R] & low, g1 = list.keys[b + (r1 - 1u) / R] & low;
+      uint32_t read = 0;
+      for (uint32_t g = g0; g <= g1; ++g) read |= g ^ (g >> 1);
+      cost = __popc(read);
+    } else if (r0 < r1) {
+      cost = (4u * (r1 - r0) + tile_rows - 1u) / tile_rows;
+    }
+    const uint32_t c = kTileClasses - 1u - min(cost, kTileClasses - 1u);
+    tiles[(uint64_t)c * tile_stride + atomicAdd(tile_count + c, 1u)] = make_uint4(s, i, b, e - b);
+  }
 }
+
+// The tiles, dear ones first.
+struct TileOrder {
+  const uint4 *tiles;
+  uint32_t stride, end[kTileClasses];
+  __device__ __forceinline__ explicit TileOrder(const AttnArgs &a)
+      : tiles(a.tiles), stride(a.tile_stride) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < kTileClasses; ++c) end[c] = sum += a.tile_count[c];
+  }
+  __device__ __forceinline__ uint32_t size() const { return end[kTileClasses - 1u]; }
+  __device__ __forceinline__ uint4 operator[](uint32_t i) const {
+    const uint4 *p = tiles + i;
+#pragma unroll
+    for (uint32_t c = 1; c < kTileClasses; ++c)
+      if (i >= end[c - 1u]) p = tiles + ((uint64_t)c * stride + (i - end[c - 1u]));
+    return *p;
+  }
+};
 
 // -------------------------------------------------------------- forward
 
@@ -545,7 +586,8 @@ attend_tiles(const AttnArgs a) {
   const float sign = a.scale == 0.f ? 0.f : a.scale < 0.f ? -1.f : 1.f;
   uint32_t phase = 0;     // of both barriers: each completes once per chunk
   bool failed = false;
-  const uint32_t work = *a.tile_count * a.gc;
+  const TileOrder order(a);
+  const uint32_t work = order.size() * a.gc;
   // What this thread's row of a tile is: asked for one tile ahead, the tile
   // itself two, as each waits for the one before.
   struct Row {
@@ -566,8 +608,8 @@ attend_tiles(const AttnArgs a) {
   };
   const uint32_t step = gridDim.x;
   uint4 tile = make_uint4(0u, 0u, 0u, 0u), tile_next = tile;
-  if (blockIdx.x < work) tile = a.tiles[blockIdx.x / a.gc];
-  if (blockIdx.x + step < work) tile_next = a.tiles[(blockIdx.x + step) / a.gc];
+  if (blockIdx.x < work) tile = order[blockIdx.x / a.gc];
+  if (blockIdx.x + step < work) tile_next = order[(blockIdx.x + step) / a.gc];
   Row mine = row_of(tile);
   for (uint32_t w = blockIdx.x; w < work; w += step) {
     const uint32_t gi = w % a.gc, g = a.g0 + gi;
@@ -588,7 +630,7 @@ attend_tiles(const AttnArgs a) {
     }
     tile = tile_next;
     mine = row_of(tile);
-    if (w + 2u * step < work) tile_next = a.tiles[(w + 2u * step) / a.gc];
+    if (w + 2u * step < work) tile_next = order[(w + 2u * step) / a.gc];
     const uint32_t warp_read = __reduce_or_sync(kFullMask, read);
     if (lane == 0) s_any[warp] = warp_read;
     s_q[tid] = q;
@@ -636,11 +678,11 @@ attend_tiles(const AttnArgs a) {
       __syncthreads();
       if (tid == 0) {
         tmem_after_sync();
+        const uint64_t q_desc = tile_desc(sq, 16u), k_desc = tile_desc(sk + buf * Shape::kChunk, 16u);
 #pragma unroll
         for (uint32_t kk = 0; kk < DP / 16; ++kk)
-          mma_ss(tm_s, tile_desc(sq + (kk >> 2) * (kTileRows * 128u) + (kk & 3u) * 32u, 16u),
-                 tile_desc(sk + buf * Shape::kChunk + (kk >> 2) * (64u * 128u) + (kk & 3u) * 32u, 16u),
-                 kScores, kk != 0u);
+          mma_ss(tm_s, further(q_desc, (kk >> 2) * (kTileRows * 128u) + (kk & 3u) * 32u),
+                 further(k_desc, (kk >> 2) * (64u * 128u) + (kk & 3u) * 32u), kScores, kk != 0u);
         mma_commit(bar_s);
       }
       __syncwarp();
@@ -726,10 +768,10 @@ attend_tiles(const AttnArgs a) {
       __syncthreads();
       if (tid == 0) {
         tmem_after_sync();
+        const uint64_t v_desc = tile_desc(sv + buf * Shape::kChunk, 64u * 128u);
 #pragma unroll
         for (uint32_t kk = 0; kk < 4u; ++kk)
-          mma_ts(tm_o, tm_s + kk * 8u, tile_desc(sv + buf * Shape::kChunk + kk * 2048u, 64u * 128u),
-                 kOutput, i != 0u || kk != 0u);
+          mma_ts(tm_o, tm_s + kk * 8u, further(v_desc, kk * 2048u), kOutput, i != 0u || kk != 0u);
         mma_commit(bar_o);
       }
       __syncwarp();
@@ -1021,12 +1063,15 @@ grad_delta(const AttnArgs a) {
 }
 
 constexpr uint32_t kGradItem = 512;    // query rows per item
-constexpr uint32_t kGradThreads = 512;
+// Warps by role: weights, results, products (one thread), loads (one warp per
+// stage).
+constexpr uint32_t kWeightWarps = 16, kResultWarps = 4, kGradStages = 3;
+constexpr uint32_t kGradThreads = 32 * (kWeightWarps + kResultWarps + 1 + kGradStages);
 
 template <int DP>  // 64 or 128
 struct GradShape {
   static constexpr uint32_t kRows = DP == 64 ? 128u : 64u;  // query rows per step
-  static constexpr uint32_t kStages = 3;                    // steps' rows in shared memory
+  static constexpr uint32_t kStages = kGradStages;          // steps' rows in shared memory
   static constexpr uint32_t kKv = DP == 64 ? 2u : 1u;       // items' keys in shared memory
   static constexpr uint32_t kKeyTile = 128u * DP * 2u, kRowTile = kRows * DP * 2u;
   static constexpr uint32_t kStage = 2u * kRowTile;         // q, dout
@@ -1044,7 +1089,7 @@ struct GradShape {
 
 // What the roles of the gradient kernel know of an item.
 struct GradItem {
-  uint32_t gi, g, place, b, key0, len, e0, row0, rows, all_rows, steps;
+  uint32_t gi, g, span, index, b, key0, len, e0, row0, rows, all_rows, steps;
 };
 
 // Items of up to kGradItem rows of one span of 128 keys and key head, CTAs
@@ -1089,32 +1134,33 @@ attend_grad(const AttnArgs a) {
   if (tid == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
       bar_init(full(i));
-      bar_init(empty(i), 5u);  // the products, and four warps' reading of the places
+      bar_init(empty(i), 1u + kResultWarps);  // the products, and four warps' reading of the places
     }
     for (uint32_t i = 0; i < 2u; ++i) {
-      bar_init(kv_full(i), 4u);
+      bar_init(kv_full(i), kResultWarps);
       bar_init(kv_empty(i));
     }
     bar_init(s_ready);
-    bar_init(s_free, 8u);
-    bar_init(p_ready, 8u);
+    bar_init(s_free, kWeightWarps);
+    bar_init(p_ready, kWeightWarps);
     bar_init(g_done);
-    bar_init(dq_free, 4u);
-    bar_init(acc_free, 4u);
+    bar_init(dq_free, kResultWarps);
+    bar_init(acc_free, kResultWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
   const uint32_t tm = s_tmem;
-  const uint32_t work = *a.tile_count * a.gc;
+  const TileOrder order(a);
+  const uint32_t work = order.size() * a.gc;
   // Every role walks the same items; the next one's tile is asked for ahead.
   struct Items {
     uint32_t w;
     uint4 tile, next;
   };
   auto tile_at = [&](uint32_t w) {
-    return w < work ? a.tiles[w / a.gc] : make_uint4(0u, 0u, 0u, 0u);
+    return w < work ? order[w / a.gc] : make_uint4(0u, 0u, 0u, 0u);
   };
   auto items = [&]() {
     return Items{blockIdx.x, tile_at(blockIdx.x), tile_at(blockIdx.x + gridDim.x)};
@@ -1132,7 +1178,8 @@ attend_grad(const AttnArgs a) {
     GradItem x;
     x.gi = y.w % a.gc;
     x.g = a.g0 + x.gi;
-    x.place = y.w / a.gc;
+    x.span = y.tile.x;
+    x.index = y.tile.y;
     x.b = y.tile.x / a.nsb;
     x.key0 = (y.tile.x - x.b * a.nsb) * 128u;
     x.len = cloud_length(a.lengths, x.b, a.N);
@@ -1150,10 +1197,11 @@ attend_grad(const AttnArgs a) {
   // n counts the steps, k the items
   // with steps.  Use u of a buffer or result waits for completion u - 1 of its
   // release, whose parity is (u - 1) & 1.
-  if (warp < 8u) {
-    // ---- weights: lanes 32 quad.. of tensor memory, half the columns
-    const uint32_t quad = warp & 3u, half = warp >> 2, my = (quad * 32u) << 16;
-    constexpr uint32_t kCols = kRows / 2u;
+  if (warp < kWeightWarps) {
+    // ---- weights: lanes 32 quad.. of tensor memory, a quarter of the columns
+    const uint32_t quad = warp & 3u, my = (quad * 32u) << 16;
+    constexpr uint32_t kCols = kRows / (kWeightWarps / 4u);
+    const uint32_t col0 = (warp >> 2) * kCols;
     const uint32_t key_in = quad * 32u + lane, block = key_in >> a.block_log2;
     const float c2 = a.scale * kLog2e;
     uint32_t n = 0;
@@ -1167,61 +1215,62 @@ attend_grad(const AttnArgs a) {
         wait(s_ready, n & 1u);
         __syncwarp();
         tmem_after_sync();
-        constexpr uint32_t kPieces = kCols / 16u;  // of 16 rows, the next in flight
-        uint32_t s[2][16], d[2][16];
-        tmem_ld16(s[0], tm + my + half * kCols);
-        tmem_ld16(d[0], tm + Shape::kDp + my + half * kCols);
+        constexpr uint32_t kPieces = kCols / 16u;  // of 16 rows
+        uint32_t p[kPieces][8], e[kPieces][8];
 #pragma unroll
         for (uint32_t x = 0; x < kPieces; ++x) {
-          const uint32_t col = half * kCols + x * 16u;
+          const uint32_t col = col0 + x * 16u;
+          uint32_t sx[16], dx[16];
+          tmem_ld16(sx, tm + my + col);
+          tmem_ld16(dx, tm + Shape::kDp + my + col);
           // which of the 16 rows read this key
           uint32_t in = reinterpret_cast<const uint16_t *>(info + Shape::kBitsAt)[block * 8u + col / 16u];
           if (!key_live) in = 0u;
           tmem_ld_wait();
-          if (x + 1u < kPieces) {
-            tmem_ld16(s[(x + 1u) & 1u], tm + my + col + 16u);
-            tmem_ld16(d[(x + 1u) & 1u], tm + Shape::kDp + my + col + 16u);
-          } else {
+          if (x + 1u == kPieces) {
             tmem_before_sync();
             __syncwarp();
             if (lane == 0) bar_arrive(s_free);
           }
-          uint32_t *sx = s[x & 1u], *dx = d[x & 1u];
-          uint32_t p16[8], e16[8];
+          uint32_t *p16 = p[x], *e16 = e[x];
           const bool all = __all_sync(kFullMask, in == 0xffffu);
           if (__any_sync(kFullMask, in != 0u)) {
 #pragma unroll
             for (uint32_t y = 0; y < 16u; y += 2u) {
               // (lse, delta) of two rows
               const float4 z = reinterpret_cast<const float4 *>(info)[col / 2u + y / 2u];
-              float2 p = fma2(make_float2(__uint_as_float(sx[y]), __uint_as_float(sx[y + 1])),
+              float2 f = fma2(make_float2(__uint_as_float(sx[y]), __uint_as_float(sx[y + 1])),
                               make_float2(c2, c2), make_float2(-z.x, -z.z));
-              p.x = exp2_fast(p.x);
-              p.y = exp2_fast(p.y);
+              f.x = exp2_fast(f.x);
+              f.y = exp2_fast(f.y);
               if (!all) {
-                p.x = (in >> y) & 1u ? p.x : 0.f;
-                p.y = (in >> (y + 1u)) & 1u ? p.y : 0.f;
+                f.x = (in >> y) & 1u ? f.x : 0.f;
+                f.y = (in >> (y + 1u)) & 1u ? f.y : 0.f;
               }
-              const float2 e = mul2(p, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
+              const float2 g = mul2(f, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
                                             make_float2(-z.y, -z.w)));
-              p16[y / 2u] = pack2<T>(p.x, p.y);
-              e16[y / 2u] = pack2<T>(e.x, e.y);
+              p16[y / 2u] = pack2<T>(f.x, f.y);
+              e16[y / 2u] = pack2<T>(g.x, g.y);
             }
           } else {
 #pragma unroll
             for (uint32_t y = 0; y < 8u; ++y) p16[y] = e16[y] = 0u;
           }
-          if (x == 0 && n) {  // the step before is done with p and ds
-            wait(g_done, (n - 1u) & 1u);
-            __syncwarp();
-            tmem_after_sync();
-          }
-          tmem_st8(tm + Shape::kP + my + col / 2u, p16);
+        }
+        if (n) {  // the step before is done with p and ds
+          wait(g_done, (n - 1u) & 1u);
+          __syncwarp();
+          tmem_after_sync();
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < kPieces; ++x) {
+          const uint32_t col = col0 + x * 16u;
+          tmem_st8(tm + Shape::kP + my + col / 2u, p[x]);
 #pragma unroll
           for (uint32_t c = 0; c < 2u; ++c)
             *reinterpret_cast<uint4 *>(smem + Shape::kDsAt + (col / 64u) * 16384u +
                                        swizzled(key_in, (col % 64u) / 8u + c)) =
-                make_uint4(e16[4 * c], e16[4 * c + 1], e16[4 * c + 2], e16[4 * c + 3]);
+                make_uint4(e[x][4 * c], e[x][4 * c + 1], e[x][4 * c + 2], e[x][4 * c + 3]);
         }
         tmem_st_wait();
         smem_to_mma();
@@ -1230,9 +1279,10 @@ attend_grad(const AttnArgs a) {
         if (lane == 0) bar_arrive(p_ready);
       }
     }
-  } else if (warp < 12u) {
-    // ---- results: lanes 32 (warp - 8).. of tensor memory
+  } else if (warp < kWeightWarps + kResultWarps) {
+    // ---- results: lanes 32 (warp & 3).. of tensor memory
     const uint32_t at_lane = (warp & 3u) * 32u + lane, my = (at_lane & ~31u) << 16;
+    const uint32_t role_tid = tid - 32u * kWeightWarps;
     uint32_t n = 0;
     // These warps also load the items' keys: item k's at the beginning, then
     // one ahead where there are two buffers.
@@ -1249,8 +1299,8 @@ attend_grad(const AttnArgs a) {
         const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
         const char *kh = a.k + 2 * ((int64_t)x.b * a.ks[0] + (int64_t)x.g * a.ks[2]) + x.key0 * ks;
         const char *vh = a.v + 2 * ((int64_t)x.b * a.vs[0] + (int64_t)x.g * a.vs[2]) + x.key0 * vs;
-        load_strided<DP, 128, 128>(sk, a.D, tid - 256u, kh, ks, x.len - x.key0);
-        load_strided<DP, 128, 128>(sk + Shape::kKeyTile, a.D, tid - 256u, vh, vs, x.len - x.key0);
+        load_strided<DP, 128, 128>(sk, a.D, role_tid, kh, ks, x.len - x.key0);
+        load_strided<DP, 128, 128>(sk + Shape::kKeyTile, a.D, role_tid, vh, vs, x.len - x.key0);
         copy_commit();
         advance(later);
         return true;
@@ -1280,40 +1330,44 @@ attend_grad(const AttnArgs a) {
         wait(g_done, n & 1u);
         __syncwarp();
         tmem_after_sync();
-        uint32_t o[2][32];
-        tmem_ld32(o[0], tm + Shape::kDq + my);
-        tmem_ld32(o[1], tm + Shape::kDq + my + 32u);
-        tmem_ld_wait();
-        tmem_before_sync();
-        __syncwarp();
-        if (lane == 0) bar_arrive(dq_free);
         const float f = failed ? NAN : 1.f;
-        if (DP == 64) {  // a lane has a row
-          const uint32_t to = place[at_lane];
-          __syncwarp();
-          if (lane == 0) bar_arrive(empty(st));
-          if (to != 0xffffffffu) {
-            float *p = a.part + (uint64_t)to * a.D;
+        // (places first: behind the second half the stage is given back)
+        const uint32_t mine = DP == 64 ? place[at_lane] : 0u;
 #pragma unroll
-            for (uint32_t y = 0; y < 64u; y += 8u)
-              if (y < a.D) store8(p + y, &o[y / 32u][y % 32u], f);
+        for (uint32_t h = 0; h < 2u; ++h) {
+          uint32_t o[32];
+          tmem_ld32(o, tm + Shape::kDq + my + h * 32u);
+          tmem_ld_wait();
+          if (h) {
+            tmem_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(dq_free);
           }
-        } else {         // a lane has one element of 64 rows
+          if (DP == 64) {  // a lane has a row
+            if (mine != 0xffffffffu) {
+              float *to = a.part + (uint64_t)mine * a.D + h * 32u;
 #pragma unroll
-          for (uint32_t y = 0; y < 64u; ++y) {
-            const uint32_t to = place[y];
-            if (to != 0xffffffffu && at_lane < a.D)
-              a.part[(uint64_t)to * a.D + at_lane] = __uint_as_float(o[y / 32u][y % 32u]) * f;
+              for (uint32_t y = 0; y < 32u; y += 8u)
+                if (h * 32u + y < a.D) store8(to + y, &o[y], f);
+            }
+          } else {         // a lane has one element of 32 rows
+#pragma unroll
+            for (uint32_t y = 0; y < 32u; ++y) {
+              const uint32_t to = place[h * 32u + y];
+              if (to != 0xffffffffu && at_lane < a.D)
+                a.part[(uint64_t)to * a.D + at_lane] = __uint_as_float(o[y]) * f;
+            }
           }
           __syncwarp();
-          if (lane == 0) bar_arrive(empty(st));
         }
+        if (lane == 0) bar_arrive(empty(st));
       }
       // the span's dk and dv, or this item's share of them: a lane has a key
       const bool whole = it.all_rows <= kGradItem, some = key < a.N;
       if (it.steps) {
         const float f = failed ? NAN : 1.f;
-        float *share = a.part_kv + (((uint64_t)it.place * a.gc + it.gi) * 256u + at_lane) * a.D;
+        const uint64_t place = whole ? 0u : a.span[it.span].z + it.index;
+        float *share = a.part_kv + ((place * a.gc + it.gi) * 256u + at_lane) * a.D;
 #pragma unroll
         for (uint32_t j = 0; j < DP / 16; ++j) {
           const bool is_k = j >= DP / 32;
@@ -1354,7 +1408,7 @@ attend_grad(const AttnArgs a) {
         }
       }
     }
-  } else if (warp == 12u) {
+  } else if (warp == kWeightWarps + kResultWarps) {
     // ---- products: one thread
     if (lane == 0) {
       constexpr uint32_t kScores = mma_desc<T>(128, kRows, false, false);
@@ -1376,7 +1430,8 @@ attend_grad(const AttnArgs a) {
         advance(x.y);
         settle(x);
       };
-      const uint32_t sds = base + Shape::kDsAt;
+      // (the distance of further columns means nothing where there are none)
+      const uint64_t ds_desc = tile_desc(base + Shape::kDsAt, 16384u);
       auto keys_at = [&](uint32_t k) { return base + (k % Shape::kKv) * 2u * Shape::kKeyTile; };
       auto rows_at = [&](uint32_t n) { return base + Shape::kRowsAt + (n % kStages) * Shape::kStage; };
       auto scores = [&](Walk &x) {
@@ -1384,16 +1439,17 @@ attend_grad(const AttnArgs a) {
         if (x.i == 0) wait(kv_full(x.k), (x.k >> 1) & 1u);
         if (x.n) wait(s_free, (x.n - 1u) & 1u);
         tmem_after_sync();
-        const uint32_t sk = keys_at(x.k), sv = sk + Shape::kKeyTile;
-        const uint32_t q = rows_at(x.n), o = q + Shape::kRowTile;
+        const uint64_t k_desc = tile_desc(keys_at(x.k), 16u), q_desc = tile_desc(rows_at(x.n), 16u);
 #pragma unroll
         for (uint32_t kk = 0; kk < DP / 16; ++kk)
-          mma_ss(tm, tile_desc(sk + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
-                 tile_desc(q + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u, 16u), kScores, kk != 0u);
+          mma_ss(tm, further(k_desc, (kk >> 2) * 16384u + (kk & 3u) * 32u),
+                 further(q_desc, (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u), kScores, kk != 0u);
 #pragma unroll
         for (uint32_t kk = 0; kk < DP / 16; ++kk)
-          mma_ss(tm + Shape::kDp, tile_desc(sv + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
-                 tile_desc(o + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u, 16u), kScores, kk != 0u);
+          mma_ss(tm + Shape::kDp,
+                 further(k_desc, Shape::kKeyTile + (kk >> 2) * 16384u + (kk & 3u) * 32u),
+                 further(q_desc, Shape::kRowTile + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u),
+                 kScores, kk != 0u);
         mma_commit(s_ready);
         next(x);
       };
@@ -1402,19 +1458,20 @@ attend_grad(const AttnArgs a) {
         if (x.n) wait(dq_free, (x.n - 1u) & 1u);
         if (x.i == 0 && x.k) wait(acc_free, (x.k - 1u) & 1u);
         tmem_after_sync();
-        const uint32_t sk = keys_at(x.k), q = rows_at(x.n), o = q + Shape::kRowTile;
+        const uint64_t k_desc = tile_desc(keys_at(x.k), 16384u);
+        const uint64_t q_desc = tile_desc(rows_at(x.n), kRows * 128u);
+        const bool add = x.i != 0u;
 #pragma unroll
         for (uint32_t kk = 0; kk < kRows / 16; ++kk)
-          mma_ts(tm + Shape::kDv, tm + Shape::kP + kk * 8u, tile_desc(o + kk * 2048u, kRows * 128u),
-                 kRowsBy, x.i != 0u || kk != 0u);
+          mma_ts(tm + Shape::kDv, tm + Shape::kP + kk * 8u,
+                 further(q_desc, Shape::kRowTile + kk * 2048u), kRowsBy, add || kk != 0u);
 #pragma unroll
         for (uint32_t kk = 0; kk < kRows / 16; ++kk)
-          mma_ss(tm + Shape::kDk, tile_desc(sds + (kk >> 2) * 16384u + (kk & 3u) * 32u, 16u),
-                 tile_desc(q + kk * 2048u, kRows * 128u), kRowsBy, x.i != 0u || kk != 0u);
+          mma_ss(tm + Shape::kDk, further(ds_desc, (kk >> 2) * 16384u + (kk & 3u) * 32u),
+                 further(q_desc, kk * 2048u), kRowsBy, add || kk != 0u);
 #pragma unroll
         for (uint32_t kk = 0; kk < 8u; ++kk) {
-          const uint64_t ds = tile_desc(sds + kk * 2048u, 16384u);
-          const uint64_t ky = tile_desc(sk + kk * 2048u, 16384u);
+          const uint64_t ds = further(ds_desc, kk * 2048u), ky = further(k_desc, kk * 2048u);
           mma_ss(tm + Shape::kDq, DP == 64 ? ds : ky, DP == 64 ? ky : ds, kDqBy, kk != 0u);
         }
         mma_commit(g_done);
@@ -1436,8 +1493,8 @@ attend_grad(const AttnArgs a) {
     }
     __syncwarp();
   } else {
-    // ---- loads: steps n with n % 3 == stage
-    const uint32_t stage = warp - 13u;
+    // ---- loads: steps n with n % kStages == stage
+    const uint32_t stage = warp - (kWeightWarps + kResultWarps + 1u);
     char *info = smem + Shape::kInfoAt + stage * Shape::kInfo;
     longlong2 *from = reinterpret_cast<longlong2 *>(smem + Shape::kFromAt + stage * Shape::kFrom);
     const uint32_t at = base + Shape::kRowsAt + stage * Shape::kStage;
@@ -1667,8 +1724,8 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.mask = c.take<uint32_t>(w.pairs);
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
   w.span = c.take<uint4>(w.spans);
-  w.tile_count = c.take<uint32_t>(1);
-  w.tiles = c.take<uint4>(w.max_tiles);
+  w.tile_count = c.take<uint32_t>(kTileClasses + 1);
+  w.tiles = c.take<uint4>(kTileClasses * w.max_tiles);
   w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
     w.delta = c.take<float>(w.bc * d.queries * d.heads);
@@ -1693,6 +1750,7 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   a.scale = d.scale;
   a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
   a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
+  a.tile_stride = (uint32_t)w.max_tiles;
   a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
   a.part_kv = w.part_kv; a.splits = w.splits; a.gc = w.gc;
   return a;
@@ -1734,7 +1792,7 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
     if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
   } else {  // no pair, or no key to form one with
     if ((err = cudaMemsetAsync(w.sort.kept, 0, 4, st))) return err;
-    if ((err = cudaMemsetAsync(w.tile_count, 0, 4, st))) return err;
+    if ((err = cudaMemsetAsync(w.tile_count, 0, 4 * (kTileClasses + 1), st))) return err;
     if (a.B * a.M &&
         (err = cudaMemsetAsync(w.lead, 0, sizeof(*w.lead) * (uint64_t)a.B * a.M, st)))
       return err;
@@ -1742,9 +1800,9 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   a.vals = list.vals;
   a.skeys = list.keys;
   if (spans)
-    plan_spans<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(list, spans, shift, a.R, w.tile_rows,
-                                                             w.least, w.span, w.tiles,
-                                                             w.tile_count);
+    plan_spans<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(
+        list, spans, shift, a.R, w.tile_rows, w.least, w.least == 0u, w.span, w.tiles,
+        a.tile_stride, w.tile_count);
   return cudaGetLastError();
 }
 

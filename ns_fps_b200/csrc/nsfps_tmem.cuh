@@ -28,6 +28,13 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lead) {
          (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// The tile `bytes` behind (its address stays below the field's 256 KB).  One
+// thread issues all products of a CTA: what it computes per product is time
+// that the tensor core waits.
+__device__ __forceinline__ uint64_t further(uint64_t desc, uint32_t bytes) {
+  return desc + (bytes >> 4);
+}
+
 // Instruction descriptor: fp32 accumulator, both operands of type T, M x N.
 template <class T>
 __device__ constexpr uint32_t mma_desc(uint32_t m, uint32_t n, bool a_mn, bool b_mn);
@@ -134,6 +141,16 @@ __device__ __forceinline__ void tmem_ld_wait() {
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// (all warps of a group of four) the registers of a thread from here on
+template <int N>
+__device__ __forceinline__ void reg_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_less() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // A barrier whose phase completes after `count` arrivals (a commit is one).
