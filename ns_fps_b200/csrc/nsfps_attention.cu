@@ -564,7 +564,7 @@ attend_tiles(const AttnArgs a) {
   __shared__ __align__(8) uint64_t s_bar[2];
   __shared__ uint32_t s_tmem, s_any[4];
   __shared__ const char *s_q[kTileRows];
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = warp_value(tid >> 5);
   const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the swizzle's pattern
   const uint32_t sk = sq + Shape::kQ, sv = sk + 2u * Shape::kChunk;
   const uint32_t bar_s = smem_u32(&s_bar[0]), bar_o = smem_u32(&s_bar[1]);
@@ -578,7 +578,7 @@ attend_tiles(const AttnArgs a) {
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
-  const uint32_t tm = s_tmem, tm_s = tm, tm_o = tm + 64u;
+  const uint32_t tm = warp_value(s_tmem), tm_s = tm, tm_o = tm + 64u;
   const uint32_t my = (warp * 32u) << 16;  // this warp's lanes
   constexpr uint32_t kScores = mma_desc<T>(128, 64, false, false);
   constexpr uint32_t kOutput = mma_desc<T>(128, DP, false, true);
@@ -635,7 +635,7 @@ attend_tiles(const AttnArgs a) {
     if (lane == 0) s_any[warp] = warp_read;
     s_q[tid] = q;
     __syncthreads();
-    uint32_t todo = s_any[0] | s_any[1] | s_any[2] | s_any[3];
+    uint32_t todo = warp_value(s_any[0] | s_any[1] | s_any[2] | s_any[3]);
     const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
     const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
     auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
@@ -676,7 +676,7 @@ attend_tiles(const AttnArgs a) {
       smem_to_mma();
       tmem_before_sync();
       __syncthreads();
-      if (tid == 0) {
+      if (warp == 0) {
         tmem_after_sync();
         const uint64_t q_desc = tile_desc(sq, 16u), k_desc = tile_desc(sk + buf * Shape::kChunk, 16u);
 #pragma unroll
@@ -766,7 +766,7 @@ attend_tiles(const AttnArgs a) {
       tmem_st_wait();
       tmem_before_sync();
       __syncthreads();
-      if (tid == 0) {
+      if (warp == 0) {
         tmem_after_sync();
         const uint64_t v_desc = tile_desc(sv + buf * Shape::kChunk, 64u * 128u);
 #pragma unroll
@@ -1063,7 +1063,7 @@ grad_delta(const AttnArgs a) {
 }
 
 constexpr uint32_t kGradItem = 512;    // query rows per item
-// Warps by role: weights, results, products (one thread), loads (one warp per
+// Warps by role: weights, results, products (one warp), loads (one warp per
 // stage).
 constexpr uint32_t kWeightWarps = 16, kResultWarps = 4, kGradStages = 3;
 constexpr uint32_t kGradThreads = 32 * (kWeightWarps + kResultWarps + 1 + kGradStages);
@@ -1106,8 +1106,8 @@ struct GradItem {
 // Done in turns by all warps, the stages of a step took 11,000 cycles, of
 // which the weights were 2,500.  So the warps have roles and meet at barriers:
 // eight make weights, three load a step's rows each (the loads of three steps
-// are in the air), four take dq, dk and dv out, and one thread issues the
-// products, the next step's scores before this step's gradients.
+// are in the air), four take dq, dk and dv out, and one issues the products,
+// the next step's scores before this step's gradients.
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
@@ -1116,7 +1116,7 @@ attend_grad(const AttnArgs a) {
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[kStages * 2 + 4 + 6];
   __shared__ uint32_t s_tmem;
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = warp_value(tid >> 5);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char *smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = smem_u32(s_bar);
@@ -1151,9 +1151,9 @@ attend_grad(const AttnArgs a) {
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
-  const uint32_t tm = s_tmem;
+  const uint32_t tm = warp_value(s_tmem);
   const TileOrder order(a);
-  const uint32_t work = order.size() * a.gc;
+  const uint32_t work = warp_value(order.size() * a.gc);
   // Every role walks the same items; the next one's tile is asked for ahead.
   struct Items {
     uint32_t w;
@@ -1409,8 +1409,8 @@ attend_grad(const AttnArgs a) {
       }
     }
   } else if (warp == kWeightWarps + kResultWarps) {
-    // ---- products: one thread
-    if (lane == 0) {
+    // ---- products: the warp in step
+    {
       constexpr uint32_t kScores = mma_desc<T>(128, kRows, false, false);
       constexpr uint32_t kRowsBy = mma_desc<T>(128, DP, false, true);  // dv, dk
       constexpr uint32_t kDqBy = mma_desc<T>(128, 64, true, true);
@@ -1420,7 +1420,7 @@ attend_grad(const AttnArgs a) {
       };
       auto settle = [&](Walk &x) {  // on the next item with steps
         for (; x.y.w < work; advance(x.y))
-          if ((x.steps = steps_of(x.y.tile))) return;
+          if ((x.steps = warp_value(steps_of(x.y.tile)))) return;
       };
       auto next = [&](Walk &x) {
         ++x.n;
@@ -1438,6 +1438,7 @@ attend_grad(const AttnArgs a) {
         wait(full(x.n % kStages), (x.n / kStages) & 1u);
         if (x.i == 0) wait(kv_full(x.k), (x.k >> 1) & 1u);
         if (x.n) wait(s_free, (x.n - 1u) & 1u);
+        __syncwarp();
         tmem_after_sync();
         const uint64_t k_desc = tile_desc(keys_at(x.k), 16u), q_desc = tile_desc(rows_at(x.n), 16u);
 #pragma unroll
@@ -1457,6 +1458,7 @@ attend_grad(const AttnArgs a) {
         wait(p_ready, x.n & 1u);
         if (x.n) wait(dq_free, (x.n - 1u) & 1u);
         if (x.i == 0 && x.k) wait(acc_free, (x.k - 1u) & 1u);
+        __syncwarp();
         tmem_after_sync();
         const uint64_t k_desc = tile_desc(keys_at(x.k), 16384u);
         const uint64_t q_desc = tile_desc(rows_at(x.n), kRows * 128u);

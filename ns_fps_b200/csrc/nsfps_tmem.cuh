@@ -1,6 +1,12 @@
 // nsfps_tmem.cuh -- the fifth-generation tensor core as the feature operators
-// use it: tcgen05.mma issued by one thread of a CTA on shared tiles, results in
+// use it: tcgen05.mma issued by one warp of a CTA on shared tiles, results in
 // tensor memory.
+//
+// The issuing calls (mma_*) are made by a whole warp in step, and one elected
+// lane issues.  Their operands live in registers that a warp shares; computed
+// by one lane alone, every descriptor was moved there first, and a product took
+// some 100 cycles to issue.  warp_value() tells the compiler that a value is
+// the same in all lanes.
 //
 // Shared tiles hold rows of 64 16-bit elements (128 bytes) in the 128-byte
 // swizzle: 16-byte chunk c of row r lies at r * 128 + ((c ^ (r & 7)) << 4), so
@@ -16,6 +22,10 @@
 
 namespace nsfps {
 
+__device__ __forceinline__ uint32_t warp_value(uint32_t x) {
+  return __shfl_sync(0xffffffffu, x, 0);
+}
+
 __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) {
   return r * 128u + ((c ^ (r & 7u)) << 4);
 }
@@ -28,9 +38,7 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lead) {
          (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// The tile `bytes` behind (its address stays below the field's 256 KB).  One
-// thread issues all products of a CTA: what it computes per product is time
-// that the tensor core waits.
+// The tile `bytes` behind (its address stays below the field's 256 KB).
 __device__ __forceinline__ uint64_t further(uint64_t desc, uint32_t bytes) {
   return desc + (bytes >> 4);
 }
@@ -52,8 +60,8 @@ __device__ constexpr uint32_t mma_desc<__nv_bfloat16>(uint32_t m, uint32_t n, bo
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
                                        bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
       ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
       : "memory");
 }
@@ -61,15 +69,17 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
                                        bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
       ::"r"(d), "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
       : "memory");
 }
 // The barrier completes when the products issued so far have.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar)
+      : "memory");
 }
 
 // (one warp) COLS columns of tensor memory; the address is put at shared `at`.
