@@ -22,11 +22,10 @@ With the sampler and the grouping operators:
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 
 from . import capi
-from .group import _cloud_batch, _dtype_code, _on
+from .group import _cloud_batch, _dtype_code, _enter, _leave, _Plans
 
 __all__ = ["select_blocks", "block_attention"]
 
@@ -42,24 +41,38 @@ def _check_block(block, top):
 
 
 def _check_lengths(lengths, B, device):
-    """Address of the clouds' lengths (0 for None)."""
     import torch
     if lengths is None:
-        return 0, None
+        return
     if not isinstance(lengths, torch.Tensor) or not lengths.is_cuda or lengths.dtype != torch.int32:
         raise TypeError("lengths must be an int32 CUDA tensor")
     if lengths.numel() != B or lengths.dim() > 1:
         raise ValueError("lengths must hold one length per cloud")
     if lengths.device != device:
         raise ValueError("lengths must be on the clouds' device")
-    lengths = lengths.contiguous()
-    return lengths.data_ptr(), lengths
 
 
-@functools.lru_cache(maxsize=256)
-def _select_desc(B, N, M, block, top):
+def _look(t):
+    """What a call's checks read of a tensor (None: None)."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+_select_plans, _attention_plans = _Plans(), _Plans()
+
+
+def _select_plan(points, centers, block, top, lengths):
+    pts, single = _cloud_batch(points, "points")
+    ctr, single_c = _cloud_batch(centers, "centers")
+    if single != single_c or pts.shape[0] != ctr.shape[0]:
+        raise ValueError("points and centers must have the same batch layout")
+    if pts.device != ctr.device:
+        raise ValueError("points and centers must be on the same device")
+    _check_block(block, top)
+    B, N, M = int(pts.shape[0]), int(pts.shape[1]), int(ctr.shape[1])
+    _check_lengths(lengths, B, pts.device)
     desc = capi.SelectDesc(B, N, M, block, top)
-    return desc, capi.select_blocks_workspace(desc)
+    return (desc, ctypes.addressof(desc), capi.select_blocks_workspace(desc),
+            (M, top) if single else (B, M, top))
 
 
 def select_blocks(points, centers, block: int, top: int, lengths=None):
@@ -79,85 +92,154 @@ def select_blocks(points, centers, block: int, top: int, lengths=None):
     radius: ``blocks.masked_fill(d2 > radius * radius, -1)``.
     """
     import torch
-    pts, single = _cloud_batch(points, "points")
-    ctr, single_c = _cloud_batch(centers, "centers")
-    if single != single_c or pts.shape[0] != ctr.shape[0]:
-        raise ValueError("points and centers must have the same batch layout")
-    if pts.device != ctr.device:
-        raise ValueError("points and centers must be on the same device")
     block, top = int(block), int(top)
-    _check_block(block, top)
-    B, N, M = int(pts.shape[0]), int(pts.shape[1]), int(ctr.shape[1])
-    len_ptr, _len = _check_lengths(lengths, B, pts.device)
-    blocks = pts.new_empty((B, M, top), dtype=torch.int64)
-    d2 = pts.new_empty((B, M, top))
-    desc, need = _select_desc(B, N, M, block, top)
-    with _on(pts) as stream:
-        work = pts.new_empty(need, dtype=torch.uint8)
-        capi.select_blocks_device(desc, pts.data_ptr(), len_ptr, ctr.data_ptr(),
-                                  blocks.data_ptr(), d2.data_ptr(), work.data_ptr(), need, stream)
-    return (blocks[0], d2[0]) if single else (blocks, d2)
-
-
-def _rows16(t):
-    """t with contiguous heads, 16-byte aligned rows: t itself when it is."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in _strides(t)):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+    try:
+        key = (_look(points), _look(centers), _look(lengths), block, top)
+        plan = _select_plans.get(key)
+    except AttributeError:  # not tensors
+        key = plan = None
+    if plan is None:
+        plan = _select_plans.keep(key, _select_plan(points, centers, block, top, lengths))
+    points, centers = points.contiguous(), centers.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    blocks = points.new_empty(plan[3], dtype=torch.int64)
+    d2 = points.new_empty(plan[3])
+    device = points.get_device()
+    before = _enter(device)
+    try:
+        work = points.new_empty(plan[2], dtype=torch.uint8)
+        capi.call("nsfps_select_blocks_device", plan[1], points.data_ptr(),
+                  0 if lengths is None else lengths.data_ptr(), centers.data_ptr(),
+                  blocks.data_ptr(), d2.data_ptr(), work.data_ptr(), plan[2],
+                  torch._C._cuda_getCurrentRawStream(device))
+    finally:
+        _leave(before)
+    return blocks, d2
 
 
 def _strides(t):
     """Strides of batch, row and head; an axis of one entry is never stepped."""
-    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])])
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
 
 
-@functools.lru_cache(maxsize=256)
-def _make_desc(q_shape, k_shape, top, q_strides, k_strides, v_strides, code, block, scale,
-               backward):
-    B, M, H, D = q_shape
-    three = ctypes.c_int64 * 3
-    desc = capi.AttentionDesc(B, M, k_shape[1], H, k_shape[2], D, block, top, code,
-                              three(*q_strides), three(*k_strides), three(*v_strides), scale, 0)
-    return desc, capi.block_attention_workspace(desc, backward)
+def _needs_copy(t):
+    return t.stride(-1) != 1 or any(s % 8 for s in _strides(t))
 
 
-def _desc(q, k, v, blocks, block, scale, backward):
-    """The call's descriptor and its scratch bytes."""
-    return _make_desc(q.shape, k.shape, blocks.shape[2], _strides(q), _strides(k), _strides(v),
-                      _dtype_code(q, "q", (capi.F16, capi.BF16)), block, scale, backward)
+def _rows16(t, copy):
+    """t with contiguous heads and 16-byte aligned rows: t itself when it is."""
+    if copy:
+        t = t.contiguous()
+    return t.clone(memory_format=_contiguous()) if t.data_ptr() % 16 else t
 
 
-def _forward(q, k, v, blocks, block, lengths, scale, want_lse):
+def _contiguous():
     import torch
-    q, k, v, blocks = _rows16(q), _rows16(k), _rows16(v), blocks.contiguous()
-    len_ptr, _len = _check_lengths(lengths, q.shape[0], q.device)
+    return torch.contiguous_format
+
+
+def _attention_plan(q, k, v, blocks, block, lengths, scale):
+    """Checks a call: (q, k, v to be copied, the arguments of _desc)."""
+    import torch
+    single = isinstance(q, torch.Tensor) and q.dim() == 3
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        code = _dtype_code(t, name, (capi.F16, capi.BF16))
+        if t.dim() != (3 if single else 4):
+            raise ValueError("q: expected shape (M, H, D) or (B, M, H, D), k and v alike")
+        if t.dtype != q.dtype:
+            raise TypeError("q, k and v must have the same type")
+        if t.device != q.device:
+            raise ValueError("q, k and v must be on the same device")
+    if not isinstance(blocks, torch.Tensor) or not blocks.is_cuda or blocks.dtype != torch.int64:
+        raise TypeError("blocks must be an int64 CUDA tensor")
+    if blocks.device != q.device:
+        raise ValueError("blocks must be on q's device")
+    if single:
+        q, k, v, blocks = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), blocks.unsqueeze(0)
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    B, M, H, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("q and k must have the same batch and head size")
+    G = k.shape[2]
+    if not 1 <= H <= 256 or G < 1 or H % G:
+        raise ValueError("q's heads must be a multiple of k's, at most 256")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("the head size must be a multiple of 8 in 8..128")
+    if blocks.dim() != 3 or blocks.shape[:2] != (B, M):
+        raise ValueError("blocks must have shape (M, top) or (B, M, top)")
+    _check_block(block, blocks.shape[2])
+    _check_lengths(lengths, B, q.device)
+    copies = tuple(_needs_copy(t) for t in (q, k, v))
+    # (a copy of a view whose rows begin off a 16-byte boundary is dense, too:
+    # such a view is copied in the call, and its strides are these)
+    dense = [(n * h * D, h * D, D) for n, h in ((M, H), (k.shape[1], G), (k.shape[1], G))]
+    strides = tuple(_strides(t) for t in (q, k, v))
+    head = (B, M, k.shape[1], H, G, D, block, blocks.shape[2], code)
+    return copies, (head, strides, dense, 1.0 / math.sqrt(D) if scale is None else float(scale))
+
+
+def _desc(plan, moved, backward):
+    """The descriptor of a call whose q, k, v lie densely where moved says so:
+    (descriptor, its address, its scratch bytes)."""
+    key = (moved, backward)
+    got = plan[2].get(key)
+    if got is None:
+        head, strides, dense, scale = plan[1]
+        three = ctypes.c_int64 * 3
+        lie = [three(*(d if m else s)) for m, s, d in zip(moved, strides, dense)]
+        desc = capi.AttentionDesc(*head, *lie, scale, 0)
+        got = plan[2][key] = (desc, ctypes.addressof(desc),
+                              capi.block_attention_workspace(desc, backward))
+    return got
+
+
+def _forward(q, k, v, blocks, lengths, plan, want_lse):
+    import torch
+    copies = plan[0]
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (qp | kp | vp) & 15 or copies != (False, False, False):
+        copies = tuple(c or t.data_ptr() % 16 != 0 for c, t in zip(copies, (q, k, v)))
+        q, k, v = (_rows16(t, c) for t, c in zip((q, k, v), copies))
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    blocks = blocks.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
     out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if want_lse else None
-    desc, need = _desc(q, k, v, blocks, block, scale, False)
-    with _on(q) as stream:
+    lse = q.new_empty(q.shape[:-1], dtype=torch.float32) if want_lse else None
+    desc, address, need = _desc(plan, copies, False)
+    device = q.get_device()
+    before = _enter(device)
+    try:
         work = q.new_empty(need, dtype=torch.uint8)
-        capi.block_attention_device(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                    blocks.data_ptr(), len_ptr, out.data_ptr(),
-                                    lse.data_ptr() if want_lse else 0, work.data_ptr(), need,
-                                    stream)
+        capi.call("nsfps_block_attention_device", address, qp, kp, vp, blocks.data_ptr(),
+                  0 if lengths is None else lengths.data_ptr(), out.data_ptr(),
+                  lse.data_ptr() if want_lse else 0, work.data_ptr(), need,
+                  torch._C._cuda_getCurrentRawStream(device))
+    finally:
+        _leave(before)
     return out, lse
 
 
-def _backward(q, k, v, blocks, block, lengths, scale, out, lse, dout):
+def _backward(q, k, v, blocks, lengths, plan, out, lse, dout):
     import torch
-    q, k, v, dout, blocks = _rows16(q), _rows16(k), _rows16(v), dout.contiguous(), blocks.contiguous()
-    dout = _rows16(dout)
-    len_ptr, _len = _check_lengths(lengths, q.shape[0], q.device)
+    copies = tuple(c or t.data_ptr() % 16 != 0 for c, t in zip(plan[0], (q, k, v)))
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    desc, need = _desc(q, k, v, blocks, block, scale, True)
-    with _on(q) as stream:
+    q, k, v = (_rows16(t, c) for t, c in zip((q, k, v), copies))
+    dout, blocks = _rows16(dout, True), blocks.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    desc, address, need = _desc(plan, copies, True)
+    device = q.get_device()
+    before = _enter(device)
+    try:
         work = q.new_empty(need, dtype=torch.uint8)
-        capi.block_attention_grad_device(
-            desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), len_ptr,
-            out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), work.data_ptr(), need, stream)
+        capi.call("nsfps_block_attention_grad_device", address, q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), blocks.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                  out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                  dv.data_ptr(), work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device))
+    finally:
+        _leave(before)
     return dq, dk, dv
 
 
@@ -174,18 +256,18 @@ def _autograd():
 
         class BlockAttention(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, q, k, v, blocks, block, lengths, scale):
-                out, lse = _forward(q, k, v, blocks, block, lengths, scale, True)
+            def forward(ctx, q, k, v, blocks, lengths, plan):
+                out, lse = _forward(q, k, v, blocks, lengths, plan, True)
                 ctx.save_for_backward(q, k, v, blocks, lengths, out, lse)
-                ctx.block, ctx.scale = block, scale
+                ctx.plan = plan
                 return out
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
                 q, k, v, blocks, lengths, out, lse = ctx.saved_tensors
-                grads = _backward(q, k, v, blocks, ctx.block, lengths, ctx.scale, out, lse, dout)
-                return (*grads, None, None, None, None)
+                grads = _backward(q, k, v, blocks, lengths, ctx.plan, out, lse, dout)
+                return (*grads, None, None, None)
 
         _function = BlockAttention
     return _function
@@ -211,41 +293,15 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
     a fixed order.  Inputs whose rows are not 16-byte aligned are copied first.
     """
     import torch
-    single = isinstance(q, torch.Tensor) and q.dim() == 3
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{name} must be a CUDA tensor")
-        _dtype_code(t, name, (capi.F16, capi.BF16))
-        if t.dim() != (3 if single else 4):
-            raise ValueError("q: expected shape (M, H, D) or (B, M, H, D), k and v alike")
-        if t.dtype != q.dtype:
-            raise TypeError("q, k and v must have the same type")
-        if t.device != q.device:
-            raise ValueError("q, k and v must be on the same device")
-    if not isinstance(blocks, torch.Tensor) or not blocks.is_cuda or blocks.dtype != torch.int64:
-        raise TypeError("blocks must be an int64 CUDA tensor")
-    if blocks.device != q.device:
-        raise ValueError("blocks must be on q's device")
-    if single:
-        q, k, v, blocks = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), blocks.unsqueeze(0)
-    if k.shape != v.shape:
-        raise ValueError("k and v must have the same shape")
-    B, M, H, D = q.shape
-    if k.shape[0] != B or k.shape[3] != D:
-        raise ValueError("q and k must have the same batch and head size")
-    G = k.shape[2]
-    if not 1 <= H <= 256 or G < 1 or H % G:
-        raise ValueError("q's heads must be a multiple of k's, at most 256")
-    if D % 8 or not 8 <= D <= 128:
-        raise ValueError("the head size must be a multiple of 8 in 8..128")
-    if blocks.dim() != 3 or blocks.shape[:2] != (B, M):
-        raise ValueError("blocks must have shape (M, top) or (B, M, top)")
     block = int(block)
-    _check_block(block, blocks.shape[2])
-    _check_lengths(lengths, B, q.device)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out = _autograd().apply(q, k, v, blocks, block, lengths, scale)
-    else:
-        out = _forward(q, k, v, blocks, block, lengths, scale, False)[0]
-    return out[0] if single else out
+    try:
+        key = (_look(q), _look(k), _look(v), _look(blocks), _look(lengths), block, scale)
+        plan = _attention_plans.get(key)
+    except AttributeError:  # not tensors
+        key = plan = None
+    if plan is None:
+        copies, shape = _attention_plan(q, k, v, blocks, block, lengths, scale)
+        plan = _attention_plans.keep(key, (copies, shape, {}))
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        return _autograd().apply(q, k, v, blocks, lengths, plan)
+    return _forward(q, k, v, blocks, lengths, plan, False)[0]

@@ -334,7 +334,9 @@ def _feature_functions():
 _feature = None
 
 
-def _call(name, *args):
+def call(name, *args):
+    """A feature entry by name, on plain addresses and sizes; raises
+    RuntimeError when it fails."""
     global _feature
     if _feature is None:
         _feature = _feature_functions()
@@ -345,14 +347,14 @@ def _call(name, *args):
 
 def _bytes(name, *args):
     n = ctypes.c_uint64(0)
-    _call(name, *args, ctypes.addressof(n))
+    call(name, *args, ctypes.addressof(n))
     return n.value
 
 
 def gather_rows_device(desc: RowsDesc, d_table_ptr: int, d_idx_ptr: int, d_out_ptr: int,
                        stream_ptr: int = 0):
     """nsfps_gather_rows_device."""
-    _call("nsfps_gather_rows_device", ctypes.addressof(desc), d_table_ptr, d_idx_ptr, d_out_ptr,
+    call("nsfps_gather_rows_device", ctypes.addressof(desc), d_table_ptr, d_idx_ptr, d_out_ptr,
           stream_ptr)
 
 
@@ -364,7 +366,7 @@ def gather_rows_grad_workspace(desc: RowsDesc) -> int:
 def gather_rows_grad_device(desc: RowsDesc, d_dout_ptr: int, d_idx_ptr: int, d_dtable_ptr: int,
                             d_work_ptr: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_gather_rows_grad_device."""
-    _call("nsfps_gather_rows_grad_device", ctypes.addressof(desc), d_dout_ptr, d_idx_ptr,
+    call("nsfps_gather_rows_grad_device", ctypes.addressof(desc), d_dout_ptr, d_idx_ptr,
           d_dtable_ptr, d_work_ptr, work_bytes, stream_ptr)
 
 
@@ -377,7 +379,7 @@ def select_blocks_device(desc: SelectDesc, d_xyz_ptr: int, d_lengths_ptr: int,
                          d_centers_ptr: int, d_blocks_ptr: int, d_d2_ptr: int, d_work_ptr: int,
                          work_bytes: int, stream_ptr: int = 0):
     """nsfps_select_blocks_device (d_lengths_ptr, d_d2_ptr: 0 for NULL)."""
-    _call("nsfps_select_blocks_device", ctypes.addressof(desc), d_xyz_ptr, d_lengths_ptr,
+    call("nsfps_select_blocks_device", ctypes.addressof(desc), d_xyz_ptr, d_lengths_ptr,
           d_centers_ptr, d_blocks_ptr, d_d2_ptr, d_work_ptr, work_bytes, stream_ptr)
 
 
@@ -390,7 +392,7 @@ def block_attention_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: 
                            out: int, lse: int, work: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_block_attention_device on device addresses (lengths, lse: 0 for
     NULL)."""
-    _call("nsfps_block_attention_device", ctypes.addressof(desc), q, k, v, blocks, lengths, out,
+    call("nsfps_block_attention_device", ctypes.addressof(desc), q, k, v, blocks, lengths, out,
           lse, work, work_bytes, stream_ptr)
 
 
@@ -398,5 +400,5 @@ def block_attention_grad_device(desc: AttentionDesc, q: int, k: int, v: int, blo
                                 lengths: int, out: int, lse: int, dout: int, dq: int, dk: int,
                                 dv: int, work: int, work_bytes: int, stream_ptr: int = 0):
     """nsfps_block_attention_grad_device on device addresses."""
-    _call("nsfps_block_attention_grad_device", ctypes.addressof(desc), q, k, v, blocks, lengths,
+    call("nsfps_block_attention_grad_device", ctypes.addressof(desc), q, k, v, blocks, lengths,
           out, lse, dout, dq, dk, dv, work, work_bytes, stream_ptr)

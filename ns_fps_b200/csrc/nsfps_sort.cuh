@@ -8,8 +8,9 @@
 // in shared memory and writes runs.  The first digit reads the keys from a
 // source object and takes a position's value to be the position itself.
 // Where a list has ten million entries this moves 20 bytes per entry and
-// digit; at the usual hundred thousand it is bound by its launches, which is
-// why it has three per digit and not the five of a general scan.
+// digit; at the usual hundred thousand it is bound by its launches.  So the
+// offsets of few tiles are summed where they are used (two launches per
+// digit), and a list that fits one CTA takes one launch in all.
 #pragma once
 
 #include "nsfps_feature.cuh"
@@ -17,6 +18,13 @@
 namespace nsfps {
 
 constexpr uint32_t kSortThreads = 256, kSortWarps = kSortThreads / 32;
+
+// Lists up to this long are sorted by one CTA in shared memory.
+constexpr uint32_t kSortSmall = 8192, kSmallItems = kSortSmall / 1024;
+constexpr uint32_t kSmallSmem = kSortSmall * 8u + 32u * 256u * 2u;
+
+// Tiles whose counts each CTA of the scatter sums itself.
+constexpr uint32_t kSumTiles = 64;
 
 // Keys per tile: few enough that small lists still spread over the SMs.
 inline uint32_t sort_tile(uint32_t n) { return kSortThreads * (n <= (1u << 19) ? 4u : 16u); }
@@ -113,7 +121,8 @@ template <int ITEMS, class Source>
 __global__ void __launch_bounds__(kSortThreads)
 sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t digit_mask,
              const uint32_t *__restrict__ hist, uint32_t tiles,
-             const uint32_t *__restrict__ total, uint32_t *__restrict__ out_keys,
+             const uint32_t *__restrict__ total,  // null: hist holds counts, not offsets
+             uint32_t *__restrict__ out_keys,
              uint32_t *__restrict__ out_vals, uint32_t *__restrict__ kept) {
   __shared__ uint32_t s_count[kSortWarps][256];
   __shared__ uint32_t s_base[256], s_global[256], s_warp[kSortWarps];
@@ -156,9 +165,24 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   }
   uint32_t in_tile, all;
   const uint32_t base = sort_cta_sum(sum, s_warp, in_tile);
-  const uint32_t before = sort_cta_sum(tid <= digit_mask ? total[tid] : 0u, s_warp, all);
+  uint32_t digits = 0, earlier = 0;  // thread d: keys of digit d, those of earlier tiles
+  if (tid <= digit_mask) {
+    const uint32_t *h = hist + (size_t)tid * tiles;
+    if (total) {
+      digits = total[tid];
+      earlier = h[blockIdx.x];
+    } else {
+#pragma unroll 8
+      for (uint32_t t = 0; t < tiles; ++t) {
+        const uint32_t c = h[t];
+        digits += c;
+        earlier += t < blockIdx.x ? c : 0u;
+      }
+    }
+  }
+  const uint32_t before = sort_cta_sum(digits, s_warp, all);
   s_base[tid] = base;
-  if (tid <= digit_mask) s_global[tid] = before + hist[(size_t)tid * tiles + blockIdx.x];
+  s_global[tid] = before + earlier;
   if (blockIdx.x == 0 && tid == 0 && Source::kFirst) *kept = all;
   __syncthreads();
 #pragma unroll
@@ -181,6 +205,98 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   }
 }
 
+// All digits of a list of at most kSortSmall keys.
+template <class Source>
+__global__ void __launch_bounds__(1024)
+sort_small(const Source src, uint32_t n, uint32_t none, uint32_t passes, uint32_t digit,
+           uint32_t *__restrict__ out_keys, uint32_t *__restrict__ out_vals,
+           uint32_t *__restrict__ kept) {
+  extern __shared__ uint32_t s_small[];
+  uint32_t *s_key = s_small, *s_val = s_small + kSortSmall;
+  uint16_t(*s_count)[256] = reinterpret_cast<uint16_t(*)[256]>(s_small + 2u * kSortSmall);
+  __shared__ uint32_t s_base[256], s_warp[kSortWarps], s_m;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t dm = (1u << digit) - 1u;
+  uint32_t key[kSmallItems], val[kSmallItems], rank[kSmallItems];
+  const uint32_t first = warp * (32u * kSmallItems) + lane;
+#pragma unroll
+  for (uint32_t i = 0; i < kSmallItems; ++i) {
+    const uint32_t at = first + i * 32u;
+    key[i] = at < n ? src.key(at) : none;
+    val[i] = at < n ? src.value(at) : 0u;
+  }
+  uint32_t m = n;
+  for (uint32_t p = 0; p < passes; ++p) {
+    const uint32_t shift = p * digit;
+    if (p) {
+#pragma unroll
+      for (uint32_t i = 0; i < kSmallItems; ++i) {
+        const uint32_t at = first + i * 32u;
+        key[i] = at < m ? s_key[at] : none;
+        val[i] = at < m ? s_val[at] : 0u;
+      }
+    }
+    for (uint32_t x = tid; x < 32u * 256u / 2u; x += 1024u) reinterpret_cast<uint32_t *>(s_count)[x] = 0;
+    __syncthreads();
+    uint16_t *cnt = s_count[warp];
+#pragma unroll
+    for (uint32_t i = 0; i < kSmallItems; ++i) {
+      const bool some = key[i] != none;
+      const uint32_t d = some ? (key[i] >> shift) & dm : 256u;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      rank[i] = __popc(peers & ((1u << lane) - 1u));
+      if (some) rank[i] += cnt[d];
+      __syncwarp();
+      if (some && (peers >> lane) == 1u) cnt[d] += (uint16_t)__popc(peers);  // the last peer
+      __syncwarp();
+    }
+    __syncthreads();
+    if (tid < 256u) {  // (whole warps; the barriers of the sum are theirs)
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (uint32_t w = 0; w < 32u; ++w) {
+        const uint32_t c = s_count[w][tid];
+        s_count[w][tid] = (uint16_t)sum;
+        sum += c;
+      }
+      uint32_t x = sum;
+#pragma unroll
+      for (uint32_t o = 1; o < 32u; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31u) s_warp[warp] = x;
+      s_base[tid] = x - sum;
+    }
+    __syncthreads();
+    if (tid < 256u) {
+      uint32_t before = 0;
+      for (uint32_t w = 0; w < warp; ++w) before += s_warp[w];
+      s_base[tid] += before;
+    }
+    if (tid == 0) {
+      uint32_t all = 0;
+      for (uint32_t w = 0; w < kSortWarps; ++w) all += s_warp[w];
+      s_m = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kSmallItems; ++i) {
+      if (key[i] == none) continue;
+      const uint32_t d = (key[i] >> shift) & dm, at = s_base[d] + cnt[d] + rank[i];
+      s_key[at] = key[i];
+      s_val[at] = val[i];
+    }
+    m = s_m;
+    __syncthreads();
+  }
+  for (uint32_t at = tid; at < m; at += 1024u) {
+    out_keys[at] = s_key[at];
+    out_vals[at] = s_val[at];
+  }
+  if (tid == 0) *kept = m;
+}
+
 // Sorts the positions of src (n of them; keys below `none`, or `none` to be
 // dropped; none > 0).
 template <class Source>
@@ -191,15 +307,25 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
   const uint32_t passes = (bits + 7u) / 8u, digit = (bits + passes - 1u) / passes;
   const uint32_t tile = sort_tile(n), tiles = (uint32_t)ceil_div(n, tile);
   const uint32_t dm = (1u << digit) - 1u;
+  if (n <= kSortSmall) {
+    cudaError_t err = cudaFuncSetAttribute(sort_small<Source>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem);
+    if (err) return err;
+    sort_small<<<1, 1024, kSmallSmem, st>>>(src, n, none, passes, digit, w.keys1, w.vals1, w.kept);
+    *out = SortedList{w.keys1, w.vals1, w.kept};
+    return cudaGetLastError();
+  }
+  const bool few = tiles <= kSumTiles;
   uint32_t *keys = w.keys0, *vals = w.vals0, *keys_next = w.keys1, *vals_next = w.vals1;
   for (uint32_t p = 0; p < passes; ++p) {
     const uint32_t shift = p * digit;
     const StoredKeys stored{keys, vals, w.kept};
 #define NSFPS_SORT_PASS(ITEMS, FROM)                                                              \
     sort_count<ITEMS><<<tiles, kSortThreads, 0, st>>>(FROM, n, none, shift, dm, w.hist, tiles);   \
-    sort_offsets<<<dm + 1u, kSortThreads, 0, st>>>(w.hist, tiles, w.total);                       \
+    if (!few) sort_offsets<<<dm + 1u, kSortThreads, 0, st>>>(w.hist, tiles, w.total);             \
     sort_scatter<ITEMS><<<tiles, kSortThreads, 0, st>>>(FROM, n, none, shift, dm, w.hist, tiles,  \
-                                                        w.total, keys_next, vals_next, w.kept)
+                                                        few ? nullptr : w.total, keys_next,       \
+                                                        vals_next, w.kept)
     if (p == 0) {
       if (tile == 4u * kSortThreads) { NSFPS_SORT_PASS(4, src); }
       else { NSFPS_SORT_PASS(16, src); }

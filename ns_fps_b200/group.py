@@ -19,7 +19,7 @@ per operation without multiply-add contraction, hit iff d2 < radius * radius.
 """
 from __future__ import annotations
 
-import functools
+import ctypes
 
 from . import capi
 
@@ -126,67 +126,98 @@ def _dtype_code(t, name, allowed):
     return code
 
 
-class _on:
-    """The current stream of a tensor's device, with that device current.  (The
-    switch is skipped where it is current already: it costs a small call more
-    than its kernels.)"""
+def _enter(index):
+    """Makes device `index` current; what it was, or None.  (Small calls cost
+    their launches and little else, so the common case is one comparison.)"""
+    import torch
+    before = torch._C._cuda_getDevice()
+    if before == index:
+        return None
+    torch.cuda.set_device(index)
+    return before
 
-    __slots__ = ("index", "guard")
 
-    def __init__(self, t):
-        self.index = t.get_device()
-
-    def __enter__(self):
+def _leave(before):
+    if before is not None:
         import torch
-        self.guard = None
-        if torch._C._cuda_getDevice() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        torch.cuda.set_device(before)
 
 
-@functools.lru_cache(maxsize=256)
-def _rows_desc(B, N, C, P, batch_stride, row_stride, scale, code):
-    return capi.RowsDesc(B, N, C, P, batch_stride, row_stride, scale, code)
+class _Plans(dict):
+    """What a call's shapes, strides and types settle once: its checks, its
+    descriptor, its scratch.  Bounded; a plan holds no tensor."""
+
+    def keep(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
 
 
-@functools.lru_cache(maxsize=256)
-def _rows_grad_desc(B, N, C, P, scale, code):
-    desc = capi.RowsDesc(B, N, C, P, 0, 0, scale, code)
-    return desc, capi.gather_rows_grad_workspace(desc)
+_rows_plans, _rows_grad_plans = _Plans(), _Plans()
 
 
-def _gather_rows_forward(table, idx, scale):
+def _rows_plan(table, idx, scale):
+    """Checks a lookup: (descriptor, its address, shape of the result, whether
+    the table has to be copied)."""
+    import torch
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise TypeError("table must be a CUDA tensor")
+    if not isinstance(idx, torch.Tensor) or not idx.is_cuda or idx.dtype != torch.int64:
+        raise TypeError("idx must be an int64 CUDA tensor")
+    code = _dtype_code(table, "table", _FLOATS)
+    if table.dim() not in (2, 3):
+        raise ValueError("table: expected shape (N, C) or (B, N, C)")
+    if table.dim() == 3 and (idx.dim() < 1 or idx.shape[0] != table.shape[0]):
+        raise ValueError("idx must have shape (B, ...) for a (B, N, C) table")
+    if table.device != idx.device:
+        raise ValueError("table and idx must be on the same device")
     shape = table.shape
     B, N, C = (1, *shape) if len(shape) == 2 else shape
-    if (C > 1 and table.stride(-1) != 1) or C == 0:
+    copy = (C > 1 and table.stride(-1) != 1) or C == 0
+    strides = (N * C, C, 1) if copy else (0, *table.stride())[-3:]
+    desc = capi.RowsDesc(B, N, C, idx.numel() // B if B else 0,
+                         strides[0] if len(shape) == 3 else 0, strides[1], scale, code)
+    return desc, ctypes.addressof(desc), (*idx.shape, C), copy
+
+
+def _gather_rows_forward(table, idx, scale, plan):
+    import torch
+    if plan[3]:
         table = table.contiguous()
     idx = idx.contiguous()
-    out = table.new_empty((*idx.shape, C))
-    strides = table.stride()
-    desc = _rows_desc(B, N, C, idx.numel() // B if B else 0,
-                      strides[0] if len(shape) == 3 else 0, strides[-2], scale,
-                      _dtype_code(table, "table", _FLOATS))
-    with _on(table) as stream:
-        capi.gather_rows_device(desc, table.data_ptr(), idx.data_ptr(), out.data_ptr(), stream)
+    out = table.new_empty(plan[2])
+    device = table.get_device()
+    before = _enter(device)
+    try:
+        capi.call("nsfps_gather_rows_device", plan[1], table.data_ptr(), idx.data_ptr(),
+                  out.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
+    finally:
+        _leave(before)
     return out
 
 
 def _gather_rows_backward(dout, idx, shape, scale):
     import torch
-    B, N, C = (1, *shape) if len(shape) == 2 else shape
     dout, idx = dout.contiguous(), idx.contiguous()
     grad = dout.new_empty(shape)
-    desc, need = _rows_grad_desc(B, N, C, idx.numel() // B if B else 0, scale,
-                                 _dtype_code(dout, "grad", _FLOATS))
-    with _on(dout) as stream:
-        work = dout.new_empty(need, dtype=torch.uint8)
-        capi.gather_rows_grad_device(desc, dout.data_ptr(), idx.data_ptr(), grad.data_ptr(),
-                                     work.data_ptr(), need, stream)
+    key = (shape, idx.shape, scale, dout.dtype)
+    plan = _rows_grad_plans.get(key)
+    if plan is None:
+        B, N, C = (1, *shape) if len(shape) == 2 else shape
+        desc = capi.RowsDesc(B, N, C, idx.numel() // B if B else 0, 0, 0, scale,
+                             _dtype_code(dout, "grad", _FLOATS))
+        plan = _rows_grad_plans.keep(key, (desc, ctypes.addressof(desc),
+                                           capi.gather_rows_grad_workspace(desc)))
+    device = dout.get_device()
+    before = _enter(device)
+    try:
+        work = dout.new_empty(plan[2], dtype=torch.uint8)
+        capi.call("nsfps_gather_rows_grad_device", plan[1], dout.data_ptr(), idx.data_ptr(),
+                  grad.data_ptr(), work.data_ptr(), plan[2],
+                  torch._C._cuda_getCurrentRawStream(device))
+    finally:
+        _leave(before)
     return grad
 
 
@@ -203,16 +234,16 @@ def _gather_rows_autograd():
 
         class GatherRows(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, table, idx, scale):
+            def forward(ctx, table, idx, scale, plan):
                 ctx.save_for_backward(idx)
                 ctx.shape, ctx.scale = table.shape, scale
-                return _gather_rows_forward(table, idx, scale)
+                return _gather_rows_forward(table, idx, scale, plan)
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
                 idx, = ctx.saved_tensors
-                return _gather_rows_backward(dout, idx, ctx.shape, ctx.scale), None, None
+                return _gather_rows_backward(dout, idx, ctx.shape, ctx.scale), None, None, None
 
         _gather_rows_function = GatherRows
     return _gather_rows_function
@@ -233,18 +264,15 @@ def gather_rows(table, idx, scale: float = 1.0):
     waiting for it.
     """
     import torch
-    if not isinstance(table, torch.Tensor) or not table.is_cuda:
-        raise TypeError("table must be a CUDA tensor")
-    if not isinstance(idx, torch.Tensor) or not idx.is_cuda or idx.dtype != torch.int64:
-        raise TypeError("idx must be an int64 CUDA tensor")
-    _dtype_code(table, "table", _FLOATS)
-    if table.dim() not in (2, 3):
-        raise ValueError("table: expected shape (N, C) or (B, N, C)")
-    if table.dim() == 3 and (idx.dim() < 1 or idx.shape[0] != table.shape[0]):
-        raise ValueError("idx must have shape (B, ...) for a (B, N, C) table")
-    if table.device != idx.device:
-        raise ValueError("table and idx must be on the same device")
     scale = float(scale)
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _gather_rows_autograd().apply(table, idx, scale)
-    return _gather_rows_forward(table, idx, scale)
+    try:
+        key = (table.shape, table.stride(), table.dtype, table.device, idx.shape, idx.dtype,
+               idx.device, scale)
+        plan = _rows_plans.get(key)
+    except AttributeError:  # not tensors
+        key = plan = None
+    if plan is None:
+        plan = _rows_plans.keep(key, _rows_plan(table, idx, scale))
+    if table.requires_grad and torch.is_grad_enabled():
+        return _gather_rows_autograd().apply(table, idx, scale, plan)
+    return _gather_rows_forward(table, idx, scale, plan)
