@@ -59,7 +59,8 @@ struct AttnArgs {
   float *part_lse;         // [pair][gc * R], base 2
   float *delta;            // [query][H]
   float *part_kv;          // [share][gc][2][span][D]
-  uint32_t splits;         // direct path: partials per query
+  // direct path: partials per query, rounds per partial, 16-row parts of R
+  uint32_t splits, rounds, row_parts;
 };
 
 __device__ __forceinline__ uint32_t cloud_length(const int32_t *lengths, uint32_t b, uint32_t n) {
@@ -909,61 +910,39 @@ attend_join_direct(const AttnArgs a) {
   if (a.lse && sub == 0) a.lse[row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
 }
 
-// Direct path: a CTA takes kDirectKeys of one query's listed keys and one key
-// head; each warp a run of 16-key slices, joined through shared memory.
+// Direct path: a CTA takes `rounds` times kDirectKeys of one query's listed
+// keys and one key head, the next round's keys in flight; each warp has 16 of
+// a round's keys.  The warps' rows meet in shared memory at the end.
 constexpr uint32_t kDirectKeys = 64;
 constexpr uint32_t kDirectWarps = 4;
+
+template <int DP>
+struct DirectShape {
+  static constexpr uint32_t kSlice = 16u * DP * 2u;            // k or v of a warp's round
+  static constexpr uint32_t kTiles = kDirectWarps * 4u * kSlice;  // two rounds
+  static constexpr uint32_t kJoin = kDirectWarps * 16u * DP * 4u;
+  // (the join lies over the tiles)
+  static constexpr uint32_t kSmem = kTiles > kJoin ? kTiles : kJoin;
+};
 
 template <class T, int DP>
 __global__ void __launch_bounds__(kDirectWarps * 32)
 attend_direct(const AttnArgs a) {
+  using Shape = DirectShape<DP>;
   extern __shared__ __align__(128) char smem[];
-  constexpr uint32_t kSlices = kDirectKeys / 16 / kDirectWarps;  // per warp
-  constexpr uint32_t kTile = 16u * kSlices * DP * 2u;
   __shared__ float s_stat[kDirectWarps][2][16];
+  __shared__ int64_t s_list[64];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t split = blockIdx.x, bm = blockIdx.y, g = blockIdx.z;
+  const uint32_t split = blockIdx.x, bm = blockIdx.y;
+  const uint32_t g = blockIdx.z / a.row_parts, h0 = (blockIdx.z % a.row_parts) * 16u;
   const uint32_t b = bm / a.M, m = bm - b * a.M;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
   const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
   const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-  const uint32_t sk = smem_u32(smem) + warp * 2u * kTile, sv = sk + kTile;
-  const int64_t *list = a.blocks + (uint64_t)bm * a.top;
-
-  uint32_t key[kSlices];
-  bool use[kSlices];
-  bool some = false;
-#pragma unroll
-  for (uint32_t i = 0; i < kSlices; ++i) {
-    const uint32_t at = split * kDirectKeys + (warp * kSlices + i) * 16u;  // of the listed keys
-    const uint32_t s = at >> a.block_log2;
-    use[i] = false;
-    key[i] = 0;
-    if (s < a.top) {
-      const int64_t j = list[s];
-      // an entry that an earlier slot holds already counts for nothing
-      bool again = false;
-      if (lane < s) again = list[lane] == j;
-      if (lane + 32u < s) again = again || list[lane + 32u] == j;
-      again = __any_sync(kFullMask, again);
-      if (!again && j >= 0 && j < (int64_t)a.nb) {
-        key[i] = ((uint32_t)j << a.block_log2) + (at & ((1u << a.block_log2) - 1u));
-        use[i] = key[i] < len;
-      }
-    }
-    some = some || use[i];
-    if (use[i]) {
-      load_keys<DP, 16, 32>(sk + i * 16u * DP * 2u, kh, a.ks[1], key[i], len, a.D, lane);
-      load_keys<DP, 16, 32>(sv + i * 16u * DP * 2u, vh, a.vs[1], key[i], len, a.D, lane);
-    }
-  }
-  copy_commit();
-  copy_wait<0>();
-  __syncwarp();
-  const ScoreScale sc(a.scale);
-  const uint32_t t = lane & 3u;
-  float *s_o = reinterpret_cast<float *>(smem);  // [warp][16][DP], over the tiles
-  for (uint32_t h0 = 0; h0 < a.R; h0 += 16u) {
+  const uint32_t tiles = smem_u32(smem) + warp * 4u * Shape::kSlice;
+  if (tid < 64u) s_list[tid] = tid < a.top ? a.blocks[(uint64_t)bm * a.top + tid] : -1;
+  uint32_t qf[DP / 16][4];
+  {
     const char *qrow[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -972,71 +951,99 @@ attend_direct(const AttnArgs a) {
                                       (int64_t)(g * a.R + hh) * a.qs[2])
                          : nullptr;
     }
-    RowsState<T, DP> st;
-    st.clear();
-    if (some) {
-      uint32_t qf[DP / 16][4];
-      load_rows<DP>(qf, qrow[0], qrow[1], a.D, t);
-      sc.apply(qf);
-#pragma unroll
-      for (uint32_t i = 0; i < kSlices; ++i)
-        if (use[i])
-          st.template add<1>(qf, sk, sv, i * 16u, key[i], len, sc.c2, lane,
-                             [](int) { return true; }, [](int) { return true; },
-                             [](int, int) { return true; });
+    load_rows<DP>(qf, qrow[0], qrow[1], a.D, lane & 3u);
+  }
+  const ScoreScale sc(a.scale);
+  sc.apply(qf);
+  __syncthreads();
+
+  // the warp's first key of round i, or none
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto key_of = [&](uint32_t i) {
+    const uint32_t at = (split * a.rounds + i) * kDirectKeys + warp * 16u;  // of the listed keys
+    const uint32_t s = at >> a.block_log2;
+    if (i >= a.rounds || s >= a.top) return kNone;
+    const int64_t j = s_list[s];
+    // an entry that an earlier slot holds already counts for nothing
+    const bool again = __any_sync(kFullMask, (lane < s && s_list[lane] == j) ||
+                                                 (lane + 32u < s && s_list[lane + 32u] == j));
+    if (again || j < 0 || j >= (int64_t)a.nb) return kNone;
+    const uint32_t key = ((uint32_t)j << a.block_log2) + (at & ((1u << a.block_log2) - 1u));
+    return key < len ? key : kNone;
+  };
+  auto fetch = [&](uint32_t i) {
+    const uint32_t key = key_of(i), to = tiles + (i & 1u) * 2u * Shape::kSlice;
+    if (key != kNone) {
+      load_keys<DP, 16, 32>(to, kh, a.ks[1], key, len, a.D, lane);
+      load_keys<DP, 16, 32>(to + Shape::kSlice, vh, a.vs[1], key, len, a.D, lane);
     }
-    st.finish(sc.c2);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (t == 0) {
-        s_stat[warp][0][(lane >> 2) + 8 * h] = st.mx[h];
-        s_stat[warp][1][(lane >> 2) + 8 * h] = st.sum[h];
-      }
-    if (a.R > 16u) {
-      // the tiles are needed again: the joint buffer lies behind them
-      s_o = reinterpret_cast<float *>(smem + kDirectWarps * 2u * kTile);
+    copy_commit();
+    return key;
+  };
+  RowsState<T, DP> st;
+  st.clear();
+  uint32_t key = fetch(0);
+  for (uint32_t i = 0; i < a.rounds; ++i) {
+    const uint32_t next = fetch(i + 1u);
+    copy_wait<1>();
+    __syncwarp();
+    if (key != kNone) {
+      const uint32_t at = tiles + (i & 1u) * 2u * Shape::kSlice;
+      st.template add<1>(qf, at, at + Shape::kSlice, 0u, key, len, sc.c2, lane,
+                         [](int) { return true; }, [](int) { return true; },
+                         [](int, int) { return true; });
     }
-    __syncthreads();  // statistics written, and every warp is done with its tiles
-    // rows of this m-tile that exist, scaled to the common maximum
+    __syncwarp();
+    key = next;
+  }
+  copy_wait<0>();
+  st.finish(sc.c2);
+  const uint32_t t = lane & 3u;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t r = (lane >> 2) + 8u * h;
-      if (h0 + r >= a.R) continue;
-      float mx = -INFINITY;
-      for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
-      const float c = st.mx[h] == -INFINITY ? 0.f : exp2_fast(st.mx[h] - mx);
+  for (int h = 0; h < 2; ++h)
+    if (t == 0) {
+      s_stat[warp][0][(lane >> 2) + 8 * h] = st.mx[h];
+      s_stat[warp][1][(lane >> 2) + 8 * h] = st.sum[h];
+    }
+  __syncthreads();  // statistics written, and every warp is done with its tiles
+  float *s_o = reinterpret_cast<float *>(smem);  // [warp][16][DP]
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
-        *reinterpret_cast<float2 *>(s_o + (warp * 16u + r) * DP + j * 8 + 2 * t) =
-            make_float2(st.o[j][2 * h] * c, st.o[j][2 * h + 1] * c);
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t r = (lane >> 2) + 8u * h;
+    if (h0 + r >= a.R) continue;
+    float mx = -INFINITY;
+    for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
+    const float c = st.mx[h] == -INFINITY ? 0.f : exp2_fast(st.mx[h] - mx);
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+      *reinterpret_cast<float2 *>(s_o + (warp * 16u + r) * DP + j * 8 + 2 * t) =
+          make_float2(st.o[j][2 * h] * c, st.o[j][2 * h + 1] * c);
+  }
+  __syncthreads();
+  const uint32_t live = min(16u, a.R - h0);
+  for (uint32_t i = tid; i < live * (DP / 4); i += kDirectWarps * 32) {
+    const uint32_t r = i / (DP / 4), d = (i % (DP / 4)) * 4;
+    if (d >= a.D) continue;
+    float mx = -INFINITY, sum = 0.f;
+    for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t w = 0; w < kDirectWarps; ++w) {
+      if (s_stat[w][0][r] == -INFINITY) continue;
+      sum += s_stat[w][1][r] * exp2_fast(s_stat[w][0][r] - mx);
+      const float4 y = *reinterpret_cast<const float4 *>(s_o + (w * 16u + r) * DP + d);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    __syncthreads();
-    const uint32_t live = min(16u, a.R - h0);
-    for (uint32_t i = tid; i < live * (DP / 4); i += kDirectWarps * 32) {
-      const uint32_t r = i / (DP / 4), d = (i % (DP / 4)) * 4;
-      if (d >= a.D) continue;
-      float mx = -INFINITY, sum = 0.f;
-      for (uint32_t w = 0; w < kDirectWarps; ++w) mx = fmaxf(mx, s_stat[w][0][r]);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t w = 0; w < kDirectWarps; ++w) {
-        if (s_stat[w][0][r] == -INFINITY) continue;
-        sum += s_stat[w][1][r] * exp2_fast(s_stat[w][0][r] - mx);
-        const float4 y = *reinterpret_cast<const float4 *>(s_o + (w * 16u + r) * DP + d);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      const uint64_t row = (uint64_t)bm * a.H + g * a.R + h0 + r;
-      if (a.splits == 1u) {
-        *reinterpret_cast<uint2 *>(a.out + (row * a.D + d) * 2) =
-            make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-        if (a.lse && d == 0) a.lse[row] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
-      } else {
-        *reinterpret_cast<float4 *>(a.part + (row * a.splits + split) * a.D + d) =
-            make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        if (d == 0) a.part_lse[row * a.splits + split] = sum > 0.f ? mx + log2f(sum) : -INFINITY;
-      }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const uint64_t row = (uint64_t)bm * a.H + g * a.R + h0 + r;
+    if (a.splits == 1u) {
+      *reinterpret_cast<uint2 *>(a.out + (row * a.D + d) * 2) =
+          make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+      if (a.lse && d == 0) a.lse[row] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+    } else {
+      *reinterpret_cast<float4 *>(a.part + (row * a.splits + split) * a.D + d) =
+          make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      if (d == 0) a.part_lse[row * a.splits + split] = sum > 0.f ? mx + log2f(sum) : -INFINITY;
     }
-    __syncthreads();
   }
 }
 
@@ -1672,7 +1679,7 @@ struct AttnPlan {
   bool direct;
   uint32_t bc;             // clouds per turn
   uint32_t gc;             // key heads per turn
-  uint32_t span_log2, tile_rows, least, splits;
+  uint32_t span_log2, tile_rows, least, splits, rounds;
   uint64_t pairs, spans, max_tiles;  // of one turn
   SortScratch sort;
   uint32_t *mask, *tile_count;
@@ -1697,7 +1704,14 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.bc = (uint32_t)d.batch;
   w.gc = d.kv_heads;
   if (w.direct) {
-    w.splits = (uint32_t)ceil_div((uint64_t)d.top * d.block, kDirectKeys);
+    // as many rounds per CTA as leave six CTAs for every SM, their limit by
+    // shared memory: one query of 1,024 keys takes a round each, 16 of 8,192
+    // keys and heads of 128 four (40 us, with a round each 61: a partial costs
+    // its write, its read and a CTA's start)
+    const uint64_t all = ceil_div((uint64_t)d.top * d.block, kDirectKeys);
+    const uint64_t ctas = all * d.batch * d.queries * d.kv_heads * ceil_div(R, 16);
+    w.rounds = (uint32_t)std::min(all, std::max<uint64_t>(1, ctas / (148 * 6)));
+    w.splits = (uint32_t)ceil_div(all, w.rounds);
     if (w.splits > 1) {
       const uint64_t rows = d.batch * d.queries * d.heads * w.splits;
       w.part = c.take<float>(rows * d.head_dim);
@@ -1754,7 +1768,8 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
   a.tile_stride = (uint32_t)w.max_tiles;
   a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
-  a.part_kv = w.part_kv; a.splits = w.splits; a.gc = w.gc;
+  a.part_kv = w.part_kv; a.splits = w.splits; a.rounds = w.rounds;
+  a.row_parts = (uint32_t)ceil_div(a.R, 16); a.gc = w.gc;
   return a;
 }
 
@@ -1821,9 +1836,10 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
   cudaError_t err;
   if (w.direct) {
     AttnArgs a = all;
-    const uint32_t smem = kDirectKeys * DP * 4u + (a.R > 16 ? kDirectWarps * 16 * DP * 4u : 0u);
+    const uint32_t smem = DirectShape<DP>::kSmem;
     if ((err = opt_in(attend_direct<T, DP>, smem))) return err;
-    attend_direct<T, DP><<<dim3(w.splits, a.B * a.M, a.G), kDirectWarps * 32, smem, st>>>(a);
+    attend_direct<T, DP><<<dim3(w.splits, a.B * a.M, a.G * a.row_parts), kDirectWarps * 32, smem,
+                           st>>>(a);
     if ((err = cudaGetLastError())) return err;
     if (w.splits > 1) {
       const uint64_t rows = (uint64_t)a.B * a.M * a.H;

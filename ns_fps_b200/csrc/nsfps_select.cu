@@ -5,12 +5,14 @@
 // block_boxes reduces each block of points to its box, and each group of 32
 // blocks to one box around theirs.  choose_blocks, one warp per centre, looks
 // at the groups first: rounding is monotone, so a group's distance is never
-// above a block's of it, exactly.  It takes the nearest group for a first list
-// of `top`, then every group that is not beyond the list's last distance, and
-// keeps the list sorted over the lanes.  Distances are never negative or NaN,
-// so (distance bits, index) order as one 64-bit key, lower indices first among
-// equals.  (Scanning every block cost 3.6 ns of the machine per centre over 512
-// blocks, most of it insertions; the order by groups leaves few.)
+// above a block's of it, exactly.  The nearest groups give a bound on the
+// `top`-th distance; the blocks of all groups within it are looked at in index
+// order, and those within it are listed.  Then the minimum is taken out of the
+// list `top` times.  Distances are never negative or NaN, so their bits order
+// as integers, and a list in index order gives the lower index among equals
+// first.  What it costs is instructions: for 512 blocks and top 16 about 900
+// per centre (a list kept sorted by insertion took 1,500, one over all blocks
+// without groups 4,000).
 #include <algorithm>
 
 #include "nsfps_feature.cuh"
@@ -19,7 +21,7 @@ namespace nsfps {
 namespace {
 
 constexpr uint32_t kFullMask = 0xffffffffu;
-constexpr uint64_t kNoKey = (uint64_t)0x7f800001u << 32;  // above +inf: an empty slot
+constexpr uint32_t kNoDist = 0xffffffffu;  // above every distance
 
 struct SelectArgs {
   const float *xyz, *centers;
@@ -98,83 +100,65 @@ __device__ __forceinline__ uint32_t box_distance(const float *__restrict__ box, 
       __fadd_rn(__fadd_rn(__fmul_rn(dx, dx), __fmul_rn(dy, dy)), __fmul_rn(dz, dz)));
 }
 
-__device__ __forceinline__ uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
-__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a < b ? b : a; }
+constexpr int kAhead = 4;            // group distances in flight per lane
+constexpr int kNear = 4;             // groups that the bound is taken from
+constexpr uint32_t kListMax = 128;   // candidates listed per centre
+constexpr int kListRegs = kListMax / 32;
 
-// Ascending sort of one key per lane; from_stage 32 merges a sequence that
-// rises and then falls.
-template <int FROM>
-__device__ __forceinline__ uint64_t sort_lanes(uint64_t v, uint32_t lane) {
-#pragma unroll
-  for (uint32_t k = FROM; k <= 32u; k <<= 1)
-#pragma unroll
-    for (uint32_t j = k >> 1; j; j >>= 1) {
-      const uint64_t o = __shfl_xor_sync(kFullMask, v, j);
-      const bool up = (lane & k) == 0u, low = (lane & j) == 0u;
-      v = (low == up) ? min64(v, o) : max64(v, o);
-    }
-  return v;
-}
+// The candidates of a centre, in shared memory: distance bits and block, in an
+// order that has the lower block first among equal distances.
+struct Candidates {
+  uint32_t *d, *j;
+  uint32_t n;
 
-// The smallest keys so far, ascending over lane + 32 * slot.
-template <int SLOTS>
-struct BestList {
-  uint64_t v[SLOTS];
-  __device__ __forceinline__ void clear() {
+  // Takes the minimum out `count` times: afterwards lane i has the place and
+  // distance of the i-th (and with SLOTS 2 of the 32 + i-th).
+  template <int SLOTS>
+  __device__ __forceinline__ void smallest(uint32_t count, uint32_t lane, uint32_t (&place)[SLOTS],
+                                           uint32_t (&dist)[SLOTS]) const {
+    uint32_t v[kListRegs];
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) v[s] = kNoKey;
-  }
-  __device__ __forceinline__ uint64_t limit(uint32_t top) const {
-    return __shfl_sync(kFullMask, v[SLOTS - 1], (top - 1u) & 31u);
-  }
-  __device__ __forceinline__ void insert(uint64_t c, uint32_t lane) {
-    uint32_t at = 0;
+    for (int r = 0; r < kListRegs; ++r) v[r] = lane + 32u * r < n ? d[lane + 32u * r] : kNoDist;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) at += __popc(__ballot_sync(kFullMask, v[s] < c));
-    uint64_t carry = 0;
+    for (int s = 0; s < SLOTS; ++s) place[s] = 0u, dist[s] = kNoDist;
+    for (uint32_t i = 0; i < count; ++i) {
+      uint32_t m = v[0];
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const uint64_t last = __shfl_sync(kFullMask, v[s], 31);
-      uint64_t up = __shfl_up_sync(kFullMask, v[s], 1);
-      if (lane == 0u) up = carry;
-      const uint32_t me = lane + 32u * s;
-      v[s] = me > at ? up : me == at ? c : v[s];
-      carry = last;
-    }
-  }
-  // One key per lane (kNoKey: none), all different from the list's.  Few are
-  // inserted one by one (about 15 instructions each); many are sorted and
-  // merged (about 200).
-  __device__ __forceinline__ void offer(uint64_t c, uint32_t top, uint32_t lane, uint64_t &lim) {
-    uint32_t want = __ballot_sync(kFullMask, c < lim);
-    if (__popc(want) > 10) {
-      uint64_t x = sort_lanes<2>(c, lane);
+      for (int r = 1; r < kListRegs; ++r)
+        if (32u * r < n) m = min(m, v[r]);
+      m = __reduce_min_sync(kFullMask, m);
+      uint32_t at = 0;
 #pragma unroll
-      for (int s = 0; s < SLOTS; ++s) {
-        const uint64_t y = __shfl_sync(kFullMask, x, 31u - lane);
-        const uint64_t lo = min64(v[s], y), hi = max64(v[s], y);
-        v[s] = sort_lanes<32>(lo, lane);
-        if (s + 1 < SLOTS) x = sort_lanes<32>(hi, lane);
+      for (int r = kListRegs - 1; r >= 0; --r) {
+        if (32u * r >= n) continue;
+        const uint32_t who = __ballot_sync(kFullMask, v[r] == m);
+        if (who) at = 32u * r + __ffs(who) - 1u;
       }
-      lim = limit(top);
-      return;
-    }
-    while (want) {
-      const int src = __ffs(want) - 1;
-      insert(__shfl_sync(kFullMask, c, src), lane);
-      lim = limit(top);
-      want &= __ballot_sync(kFullMask, c < lim) & ~((2u << src) - 1u);
+#pragma unroll
+      for (int r = 0; r < kListRegs; ++r)
+        if (at == lane + 32u * r) v[r] = kNoDist;
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s)
+        if (i == lane + 32u * s) place[s] = at, dist[s] = m;
     }
   }
 };
 
-constexpr int kAhead = 4;  // group distances in flight per lane
+// Clouds of at most this many blocks: every distance is computed once and held
+// in registers, without groups.  For 512 blocks and top 16 that is 750
+// instructions per centre where the groups take 1,500 (most of 16 groups are
+// within the bound); for 1,920 blocks the groups take less than the distances
+// alone.
+constexpr int kHeldRegs = 16;
+constexpr uint32_t kHeldBlocks = 32 * kHeldRegs;
 
-template <int SLOTS>
+// SLOTS: 32-entry parts of the result.
+template <int SLOTS, bool HELD>
 __global__ void __launch_bounds__(256)
 choose_blocks(const SelectArgs a) {
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint32_t c = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  __shared__ uint32_t s_d[8][kListMax], s_j[8][kListMax];
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  const uint32_t c = blockIdx.x * (blockDim.x >> 5) + warp;
   if (c >= a.B * a.m) return;
   const uint32_t b = c / a.m;
   const uint32_t len = cloud_length(a.lengths, b, a.n);
@@ -184,68 +168,126 @@ choose_blocks(const SelectArgs a) {
               z = a.centers[3 * (uint64_t)c + 2];
   const uint64_t groups = (uint64_t)a.B * a.ng;
   const float *gbox = a.group + (uint64_t)b * a.ng, *bbox = a.box + (uint64_t)b * a.ng * 32u;
-  BestList<SLOTS> best;
-  best.clear();
-  uint64_t lim = kNoKey;
-  auto take = [&](uint32_t g) {
-    const uint32_t j = g * 32u + lane;
-    uint64_t key = kNoKey;
-    if (j < nv) key = (uint64_t)box_distance(bbox, groups * 32u, j, x, y, z) << 32 | j;
-    best.offer(key, a.top, lane, lim);
+  auto block_distance = [&](uint32_t j) {
+    return j < nv ? box_distance(bbox, groups * 32u, j, x, y, z) : kNoDist;
   };
-  // the nearest groups, until the list is full
-  uint32_t done[SLOTS + 1];
+
+  // A bound on the top-th distance: of the nearest groups' blocks each lane
+  // keeps its smallest distance (with SLOTS 2 the smallest of every other
+  // group); `top` of these are as many blocks within their top-th.
+  uint32_t limit = 0x7f800000u;
+  uint32_t held[HELD ? kHeldRegs : 1];
+  if (HELD) {
 #pragma unroll
-  for (int i = 0; i <= SLOTS; ++i) {
-    done[i] = 0xffffffffu;
-    if (i && lim != kNoKey) continue;
-    uint64_t near = ~0ull;
-    for (uint32_t g0 = 0; g0 < ng; g0 += 32u * kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const uint32_t g = g0 + u * 32u + lane;
-        bool free = g < ng;
-#pragma unroll
-        for (int k = 0; k < i; ++k) free = free && g != done[k];
-        if (free) near = min64(near, (uint64_t)box_distance(gbox, groups, g, x, y, z) << 32 | g);
-      }
+    for (int r = 0; r < kHeldRegs; ++r) {
+      held[r] = kNoDist;
+      if (32u * r < nv) held[r] = block_distance(32u * r + lane);
     }
-    const uint32_t d = __reduce_min_sync(kFullMask, (uint32_t)(near >> 32));
-    if (d == 0xffffffffu) continue;  // no group is left
-    done[i] = __reduce_min_sync(kFullMask, (uint32_t)(near >> 32) == d ? (uint32_t)near : ~0u);
-    take(done[i]);
   }
-  // every other group that may hold a nearer block
-  for (uint32_t g0 = 0; g0 < ng; g0 += 32u * kAhead) {
-    uint32_t d[kAhead];
+  if (nv > a.top) {
+    uint32_t done[kNear], v[SLOTS];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) v[s] = kNoDist;
+    if (HELD) {
+#pragma unroll
+      for (int r = 0; r < kHeldRegs; ++r) v[r % SLOTS] = min(v[r % SLOTS], held[r]);
+    }
+#pragma unroll
+    for (int i = 0; i < (HELD ? 0 : kNear); ++i) {
+      uint32_t near = kNoDist, who = kNoDist;
+      for (uint32_t g0 = 0; g0 < ng; g0 += 32u) {
+        const uint32_t g = g0 + lane;
+        uint32_t d = g < ng ? box_distance(gbox, groups, g, x, y, z) : kNoDist;
+#pragma unroll
+        for (int k = 0; k < i; ++k)
+          if (g == done[k]) d = kNoDist;
+        if (d < near) near = d, who = g;
+      }
+      const uint32_t d = __reduce_min_sync(kFullMask, near);
+      done[i] = __reduce_min_sync(kFullMask, near == d ? who : kNoDist);
+      if (d == kNoDist) continue;  // no group is left
+      v[i % SLOTS] = min(v[i % SLOTS], block_distance(done[i] * 32u + lane));
+    }
+    // the smallest 15-bit prefix that `top` of the lanes do not exceed (all
+    // bits set where fewer have a block)
+    uint32_t prefix = 0;
+#pragma unroll
+    for (int bit = 30; bit >= 16; --bit) {
+      const uint32_t below = prefix | (1u << bit);  // first value with this bit
+      uint32_t count = 0;
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) count += __popc(__ballot_sync(kFullMask, v[s] < below));
+      if (count < a.top) prefix = below;
+    }
+    limit = min(prefix | 0xffffu, limit);
+  }
+
+  // The blocks within the bound, in index order.
+  Candidates list{s_d[warp], s_j[warp], 0u};
+  uint32_t place[SLOTS], dist[SLOTS];
+  bool open = true;  // false: nothing further can be nearer
+  auto add = [&](uint32_t d, uint32_t j0) {  // blocks j0 .. j0 + 31
+    const uint32_t in = __ballot_sync(kFullMask, d <= limit);
+    if (!in) return;
+    if (d <= limit) {
+      const uint32_t at = list.n + __popc(in & ((1u << lane) - 1u));
+      list.d[at] = d;
+      list.j[at] = j0 + lane;
+    }
+    list.n += __popc(in);
+    __syncwarp();
+    if (list.n + 32u <= kListMax) return;
+    // the list is full: keep its best, in order (what follows has higher
+    // indices, so from here on only smaller distances matter)
+    list.smallest<SLOTS>(a.top, lane, place, dist);
+    uint32_t j[SLOTS];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) j[s] = list.j[place[s]];
+    __syncwarp();
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+      if (lane + 32u * s < a.top) list.d[lane + 32u * s] = dist[s], list.j[lane + 32u * s] = j[s];
+    __syncwarp();
+    list.n = a.top;
+    const uint32_t last = list.d[a.top - 1u];
+    open = last != 0u;
+    limit = last - 1u;
+  };
+  if (HELD) {
+#pragma unroll
+    for (int r = 0; r < kHeldRegs; ++r)
+      if (32u * r < nv && open) add(held[r], 32u * r);
+  }
+  for (uint32_t g0 = 0; !HELD && g0 < ng && open; g0 += 32u * kAhead) {
+    uint32_t gd[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const uint32_t g = g0 + u * 32u + lane;
-      d[u] = 0xffffffffu;
-      bool free = g < ng;
-#pragma unroll
-      for (int k = 0; k <= SLOTS; ++k) free = free && g != done[k];
-      if (free) d[u] = box_distance(gbox, groups, g, x, y, z);
+      gd[u] = kNoDist;
+      if (g0 + u * 32u >= ng) continue;
+      gd[u] = g < ng ? box_distance(gbox, groups, g, x, y, z) : kNoDist;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      // (an equal distance may go with a lower index)
-      uint32_t want = __ballot_sync(kFullMask, d[u] <= (uint32_t)(lim >> 32));
-      while (want) {
-        const int src = __ffs(want) - 1;
-        take(g0 + u * 32u + src);
-        want &= __ballot_sync(kFullMask, d[u] <= (uint32_t)(lim >> 32)) & ~((2u << src) - 1u);
+      if (g0 + u * 32u >= ng) break;
+      uint32_t want = __ballot_sync(kFullMask, gd[u] <= limit);
+      while (want && open) {
+        const uint32_t g = g0 + u * 32u + __ffs(want) - 1u;
+        want &= want - 1u;
+        add(block_distance(g * 32u + lane), g * 32u);
+        want &= __ballot_sync(kFullMask, gd[u] <= limit);
       }
     }
   }
+  const uint32_t found = min(a.top, list.n);
+  list.smallest<SLOTS>(found, lane, place, dist);
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const uint32_t i = lane + 32u * s;
     if (i >= a.top) continue;
-    const bool some = best.v[s] < kNoKey;
     const uint64_t o = (uint64_t)c * a.top + i;
-    a.out[o] = some ? (int64_t)(uint32_t)best.v[s] : -1;
-    if (a.out_d2) a.out_d2[o] = __uint_as_float(some ? (uint32_t)(best.v[s] >> 32) : 0x7f800000u);
+    a.out[o] = i < found ? (int64_t)list.j[place[s]] : -1;
+    if (a.out_d2) a.out_d2[o] = __uint_as_float(i < found ? dist[s] : 0x7f800000u);
   }
 }
 
@@ -254,7 +296,11 @@ cudaError_t launch_choose(const SelectArgs &a, cudaStream_t st) {
   // one warp per CTA while there is an SM for each centre, up to eight
   const uint32_t centres = a.B * a.m;
   const uint32_t warps = std::min(8u, std::max(1u, centres / (uint32_t)sm_count()));
-  choose_blocks<SLOTS><<<(uint32_t)ceil_div(centres, warps), warps * 32u, 0, st>>>(a);
+  const uint32_t grid = (uint32_t)ceil_div(centres, warps);
+  if (ceil_div(a.n, 1ull << a.block_log2) <= kHeldBlocks)
+    choose_blocks<SLOTS, true><<<grid, warps * 32u, 0, st>>>(a);
+  else
+    choose_blocks<SLOTS, false><<<grid, warps * 32u, 0, st>>>(a);
   return cudaGetLastError();
 }
 
