@@ -103,7 +103,6 @@ __device__ __forceinline__ uint32_t box_distance(const float *__restrict__ box, 
 constexpr int kAhead = 4;            // group distances in flight per lane
 constexpr int kNear = 4;             // groups that the bound is taken from
 constexpr uint32_t kListMax = 128;   // candidates listed per centre
-constexpr int kListRegs = kListMax / 32;
 
 // The candidates of a centre, in shared memory: distance bits and block, in an
 // order that has the lower block first among equal distances.
@@ -111,36 +110,31 @@ struct Candidates {
   uint32_t *d, *j;
   uint32_t n;
 
-  // Takes the minimum out `count` times: afterwards lane i has the place and
-  // distance of the i-th (and with SLOTS 2 of the 32 + i-th).
-  template <int SLOTS>
-  __device__ __forceinline__ void smallest(uint32_t count, uint32_t lane, uint32_t (&place)[SLOTS],
-                                           uint32_t (&dist)[SLOTS]) const {
-    uint32_t v[kListRegs];
-#pragma unroll
-    for (int r = 0; r < kListRegs; ++r) v[r] = lane + 32u * r < n ? d[lane + 32u * r] : kNoDist;
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s) place[s] = 0u, dist[s] = kNoDist;
-    for (uint32_t i = 0; i < count; ++i) {
-      uint32_t m = v[0];
-#pragma unroll
-      for (int r = 1; r < kListRegs; ++r)
-        if (32u * r < n) m = min(m, v[r]);
-      m = __reduce_min_sync(kFullMask, m);
-      uint32_t at = 0;
-#pragma unroll
-      for (int r = kListRegs - 1; r >= 0; --r) {
-        if (32u * r >= n) continue;
-        const uint32_t who = __ballot_sync(kFullMask, v[r] == m);
-        if (who) at = 32u * r + __ffs(who) - 1u;
+  // Calls f(rank, distance, block) for every candidate, one per lane and turn;
+  // the rank is the number of candidates before it in (distance, place) order,
+  // found by comparing with all of them, which for the usual 25 is cheaper than
+  // any sort.
+  template <class F>
+  __device__ __forceinline__ void ranked(uint32_t lane, F f) const {
+    for (uint32_t base = 0; base < n; base += 32u) {
+      const uint32_t me = base + lane;
+      const bool some = me < n;
+      const uint32_t mine = some ? d[me] : kNoDist, block = some ? j[me] : 0u;
+      uint32_t rank = 0;
+      for (uint32_t k = 0; k < n; k += 4u) {
+        const uint4 o = *reinterpret_cast<const uint4 *>(d + k);  // (unused places hold kNoDist)
+        rank += o.x < mine + (k < me) ? 1u : 0u;
+        rank += o.y < mine + (k + 1u < me) ? 1u : 0u;
+        rank += o.z < mine + (k + 2u < me) ? 1u : 0u;
+        rank += o.w < mine + (k + 3u < me) ? 1u : 0u;
       }
-#pragma unroll
-      for (int r = 0; r < kListRegs; ++r)
-        if (at == lane + 32u * r) v[r] = kNoDist;
-#pragma unroll
-      for (int s = 0; s < SLOTS; ++s)
-        if (i == lane + 32u * s) place[s] = at, dist[s] = m;
+      f(some, rank, mine, block);
     }
+  }
+  // Fills the places up to a multiple of four.
+  __device__ __forceinline__ void pad(uint32_t lane) {
+    if (lane < 4u) d[n + lane] = kNoDist;
+    __syncwarp();
   }
 };
 
@@ -156,7 +150,7 @@ constexpr uint32_t kHeldBlocks = 32 * kHeldRegs;
 template <int SLOTS, bool HELD>
 __global__ void __launch_bounds__(256)
 choose_blocks(const SelectArgs a) {
-  __shared__ uint32_t s_d[8][kListMax], s_j[8][kListMax];
+  __shared__ __align__(16) uint32_t s_d[8][kListMax + 4], s_j[8][kListMax];
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   const uint32_t c = blockIdx.x * (blockDim.x >> 5) + warp;
   if (c >= a.B * a.m) return;
@@ -224,7 +218,6 @@ choose_blocks(const SelectArgs a) {
 
   // The blocks within the bound, in index order.
   Candidates list{s_d[warp], s_j[warp], 0u};
-  uint32_t place[SLOTS], dist[SLOTS];
   bool open = true;  // false: nothing further can be nearer
   auto add = [&](uint32_t d, uint32_t j0) {  // blocks j0 .. j0 + 31
     const uint32_t in = __ballot_sync(kFullMask, d <= limit);
@@ -239,14 +232,18 @@ choose_blocks(const SelectArgs a) {
     if (list.n + 32u <= kListMax) return;
     // the list is full: keep its best, in order (what follows has higher
     // indices, so from here on only smaller distances matter)
-    list.smallest<SLOTS>(a.top, lane, place, dist);
-    uint32_t j[SLOTS];
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s) j[s] = list.j[place[s]];
+    list.pad(lane);
+    uint32_t rank[kListMax / 32], dist[kListMax / 32], block[kListMax / 32];
+    int turn = 0;
+    list.ranked(lane, [&](bool some, uint32_t r, uint32_t d, uint32_t j) {
+      rank[turn] = some ? r : kNoDist;
+      dist[turn] = d;
+      block[turn++] = j;
+    });
     __syncwarp();
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s)
-      if (lane + 32u * s < a.top) list.d[lane + 32u * s] = dist[s], list.j[lane + 32u * s] = j[s];
+    for (int i = 0; i < (int)kListMax / 32; ++i)
+      if (i < turn && rank[i] < a.top) list.d[rank[i]] = dist[i], list.j[rank[i]] = block[i];
     __syncwarp();
     list.n = a.top;
     const uint32_t last = list.d[a.top - 1u];
@@ -280,14 +277,16 @@ choose_blocks(const SelectArgs a) {
     }
   }
   const uint32_t found = min(a.top, list.n);
-  list.smallest<SLOTS>(found, lane, place, dist);
-#pragma unroll
-  for (int s = 0; s < SLOTS; ++s) {
-    const uint32_t i = lane + 32u * s;
-    if (i >= a.top) continue;
-    const uint64_t o = (uint64_t)c * a.top + i;
-    a.out[o] = i < found ? (int64_t)list.j[place[s]] : -1;
-    if (a.out_d2) a.out_d2[o] = __uint_as_float(i < found ? dist[s] : 0x7f800000u);
+  const uint64_t to = (uint64_t)c * a.top;
+  list.pad(lane);
+  list.ranked(lane, [&](bool some, uint32_t rank, uint32_t d, uint32_t j) {
+    if (!some || rank >= a.top) return;
+    a.out[to + rank] = (int64_t)j;
+    if (a.out_d2) a.out_d2[to + rank] = __uint_as_float(d);
+  });
+  for (uint32_t i = found + lane; i < a.top; i += 32u) {
+    a.out[to + i] = -1;
+    if (a.out_d2) a.out_d2[to + i] = __uint_as_float(0x7f800000u);
   }
 }
 
