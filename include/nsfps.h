@@ -328,7 +328,10 @@ NSFPS_API int nsfps_select_blocks_device(const nsfps_select_desc *desc, const fl
  * blocks that blocks[b][m][0 .. top) lists.  The list is a set: an entry that
  * occurs again, is negative or names no block of the cloud counts for nothing.
  * A query without a key gets zeros (and no gradient).  What lies behind a
- * cloud's length is never part of a result, whatever its value.
+ * cloud's length, in blocks that no query of the cloud lists, or in rows of
+ * queries that list nothing, is never part of a result, whatever its value;
+ * what is listed has to be finite (a value that is not may also reach results
+ * of queries and keys nearby that do not list it).
  * q, k and v: F16 or BF16, elements of a head contiguous, 16-byte aligned, the
  * strides (batch, row, head, in elements) multiples of 8.  blocks (batch x
  * queries x top int64), out (batch x queries x heads x head_dim) and lse

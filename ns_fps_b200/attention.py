@@ -283,7 +283,8 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
              set of blocks of ``block`` consecutive keys; entries that are
              negative, repeated, or name no block count for nothing
     lengths  None, or int32 (B,): the keys of each padded cloud; what lies
-             behind them is never read into a result
+             behind them, or in blocks that no query lists, is never part of a
+             result.  Values that are listed have to be finite.
     scale    default 1 / sqrt(D)
 
     D is a multiple of 8 up to 128, H at most 256.  Returns a tensor like q,

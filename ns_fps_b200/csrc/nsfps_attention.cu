@@ -49,6 +49,7 @@ struct AttnArgs {
   const uint32_t *mask;    // per query slot: blocks of the span that are listed
   const unsigned long long *lead;  // per query: bit s = slot s leads a pair
   const uint32_t *skeys;   // their sort keys: span, then the chunks read
+  const uint4 *listed;     // per span: 16 bytes, 1 for each block that some query lists
   const uint4 *span;       // per span: first pair, end, first share, tiles
   const uint4 *tiles;      // by cost: (span, tile within it, first pair, pairs of the span)
   uint32_t tile_stride;    // places per cost class
@@ -201,9 +202,8 @@ template <int SLOTS>  // 32-slot parts of a list
 __global__ void __launch_bounds__(256)
 plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
            uint32_t *__restrict__ mask, unsigned long long *__restrict__ lead,
-           uint32_t *__restrict__ tile_count) {
+           uint8_t *__restrict__ listed) {
   const uint32_t lane = threadIdx.x & 31u;
-  if (blockIdx.x == 0 && threadIdx.x <= kTileClasses) tile_count[threadIdx.x] = 0;  // for plan_spans
   const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (bm >= a.B * a.M) return;
   const uint32_t b = bm / a.M;
@@ -221,6 +221,8 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
     bit[i] = use ? 1u << ((uint32_t)j & ((1u << in_log2) - 1u)) : 0u;
     m[i] = 0u;
     lead_of[i] = none;
+    // (every query that lists the block stores the same byte)
+    if (use) listed[16u * (b * a.nsb + sb[i]) + ((uint32_t)j & ((1u << in_log2) - 1u))] = 1u;
   }
 #pragma unroll
   for (int part = SLOTS - 1; part >= 0; --part) {
@@ -303,6 +305,12 @@ plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, ui
     const uint32_t c = kTileClasses - 1u - min(cost, kTileClasses - 1u);
     tiles[(uint64_t)c * tile_stride + atomicAdd(tile_count + c, 1u)] = make_uint4(s, i, b, e - b);
   }
+}
+
+// A span's marks as bits.
+__device__ __forceinline__ uint32_t marked(const uint4 &x) {
+  auto four = [](uint32_t y) { return (y * 0x10204080u) >> 28; };  // bytes of 0 or 1
+  return four(x.x) | four(x.y) << 4 | four(x.z) << 8 | four(x.w) << 12;
 }
 
 // The tiles, dear ones first.
@@ -529,11 +537,15 @@ __device__ __forceinline__ void load_rows_by(uint32_t dst, uint32_t D, uint32_t 
   }
 }
 
-// The same for rows `stride` bytes apart, the first `live` of them; zeros
-// behind.
+// The same for keys `stride` bytes apart: those below `live` of the blocks that
+// `blocks` names (bit r >> block_log2), zeros for the others.  Whatever lies in
+// a block that no query lists meets weights of zero, and must not be a NaN.
 template <int DP, uint32_t ROWS, uint32_t THREADS>
 __device__ __forceinline__ void load_strided(uint32_t dst, uint32_t D, uint32_t tid,
-                                             const char *first, int64_t stride, uint32_t live) {
+                                             const char *first, int64_t stride, uint32_t live,
+                                             uint32_t blocks, uint32_t block_log2) {
+  const uint32_t n = ROWS >> block_log2, every = n ? (1u << n) - 1u : 1u;
+  const bool all = (blocks & every) == every;
   constexpr uint32_t kChunks = DP / 8, kStep = THREADS / kChunks;
   const uint32_t c = tid % kChunks, r0 = tid / kChunks;
   const uint32_t at = dst + (c >> 3) * (ROWS * 128u) + swizzled(r0, c & 7u);
@@ -541,7 +553,8 @@ __device__ __forceinline__ void load_strided(uint32_t dst, uint32_t D, uint32_t 
   const bool in = c * 8u < D;
 #pragma unroll
   for (uint32_t i = 0; i < ROWS / kStep; ++i) {
-    const bool some = in && r0 + i * kStep < live;
+    const uint32_t r = r0 + i * kStep;
+    const bool some = in && r < live && (all || ((blocks >> (r >> block_log2)) & 1u));
     copy16(at + i * kStep * 128u, some ? p : first, some);
     p += (int64_t)kStep * stride;
   }
@@ -594,9 +607,11 @@ attend_tiles(const AttnArgs a) {
   struct Row {
     uint32_t pair, head, read;
     bool live;
+    uint32_t listed;  // of the tile's span
   };
   auto row_of = [&](const uint4 &tile) {
-    Row x{0xffffffffu, 0u, 0u, false};
+    Row x{0xffffffffu, 0u, 0u, false, 0u};
+    if (tile.w) x.listed = marked(a.listed[tile.x]);
     const uint32_t r = tile.y * kTileRows + tid;
     x.live = r < tile.w * a.R;
     if (x.live) {
@@ -620,6 +635,7 @@ attend_tiles(const AttnArgs a) {
     // this thread's row, and the chunks that any row reads
     const uint32_t pair = mine.pair, head = mine.head;
     const bool live_row = mine.live;
+    const uint32_t listed = mine.listed;
     uint32_t read = mine.read & ((1u << kChunkBits) - 1u), mask = 0u;
     read ^= read >> 1;  // from the place in the Gray code
     const char *q = nullptr;
@@ -642,12 +658,15 @@ attend_tiles(const AttnArgs a) {
     auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
       if (some) {
         const uint32_t key = key0 + c * 64u, live = key < len ? len - key : 0u;
+        const uint32_t blocks = listed >> ((c * 64u) >> a.block_log2);
         const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
         // (a chunk wholly behind the end reads nothing, but its address is formed)
         load_strided<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid,
-                                           kh + (live ? (int64_t)key * ks : 0), ks, live);
+                                           kh + (live ? (int64_t)key * ks : 0), ks, live, blocks,
+                                           a.block_log2);
         load_strided<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid,
-                                           vh + (live ? (int64_t)key * vs : 0), vs, live);
+                                           vh + (live ? (int64_t)key * vs : 0), vs, live, blocks,
+                                           a.block_log2);
       }
       copy_commit();
     };
@@ -1250,12 +1269,13 @@ attend_grad(const AttnArgs a) {
                               make_float2(c2, c2), make_float2(-z.x, -z.z));
               f.x = exp2_fast(f.x);
               f.y = exp2_fast(f.y);
+              float2 g = mul2(f, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
+                                      make_float2(-z.y, -z.w)));
               if (!all) {
-                f.x = (in >> y) & 1u ? f.x : 0.f;
-                f.y = (in >> (y + 1u)) & 1u ? f.y : 0.f;
+                const bool in0 = (in >> y) & 1u, in1 = (in >> (y + 1u)) & 1u;
+                f.x = in0 ? f.x : 0.f, g.x = in0 ? g.x : 0.f;
+                f.y = in1 ? f.y : 0.f, g.y = in1 ? g.y : 0.f;
               }
-              const float2 g = mul2(f, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
-                                            make_float2(-z.y, -z.w)));
               p16[y / 2u] = pack2<T>(f.x, f.y);
               e16[y / 2u] = pack2<T>(g.x, g.y);
             }
@@ -1306,8 +1326,10 @@ attend_grad(const AttnArgs a) {
         const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
         const char *kh = a.k + 2 * ((int64_t)x.b * a.ks[0] + (int64_t)x.g * a.ks[2]) + x.key0 * ks;
         const char *vh = a.v + 2 * ((int64_t)x.b * a.vs[0] + (int64_t)x.g * a.vs[2]) + x.key0 * vs;
-        load_strided<DP, 128, 128>(sk, a.D, role_tid, kh, ks, x.len - x.key0);
-        load_strided<DP, 128, 128>(sk + Shape::kKeyTile, a.D, role_tid, vh, vs, x.len - x.key0);
+        const uint32_t blocks = marked(a.listed[x.span]), live = x.len - x.key0;
+        load_strided<DP, 128, 128>(sk, a.D, role_tid, kh, ks, live, blocks, a.block_log2);
+        load_strided<DP, 128, 128>(sk + Shape::kKeyTile, a.D, role_tid, vh, vs, live, blocks,
+                                   a.block_log2);
         copy_commit();
         advance(later);
         return true;
@@ -1671,7 +1693,9 @@ int padded_dim(uint32_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 constexpr uint32_t kGradSpanLog2 = 7;  // one key per lane of tensor memory
 
 // Partials of a pass stay below this, by taking the key heads, then the clouds
-// of a call, in turns.
+// of a call, in turns.  Turns small enough to keep their partials in L2 cost
+// more in launches and half-empty waves than they save: a scan's attention
+// took 199 us in one turn, 207 in two, 267 in four.
 constexpr uint64_t kMaxPartBytes = 1ull << 30;
 
 // How a call is cut up, and its scratch.
@@ -1683,6 +1707,7 @@ struct AttnPlan {
   uint64_t pairs, spans, max_tiles;  // of one turn
   SortScratch sort;
   uint32_t *mask, *tile_count;
+  uint8_t *listed;
   uint4 *span;
   unsigned long long *lead;
   uint4 *tiles;
@@ -1690,10 +1715,16 @@ struct AttnPlan {
   uint64_t bytes;
 };
 
-// Forward calls whose queries would not fill the machine's tiles go the direct
-// way: it reads each query's keys once per query instead of once per tile.
+// The direct path reads each query's keys once per query, the tiles once per
+// 128 of them, behind a sort.  Up to some 200 MB of keys the former is less:
+// 64 queries of 8 heads and 1,024 keys of 64 (134 MB) took 28 us direct and 34
+// by tiles, 128 queries (268 MB) 37 and 38, 512 queries 135 and 47; 1,024
+// queries of 4 heads and 64 keys (67 MB) 23 and 31, 4,096 (268 MB) 84 and 39;
+// one query 4 and 24.
 bool takes_direct(const nsfps_attention_desc &d) {
-  return d.batch * d.queries * d.kv_heads <= 512 && d.batch * d.queries <= 65535;
+  const uint64_t keys = std::min<uint64_t>((uint64_t)d.top * d.block, d.keys);
+  return d.batch * d.queries <= 65535 &&
+         d.batch * d.queries * d.kv_heads * keys * d.head_dim * 4 <= 200000000;
 }
 
 AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base) {
@@ -1740,7 +1771,9 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.mask = c.take<uint32_t>(w.pairs);
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
   w.span = c.take<uint4>(w.spans);
-  w.tile_count = c.take<uint32_t>(kTileClasses + 1);
+  static_assert(4 * (kTileClasses + 1) <= 32, "the marks begin 32 bytes behind");
+  w.tile_count = (uint32_t *)c.take<char>(32 + 16 * w.spans);
+  w.listed = (uint8_t *)w.tile_count + (base ? 32 : 0);
   w.tiles = c.take<uint4>(kTileClasses * w.max_tiles);
   w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
@@ -1766,6 +1799,7 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   a.scale = d.scale;
   a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
   a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
+  a.listed = (const uint4 *)w.listed;
   a.tile_stride = (uint32_t)w.max_tiles;
   a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
   a.part_kv = w.part_kv; a.splits = w.splits; a.rounds = w.rounds;
@@ -1797,19 +1831,20 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   const uint32_t shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
   SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
+  // (the tile counters and the spans' marks, cleared together)
+  if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + 16 * (uint64_t)spans, st))) return err;
   if (n && spans) {
     const uint32_t grid = (uint32_t)ceil_div(a.B * a.M, 8);
     if (a.top <= 32)
       plan_pairs<1><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
-                                          w.tile_count);
+                                          w.listed);
     else
       plan_pairs<2><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
-                                          w.tile_count);
+                                          w.listed);
     if ((err = cudaGetLastError())) return err;
     if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
   } else {  // no pair, or no key to form one with
     if ((err = cudaMemsetAsync(w.sort.kept, 0, 4, st))) return err;
-    if ((err = cudaMemsetAsync(w.tile_count, 0, 4 * (kTileClasses + 1), st))) return err;
     if (a.B * a.M &&
         (err = cudaMemsetAsync(w.lead, 0, sizeof(*w.lead) * (uint64_t)a.B * a.M, st)))
       return err;

@@ -163,6 +163,33 @@ def test_padded_clouds_and_lists_that_name_nothing(block):
     assert not out[1].any() and not out[:, 4::7].any()
 
 
+@pytest.mark.parametrize("M", [40, 6000])  # the direct path and the tiles
+@pytest.mark.parametrize("block", [16, 64])
+def test_blocks_that_nobody_lists_are_never_part_of_a_result(M, block):
+    """NaN and infinities beside listed blocks, and in rows of q and dout whose
+    query lists nothing; q, k and v gradients zero there and right elsewhere."""
+    from ns_fps_b200 import attention
+    B, N, H, G, D = 1, 1000, 4, 2, 64
+    q, k, v = _normal((B, M, H, D), torch.bfloat16, 1), _normal((B, N, G, D), torch.bfloat16, 2), \
+        _normal((B, N, G, D), torch.bfloat16, 3)
+    nb = (N + block - 1) // block
+    blocks = _lists(B, M, nb, 5, 4)
+    blocks[blocks % 2 == 1] = -1  # odd blocks: not listed
+    blocks[:, ::9] = -1
+    dout = _normal(q.shape, torch.bfloat16, 5)
+    ref = Exact(q, k, v, blocks, block, None, None, dout)
+    odd = (torch.arange(N, device="cuda") // block) % 2 == 1
+    k[:, odd], v[:, odd] = math.nan, math.inf
+    q[:, ::9], dout[:, ::9] = math.nan, math.inf
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention.block_attention(*leaves, blocks, block)
+    got = (out.detach(), *torch.autograd.grad(out, leaves, dout))
+    for g, name in zip(got, ("out", "dq", "dk", "dv")):
+        off = (g.double() - getattr(ref, name)).abs()
+        assert bool((off <= getattr(ref, name + "_off")).all()), name
+    assert not got[2][:, odd].any() and not got[3][:, odd].any() and not got[0][:, ::9].any()
+
+
 def test_every_query_lists_the_same_block():
     q, k, v = _normal((1, 5000, 2, 64), torch.bfloat16, 1), \
         _normal((1, 100, 1, 64), torch.bfloat16, 2), _normal((1, 100, 1, 64), torch.bfloat16, 3)
