@@ -1858,21 +1858,13 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// More than 48 KB a CTA, static shared memory included, has to be asked for.
-template <class K>
-cudaError_t opt_in(K kernel, uint32_t smem) {
-  return smem <= 40u << 10 ? cudaSuccess
-                           : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  (int)smem);
-}
-
 template <class T, int DP>
 cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
   cudaError_t err;
   if (w.direct) {
     AttnArgs a = all;
     const uint32_t smem = DirectShape<DP>::kSmem;
-    if ((err = opt_in(attend_direct<T, DP>, smem))) return err;
+    if ((err = opt_in<attend_direct<T, DP>>(smem))) return err;
     attend_direct<T, DP><<<dim3(w.splits, a.B * a.M, a.G * a.row_parts), kDirectWarps * 32, smem,
                            st>>>(a);
     if ((err = cudaGetLastError())) return err;
@@ -1884,7 +1876,7 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
   }
   constexpr int TP = DP < 64 ? 64 : DP;  // the tiles' rows are 64 or 128 elements
   const uint32_t smem = TileShape<TP>::kSmem;
-  if ((err = opt_in(attend_tiles<T, TP>, smem))) return err;
+  if ((err = opt_in<attend_tiles<T, TP>>(smem))) return err;
   const uint64_t resident = (uint64_t)sm_count() * TileShape<TP>::kCtas;
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);
@@ -1909,7 +1901,7 @@ template <class T, int DP>
 cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t st) {
   cudaError_t err;
   const uint32_t smem = GradShape<DP>::kSmem;
-  if ((err = opt_in(attend_grad<T, DP>, smem))) return err;
+  if ((err = opt_in<attend_grad<T, DP>>(smem))) return err;
   const uint64_t resident = (uint64_t)sm_count();
   for (uint32_t b0 = 0; b0 < all.B; b0 += w.bc) {
     AttnArgs a = turn_args(all, b0, w.bc);

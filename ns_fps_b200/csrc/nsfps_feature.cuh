@@ -7,6 +7,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "nsfps_internal.cuh"
 #include "nsfps_kernels.h"
 
@@ -35,11 +38,36 @@ struct WorkCarver {
 
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
-inline int sm_count() {
-  int dev = 0, sms = 148;
+// What a launch asks of the current device, once per device (up to 64).
+inline int current_device() {
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return dev;
+}
+
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  const int dev = current_device();
+  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
+}
+
+// More than 48 KB of shared memory a CTA, the static included, has to be asked
+// for, per kernel (hence the template) and device.
+template <auto Kernel>
+cudaError_t opt_in(uint32_t smem) {
+  if (smem <= 40u << 10) return cudaSuccess;
+  static std::atomic<uint64_t> asked;
+  const int dev = current_device();
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (asked.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t err =
+      cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (err == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return err;
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }

@@ -19,8 +19,11 @@ namespace nsfps {
 
 constexpr uint32_t kSortThreads = 256, kSortWarps = kSortThreads / 32;
 
-// Lists up to this long are sorted by one CTA in shared memory.
-constexpr uint32_t kSortSmall = 8192, kSmallItems = kSortSmall / 1024;
+// Lists up to this long are sorted by one CTA in shared memory.  On the GPU
+// alone that is within a tenth of the launches per digit at 4,096 keys (a whole
+// row gradient of 4,000 entries, 25 us and 23; of 8,000, 35 and 23); in a
+// program that waits for its launches it saves three to five of them.
+constexpr uint32_t kSortSmall = 4096, kSmallItems = kSortSmall / 1024;
 constexpr uint32_t kSmallSmem = kSortSmall * 8u + 32u * 256u * 2u;
 
 // Tiles whose counts each CTA of the scatter sums itself.
@@ -308,8 +311,7 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
   const uint32_t tile = sort_tile(n), tiles = (uint32_t)ceil_div(n, tile);
   const uint32_t dm = (1u << digit) - 1u;
   if (n <= kSortSmall) {
-    cudaError_t err = cudaFuncSetAttribute(sort_small<Source>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem);
+    const cudaError_t err = opt_in<sort_small<Source>>(kSmallSmem);
     if (err) return err;
     sort_small<<<1, 1024, kSmallSmem, st>>>(src, n, none, passes, digit, w.keys1, w.vals1, w.kept);
     *out = SortedList{w.keys1, w.vals1, w.kept};
