@@ -627,70 +627,96 @@ attend_tiles(const AttnArgs a) {
   if (blockIdx.x < work) tile = order[blockIdx.x / a.gc];
   if (blockIdx.x + step < work) tile_next = order[(blockIdx.x + step) / a.gc];
   Row mine = row_of(tile);
-  for (uint32_t w = blockIdx.x; w < work; w += step) {
-    const uint32_t gi = w % a.gc, g = a.g0 + gi;
-    const uint32_t b = tile.x / a.nsb, sb = tile.x - b * a.nsb;
-    const uint32_t len = cloud_length(a.lengths, b, a.N);
-    const uint32_t key0 = sb << kSpanLog2;
-    // this thread's row, and the chunks that any row reads
-    const uint32_t pair = mine.pair, head = mine.head;
-    const bool live_row = mine.live;
-    const uint32_t listed = mine.listed;
-    uint32_t read = mine.read & ((1u << kChunkBits) - 1u), mask = 0u;
+  struct Tile {
+    uint32_t gi, key0, len, listed, todo;  // todo: chunks that some row reads
+    const char *kh, *vh;
+    uint32_t pair, head, mask;             // this thread's row
+    bool live;
+  };
+  // Takes the next tile: puts its rows' places and chunks into shared memory
+  // (todo is known behind a barrier) and asks for the one after it.
+  auto open = [&](uint32_t w) {
+    Tile x;
+    const uint32_t b = tile.x / a.nsb, g = a.g0 + w % a.gc;
+    x.gi = w % a.gc;
+    x.key0 = (tile.x - b * a.nsb) << kSpanLog2;
+    x.len = cloud_length(a.lengths, b, a.N);
+    x.listed = mine.listed;
+    x.kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
+    x.vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
+    x.pair = mine.pair;
+    x.head = mine.head;
+    x.live = mine.live;
+    x.mask = 0u;
+    uint32_t read = mine.read & ((1u << kChunkBits) - 1u);
     read ^= read >> 1;  // from the place in the Gray code
     const char *q = nullptr;
-    if (live_row) {
-      mask = a.mask[pair];
-      const uint32_t m = pair / a.top - b * a.M;
+    if (x.live) {
+      x.mask = a.mask[x.pair];
+      const uint32_t m = x.pair / a.top - b * a.M;
       q = a.q + 2 * ((int64_t)b * a.qs[0] + (int64_t)m * a.qs[1] +
-                     (int64_t)(g * a.R + head) * a.qs[2]);
+                     (int64_t)(g * a.R + x.head) * a.qs[2]);
     }
+    read = __reduce_or_sync(kFullMask, read);
+    if (lane == 0) s_any[warp] = read;
+    s_q[tid] = q;
     tile = tile_next;
     mine = row_of(tile);
     if (w + 2u * step < work) tile_next = order[(w + 2u * step) / a.gc];
-    const uint32_t warp_read = __reduce_or_sync(kFullMask, read);
-    if (lane == 0) s_any[warp] = warp_read;
-    s_q[tid] = q;
-    __syncthreads();
-    uint32_t todo = warp_value(s_any[0] | s_any[1] | s_any[2] | s_any[3]);
-    const char *kh = a.k + 2 * ((int64_t)b * a.ks[0] + (int64_t)g * a.ks[2]);
-    const char *vh = a.v + 2 * ((int64_t)b * a.vs[0] + (int64_t)g * a.vs[2]);
-    auto fetch = [&](uint32_t c, uint32_t buf, bool some) {
-      if (some) {
-        const uint32_t key = key0 + c * 64u, live = key < len ? len - key : 0u;
-        const uint32_t blocks = listed >> ((c * 64u) >> a.block_log2);
-        const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
-        // (a chunk wholly behind the end reads nothing, but its address is formed)
-        load_strided<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid,
-                                           kh + (live ? (int64_t)key * ks : 0), ks, live, blocks,
-                                           a.block_log2);
-        load_strided<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid,
-                                           vh + (live ? (int64_t)key * vs : 0), vs, live, blocks,
-                                           a.block_log2);
-      }
-      copy_commit();
-    };
-    uint32_t ahead = todo;
-    load_rows_by<DP, kTileRows, kTileThreads>(sq, a.D, tid, a.q,
-                                              [&](uint32_t x) { return s_q[x]; });
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {  // (q goes with the first chunk)
-      fetch(__ffs(ahead) - 1, i, ahead != 0);
-      ahead &= ahead - 1u;
+    return x;
+  };
+  auto fetch = [&](const Tile &x, uint32_t c, uint32_t buf, bool some) {
+    if (some) {
+      const uint32_t key = x.key0 + c * 64u, live = key < x.len ? x.len - key : 0u;
+      const uint32_t blocks = x.listed >> ((c * 64u) >> a.block_log2);
+      const int64_t ks = a.ks[1] * 2, vs = a.vs[1] * 2;
+      // (a chunk wholly behind the end reads nothing, but its address is formed)
+      load_strided<DP, 64, kTileThreads>(sk + buf * Shape::kChunk, a.D, tid,
+                                         x.kh + (live ? (int64_t)key * ks : 0), ks, live, blocks,
+                                         a.block_log2);
+      load_strided<DP, 64, kTileThreads>(sv + buf * Shape::kChunk, a.D, tid,
+                                         x.vh + (live ? (int64_t)key * vs : 0), vs, live, blocks,
+                                         a.block_log2);
     }
+    copy_commit();
+  };
+  // (behind a barrier) the tile's q and first chunk, one group; then the second
+  uint32_t ahead = 0;  // chunks not yet asked for
+  auto load_first = [&](Tile &x, uint32_t buf) {
+    x.todo = warp_value(s_any[0] | s_any[1] | s_any[2] | s_any[3]);
+    ahead = x.todo;
+    load_rows_by<DP, kTileRows, kTileThreads>(sq, a.D, tid, a.q, [&](uint32_t r) { return s_q[r]; });
+    fetch(x, __ffs(ahead) - 1, buf, ahead != 0);
+    ahead &= ahead - 1u;
+  };
+  auto load_second = [&](const Tile &x, uint32_t buf) {
+    fetch(x, __ffs(ahead) - 1, buf, ahead != 0);
+    ahead &= ahead - 1u;
+  };
+  Tile now{}, coming{};
+  uint32_t buf = 0;  // of the chunk at hand
+  if (blockIdx.x < work) {
+    now = open(blockIdx.x);
+    __syncthreads();
+    load_first(now, 0u);
+    load_second(now, 1u);
+  }
+  for (uint32_t w = blockIdx.x; w < work; w += step) {
+    const bool another = w + step < work;
+    const uint32_t key0 = now.key0, len = now.len, mask = now.mask;
     const uint32_t warp_any = __reduce_or_sync(kFullMask, mask);
-    const uint32_t warp_all = __reduce_and_sync(kFullMask, q ? mask : ~0u);
+    const uint32_t warp_all = __reduce_and_sync(kFullMask, now.live ? mask : ~0u);
     float ref = -INFINITY, sum = 0.f;  // reference maximum of the signed raw scores
-    for (uint32_t i = 0; todo; ++i) {
-      const uint32_t c = __ffs(todo) - 1, buf = i & 1u;
-      todo &= todo - 1u;
+    for (uint32_t i = 0; now.todo; ++i) {
+      const uint32_t c = __ffs(now.todo) - 1;
+      now.todo &= now.todo - 1u;
       if (i) {
         // the chunk before is used up: its buffers take the next but one
+        buf ^= 1u;
         if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
         __syncwarp();
         tmem_after_sync();
-        fetch(__ffs(ahead) - 1, buf ^ 1u, ahead != 0);
-        ahead &= ahead - 1u;
+        load_second(now, buf ^ 1u);
       }
       copy_wait<1>();
       smem_to_mma();
@@ -783,6 +809,8 @@ attend_tiles(const AttnArgs a) {
       part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
       sum += part[0].x + part[0].y;
       tmem_st32(tm_s + my, s[0]);
+      const bool last = another && !now.todo;
+      if (last) coming = open(w + step);
       tmem_st_wait();
       tmem_before_sync();
       __syncthreads();
@@ -796,11 +824,17 @@ attend_tiles(const AttnArgs a) {
       }
       __syncwarp();
       phase ^= 1u;
+      // the next tile's loads go before this one's results: q is used up, and
+      // so is the other buffer
+      if (last) load_first(coming, buf ^ 1u);
     }
     if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
     __syncwarp();
     tmem_after_sync();
-    const uint64_t row = (uint64_t)pair * (a.gc * a.R) + gi * a.R + head;
+    if (another) load_second(coming, buf);
+    buf ^= 1u;
+    const bool live_row = now.live;
+    const uint64_t row = (uint64_t)now.pair * (a.gc * a.R) + now.gi * a.R + now.head;
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
     for (uint32_t j = 0; j < DP / 32; ++j) {
@@ -816,10 +850,11 @@ attend_tiles(const AttnArgs a) {
     if (live_row)  // (a wait that ran out shows as NaN)
       a.part_lse[row] = failed ? __int_as_float(0x7fc00000)
                         : sum > 0.f ? fmaf(ref, c2, log2f(sum)) : -INFINITY;
-    tmem_before_sync();
-    __syncthreads();  // every thread is done with the tiles and the output
-    tmem_after_sync();
+    now = coming;  // (the output is read before the barriers of the next chunk)
   }
+  tmem_before_sync();
+  __syncthreads();
+  tmem_after_sync();
   if (warp == 0) tmem_free<Shape::kTmem>(tm);
 }
 
