@@ -190,6 +190,36 @@ def test_blocks_that_nobody_lists_are_never_part_of_a_result(M, block):
     assert not got[2][:, odd].any() and not got[3][:, odd].any() and not got[0][:, ::9].any()
 
 
+def test_long_lists():
+    """More pairs than a pass of short tiles sorts, in two clouds."""
+    q, k, v = _normal((2, 20_000, 1, 16), torch.bfloat16, 1), \
+        _normal((2, 500, 1, 16), torch.bfloat16, 2), _normal((2, 500, 1, 16), torch.bfloat16, 3)
+    _check(q, k, v, _lists(2, 20_000, 32, 14, 4), 16)
+
+
+def test_calls_taken_in_turns_equal_calls_apart():
+    """A call whose partial results pass the limit takes its heads, then its
+    clouds, in turns; each cloud and head by itself gives the same bits."""
+    from ns_fps_b200 import attention
+    B, M, N, H, D, top, block = 5, 40_000, 2000, 2, 128, 16, 16
+    q, k, v, dout = (_normal((B, n, H, D), torch.bfloat16, i)
+                     for i, n in enumerate((M, N, N, M)))
+    blocks = _lists(B, M, (N + block - 1) // block, top, 9)
+
+    def step(*x):
+        leaves = [t.detach().requires_grad_() for t in x[:3]]
+        out = attention.block_attention(*leaves, x[3], block)
+        return (out.detach(), *torch.autograd.grad(out, leaves, x[4]))
+
+    all_at_once = step(q, k, v, blocks, dout)
+    for b in (0, B - 1):
+        for h in range(H):
+            part = step(*(t[b:b + 1, :, h:h + 1] for t in (q, k, v)), blocks[b:b + 1],
+                        dout[b:b + 1, :, h:h + 1])
+            for x, y in zip(all_at_once, part):
+                assert torch.equal(x[b:b + 1, :, h:h + 1], y)
+
+
 def test_every_query_lists_the_same_block():
     q, k, v = _normal((1, 5000, 2, 64), torch.bfloat16, 1), \
         _normal((1, 100, 1, 64), torch.bfloat16, 2), _normal((1, 100, 1, 64), torch.bfloat16, 3)

@@ -117,6 +117,18 @@ def test_gradient_of_a_row_that_many_entries_name(count):
     assert torch.equal(grad.double(), ref)
 
 
+@pytest.mark.parametrize("count,N", [(70_001, 9), (90_000, 70_001), (600_011, 70_001),
+                                     (530_000, 200)])
+def test_gradient_of_long_lists(count, N):
+    """Lists of many tiles and of two and three digits; whole numbers, exact."""
+    from ns_fps_b200 import group
+    table = torch.zeros(N, 3, device="cuda", requires_grad=True)
+    idx = _idx((count,), N, lo=-N // 50 - 1)
+    dout = _idx((count, 3), 4, seed=3).float()
+    grad, = torch.autograd.grad(group.gather_rows(table, idx), table, dout)
+    assert torch.equal(grad.double(), _backward(dout, idx, (N, 3), 1.0)[0])
+
+
 def test_indices_that_name_no_row():
     from ns_fps_b200 import group
     table = _table(2, 6, 5, torch.float32).requires_grad_()
