@@ -2,22 +2,28 @@
 // query, and its gradient.
 //
 // A query reads few keys, and neighbouring queries read the same ones, so the
-// work is turned round: the keys are cut into spans of kSpan consecutive keys,
-// and every (query, span) pair that shares a key is sorted by span.  A CTA
-// takes a run of pairs of one span, gathers their query rows into matrix
-// tiles, and meets the span's keys once for all of them (mma.sync on 16-bit
-// operands, fp32 accumulators).  Each pair leaves a partial result in fp32
-// (its normalised output and log-sum-exp; in the gradient its share of dq),
-// and a last kernel joins the partials of a query.  No atomics: every partial
-// has one writer, and the sort is stable, so dk and dv add up in one order.
+// work is turned round: the keys are cut into spans of 256 consecutive keys (of
+// 128 in the gradient), and every (query, span) pair that shares a key is
+// sorted by span.  A CTA takes a run of pairs of one span, gathers their query
+// rows into a matrix tile, and meets the span's keys once for all of them
+// (tcgen05.mma on 16-bit operands, fp32 in tensor memory).  Each pair leaves a
+// partial result in fp32 (its normalised output and log-sum-exp; in the
+// gradient its share of dq), and a last kernel joins the partials of a query.
+// No atomics in a sum: every partial has one writer, and the sort is stable, so
+// dk and dv add up in one order.
 //
 // What bounds it: per pair and head the tile products cost 4 * D * keys
 // operations against 8 * D bytes of partials (written and read), so the
-// partials and the softmax, not the matrix unit, set the pace; wide spans make
-// the pairs fewer.
+// partials, the softmax and the way to the tiles, not the matrix unit, set the
+// pace (its share of the time is 13 % forward, 15 % in the gradient).  Of a
+// scan's 200 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
+// tiles take 109, the join 42 (132 MB of partials, 3.2 TB/s), the plan 35; the
+// floor is 22 by bytes.  Spans of 512 keys make that call 3 % faster, not enough
+// for the second plan that the smaller calls would then want.
 //
 // A handful of queries does not fill tiles and would wait for the sort; they
-// take a direct path, which splits each query's own keys over CTAs.
+// take a direct path, which splits each query's own keys over CTAs (mma.sync,
+// whose 16-row tiles suit a query's few heads; the keys' bytes bound it).
 #include <algorithm>
 #include <cmath>
 
@@ -271,8 +277,8 @@ struct PairKeys {
 
 // One warp per span: its pairs, and its tiles of tile_rows rows (at least
 // `least`), listed by cost.  CTAs take the tiles in turns, so with the dear
-// ones first the turns come out even (unsorted, the longest CTA of the
-// gradient had 1.4 times the mean).  A tile's place in its class comes from a
+// ones first the turns come out even (the gradient of shared heads took 53 us
+// unsorted, 38 sorted).  A tile's place in its class comes from a
 // counter and differs from run to run; no result depends on it.  Spans of
 // several tiles get places for their tiles' shares of dk and dv, in order.
 __global__ void __launch_bounds__(256)
@@ -502,9 +508,11 @@ struct RowsState {
 // that some row reads: s = q k^T (128 x 64) by the tensor core into tensor
 // memory, the thread takes its row's scores out, makes the weights, puts them
 // back as 16-bit values over the scores, and o += p v takes them from there.
-// Nothing but the operands' tiles passes through shared memory.  The softmax
-// (one exp2 per score, 16 per cycle and SM) bounds it; while one CTA waits for
-// its products or its loads, the others of the SM compute.
+// Nothing but the operands' tiles passes through shared memory.  Four CTAs an
+// SM (two with heads of 128): while one waits for its products or its loads,
+// the others compute.  A scan's 5,104 tiles take 109 us, 4,200 cycles each and
+// SM, of which the instructions of the softmax and the loads are 45 %; with
+// mma.sync and scores in registers it was 182.
 constexpr uint32_t kTileThreads = 128;
 
 // The reference maximum moves only when a row's maximum outgrows it by this
@@ -861,7 +869,8 @@ attend_tiles(const AttnArgs a) {
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
 // its leading slots.  A warp takes 128 consecutive elements of a query's heads,
 // four per lane: the slots are the same for all lanes, and what a slot's
-// partial holds of them is consecutive too.
+// partial holds of them is consecutive too.  A scan's 132 MB of partials, read
+// in the queries' order, take 42 us.
 template <class T>
 __global__ void __launch_bounds__(256)
 attend_join(const AttnArgs a, uint32_t parts) {
@@ -1103,7 +1112,8 @@ attend_direct(const AttnArgs a) {
 
 // -------------------------------------------------------------- gradient
 
-// delta = sum_d dout * out per row; 8 lanes per row, 8 elements per step.
+// delta = sum_d dout * out per row; 8 lanes per row, 8 elements per step; bound
+// by the bytes of the two.
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_delta(const AttnArgs a) {
@@ -1166,9 +1176,13 @@ struct GradItem {
 //
 // Done in turns by all warps, the stages of a step took 11,000 cycles, of
 // which the weights were 2,500.  So the warps have roles and meet at barriers:
-// eight make weights, three load a step's rows each (the loads of three steps
+// sixteen make weights, three load a step's rows each (the loads of three steps
 // are in the air), four take dq, dk and dv out, and one issues the products,
-// the next step's scores before this step's gradients.
+// the next step's scores before this step's gradients.  Four clouds (16,384
+// queries, 8 heads of 64) took 210 us without roles and take 128 (the matrix
+// unit 15 % busy, memory 19 %: what is left is the way of a step from barrier to
+// barrier, with the gather of 128 rows of q and dout in it), shared heads
+// (2,048 queries, 16 heads of 128 over 4) 62 and 35.
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
@@ -1658,7 +1672,7 @@ grad_join_keys(const AttnArgs a, uint32_t span) {
 }
 
 // dq of a query: the shares of its pairs, slots in order; lanes as in
-// attend_join.
+// attend_join, and bound as it is (24 us for the four clouds).
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_join_queries(const AttnArgs a, uint32_t parts) {
@@ -1770,10 +1784,10 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.bc = (uint32_t)d.batch;
   w.gc = d.kv_heads;
   if (w.direct) {
-    // as many rounds per CTA as leave six CTAs for every SM, their limit by
-    // shared memory: one query of 1,024 keys takes a round each, 16 of 8,192
-    // keys and heads of 128 four (40 us, with a round each 61: a partial costs
-    // its write, its read and a CTA's start)
+    // as many rounds per CTA as leave six CTAs for every SM: one query of 1,024
+    // keys takes a round each, 16 of 8,192 keys and heads of 128 four (40 us in
+    // all, with a round each 61: a partial costs its write, its read and a
+    // CTA's start; 134 MB of keys come at 4.2 TB/s)
     const uint64_t all = ceil_div((uint64_t)d.top * d.block, kDirectKeys);
     const uint64_t ctas = all * d.batch * d.queries * d.kv_heads * ceil_div(R, 16);
     w.rounds = (uint32_t)std::min(all, std::max<uint64_t>(1, ctas / (148 * 6)));

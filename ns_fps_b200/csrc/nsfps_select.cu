@@ -10,9 +10,9 @@
 // order, and those within it are listed.  Then the minimum is taken out of the
 // list `top` times.  Distances are never negative or NaN, so their bits order
 // as integers, and a list in index order gives the lower index among equals
-// first.  What it costs is instructions: for 512 blocks and top 16 about 900
-// per centre (a list kept sorted by insertion took 1,500, one over all blocks
-// without groups 4,000).
+// first.  What bounds it is instructions: 131,072 centres over 512 blocks and
+// top 16 take 160 us (a list kept sorted by insertion over all blocks 469, by
+// groups 260), 16,384 centres over 1,920 blocks 54 (203, 76).
 #include <algorithm>
 
 #include "nsfps_feature.cuh"
@@ -139,10 +139,10 @@ struct Candidates {
 };
 
 // Clouds of at most this many blocks: every distance is computed once and held
-// in registers, without groups.  For 512 blocks and top 16 that is 750
-// instructions per centre where the groups take 1,500 (most of 16 groups are
-// within the bound); for 1,920 blocks the groups take less than the distances
-// alone.
+// in registers, without groups.  For 512 blocks and top 16, where most of the
+// 16 groups are within the bound, 32 clouds took 233 us so and 267 by groups;
+// for 1,920 blocks the distances alone would be more than the groups' whole
+// work.
 constexpr int kHeldRegs = 16;
 constexpr uint32_t kHeldBlocks = 32 * kHeldRegs;
 

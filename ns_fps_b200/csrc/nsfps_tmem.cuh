@@ -153,16 +153,6 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// (all warps of a group of four) the registers of a thread from here on
-template <int N>
-__device__ __forceinline__ void reg_more() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void reg_less() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // A barrier whose phase completes after `count` arrivals (a commit is one).
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count = 1u) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
