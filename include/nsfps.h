@@ -336,7 +336,8 @@ NSFPS_API int nsfps_select_blocks_device(const nsfps_select_desc *desc, const fl
  * strides (batch, row, head, in elements) multiples of 8.  blocks (batch x
  * queries x top int64), out (batch x queries x heads x head_dim) and lse
  * (batch x queries x heads fp32: log of the softmax sum, -inf without a key;
- * may be NULL) are dense.  head_dim: a multiple of 8 up to 128; block: 16, 32,
+ * may be NULL) are dense; so is rest (like out; may be NULL), which takes what
+ * the rounding of out left, for the gradient.  head_dim: a multiple of 8 up to 128; block: 16, 32,
  * 64 or 128; top: 1..NSFPS_MAX_TOP; heads a multiple of kv_heads, at most 256.
  * batch below 2^27, batch * queries * top and batch * keys below 2^30, queries *
  * top * heads / kv_heads below 2^31. */
@@ -355,17 +356,20 @@ NSFPS_API int nsfps_block_attention_workspace(const nsfps_attention_desc *desc, 
 NSFPS_API int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d_q,
                                            const void *d_k, const void *d_v,
                                            const int64_t *d_blocks, const int32_t *d_lengths,
-                                           void *d_out, float *d_lse, void *d_work,
-                                           uint64_t work_bytes, void *stream);
+                                           void *d_out, float *d_lse, void *d_rest,
+                                           void *d_work, uint64_t work_bytes, void *stream);
 
 /* Gradient: dq (dense, like out), dk and dv (dense, batch x keys x kv_heads x
  * head_dim; keys that no query reads get zeros) from dout (dense, like out,
- * 16-byte aligned) and the forward's out and lse. */
+ * 16-byte aligned) and the forward's out, lse and rest.  Without rest (NULL)
+ * the gradient takes out as it is rounded, which dq and dk of queries with few
+ * weighty keys feel. */
 NSFPS_API int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const void *d_q,
                                                 const void *d_k, const void *d_v,
                                                 const int64_t *d_blocks,
                                                 const int32_t *d_lengths, const void *d_out,
-                                                const float *d_lse, const void *d_dout,
+                                                const float *d_lse, const void *d_rest,
+                                                const void *d_dout,
                                                 void *d_dq, void *d_dk, void *d_dv, void *d_work,
                                                 uint64_t work_bytes, void *stream);
 

@@ -196,7 +196,9 @@ def _desc(plan, moved, backward):
     return got
 
 
-def _forward(q, k, v, blocks, lengths, plan, want_lse):
+def _forward(q, k, v, blocks, lengths, plan, train):
+    """out, and for the gradient the log of the softmax sums and what the
+    rounding of out left."""
     import torch
     copies = plan[0]
     qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -207,7 +209,8 @@ def _forward(q, k, v, blocks, lengths, plan, want_lse):
     blocks = blocks.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:-1], dtype=torch.float32) if want_lse else None
+    lse = q.new_empty(q.shape[:-1], dtype=torch.float32) if train else None
+    rest = q.new_empty(q.shape) if train else None
     desc, address, need = _desc(plan, copies, False)
     device = q.get_device()
     before = _enter(device)
@@ -215,14 +218,15 @@ def _forward(q, k, v, blocks, lengths, plan, want_lse):
         work = q.new_empty(need, dtype=torch.uint8)
         capi.call("nsfps_block_attention_device", address, qp, kp, vp, blocks.data_ptr(),
                   0 if lengths is None else lengths.data_ptr(), out.data_ptr(),
-                  lse.data_ptr() if want_lse else 0, work.data_ptr(), need,
+                  lse.data_ptr() if train else 0, rest.data_ptr() if train else 0,
+                  work.data_ptr(), need,
                   torch._C._cuda_getCurrentRawStream(device))
     finally:
         _leave(before)
-    return out, lse
+    return out, lse, rest
 
 
-def _backward(q, k, v, blocks, lengths, plan, out, lse, dout):
+def _backward(q, k, v, blocks, lengths, plan, out, lse, rest, dout):
     import torch
     copies = tuple(c or t.data_ptr() % 16 != 0 for c, t in zip(plan[0], (q, k, v)))
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
@@ -236,8 +240,9 @@ def _backward(q, k, v, blocks, lengths, plan, out, lse, dout):
         work = q.new_empty(need, dtype=torch.uint8)
         capi.call("nsfps_block_attention_grad_device", address, q.data_ptr(), k.data_ptr(),
                   v.data_ptr(), blocks.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                  out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                  dv.data_ptr(), work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device))
+                  out.data_ptr(), lse.data_ptr(), rest.data_ptr(), dout.data_ptr(),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), need,
+                  torch._C._cuda_getCurrentRawStream(device))
     finally:
         _leave(before)
     return dq, dk, dv
@@ -257,16 +262,15 @@ def _autograd():
         class BlockAttention(torch.autograd.Function):
             @staticmethod
             def forward(ctx, q, k, v, blocks, lengths, plan):
-                out, lse = _forward(q, k, v, blocks, lengths, plan, True)
-                ctx.save_for_backward(q, k, v, blocks, lengths, out, lse)
+                out, lse, rest = _forward(q, k, v, blocks, lengths, plan, True)
+                ctx.save_for_backward(q, k, v, blocks, lengths, out, lse, rest)
                 ctx.plan = plan
                 return out
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
-                q, k, v, blocks, lengths, out, lse = ctx.saved_tensors
-                grads = _backward(q, k, v, blocks, lengths, ctx.plan, out, lse, dout)
+                grads = _backward(*ctx.saved_tensors[:5], ctx.plan, *ctx.saved_tensors[5:], dout)
                 return (*grads, None, None, None)
 
         _function = BlockAttention

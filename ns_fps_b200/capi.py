@@ -318,8 +318,8 @@ def _feature_functions():
         "nsfps_select_blocks_workspace": [p, p],
         "nsfps_select_blocks_device": [p] * 7 + [u, p],
         "nsfps_block_attention_workspace": [p, ctypes.c_int, p],
-        "nsfps_block_attention_device": [p] * 9 + [u, p],
-        "nsfps_block_attention_grad_device": [p] * 13 + [u, p],
+        "nsfps_block_attention_device": [p] * 10 + [u, p],
+        "nsfps_block_attention_grad_device": [p] * 14 + [u, p],
     }
     # a second handle of the library: other callers of lib() set no types
     handle = ctypes.CDLL(lib()._name)
@@ -389,16 +389,19 @@ def block_attention_workspace(desc: AttentionDesc, backward: bool) -> int:
 
 
 def block_attention_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int, lengths: int,
-                           out: int, lse: int, work: int, work_bytes: int, stream_ptr: int = 0):
-    """nsfps_block_attention_device on device addresses (lengths, lse: 0 for
-    NULL)."""
+                           out: int, lse: int, work: int, work_bytes: int, stream_ptr: int = 0,
+                           rest: int = 0):
+    """nsfps_block_attention_device on device addresses (lengths, lse, rest: 0
+    for NULL)."""
     call("nsfps_block_attention_device", ctypes.addressof(desc), q, k, v, blocks, lengths, out,
-          lse, work, work_bytes, stream_ptr)
+         lse, rest, work, work_bytes, stream_ptr)
 
 
 def block_attention_grad_device(desc: AttentionDesc, q: int, k: int, v: int, blocks: int,
                                 lengths: int, out: int, lse: int, dout: int, dq: int, dk: int,
-                                dv: int, work: int, work_bytes: int, stream_ptr: int = 0):
-    """nsfps_block_attention_grad_device on device addresses."""
+                                dv: int, work: int, work_bytes: int, stream_ptr: int = 0,
+                                rest: int = 0):
+    """nsfps_block_attention_grad_device on device addresses (lengths, rest: 0
+    for NULL)."""
     call("nsfps_block_attention_grad_device", ctypes.addressof(desc), q, k, v, blocks, lengths,
-          out, lse, dout, dq, dk, dv, work, work_bytes, stream_ptr)
+         out, lse, rest, dout, dq, dk, dv, work, work_bytes, stream_ptr)

@@ -39,8 +39,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
-  const char *q, *k, *v, *dout, *out_in;
-  char *out, *dq, *dk, *dv;
+  const char *q, *k, *v, *dout, *out_in, *rest_in;
+  char *out, *rest, *dq, *dk, *dv;  // rest: may be null, as rest_in
   float *lse;              // forward: may be null
   const float *lse_in;
   const int64_t *blocks;
@@ -866,6 +866,18 @@ attend_tiles(const AttnArgs a) {
   if (warp == 0) tmem_free<Shape::kTmem>(tm);
 }
 
+// Four consecutive elements of the output, rounded, and what the rounding left.
+template <class T>
+__device__ __forceinline__ void store_out(const AttnArgs &a, uint64_t at, float4 x) {
+  const uint2 y = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+  *reinterpret_cast<uint2 *>(a.out + at * 2) = y;
+  if (!a.rest) return;
+  const T *e = reinterpret_cast<const T *>(&y);
+  *reinterpret_cast<uint2 *>(a.rest + at * 2) =
+      make_uint2(pack2<T>(x.x - to_f32(e[0]), x.y - to_f32(e[1])),
+                 pack2<T>(x.z - to_f32(e[2]), x.w - to_f32(e[3])));
+}
+
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
 // its leading slots.  A warp takes 128 consecutive elements of a query's heads,
 // four per lane: the slots are the same for all lanes, and what a slot's
@@ -918,8 +930,7 @@ attend_join(const AttnArgs a, uint32_t parts) {
   }
   const float inv = total > 0.f ? 1.f / total : 0.f;
   const uint64_t out = ((uint64_t)bm * a.H + a.g0 * a.R) * a.D + d;
-  *reinterpret_cast<uint2 *>(a.out + out * 2) =
-      make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  store_out<T>(a, out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   if (a.lse && d == hh * a.D)
     a.lse[(uint64_t)bm * a.H + a.g0 * a.R + hh] =
         total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
@@ -968,8 +979,8 @@ attend_join_direct(const AttnArgs a) {
   }
   const float inv = total > 0.f ? 1.f / total : 0.f;
   if (4u * sub < a.D)
-    *reinterpret_cast<uint2 *>(a.out + (row * a.D + 4 * sub) * 2) =
-        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    store_out<T>(a, row * a.D + 4 * sub,
+                 make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   if (a.lse && sub == 0) a.lse[row] = total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
 }
 
@@ -1099,8 +1110,7 @@ attend_direct(const AttnArgs a) {
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     const uint64_t row = (uint64_t)bm * a.H + g * a.R + h0 + r;
     if (a.splits == 1u) {
-      *reinterpret_cast<uint2 *>(a.out + (row * a.D + d) * 2) =
-          make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+      store_out<T>(a, row * a.D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
       if (a.lse && d == 0) a.lse[row] = sum > 0.f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
     } else {
       *reinterpret_cast<float4 *>(a.part + (row * a.splits + split) * a.D + d) =
@@ -1112,8 +1122,21 @@ attend_direct(const AttnArgs a) {
 
 // -------------------------------------------------------------- gradient
 
+// Whether a query reads one key: the first of the cloud's last block, alone.
+__device__ __forceinline__ bool one_key(const AttnArgs &a, uint32_t bm) {
+  const unsigned long long lead = a.lead[bm];
+  if (__popcll(lead) != 1) return false;
+  const uint64_t slot = (uint64_t)bm * a.top + __ffsll(lead) - 1;
+  return __popc(a.mask[slot]) == 1 &&
+         ((uint64_t)a.blocks[slot] << a.block_log2) + 1u == cloud_length(a.lengths, bm / a.M, a.N);
+}
+
 // delta = sum_d dout * out per row; 8 lanes per row, 8 elements per step; bound
-// by the bytes of the two.
+// by the bytes read.  out comes with what its rounding left: ds = p (dp - delta)
+// is a difference of like numbers where few keys have the weight, and with the
+// rounded out alone dq and dk were off 2.3 times as far as their own rounding
+// puts them (two keys).  With one key the difference is zero by definition, not
+// nearly: delta = inf stands for that.
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_delta(const AttnArgs a) {
@@ -1124,13 +1147,18 @@ grad_delta(const AttnArgs a) {
     for (uint32_t d = sub * 8; d < a.D; d += 64) {
       const uint4 x = *reinterpret_cast<const uint4 *>(a.dout + (row * a.D + d) * 2);
       const uint4 y = *reinterpret_cast<const uint4 *>(a.out_in + (row * a.D + d) * 2);
+      const uint4 z = a.rest_in
+                          ? *reinterpret_cast<const uint4 *>(a.rest_in + (row * a.D + d) * 2)
+                          : make_uint4(0u, 0u, 0u, 0u);
       const T *xe = reinterpret_cast<const T *>(&x), *ye = reinterpret_cast<const T *>(&y);
+      const T *ze = reinterpret_cast<const T *>(&z);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += to_f32(xe[i]) * to_f32(ye[i]);
+      for (int i = 0; i < 8; ++i) s += to_f32(xe[i]) * (to_f32(ye[i]) + to_f32(ze[i]));
     }
 #pragma unroll
   for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-  if (sub == 0 && row < (uint64_t)a.B * a.M * a.H) a.delta[row] = s;
+  if (sub == 0 && row < (uint64_t)a.B * a.M * a.H)
+    a.delta[row] = one_key(a, (uint32_t)(row / a.H)) ? INFINITY : s;
 }
 
 constexpr uint32_t kGradItem = 512;    // query rows per item
@@ -1322,8 +1350,10 @@ attend_grad(const AttnArgs a) {
                                       make_float2(-z.y, -z.w)));
               if (!all) {
                 const bool in0 = (in >> y) & 1u, in1 = (in >> (y + 1u)) & 1u;
-                f.x = in0 ? f.x : 0.f, g.x = in0 ? g.x : 0.f;
-                f.y = in1 ? f.y : 0.f, g.y = in1 ? g.y : 0.f;
+                // (a block with one key leaves the other lanes out: rows of
+                // one key come here)
+                f.x = in0 ? f.x : 0.f, g.x = in0 && z.y != INFINITY ? g.x : 0.f;
+                f.y = in1 ? f.y : 0.f, g.y = in1 && z.w != INFINITY ? g.y : 0.f;
               }
               p16[y / 2u] = pack2<T>(f.x, f.y);
               e16[y / 2u] = pack2<T>(g.x, g.y);
@@ -1868,6 +1898,8 @@ AttnArgs turn_args(const AttnArgs &all, uint32_t b0, uint32_t bc) {
   if (a.lengths) a.lengths += b0;
   const uint64_t ro = 2 * rows * a.H * a.D, ko = 2 * (uint64_t)b0 * a.N * a.G * a.D;
   if (a.out) a.out += ro;
+  if (a.rest) a.rest += ro;
+  if (a.rest_in) a.rest_in += ro;
   if (a.lse) a.lse += rows * a.H;
   if (a.dout) a.dout += ro, a.out_in += ro, a.dq += ro, a.lse_in += rows * a.H;
   if (a.dk) a.dk += ko, a.dv += ko;
@@ -2029,7 +2061,7 @@ int nsfps_block_attention_workspace(const nsfps_attention_desc *desc, int backwa
 int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d_q,
                                  const void *d_k, const void *d_v, const int64_t *d_blocks,
                                  const int32_t *d_lengths, void *d_out, float *d_lse,
-                                 void *d_work, uint64_t work_bytes, void *stream) {
+                                 void *d_rest, void *d_work, uint64_t work_bytes, void *stream) {
   clear_error();
   int rc = check_attention(desc);
   if (rc) return rc;
@@ -2037,8 +2069,8 @@ int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d
   if (d.batch * d.queries == 0) return NSFPS_OK;
   if (!d_q || !d_out || !d_blocks || (d.keys && (!d_k || !d_v)))
     return set_error(NSFPS_ERR_ARG, "NULL argument");
-  if (((uint64_t)d_q | (uint64_t)d_k | (uint64_t)d_v | (uint64_t)d_out) % 16)
-    return set_error(NSFPS_ERR_ARG, "q, k, v and out must be 16-byte aligned");
+  if (((uint64_t)d_q | (uint64_t)d_k | (uint64_t)d_v | (uint64_t)d_out | (uint64_t)d_rest) % 16)
+    return set_error(NSFPS_ERR_ARG, "q, k, v, out and rest must be 16-byte aligned");
   if ((uint64_t)d_blocks % 8 || ((uint64_t)d_lse | (uint64_t)d_lengths) % 4)
     return set_error(NSFPS_ERR_ARG, "a pointer is not aligned to its elements");
   const AttnPlan w = plan_attention(d, false, d_work);
@@ -2047,6 +2079,7 @@ int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d
   AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths, w);
   a.out = (char *)d_out;
   a.lse = d_lse;
+  a.rest = (char *)d_rest;
   cudaStream_t st = (cudaStream_t)stream;
   NSFPS_FEATURE_CUDA(d.dtype == NSFPS_F16 ? forward_of<__half>(a, w, st)
                                           : forward_of<__nv_bfloat16>(a, w, st));
@@ -2056,7 +2089,8 @@ int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d
 int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const void *d_q,
                                       const void *d_k, const void *d_v, const int64_t *d_blocks,
                                       const int32_t *d_lengths, const void *d_out,
-                                      const float *d_lse, const void *d_dout, void *d_dq,
+                                      const float *d_lse, const void *d_rest,
+                                      const void *d_dout, void *d_dq,
                                       void *d_dk, void *d_dv, void *d_work, uint64_t work_bytes,
                                       void *stream) {
   clear_error();
@@ -2069,8 +2103,8 @@ int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const vo
       (nk && (!d_k || !d_v || !d_dk || !d_dv)))
     return set_error(NSFPS_ERR_ARG, "NULL argument");
   if (((uint64_t)d_q | (uint64_t)d_k | (uint64_t)d_v | (uint64_t)d_out | (uint64_t)d_dout |
-       (uint64_t)d_dq | (uint64_t)d_dk | (uint64_t)d_dv) % 16)
-    return set_error(NSFPS_ERR_ARG, "q, k, v, out and the gradients must be 16-byte aligned");
+       (uint64_t)d_rest | (uint64_t)d_dq | (uint64_t)d_dk | (uint64_t)d_dv) % 16)
+    return set_error(NSFPS_ERR_ARG, "q, k, v, out, rest and the gradients must be 16-byte aligned");
   if ((uint64_t)d_blocks % 8 || ((uint64_t)d_lse | (uint64_t)d_lengths) % 4)
     return set_error(NSFPS_ERR_ARG, "a pointer is not aligned to its elements");
   const AttnPlan w = plan_attention(d, true, d_work);
@@ -2078,6 +2112,7 @@ int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const vo
   if (rc) return rc;
   AttnArgs a = common_args(d, d_q, d_k, d_v, d_blocks, d_lengths, w);
   a.out_in = (const char *)d_out; a.lse_in = d_lse; a.dout = (const char *)d_dout;
+  a.rest_in = (const char *)d_rest;
   a.dq = (char *)d_dq; a.dk = (char *)d_dk; a.dv = (char *)d_dv;
   cudaStream_t st = (cudaStream_t)stream;
   NSFPS_FEATURE_CUDA(d.dtype == NSFPS_F16 ? backward_of<__half>(a, w, st)

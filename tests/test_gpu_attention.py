@@ -376,3 +376,63 @@ def test_refusals():
             ((q, k, k, blocks, 16, None, math.inf), RuntimeError)]:
         with pytest.raises(error):
             attention.block_attention(*args)
+
+
+def _one_block(B, M, N, H, G, D, dtype, seed):
+    """A call in which every query reads all N keys, of one block of 16."""
+    q, dout = _normal((B, M, H, D), dtype, seed), _normal((B, M, H, D), dtype, seed + 1)
+    k, v = _normal((B, N, G, D), dtype, seed + 2), _normal((B, N, G, D), dtype, seed + 3)
+    return q, k, v, torch.zeros(B, M, 1, dtype=torch.int64, device="cuda"), dout
+
+
+def _grads(q, k, v, blocks, dout, block=16, lengths=None):
+    from ns_fps_b200 import attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention.block_attention(*leaves, blocks, block, lengths=lengths)
+    return torch.autograd.grad(out, leaves, dout)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,queries", [(64, 1), (64, 300), (128, 70), (24, 9)])
+def test_one_key_moves_no_score(D, queries, dtype):
+    """A query with one key gives it weight one wherever it lies: dq and dk
+    are zero, dv is dout.  Queries beside it that read more keys keep theirs."""
+    B, N, H, G = 2, 33, 4, 2
+    q, k, v = (_normal(s, dtype, i) for i, s in
+               enumerate([(B, queries, H, D), (B, N, G, D), (B, N, G, D)]))
+    dout = _normal(q.shape, dtype, 7)
+    blocks = torch.full((B, queries, 2), 2, dtype=torch.int64, device="cuda")
+    dq, dk, dv = _grads(q, k, v, blocks, dout)
+    assert not bool(dq.any()) and not bool(dk.any())
+    # p is 1 up to the errors of an fp32 score, far less than the 2^-12 that
+    # would round it to anything but 1; the sum's 600 terms are added in fp32
+    sums = dout.double().reshape(B, queries, G, H // G, D).sum((1, 3))
+    mag = dout.double().abs().reshape(B, queries, G, H // G, D).sum((1, 3))
+    u = torch.finfo(dtype).eps / 2
+    assert bool(((dv[:, 32].double() - sums).abs() <= u * sums.abs() + 1e-4 * mag + 2e-7).all())
+    assert not bool(dv[:, :32].any())
+    blocks[:, ::2, 1] = 0  # every other query reads 16 keys more
+    dq = _grads(q, k, v, blocks, dout)[0]
+    assert bool(dq[:, ::2].any()) and not bool(dq[:, 1::2].any())
+    lengths = torch.tensor([1, 17], dtype=torch.int32, device="cuda")
+    dq, dk, _ = _grads(q, k, v, torch.ones_like(blocks) * lengths[:, None, None] // 17, dout,
+                       lengths=lengths)
+    assert not bool(dq.any()) and not bool(dk.any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [2, 3, 5, 11])
+def test_gradients_of_few_keys(N, dtype):
+    """dp - delta cancels where few keys share the weight.  dq and dk are off
+    by the roundings of ds and of themselves alone.  A rounding error is uniform
+    within half a step, at most u of the value, so over many independent values
+    its 2-norm is at most u / sqrt(3) of theirs, and that of the two roundings
+    together at most sqrt(2 / 3) u."""
+    B, M, H, G, D = 2, 400, 4, 2, 64
+    q, k, v, blocks, dout = _one_block(B, M, N, H, G, D, dtype, 3)
+    ref = Exact(q, k, v, blocks, 16, dout=dout)
+    dq, dk, _ = _grads(q, k, v, blocks, dout)
+    u = torch.finfo(dtype).eps / 2
+    for name, got, want in (("dq", dq, ref.dq), ("dk", dk, ref.dk)):
+        off = float((got.double() - want).norm() / want.norm())
+        assert off <= math.sqrt(2 / 3) * u, (name, off / u)
