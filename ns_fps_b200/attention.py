@@ -197,8 +197,8 @@ def _desc(plan, moved, backward):
 
 
 def _forward(q, k, v, blocks, lengths, plan, train):
-    """out, and for the gradient the log of the softmax sums and what the
-    rounding of out left."""
+    """out, and what the gradient needs besides: what the rounding of out left,
+    and behind it the logs of the softmax sums, as bytes."""
     import torch
     copies = plan[0]
     qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -209,8 +209,11 @@ def _forward(q, k, v, blocks, lengths, plan, train):
     blocks = blocks.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:-1], dtype=torch.float32) if train else None
-    rest = q.new_empty(q.shape) if train else None
+    keep, rest, lse = None, 0, 0
+    if train:
+        keep = q.new_empty(2 * q.numel() + 4 * (q.numel() // q.shape[-1]), dtype=torch.uint8)
+        rest = keep.data_ptr()
+        lse = rest + 2 * q.numel()
     desc, address, need = _desc(plan, copies, False)
     device = q.get_device()
     before = _enter(device)
@@ -218,21 +221,21 @@ def _forward(q, k, v, blocks, lengths, plan, train):
         work = q.new_empty(need, dtype=torch.uint8)
         capi.call("nsfps_block_attention_device", address, qp, kp, vp, blocks.data_ptr(),
                   0 if lengths is None else lengths.data_ptr(), out.data_ptr(),
-                  lse.data_ptr() if train else 0, rest.data_ptr() if train else 0,
-                  work.data_ptr(), need,
+                  lse, rest, work.data_ptr(), need,
                   torch._C._cuda_getCurrentRawStream(device))
     finally:
         _leave(before)
-    return out, lse, rest
+    return out, keep
 
 
-def _backward(q, k, v, blocks, lengths, plan, out, lse, rest, dout):
+def _backward(q, k, v, blocks, lengths, plan, out, keep, dout):
     import torch
     copies = tuple(c or t.data_ptr() % 16 != 0 for c, t in zip(plan[0], (q, k, v)))
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     q, k, v = (_rows16(t, c) for t, c in zip((q, k, v), copies))
     dout, blocks = _rows16(dout, True), blocks.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
+    rest = keep.data_ptr()
     desc, address, need = _desc(plan, copies, True)
     device = q.get_device()
     before = _enter(device)
@@ -240,7 +243,7 @@ def _backward(q, k, v, blocks, lengths, plan, out, lse, rest, dout):
         work = q.new_empty(need, dtype=torch.uint8)
         capi.call("nsfps_block_attention_grad_device", address, q.data_ptr(), k.data_ptr(),
                   v.data_ptr(), blocks.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                  out.data_ptr(), lse.data_ptr(), rest.data_ptr(), dout.data_ptr(),
+                  out.data_ptr(), rest + 2 * q.numel(), rest, dout.data_ptr(),
                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), need,
                   torch._C._cuda_getCurrentRawStream(device))
     finally:
@@ -262,15 +265,16 @@ def _autograd():
         class BlockAttention(torch.autograd.Function):
             @staticmethod
             def forward(ctx, q, k, v, blocks, lengths, plan):
-                out, lse, rest = _forward(q, k, v, blocks, lengths, plan, True)
-                ctx.save_for_backward(q, k, v, blocks, lengths, out, lse, rest)
+                out, keep = _forward(q, k, v, blocks, lengths, plan, True)
+                ctx.save_for_backward(q, k, v, blocks, lengths, out, keep)
                 ctx.plan = plan
                 return out
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
-                grads = _backward(*ctx.saved_tensors[:5], ctx.plan, *ctx.saved_tensors[5:], dout)
+                q, k, v, blocks, lengths, out, keep = ctx.saved_tensors
+                grads = _backward(q, k, v, blocks, lengths, ctx.plan, out, keep, dout)
                 return (*grads, None, None, None)
 
         _function = BlockAttention

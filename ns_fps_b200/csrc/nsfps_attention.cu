@@ -1207,10 +1207,10 @@ struct GradItem {
 // sixteen make weights, three load a step's rows each (the loads of three steps
 // are in the air), four take dq, dk and dv out, and one issues the products,
 // the next step's scores before this step's gradients.  Four clouds (16,384
-// queries, 8 heads of 64) took 210 us without roles and take 128 (the matrix
+// queries, 4 heads of 64) took 210 us without roles and take 130 (the matrix
 // unit 15 % busy, memory 19 %: what is left is the way of a step from barrier to
 // barrier, with the gather of 128 rows of q and dout in it), shared heads
-// (2,048 queries, 16 heads of 128 over 4) 62 and 35.
+// (2,046 queries, 8 heads of 128 over 2) 62 and 37.
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
@@ -1310,7 +1310,13 @@ attend_grad(const AttnArgs a) {
     uint32_t n = 0;
     for (Items y = items(); y.w < work; advance(y)) {
       const GradItem it = item_of(y);
-      const bool key_live = it.key0 + key_in < it.len;
+      // rows that may read this key; kLone: it is a block's only key
+      constexpr uint32_t kLone = 0x10000u;
+      const uint32_t key = it.key0 + key_in;
+      const uint32_t live = key >= it.len ? 0u
+                            : key + 1u == it.len && !(key & ((1u << a.block_log2) - 1u))
+                                ? 0xffffu | kLone
+                                : 0xffffu;
       for (uint32_t i = 0; i < it.steps; ++i, ++n) {
         const uint32_t st = n % kStages;
         const char *info = smem + Shape::kInfoAt + st * Shape::kInfo;
@@ -1328,7 +1334,7 @@ attend_grad(const AttnArgs a) {
           tmem_ld16(dx, tm + Shape::kDp + my + col);
           // which of the 16 rows read this key
           uint32_t in = reinterpret_cast<const uint16_t *>(info + Shape::kBitsAt)[block * 8u + col / 16u];
-          if (!key_live) in = 0u;
+          in &= live;
           tmem_ld_wait();
           if (x + 1u == kPieces) {
             tmem_before_sync();
@@ -1350,10 +1356,8 @@ attend_grad(const AttnArgs a) {
                                       make_float2(-z.y, -z.w)));
               if (!all) {
                 const bool in0 = (in >> y) & 1u, in1 = (in >> (y + 1u)) & 1u;
-                // (a block with one key leaves the other lanes out: rows of
-                // one key come here)
-                f.x = in0 ? f.x : 0.f, g.x = in0 && z.y != INFINITY ? g.x : 0.f;
-                f.y = in1 ? f.y : 0.f, g.y = in1 && z.w != INFINITY ? g.y : 0.f;
+                f.x = in0 ? f.x : 0.f, g.x = in0 ? g.x : 0.f;
+                f.y = in1 ? f.y : 0.f, g.y = in1 ? g.y : 0.f;
               }
               p16[y / 2u] = pack2<T>(f.x, f.y);
               e16[y / 2u] = pack2<T>(g.x, g.y);
@@ -1378,6 +1382,12 @@ attend_grad(const AttnArgs a) {
                                        swizzled(key_in, (col % 64u) / 8u + c)) =
                 make_uint4(e[x][4 * c], e[x][4 * c + 1], e[x][4 * c + 2], e[x][4 * c + 3]);
         }
+        if (live & kLone)  // rows of one key are here only (tested per element: 11 us of 140)
+#pragma unroll 1
+          for (uint32_t col = col0; col < col0 + kCols; ++col)
+            if (reinterpret_cast<const float2 *>(info)[col].y == INFINITY)
+              *reinterpret_cast<uint16_t *>(smem + Shape::kDsAt + (col / 64u) * 16384u +
+                                            swizzled(key_in, (col % 64u) / 8u) + (col % 8u) * 2u) = 0u;
         tmem_st_wait();
         smem_to_mma();
         tmem_before_sync();
