@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(256)
 plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
            uint32_t *__restrict__ mask, unsigned long long *__restrict__ lead,
            uint8_t *__restrict__ listed) {
+  after_previous();
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (bm >= a.B * a.M) return;
@@ -285,6 +286,7 @@ __global__ void __launch_bounds__(256)
 plan_spans(const SortedList list, uint32_t spans, uint32_t shift, uint32_t R, uint32_t tile_rows,
            uint32_t least, bool by_chunks, uint4 *__restrict__ span, uint4 *__restrict__ tiles,
            uint32_t tile_stride, uint32_t *__restrict__ tile_count) {
+  after_previous();
   const uint32_t s = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
   if (s >= spans) return;
   const uint32_t n = *list.kept;
@@ -581,6 +583,7 @@ __device__ __forceinline__ void store8(float *to, const uint32_t *x, float f) {
 template <class T, int DP>
 __global__ void __launch_bounds__(kTileThreads, TileShape<DP>::kCtas)
 attend_tiles(const AttnArgs a) {
+  after_previous();
   using Shape = TileShape<DP>;
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[2];
@@ -886,6 +889,7 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, uint64_t at, float4
 template <class T>
 __global__ void __launch_bounds__(256)
 attend_join(const AttnArgs a, uint32_t parts) {
+  after_previous();
   const uint32_t lane = threadIdx.x & 31u, hc = a.gc * a.R;
   const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
   const uint32_t bm = (uint32_t)(w / parts);
@@ -941,6 +945,7 @@ attend_join(const AttnArgs a, uint32_t parts) {
 template <class T, int LANES>
 __global__ void __launch_bounds__(256)
 attend_join_direct(const AttnArgs a) {
+  after_previous();
   constexpr uint32_t kGroups = 256 / LANES;
   __shared__ float s_mx[8];
   __shared__ float4 s_acc[kGroups][LANES];
@@ -1002,6 +1007,7 @@ struct DirectShape {
 template <class T, int DP>
 __global__ void __launch_bounds__(kDirectWarps * 32)
 attend_direct(const AttnArgs a) {
+  after_previous();
   using Shape = DirectShape<DP>;
   extern __shared__ __align__(128) char smem[];
   __shared__ float s_stat[kDirectWarps][2][16];
@@ -1140,6 +1146,7 @@ __device__ __forceinline__ bool one_key(const AttnArgs &a, uint32_t bm) {
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_delta(const AttnArgs a) {
+  after_previous();
   const uint64_t row = (uint64_t)blockIdx.x * 32u + (threadIdx.x >> 3);
   const uint32_t sub = threadIdx.x & 7u;
   float s = 0.f;
@@ -1214,6 +1221,7 @@ struct GradItem {
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {
+  after_previous();
   using Shape = GradShape<DP>;
   constexpr uint32_t kRows = Shape::kRows, kStages = Shape::kStages, kChunks = DP / 8;
   extern __shared__ char smem_raw[];
@@ -1690,6 +1698,7 @@ attend_grad(const AttnArgs a) {
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_join_keys(const AttnArgs a, uint32_t span) {
+  after_previous();
   const uint32_t s = blockIdx.x, gi = blockIdx.y, g = a.g0 + gi;
   const uint4 sp = a.span[s];
   const uint32_t i0 = sp.z, i1 = sp.z + sp.w;
@@ -1716,6 +1725,7 @@ grad_join_keys(const AttnArgs a, uint32_t span) {
 template <class T>
 __global__ void __launch_bounds__(256)
 grad_join_queries(const AttnArgs a, uint32_t parts) {
+  after_previous();
   const uint32_t lane = threadIdx.x & 31u, hc = a.gc * a.R;
   const uint64_t w = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
   const uint32_t bm = (uint32_t)(w / parts);
@@ -1926,13 +1936,9 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + 16 * (uint64_t)spans, st))) return err;
   if (n && spans) {
     const uint32_t grid = (uint32_t)ceil_div(a.B * a.M, 8);
-    if (a.top <= 32)
-      plan_pairs<1><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
-                                          w.listed);
-    else
-      plan_pairs<2><<<grid, 256, 0, st>>>(a, w.span_log2, w.sort.keys0, w.mask, w.lead,
-                                          w.listed);
-    if ((err = cudaGetLastError())) return err;
+    if ((err = launch_next(a.top <= 32 ? plan_pairs<1> : plan_pairs<2>, grid, 256, 0, st, a,
+                           w.span_log2, w.sort.keys0, w.mask, w.lead, w.listed)))
+      return err;
     if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
   } else {  // no pair, or no key to form one with
     if ((err = cudaMemsetAsync(w.sort.kept, 0, 4, st))) return err;
@@ -1942,11 +1948,10 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   }
   a.vals = list.vals;
   a.skeys = list.keys;
-  if (spans)
-    plan_spans<<<(uint32_t)ceil_div(spans, 8), 256, 0, st>>>(
-        list, spans, shift, a.R, w.tile_rows, w.least, w.least == 0u, w.span, w.tiles,
-        a.tile_stride, w.tile_count);
-  return cudaGetLastError();
+  if (!spans) return cudaSuccess;
+  return launch_next(plan_spans, (uint32_t)ceil_div(spans, 8), 256, 0, st, list, spans, shift, a.R,
+                     w.tile_rows, w.least, w.least == 0u, w.span, w.tiles, a.tile_stride,
+                     w.tile_count);
 }
 
 template <class T, int DP>
@@ -1956,14 +1961,10 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
     AttnArgs a = all;
     const uint32_t smem = DirectShape<DP>::kSmem;
     if ((err = opt_in<attend_direct<T, DP>>(smem))) return err;
-    attend_direct<T, DP><<<dim3(w.splits, a.B * a.M, a.G * a.row_parts), kDirectWarps * 32, smem,
-                           st>>>(a);
-    if ((err = cudaGetLastError())) return err;
-    if (w.splits > 1) {
-      const uint64_t rows = (uint64_t)a.B * a.M * a.H;
-      attend_join_direct<T, DP / 4><<<(uint32_t)rows, 256, 0, st>>>(a);
-    }
-    return cudaGetLastError();
+    const dim3 grid(w.splits, a.B * a.M, a.G * a.row_parts);
+    err = launch_next(attend_direct<T, DP>, grid, kDirectWarps * 32, smem, st, a);
+    if (err || w.splits == 1) return err;
+    return launch_next(attend_join_direct<T, DP / 4>, a.B * a.M * a.H, 256, 0, st, a);
   }
   constexpr int TP = DP < 64 ? 64 : DP;  // the tiles' rows are 64 or 128 elements
   const uint32_t smem = TileShape<TP>::kSmem;
@@ -1975,14 +1976,15 @@ cudaError_t launch_forward(const AttnArgs &all, const AttnPlan &w, cudaStream_t 
     const uint64_t tiles = (uint64_t)a.B * a.M * a.top * a.R / w.tile_rows + (uint64_t)a.B * a.nsb;
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
-      if (tiles)
-        attend_tiles<T, TP><<<(uint32_t)std::min(tiles * a.gc, resident), kTileThreads, smem, st>>>(
-            a);
-      if ((err = cudaGetLastError())) return err;
+      if (tiles && (err = launch_next(attend_tiles<T, TP>,
+                                      (uint32_t)std::min(tiles * a.gc, resident), kTileThreads,
+                                      smem, st, a)))
+        return err;
       const uint64_t rows = (uint64_t)a.B * a.M;
       const uint32_t parts = (uint32_t)ceil_div((uint64_t)a.gc * a.R * a.D, 128);
-      attend_join<T><<<(uint32_t)ceil_div(rows * parts, 8), 256, 0, st>>>(a, parts);
-      if ((err = cudaGetLastError())) return err;
+      if ((err = launch_next(attend_join<T>, (uint32_t)ceil_div(rows * parts, 8), 256, 0, st, a,
+                             parts)))
+        return err;
     }
   }
   return cudaSuccess;
@@ -1998,26 +2000,25 @@ cudaError_t launch_backward(const AttnArgs &all, const AttnPlan &w, cudaStream_t
     AttnArgs a = turn_args(all, b0, w.bc);
     const uint64_t nq = (uint64_t)a.B * a.M;
     if ((err = run_plan(a, w, st))) return err;
-    if (nq) {
-      grad_delta<T><<<(uint32_t)ceil_div(nq * a.H, 32), 256, 0, st>>>(a);
-      if ((err = cudaGetLastError())) return err;
-    }
+    if (nq && (err = launch_next(grad_delta<T>, (uint32_t)ceil_div(nq * a.H, 32), 256, 0, st, a)))
+      return err;
     const uint32_t spans = a.B * a.nsb;
     const uint64_t tiles = nq * a.top * a.R / w.tile_rows + spans;
     for (a.g0 = 0; a.g0 < a.G; a.g0 += w.gc) {
       a.gc = std::min(w.gc, a.G - a.g0);
-      if (tiles)
-        attend_grad<T, DP><<<(uint32_t)std::min(tiles * a.gc, resident), kGradThreads, smem, st>>>(
-            a);
-      if ((err = cudaGetLastError())) return err;
-      if (nq * a.top * a.R > w.tile_rows && spans) {
-        grad_join_keys<T><<<dim3(spans, a.gc, 4), 256, 0, st>>>(a, 1u << kGradSpanLog2);
-        if ((err = cudaGetLastError())) return err;
-      }
+      if (tiles && (err = launch_next(attend_grad<T, DP>,
+                                      (uint32_t)std::min(tiles * a.gc, resident), kGradThreads,
+                                      smem, st, a)))
+        return err;
+      if (nq * a.top * a.R > w.tile_rows && spans &&
+          (err = launch_next(grad_join_keys<T>, dim3(spans, a.gc, 4), 256, 0, st, a,
+                             1u << kGradSpanLog2)))
+        return err;
       if (nq) {
         const uint32_t parts = (uint32_t)ceil_div((uint64_t)a.gc * a.R * a.D, 128);
-        grad_join_queries<T><<<(uint32_t)ceil_div(nq * parts, 8), 256, 0, st>>>(a, parts);
-        if ((err = cudaGetLastError())) return err;
+        if ((err = launch_next(grad_join_queries<T>, (uint32_t)ceil_div(nq * parts, 8), 256, 0, st,
+                               a, parts)))
+          return err;
       }
     }
   }

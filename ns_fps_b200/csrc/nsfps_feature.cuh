@@ -70,6 +70,28 @@ cudaError_t opt_in(uint32_t smem) {
   return err;
 }
 
+// Launches a kernel that begins with after_previous() behind the one before it
+// in the stream: its CTAs are set up while that one's last results go out.
+template <class... P, class... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t smem,
+                        cudaStream_t st, const A &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// First in every kernel that launch_next starts, by all threads: the kernels
+// before have ended and what they wrote is there.
+__device__ __forceinline__ void after_previous() { cudaGridDependencySynchronize(); }
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -153,6 +153,7 @@ struct WalkArgs {
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
 rows_walk(const WalkArgs a) {
+  after_previous();
   constexpr int E = Pack<T, VB>::E;
   using V = typename VecOf<VB>::type;
   const uint32_t lanes = 1u << a.lanes_log2, sub = threadIdx.x & (lanes - 1u);
@@ -231,6 +232,7 @@ constexpr uint32_t kLongChain = 32;
 template <class T, int VB>
 __global__ void __launch_bounds__(256)
 rows_join(const WalkArgs a) {
+  after_previous();
   constexpr int E = Pack<T, VB>::E;
   __shared__ float s_acc[8][32][E];
   __shared__ uint32_t s_row[8], s_len[8];
@@ -386,10 +388,11 @@ struct LaunchWalk {
   template <class T, int VB>
   cudaError_t operator()() const {
     const uint32_t tiles = (uint32_t)ceil_div(n, kWalk);
-    rows_walk<T, VB><<<dim3((uint32_t)ceil_div(tiles, 256u >> a.lanes_log2),
-                            (uint32_t)ceil_div(a.vecs, 1u << a.lanes_log2)), 256, 0, st>>>(a);
-    if (n > kWalk) rows_join<T, VB><<<(uint32_t)ceil_div(tiles, 8), 256, 0, st>>>(a);
-    return cudaGetLastError();
+    const dim3 grid((uint32_t)ceil_div(tiles, 256u >> a.lanes_log2),
+                    (uint32_t)ceil_div(a.vecs, 1u << a.lanes_log2));
+    const cudaError_t err = launch_next(rows_walk<T, VB>, grid, 256, 0, st, a);
+    if (err || n <= kWalk) return err;
+    return launch_next(rows_join<T, VB>, (uint32_t)ceil_div(tiles, 8), 256, 0, st, a);
   }
 };
 

@@ -150,6 +150,7 @@ constexpr uint32_t kHeldBlocks = 32 * kHeldRegs;
 template <int SLOTS, bool HELD>
 __global__ void __launch_bounds__(256)
 choose_blocks(const SelectArgs a) {
+  after_previous();
   __shared__ __align__(16) uint32_t s_d[8][kListMax + 4], s_j[8][kListMax];
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   const uint32_t c = blockIdx.x * (blockDim.x >> 5) + warp;
@@ -297,10 +298,8 @@ cudaError_t launch_choose(const SelectArgs &a, cudaStream_t st) {
   const uint32_t warps = std::min(8u, std::max(1u, centres / (uint32_t)sm_count()));
   const uint32_t grid = (uint32_t)ceil_div(centres, warps);
   if (ceil_div(a.n, 1ull << a.block_log2) <= kHeldBlocks)
-    choose_blocks<SLOTS, true><<<grid, warps * 32u, 0, st>>>(a);
-  else
-    choose_blocks<SLOTS, false><<<grid, warps * 32u, 0, st>>>(a);
-  return cudaGetLastError();
+    return launch_next(choose_blocks<SLOTS, true>, grid, warps * 32u, 0, st, a);
+  return launch_next(choose_blocks<SLOTS, false>, grid, warps * 32u, 0, st, a);
 }
 
 int check_select(const nsfps_select_desc *d) {

@@ -63,6 +63,7 @@ template <int ITEMS, class Source>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t digit_mask,
            uint32_t *__restrict__ hist, uint32_t tiles) {
+  after_previous();
   __shared__ uint32_t s_hist[256];
   s_hist[threadIdx.x] = 0;
   __syncthreads();
@@ -106,6 +107,7 @@ __device__ __forceinline__ uint32_t sort_cta_sum(uint32_t v, uint32_t *s_warp, u
 // One CTA per digit: its counts per tile become offsets within the digit.
 static __global__ void __launch_bounds__(kSortThreads)
 sort_offsets(uint32_t *__restrict__ hist, uint32_t tiles, uint32_t *__restrict__ total) {
+  after_previous();
   __shared__ uint32_t s_warp[kSortWarps];
   uint32_t *h = hist + (size_t)blockIdx.x * tiles;
   uint32_t base = 0;
@@ -123,10 +125,11 @@ sort_offsets(uint32_t *__restrict__ hist, uint32_t tiles, uint32_t *__restrict__
 template <int ITEMS, class Source>
 __global__ void __launch_bounds__(kSortThreads)
 sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t digit_mask,
-             const uint32_t *__restrict__ hist, uint32_t tiles,
-             const uint32_t *__restrict__ total,  // null: hist holds counts, not offsets
+             const uint32_t *hist, uint32_t tiles,
+             const uint32_t *total,  // null: hist holds counts, not offsets
              uint32_t *__restrict__ out_keys,
              uint32_t *__restrict__ out_vals, uint32_t *__restrict__ kept) {
+  after_previous();
   __shared__ uint32_t s_count[kSortWarps][256];
   __shared__ uint32_t s_base[256], s_global[256], s_warp[kSortWarps];
   __shared__ uint32_t s_key[kSortThreads * ITEMS], s_val[kSortThreads * ITEMS];
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(1024)
 sort_small(const Source src, uint32_t n, uint32_t none, uint32_t passes, uint32_t digit,
            uint32_t *__restrict__ out_keys, uint32_t *__restrict__ out_vals,
            uint32_t *__restrict__ kept) {
+  after_previous();
   extern __shared__ uint32_t s_small[];
   uint32_t *s_key = s_small, *s_val = s_small + kSortSmall;
   uint16_t(*s_count)[256] = reinterpret_cast<uint16_t(*)[256]>(s_small + 2u * kSortSmall);
@@ -313,30 +317,33 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
   if (n <= kSortSmall) {
     const cudaError_t err = opt_in<sort_small<Source>>(kSmallSmem);
     if (err) return err;
-    sort_small<<<1, 1024, kSmallSmem, st>>>(src, n, none, passes, digit, w.keys1, w.vals1, w.kept);
     *out = SortedList{w.keys1, w.vals1, w.kept};
-    return cudaGetLastError();
+    return launch_next(sort_small<Source>, 1, 1024, kSmallSmem, st, src, n, none, passes, digit,
+                       w.keys1, w.vals1, w.kept);
   }
   const bool few = tiles <= kSumTiles;
   uint32_t *keys = w.keys0, *vals = w.vals0, *keys_next = w.keys1, *vals_next = w.vals1;
   for (uint32_t p = 0; p < passes; ++p) {
     const uint32_t shift = p * digit;
     const StoredKeys stored{keys, vals, w.kept};
-#define NSFPS_SORT_PASS(ITEMS, FROM)                                                              \
-    sort_count<ITEMS><<<tiles, kSortThreads, 0, st>>>(FROM, n, none, shift, dm, w.hist, tiles);   \
-    if (!few) sort_offsets<<<dm + 1u, kSortThreads, 0, st>>>(w.hist, tiles, w.total);             \
-    sort_scatter<ITEMS><<<tiles, kSortThreads, 0, st>>>(FROM, n, none, shift, dm, w.hist, tiles,  \
-                                                        few ? nullptr : w.total, keys_next,       \
-                                                        vals_next, w.kept)
-    if (p == 0) {
-      if (tile == 4u * kSortThreads) { NSFPS_SORT_PASS(4, src); }
-      else { NSFPS_SORT_PASS(16, src); }
-    } else {
-      if (tile == 4u * kSortThreads) { NSFPS_SORT_PASS(4, stored); }
-      else { NSFPS_SORT_PASS(16, stored); }
-    }
-#undef NSFPS_SORT_PASS
-    cudaError_t err = cudaGetLastError();
+    auto pass = [&](auto count, auto scatter, const auto &from) {
+      cudaError_t err = launch_next(count, tiles, kSortThreads, 0, st, from, n, none, shift, dm,
+                                    w.hist, tiles);
+      if (!err && !few)
+        err = launch_next(sort_offsets, dm + 1u, kSortThreads, 0, st, w.hist, tiles, w.total);
+      if (!err)
+        err = launch_next(scatter, tiles, kSortThreads, 0, st, from, n, none, shift, dm, w.hist,
+                          tiles, few ? (uint32_t *)nullptr : w.total, keys_next, vals_next, w.kept);
+      return err;
+    };
+    const bool short_tiles = tile == 4u * kSortThreads;
+    cudaError_t err;
+    if (p == 0)
+      err = short_tiles ? pass(sort_count<4, Source>, sort_scatter<4, Source>, src)
+                        : pass(sort_count<16, Source>, sort_scatter<16, Source>, src);
+    else
+      err = short_tiles ? pass(sort_count<4, StoredKeys>, sort_scatter<4, StoredKeys>, stored)
+                        : pass(sort_count<16, StoredKeys>, sort_scatter<16, StoredKeys>, stored);
     if (err) return err;
     std::swap(keys, keys_next);
     std::swap(vals, vals_next);
