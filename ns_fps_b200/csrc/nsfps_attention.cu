@@ -16,8 +16,8 @@
 // operations against 8 * D bytes of partials (written and read), so the
 // partials, the softmax and the way to the tiles, not the matrix unit, set the
 // pace (its share of the time is 13 % forward, 15 % in the gradient).  Of a
-// scan's 200 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
-// tiles take 109, the join 42 (132 MB of partials, 3.2 TB/s), the plan 35; the
+// scan's 172 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
+// tiles take 109, the join 36 (132 MB of partials, 3.7 TB/s), the plan 33; the
 // floor is 22 by bytes.  Spans of 512 keys make that call 3 % faster, not enough
 // for the second plan that the smaller calls would then want.
 //
@@ -199,21 +199,21 @@ __device__ __forceinline__ uint32_t chunk_blocks(uint32_t c, uint32_t block_log2
   return ((1u << n) - 1u) << ((c << 6) >> block_log2);
 }
 
-// One warp per query: which slots lead a pair, and the blocks of each pair.
+// LANES lanes per query: which slots lead a pair, and the blocks of each pair.
 // A pair's leading slot is the first slot that lists a block of its span; a
 // repeated block sets the same bit again.  The sort key is the span and, as
 // its place in a Gray code, the set of 64-key chunks that are read: neighbours
 // in that order differ in few chunks, so the rows of a tile read alike.
-template <int SLOTS>  // 32-slot parts of a list
+template <int SLOTS, int LANES>  // slots per lane, LANES apart
 __global__ void __launch_bounds__(256)
 plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
            uint32_t *__restrict__ mask, unsigned long long *__restrict__ lead,
            uint8_t *__restrict__ listed) {
   after_previous();
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint32_t bm = blockIdx.x * 8u + (threadIdx.x >> 5);
-  if (bm >= a.B * a.M) return;
-  const uint32_t b = bm / a.M;
+  const uint32_t lane = threadIdx.x & (LANES - 1u), here = (threadIdx.x & 31u) - lane;
+  const uint32_t bm = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
+  const bool some = bm < a.B * a.M;  // (all lanes of a warp take part in its shuffles)
+  const uint32_t top = some ? a.top : 0u, b = some ? bm / a.M : 0u;
   const uint32_t len = cloud_length(a.lengths, b, a.N);
   const uint32_t live = (uint32_t)(((uint64_t)len + (1u << a.block_log2) - 1u) >> a.block_log2);
   const uint32_t in_log2 = span_log2 - a.block_log2;  // blocks per span, log2
@@ -221,8 +221,8 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
   uint32_t sb[SLOTS], bit[SLOTS], m[SLOTS], lead_of[SLOTS];
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
-    const uint32_t s = lane + 32u * i;
-    const int64_t j = s < a.top ? a.blocks[(uint64_t)bm * a.top + s] : -1;
+    const uint32_t s = lane + LANES * i;
+    const int64_t j = s < top ? a.blocks[(uint64_t)bm * a.top + s] : -1;
     const bool use = j >= 0 && j < (int64_t)live;
     sb[i] = use ? (uint32_t)j >> in_log2 : none;
     bit[i] = use ? 1u << ((uint32_t)j & ((1u << in_log2) - 1u)) : 0u;
@@ -233,16 +233,16 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
   }
 #pragma unroll
   for (int part = SLOTS - 1; part >= 0; --part) {
-    const uint32_t n = min(32u, a.top > 32u * part ? a.top - 32u * part : 0u);
+    const uint32_t n = min((uint32_t)LANES, a.top > LANES * part ? a.top - LANES * part : 0u);
 #pragma unroll 4
     for (uint32_t s = n; s-- > 0u;) {  // downwards: the last match is the first slot
-      const uint32_t osb = __shfl_sync(kFullMask, sb[part], s);
-      const uint32_t obit = __shfl_sync(kFullMask, bit[part], s);
+      const uint32_t osb = __shfl_sync(kFullMask, sb[part], s, LANES);
+      const uint32_t obit = __shfl_sync(kFullMask, bit[part], s, LANES);
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i)
         if (osb == sb[i]) {
           m[i] |= obit;
-          lead_of[i] = s + 32u * part;
+          lead_of[i] = s + LANES * part;
         }
     }
   }
@@ -250,10 +250,11 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
   const uint32_t chunks = 1u << (span_log2 - 6u);
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
-    const uint32_t s = lane + 32u * i;
+    const uint32_t s = lane + LANES * i;
     const bool first = sb[i] != none && lead_of[i] == s;
-    leaders |= (unsigned long long)__ballot_sync(kFullMask, first) << (32 * i);
-    if (s >= a.top) continue;
+    const uint32_t firsts = __ballot_sync(kFullMask, first) >> here;
+    leaders |= (unsigned long long)(firsts & (kFullMask >> (32 - LANES))) << (LANES * i);
+    if (s >= top) continue;
     uint32_t read = 0;
     for (uint32_t c = 0; c < chunks; ++c)
       read |= (m[i] & chunk_blocks(c, a.block_log2)) ? 1u << c : 0u;
@@ -264,7 +265,7 @@ plan_pairs(const AttnArgs a, uint32_t span_log2, uint32_t *__restrict__ keys,
     keys[p] = first ? ((b * a.nsb + sb[i]) << chunks) | rank : (a.B * a.nsb) << chunks;
     mask[p] = m[i];
   }
-  if (lane == 0) lead[bm] = leaders;
+  if (some && lane == 0) lead[bm] = leaders;
 }
 
 // Keys of the sort: one per query slot, in slot order.
@@ -885,7 +886,10 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, uint64_t at, float4
 // its leading slots.  A warp takes 128 consecutive elements of a query's heads,
 // four per lane: the slots are the same for all lanes, and what a slot's
 // partial holds of them is consecutive too.  A scan's 132 MB of partials, read
-// in the queries' order, take 42 us.
+// in the queries' order, take 36 us (the logs and the weights in a pass of their
+// own first: 42).
+constexpr int kJoinFlight = 8;  // partials in flight per lane
+
 template <class T>
 __global__ void __launch_bounds__(256)
 attend_join(const AttnArgs a, uint32_t parts) {
@@ -901,24 +905,14 @@ attend_join(const AttnArgs a, uint32_t parts) {
   const float *lse = a.part_lse + (uint64_t)bm * a.top * hc + hh;
   const float *part = a.part + (uint64_t)bm * a.top * hc * a.D + d;
   const uint64_t step = (uint64_t)hc * a.D;
-  float mx = -INFINITY;
-  for (unsigned long long l = lead; l;) {
-    float x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      x[u] = l ? lse[(uint64_t)(__ffsll(l) - 1) * hc] : -INFINITY;
-      l &= l - 1ull;
-    }
-    mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-  }
-  const float base = mx == -INFINITY ? 0.f : mx;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float total = 0.f;
+  float mx = -INFINITY, total = 0.f;  // the sums so far are relative to mx
   for (unsigned long long l = lead; l;) {
-    float c[4];
-    float4 x[4];
+    float c[kJoinFlight];
+    float4 x[kJoinFlight];
+    float next = mx;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kJoinFlight; ++u) {
       const uint32_t s = l ? __ffsll(l) - 1 : 0u;
       c[u] = l ? lse[(uint64_t)s * hc] : -INFINITY;
       x[u] = l ? __ldcs(reinterpret_cast<const float4 *>(part + s * step))
@@ -926,7 +920,13 @@ attend_join(const AttnArgs a, uint32_t parts) {
       l &= l - 1ull;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kJoinFlight; ++u) next = fmaxf(next, c[u]);
+    const float base = next == -INFINITY ? 0.f : next, old = exp2_fast(mx - base);
+    mx = next;
+    total *= old;
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+    for (int u = 0; u < kJoinFlight; ++u) {
       const float y = exp2_fast(c[u] - base);
       total += y;
       acc.x += y * x[u].x; acc.y += y * x[u].y; acc.z += y * x[u].z; acc.w += y * x[u].w;
@@ -1935,9 +1935,14 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   // (the tile counters and the spans' marks, cleared together)
   if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + 16 * (uint64_t)spans, st))) return err;
   if (n && spans) {
-    const uint32_t grid = (uint32_t)ceil_div(a.B * a.M, 8);
-    if ((err = launch_next(a.top <= 32 ? plan_pairs<1> : plan_pairs<2>, grid, 256, 0, st, a,
-                           w.span_log2, w.sort.keys0, w.mask, w.lead, w.listed)))
+    // a power of two of lanes that holds the list, up to a warp with two slots each
+    const uint32_t lanes = a.top <= 8 ? 8 : a.top <= 16 ? 16 : 32;
+    const auto kernel = a.top <= 8    ? plan_pairs<1, 8>
+                        : a.top <= 16 ? plan_pairs<1, 16>
+                        : a.top <= 32 ? plan_pairs<1, 32>
+                                      : plan_pairs<2, 32>;
+    if ((err = launch_next(kernel, (uint32_t)ceil_div((uint64_t)a.B * a.M * lanes, 256), 256, 0, st,
+                           a, w.span_log2, w.sort.keys0, w.mask, w.lead, w.listed)))
       return err;
     if ((err = run_sort(PairKeys{w.sort.keys0}, n, spans << shift, w.sort, &list, st))) return err;
   } else {  // no pair, or no key to form one with
