@@ -162,3 +162,12 @@ def test_python_entries_refuse_host_tensors():
     x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(TypeError, match="CUDA"):
         attention.block_attention(x, x, x, torch.zeros(4, 1, dtype=torch.int64), 16)
+
+
+def test_attention_refuses_a_rest_off_its_alignment():
+    d = _attention()
+    with pytest.raises(RuntimeError, match=f"rc={capi.ERR_ARG}.*rest"):
+        capi.block_attention_device(d, P, P, P, P, 0, P, P, P, 1 << 40, rest=P + 8)
+    with pytest.raises(RuntimeError, match=f"rc={capi.ERR_ARG}.*rest"):
+        capi.block_attention_grad_device(d, P, P, P, P, 0, P, P, P, P, P, P, P, 1 << 40,
+                                         rest=P + 2)
