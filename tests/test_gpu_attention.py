@@ -436,3 +436,19 @@ def test_gradients_of_few_keys(N, dtype):
     for name, got, want in (("dq", dq, ref.dq), ("dk", dk, ref.dk)):
         off = float((got.double() - want).norm() / want.norm())
         assert off <= math.sqrt(2 / 3) * u, (name, off / u)
+
+
+@pytest.mark.parametrize("N", [2, 7])
+def test_gradients_of_few_keys_of_many_queries(N):
+    """The same where the queries are enough to be gathered into tiles (above
+    65,535, whatever they read)."""
+    B, M, H, G, D, dtype = 2, 33_000, 1, 1, 64, torch.bfloat16
+    q, k, v, blocks, dout = _one_block(B, M, N, H, G, D, dtype, 5)
+    ref = Exact(q, k, v, blocks, 16, dout=dout)
+    dq, dk, _ = _grads(q, k, v, blocks, dout)
+    u = torch.finfo(dtype).eps / 2
+    off = float((dq.double() - ref.dq).norm() / ref.dq.norm())
+    assert off <= math.sqrt(2 / 3) * u, off / u
+    # dk adds M terms in fp32 besides
+    off = float((dk.double() - ref.dk).norm() / ref.dk.norm())
+    assert off <= math.sqrt(2 / 3) * u + M * U32, off / u
