@@ -18,8 +18,9 @@
 // pace (its share of the time is 13 % forward, 15 % in the gradient).  Of a
 // scan's 172 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
 // tiles take 109, the join 36 (132 MB of partials, 3.7 TB/s), the plan 33; the
-// floor is 22 by bytes.  Spans of 512 keys make that call 3 % faster, not enough
-// for the second plan that the smaller calls would then want.
+// floor is 22 by bytes.  Spans of 128 keys make more pairs (186 us); spans of 512
+// make that call 3 % faster, not enough for the second plan that the smaller
+// calls would then want.
 //
 // A handful of queries does not fill tiles and would wait for the sort; they
 // take a direct path, which splits each query's own keys over CTAs (mma.sync,
