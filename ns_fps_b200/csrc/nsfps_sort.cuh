@@ -30,16 +30,23 @@ constexpr uint32_t kSmallSmem = kSortSmall * 8u + 32u * 256u * 2u;
 constexpr uint32_t kSumTiles = 64;
 
 // Keys per tile: few enough that small lists still spread over the SMs.
-inline uint32_t sort_tile(uint32_t n) { return kSortThreads * (n <= (1u << 19) ? 4u : 16u); }
+constexpr uint32_t kShortTiles = 1u << 19;  // the longest list in short tiles
+inline uint32_t sort_tile(uint32_t n) { return kSortThreads * (n <= kShortTiles ? 4u : 16u); }
 
+// Scratch for any list of up to n keys.  A list just short enough for short
+// tiles has more of them than one somewhat longer, so what the longest list
+// has is not enough: a call taken in turns ends with a shorter one.
 struct SortScratch {
   uint32_t *keys0, *vals0, *keys1, *vals1, *hist, *total, *kept;
+  uint32_t tiles;  // for which hist has room
   void carve(WorkCarver &w, uint32_t n) {
+    const uint32_t few = std::min(n, kShortTiles);
+    tiles = (uint32_t)std::max(ceil_div(n, sort_tile(n)), ceil_div(few, sort_tile(few)));
     keys0 = w.take<uint32_t>(n);
     vals0 = w.take<uint32_t>(n);
     keys1 = w.take<uint32_t>(n);
     vals1 = w.take<uint32_t>(n);
-    hist = w.take<uint32_t>(256ull * ceil_div(n, sort_tile(n)));
+    hist = w.take<uint32_t>(256ull * tiles);
     total = w.take<uint32_t>(256);
     kept = w.take<uint32_t>(1);
   }
@@ -305,7 +312,7 @@ sort_small(const Source src, uint32_t n, uint32_t none, uint32_t passes, uint32_
 }
 
 // Sorts the positions of src (n of them; keys below `none`, or `none` to be
-// dropped; none > 0).
+// dropped; none > 0) in scratch carved for n keys or more.
 template <class Source>
 cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScratch &w,
                      SortedList *out, cudaStream_t st) {
@@ -321,6 +328,7 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
     return launch_next(sort_small<Source>, 1, 1024, kSmallSmem, st, src, n, none, passes, digit,
                        w.keys1, w.vals1, w.kept);
   }
+  if (tiles > w.tiles) return cudaErrorInvalidValue;
   const bool few = tiles <= kSumTiles;
   uint32_t *keys = w.keys0, *vals = w.vals0, *keys_next = w.keys1, *vals_next = w.vals1;
   for (uint32_t p = 0; p < passes; ++p) {

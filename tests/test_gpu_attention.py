@@ -452,3 +452,27 @@ def test_gradients_of_few_keys_of_many_queries(N):
     # dk adds M terms in fp32 besides
     off = float((dk.double() - ref.dk).norm() / ref.dk.norm())
     assert off <= math.sqrt(2 / 3) * u + M * U32, off / u
+
+
+@pytest.mark.parametrize("M", [16_384, 14_000])
+def test_a_last_turn_of_shorter_sort_tiles(M):
+    """Three clouds whose partial results make turns of two and one: the
+    forward's (M = 16,384) or the gradient's (14,000).  A full turn's 786,432 or
+    672,000 pairs are sorted in tiles of 4,096 keys, the last one's half in more
+    tiles of 1,024.  The last cloud by itself gives the same bits."""
+    from ns_fps_b200 import attention
+    B, N, H, G, D, top, block, dtype = 3, 600, 4, 2, 128, 24, 16, torch.bfloat16
+    q, dout = _normal((B, M, H, D), dtype, 1), _normal((B, M, H, D), dtype, 2)
+    k, v = _normal((B, N, G, D), dtype, 3), _normal((B, N, G, D), dtype, 4)
+    blocks = _lists(B, M, (N + block - 1) // block, top, 5)
+
+    def step(*x):
+        leaves = [t.detach().requires_grad_() for t in x[:3]]
+        out = attention.block_attention(*leaves, x[3], block)
+        return (out.detach(), *torch.autograd.grad(out, leaves, x[4]))
+
+    together = step(q, k, v, blocks, dout)
+    for b in range(B):
+        apart = step(*(t[b:b + 1] for t in (q, k, v, blocks, dout)))
+        for x, y in zip(together, apart):
+            assert torch.equal(x[b:b + 1], y)
