@@ -25,7 +25,7 @@ import ctypes
 import math
 
 from . import capi
-from .group import _cloud_batch, _dtype_code, _enter, _leave, _Plans
+from .group import _cloud_batch, _dtype_code, _enter, _leave, _number, _Plans
 
 __all__ = ["select_blocks", "block_attention"]
 
@@ -178,7 +178,7 @@ def _attention_plan(q, k, v, blocks, block, lengths, scale):
     dense = [(n * h * D, h * D, D) for n, h in ((M, H), (k.shape[1], G), (k.shape[1], G))]
     strides = tuple(_strides(t) for t in (q, k, v))
     head = (B, M, k.shape[1], H, G, D, block, blocks.shape[2], code)
-    return copies, (head, strides, dense, 1.0 / math.sqrt(D) if scale is None else float(scale))
+    return copies, (head, strides, dense, 1.0 / math.sqrt(D) if scale is None else scale)
 
 
 def _desc(plan, moved, backward):
@@ -293,7 +293,8 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
     lengths  None, or int32 (B,): the keys of each padded cloud; what lies
              behind them, or in blocks that no query lists, is never part of a
              result.  Values that are listed have to be finite.
-    scale    default 1 / sqrt(D)
+    scale    a number, by default 1 / sqrt(D) (what a tensor holds is read, and
+             has no gradient)
 
     D is a multiple of 8 up to 128, H at most 256.  Returns a tensor like q,
     dense; a query without any key gets zeros.  Scores and sums are float32;
@@ -302,7 +303,7 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
     a fixed order.  Inputs whose rows are not 16-byte aligned are copied first.
     """
     import torch
-    block = int(block)
+    block, scale = int(block), None if scale is None else _number(scale)
     try:
         key = (_look(q), _look(k), _look(v), _look(blocks), _look(lengths), block, scale)
         plan = _attention_plans.get(key)

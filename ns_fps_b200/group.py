@@ -143,6 +143,18 @@ def _leave(before):
         torch.cuda.set_device(before)
 
 
+def _number(scale):
+    """A scale as the plain number that it is now.  (A tensor would be another
+    number at the next call, and still the same key of a plan.)"""
+    if type(scale) is float:
+        return scale
+    if getattr(scale, "requires_grad", False):
+        import torch
+        if torch.is_grad_enabled():
+            raise TypeError("scale takes no gradient: multiply by it outside, or pass a number")
+    return float(scale)
+
+
 class _Plans(dict):
     """What a call's shapes, strides and types settle once: its checks, its
     descriptor, its scratch.  Bounded; a plan holds no tensor."""
@@ -255,6 +267,7 @@ def gather_rows(table, idx, scale: float = 1.0):
 
     table  (N, C), or (B, N, C) for B clouds: float32, float16 or bfloat16
     idx    int64: any shape for (N, C); (B, ...) for (B, N, C)
+    scale  a number (what a tensor holds is read, and has no gradient)
 
     Returns idx.shape + (C,) in the table's type (the product in float32,
     rounded once).  A negative index stands for no row: zeros, and no gradient.
@@ -264,7 +277,7 @@ def gather_rows(table, idx, scale: float = 1.0):
     waiting for it.
     """
     import torch
-    scale = float(scale)
+    scale = _number(scale)
     try:
         key = (table.shape, table.stride(), table.dtype, table.device, idx.shape, idx.dtype,
                idx.device, scale)

@@ -171,3 +171,16 @@ def test_attention_refuses_a_rest_off_its_alignment():
     with pytest.raises(RuntimeError, match=f"rc={capi.ERR_ARG}.*rest"):
         capi.block_attention_grad_device(d, P, P, P, P, 0, P, P, P, P, P, P, P, 1 << 40,
                                          rest=P + 2)
+
+
+def test_python_entries_refuse_a_scale_that_wants_a_gradient():
+    torch = pytest.importorskip("torch")
+    from ns_fps_b200 import attention, group
+    scale = torch.tensor(0.5, requires_grad=True)
+    x, idx = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 1, dtype=torch.int64)
+    with pytest.raises(TypeError, match="scale.*gradient"):
+        attention.block_attention(x, x, x, idx, 16, scale=scale)
+    with pytest.raises(TypeError, match="scale.*gradient"):
+        group.gather_rows(x[:, 0], idx, scale)
+    with torch.no_grad(), pytest.raises(TypeError, match="CUDA"):  # a number then
+        attention.block_attention(x, x, x, idx, 16, scale=scale)

@@ -476,3 +476,29 @@ def test_a_last_turn_of_shorter_sort_tiles(M):
         apart = step(*(t[b:b + 1] for t in (q, k, v, blocks, dout)))
         for x, y in zip(together, apart):
             assert torch.equal(x[b:b + 1], y)
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_a_scale_that_changes_in_place(device):
+    """A scale held in a tensor is read at every call, and not kept."""
+    import gc
+    import weakref
+
+    from ns_fps_b200 import attention
+    q, k, v = (_normal((1, n, 2, 32), torch.float16, i) for i, n in enumerate((9, 100, 100)))
+    blocks, dout = _lists(1, 9, 7, 3, 4), _normal(q.shape, torch.float16, 5)
+
+    def step(scale):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = attention.block_attention(*leaves, blocks, 16, scale=scale)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    scale = torch.tensor(0.25, device=device)
+    for value in (0.25, 2.0, 0.0):
+        scale.fill_(value)
+        for x, y in zip(step(scale), step(value)):
+            assert torch.equal(x, y)
+    kept = weakref.ref(scale)
+    del scale
+    gc.collect()
+    assert kept() is None
