@@ -25,7 +25,7 @@ import ctypes
 import math
 
 from . import capi
-from .group import _cloud_batch, _dtype_code, _enter, _leave, _number, _Plans
+from .group import _cloud_batch, _dtype_code, _enter, _leave, _no_tangents, _number, _Plans
 
 __all__ = ["select_blocks", "block_attention"]
 
@@ -89,7 +89,8 @@ def select_blocks(points, centers, block: int, top: int, lengths=None):
     bounding box, the lower index first among equals, -1 (d2 = inf) behind the
     last block.  d2 is the sampler's arithmetic, (dx*dx + dy*dy) + dz*dz in
     float32 without contraction, so the choice is exact.  To cut the list at a
-    radius: ``blocks.masked_fill(d2 > radius * radius, -1)``.
+    radius: ``blocks.masked_fill(d2 > radius * radius, -1)``.  Points and centres
+    are data here, as for ``ball_query``: d2 carries no derivative.
     """
     import torch
     block, top = int(block), int(top)
@@ -273,6 +274,7 @@ def _autograd():
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
+                _no_tangents(dout)
                 q, k, v, blocks, lengths, out, keep = ctx.saved_tensors
                 grads = _backward(q, k, v, blocks, lengths, ctx.plan, out, keep, dout)
                 return (*grads, None, None, None)
@@ -300,7 +302,8 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
     dense; a query without any key gets zeros.  Scores and sums are float32;
     the softmax weights are rounded to q's type for the product with v.
     Gradients reach q, k and v (zeros for keys that no query lists), summed in
-    a fixed order.  Inputs whose rows are not 16-byte aligned are copied first.
+    a fixed order; forward-mode derivatives are refused.  Inputs whose rows are
+    not 16-byte aligned are copied first.
     """
     import torch
     block, scale = int(block), None if scale is None else _number(scale)
@@ -312,6 +315,7 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
     if plan is None:
         copies, shape = _attention_plan(q, k, v, blocks, block, lengths, scale)
         plan = _attention_plans.keep(key, (copies, shape, {}))
+    _no_tangents(q, k, v)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         return _autograd().apply(q, k, v, blocks, lengths, plan)
     return _forward(q, k, v, blocks, lengths, plan, False)[0]

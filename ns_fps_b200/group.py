@@ -143,14 +143,26 @@ def _leave(before):
         torch.cuda.set_device(before)
 
 
+def _no_tangents(*tensors):
+    """Refuses forward-mode differentiation: a kernel's result has no tangent,
+    which would read as a derivative of zero.  (A dual tensor need not require
+    a gradient, so the autograd node would not see it.)"""
+    import torch
+    forward_ad = torch.autograd.forward_ad
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("no forward-mode derivative: only gradients (backward)")
+
+
 def _number(scale):
     """A scale as the plain number that it is now.  (A tensor would be another
     number at the next call, and still the same key of a plan.)"""
     if type(scale) is float:
         return scale
-    if getattr(scale, "requires_grad", False):
-        import torch
-        if torch.is_grad_enabled():
+    import torch
+    if isinstance(scale, torch.Tensor):
+        _no_tangents(scale)
+        if scale.requires_grad and torch.is_grad_enabled():
             raise TypeError("scale takes no gradient: multiply by it outside, or pass a number")
     return float(scale)
 
@@ -254,6 +266,7 @@ def _gather_rows_autograd():
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
+                _no_tangents(dout)
                 idx, = ctx.saved_tensors
                 return _gather_rows_backward(dout, idx, ctx.shape, ctx.scale), None, None, None
 
@@ -273,8 +286,8 @@ def gather_rows(table, idx, scale: float = 1.0):
     rounded once).  A negative index stands for no row: zeros, and no gradient.
     An index of N or more is never read: its row is NaN, and its gradient goes
     nowhere.  The gradient adds a row's entries in float32 in index order, so
-    it is the same every time.  Runs on PyTorch's current stream without
-    waiting for it.
+    it is the same every time.  Forward-mode derivatives are refused.  Runs on
+    PyTorch's current stream without waiting for it.
     """
     import torch
     scale = _number(scale)
@@ -286,6 +299,7 @@ def gather_rows(table, idx, scale: float = 1.0):
         key = plan = None
     if plan is None:
         plan = _rows_plans.keep(key, _rows_plan(table, idx, scale))
+    _no_tangents(table)
     if table.requires_grad and torch.is_grad_enabled():
         return _gather_rows_autograd().apply(table, idx, scale, plan)
     return _gather_rows_forward(table, idx, scale, plan)

@@ -502,3 +502,29 @@ def test_a_scale_that_changes_in_place(device):
     del scale
     gc.collect()
     assert kept() is None
+
+
+def test_forward_mode_derivatives_are_refused():
+    """They are not computed, and no result without a tangent stands for one."""
+    from torch.autograd import forward_ad
+
+    from ns_fps_b200 import attention
+    x = [_normal((n, 2, 32), torch.float16, i) for i, n in enumerate((9, 100, 100))]
+    blocks, dout = _lists(1, 9, 7, 3, 4)[0], _normal(x[0].shape, torch.float16, 5)
+    plain = attention.block_attention(*x, blocks, 16)
+    with forward_ad.dual_level():
+        for i in range(3):
+            for leaf in (False, True):
+                args = [t.detach().requires_grad_(leaf) for t in x]
+                args[i] = forward_ad.make_dual(args[i], torch.ones_like(x[i]))
+                with pytest.raises(RuntimeError, match="forward"):
+                    attention.block_attention(*args, blocks, 16)
+        scale = forward_ad.make_dual(torch.tensor(0.5), torch.tensor(1.0))
+        with pytest.raises(RuntimeError, match="forward"):
+            attention.block_attention(*x, blocks, 16, scale=scale)
+        leaves = [t.detach().requires_grad_() for t in x]
+        out = attention.block_attention(*leaves, blocks, 16)
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(out, leaves, forward_ad.make_dual(dout, torch.ones_like(dout)))
+        assert torch.equal(attention.block_attention(*x, blocks, 16), plain)  # no tangent: as ever
+    assert torch.equal(attention.block_attention(*x, blocks, 16), plain)

@@ -221,3 +221,26 @@ def test_refusals():
                        ((table, idx.cpu()), TypeError), ((table, idx, math.nan), RuntimeError)]:
         with pytest.raises(error):
             group.gather_rows(*bad)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """They are not computed, and no result without a tangent stands for one."""
+    from torch.autograd import forward_ad
+
+    from ns_fps_b200 import group
+    table = torch.ones(5, 4, device="cuda")
+    idx = torch.tensor([1, 3], device="cuda")
+    with forward_ad.dual_level():
+        for leaf in (False, True):
+            dual = forward_ad.make_dual(table.detach().requires_grad_(leaf), table)
+            with pytest.raises(RuntimeError, match="forward"):
+                group.gather_rows(dual, idx)
+        scale = forward_ad.make_dual(torch.tensor(0.5), torch.tensor(1.0))
+        with pytest.raises(RuntimeError, match="forward"):
+            group.gather_rows(table, idx, scale)
+        leaf = table.detach().requires_grad_()
+        out = group.gather_rows(leaf, idx)
+        dout = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(out, leaf, dout)
+        assert torch.equal(group.gather_rows(table, idx), table[idx])
