@@ -363,7 +363,10 @@ NSFPS_API int nsfps_block_attention_device(const nsfps_attention_desc *desc, con
  * head_dim; keys that no query reads get zeros) from dout (dense, like out,
  * 16-byte aligned) and the forward's out, lse and rest.  Without rest (NULL)
  * the gradient takes out as it is rounded, which dq and dk of queries with few
- * weighty keys feel. */
+ * weighty keys feel.  The weights p and the score gradients ds are rounded to
+ * the inputs' type for the products; in F16 both are first multiplied by powers
+ * of two (ds by one that follows the sizes of dout and v), so neither overflows
+ * nor sinks among the smallest numbers where the results do not. */
 NSFPS_API int nsfps_block_attention_grad_device(const nsfps_attention_desc *desc, const void *d_q,
                                                 const void *d_k, const void *d_v,
                                                 const int64_t *d_blocks,

@@ -27,6 +27,7 @@
 // whose 16-row tiles suit a query's few heads; the keys' bytes bound it).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "nsfps_feature.cuh"
 #include "nsfps_sort.cuh"
@@ -66,6 +67,7 @@ struct AttnArgs {
   float *part;             // [pair][gc * R][D]
   float *part_lse;         // [pair][gc * R], base 2
   float *delta;            // [query][H]
+  uint32_t *most;          // [cloud][G][2], float bits: |dout|^2 and |delta| at most
   float *part_kv;          // [share][gc][2][span][D]
   // direct path: partials per query, rounds per partial, 16-row parts of R
   uint32_t splits, rounds, row_parts;
@@ -1138,6 +1140,34 @@ __device__ __forceinline__ bool one_key(const AttnArgs &a, uint32_t bm) {
          ((uint64_t)a.blocks[slot] << a.block_log2) + 1u == cloud_length(a.lengths, bm / a.M, a.N);
 }
 
+// In half precision p and ds would lie among the smallest numbers, where few
+// bits are left, for a usual gradient without a scaled loss (ds is 10^-6 with
+// dout of 10^-4 and 512 keys: dk was off four times as far as its own rounding
+// puts it), and ds beyond the largest one for a large gradient and few keys.  So
+// p is taken times 2^15, which p <= 1 allows, and ds times a power of two per
+// item, undone on the fp32 sums.  By |dp| <= |dout| |v| the factor of
+//   bound = max |dout| over the queries of the cloud and key head
+//           * max |v| over the item's keys + max |delta| likewise
+// keeps every ds below 2^15, half the largest number, whatever the inputs; the
+// rows' maxima come from grad_delta, |v| from the item's keys in shared memory.
+template <class T>
+constexpr bool kScaled = std::is_same_v<T, __half>;
+constexpr float kUp = 32768.f;  // 2^15
+
+// The exponent of the factor (the bound's parts squared: dout, v; delta).
+__device__ __forceinline__ int ds_exponent(float dout2, float v2, float delta) {
+  const float bound = sqrtf(dout2 * v2) + delta;  // < 2^(e + 1)
+  const int e = (int)(__float_as_uint(bound) >> 23) - 127;
+  return min(max(14 - e, -100), 100);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// *to = max(*to, x), x >= 0.  Most rows find a larger one there already.
+__device__ __forceinline__ void raise(uint32_t *to, float x) {
+  const uint32_t bits = __float_as_uint(x);
+  if (bits > *reinterpret_cast<volatile uint32_t *>(to)) atomicMax(to, bits);
+}
+
 // delta = sum_d dout * out per row; 8 lanes per row, 8 elements per step; bound
 // by the bytes read.  out comes with what its rounding left: ds = p (dp - delta)
 // is a difference of like numbers where few keys have the weight, and with the
@@ -1150,7 +1180,7 @@ grad_delta(const AttnArgs a) {
   after_previous();
   const uint64_t row = (uint64_t)blockIdx.x * 32u + (threadIdx.x >> 3);
   const uint32_t sub = threadIdx.x & 7u;
-  float s = 0.f;
+  float s = 0.f, dout2 = 0.f;
   if (row < (uint64_t)a.B * a.M * a.H)
     for (uint32_t d = sub * 8; d < a.D; d += 64) {
       const uint4 x = *reinterpret_cast<const uint4 *>(a.dout + (row * a.D + d) * 2);
@@ -1161,12 +1191,49 @@ grad_delta(const AttnArgs a) {
       const T *xe = reinterpret_cast<const T *>(&x), *ye = reinterpret_cast<const T *>(&y);
       const T *ze = reinterpret_cast<const T *>(&z);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += to_f32(xe[i]) * (to_f32(ye[i]) + to_f32(ze[i]));
+      for (int i = 0; i < 8; ++i) {
+        s += to_f32(xe[i]) * (to_f32(ye[i]) + to_f32(ze[i]));
+        if (kScaled<T>) dout2 += to_f32(xe[i]) * to_f32(xe[i]);
+      }
     }
 #pragma unroll
-  for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-  if (sub == 0 && row < (uint64_t)a.B * a.M * a.H)
-    a.delta[row] = one_key(a, (uint32_t)(row / a.H)) ? INFINITY : s;
+  for (int o = 4; o; o >>= 1) {
+    s += __shfl_xor_sync(kFullMask, s, o);
+    if (kScaled<T>) dout2 += __shfl_xor_sync(kFullMask, dout2, o);
+  }
+  const uint32_t bm = (uint32_t)(row / a.H);
+  const bool some = row < (uint64_t)a.B * a.M * a.H, one = some && one_key(a, bm);
+  if (some && sub == 0) a.delta[row] = one ? INFINITY : s;
+  if (!kScaled<T>) return;
+  // The rows' maxima: first among the CTA's 32 rows, so that a word of a key
+  // head is raised by few (by every row, this kernel took 31 us of a training
+  // step of four clouds; so it takes 9, and 6 without the maxima).  Rows that move no score do not count,
+  // nor do those that are not finite: they spoil their own results, not the
+  // others' factor.
+  __shared__ uint32_t s_word[32];
+  __shared__ float2 s_most[32];
+  if (sub == 0) {
+    const bool counts = some && !one && a.lead[bm] && dout2 < INFINITY && fabsf(s) < INFINITY;
+    const uint32_t g = (uint32_t)(row - (uint64_t)bm * a.H) / a.R;
+    s_word[threadIdx.x >> 3] = counts ? bm / a.M * a.G + g : 0xffffffffu;
+    s_most[threadIdx.x >> 3] = make_float2(dout2, fabsf(s));
+  }
+  __syncthreads();
+  if (threadIdx.x >= 32u) return;
+  const uint32_t mine = s_word[threadIdx.x];
+  bool first = mine != 0xffffffffu;
+  float2 most = make_float2(0.f, 0.f);
+#pragma unroll 8
+  for (uint32_t r = 0; r < 32u; ++r) {
+    if (s_word[r] != mine) continue;
+    const float2 x = s_most[r];
+    most = make_float2(fmaxf(most.x, x.x), fmaxf(most.y, x.y));
+    if (r < threadIdx.x) first = false;
+  }
+  if (first) {
+    raise(a.most + 2ull * mine, most.x);
+    raise(a.most + 2ull * mine + 1u, most.y);
+  }
 }
 
 constexpr uint32_t kGradItem = 512;    // query rows per item
@@ -1208,7 +1275,8 @@ struct GradItem {
 // an operand of dq read down its rows (dq = ds k, or with heads of 128
 // elements dq^T = k^T ds^T, so that 64 rows a step suffice); dv += p^T dout
 // takes p from tensor memory.  p and ds are rounded to T for these products,
-// half a step each.
+// half a step each (in half precision clear of its ends: kScaled, which costs
+// the four clouds below 7 us here).
 //
 // Done in turns by all warps, the stages of a step took 11,000 cycles, of
 // which the weights were 2,500.  So the warps have roles and meet at barriers:
@@ -1228,6 +1296,9 @@ attend_grad(const AttnArgs a) {
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[kStages * 2 + 4 + 6];
   __shared__ uint32_t s_tmem;
+  // |v|^2 at most, per warp that loads them, of items k & 3 (a warp that is a
+  // step behind another may still read those of the item before)
+  __shared__ float s_v2[4][kResultWarps];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = warp_value(tid >> 5);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char *smem = smem_raw + (base - smem_u32(smem_raw));
@@ -1306,6 +1377,18 @@ attend_grad(const AttnArgs a) {
   auto wait = [&](uint32_t bar, uint32_t phase) {
     if (!failed) failed = !bar_wait(bar, phase);
   };
+  // The exponent of an item's factor of ds; `most` is asked for before the keys
+  // are waited for.
+  auto most_of = [&](const GradItem &x) {
+    return kScaled<T>
+               ? *reinterpret_cast<const float2 *>(a.most + 2ull * ((uint64_t)x.b * a.G + x.g))
+               : make_float2(0.f, 0.f);
+  };
+  auto exponent_of = [&](uint32_t k, const float2 &most) {
+    wait(kv_full(k), (k >> 1) & 1u);
+    const float *v2 = s_v2[k & 3u];
+    return ds_exponent(most.x, fmaxf(fmaxf(v2[0], v2[1]), fmaxf(v2[2], v2[3])), most.y);
+  };
   // n counts the steps, k the items
   // with steps.  Use u of a buffer or result waits for completion u - 1 of its
   // release, whose parity is (u - 1) & 1.
@@ -1316,9 +1399,12 @@ attend_grad(const AttnArgs a) {
     const uint32_t col0 = (warp >> 2) * kCols;
     const uint32_t key_in = quad * 32u + lane, block = key_in >> a.block_log2;
     const float c2 = a.scale * kLog2e;
-    uint32_t n = 0;
+    uint32_t n = 0, k = 0;
     for (Items y = items(); y.w < work; advance(y)) {
       const GradItem it = item_of(y);
+      const float2 most = most_of(it);
+      float f_ds = 1.f;  // of ds, over p's
+      if (kScaled<T> && it.steps) f_ds = pow2(exponent_of(k++, most) - 15);
       // rows that may read this key; kLone: it is a block's only key
       constexpr uint32_t kLone = 0x10000u;
       const uint32_t key = it.key0 + key_in;
@@ -1361,8 +1447,10 @@ attend_grad(const AttnArgs a) {
                               make_float2(c2, c2), make_float2(-z.x, -z.z));
               f.x = exp2_fast(f.x);
               f.y = exp2_fast(f.y);
-              float2 g = mul2(f, add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
-                                      make_float2(-z.y, -z.w)));
+              float2 g = add2(make_float2(__uint_as_float(dx[y]), __uint_as_float(dx[y + 1])),
+                              make_float2(-z.y, -z.w));
+              if (kScaled<T>) g = mul2(g, make_float2(f_ds, f_ds));
+              g = mul2(f, g);
               if (!all) {
                 const bool in0 = (in >> y) & 1u, in1 = (in >> (y + 1u)) & 1u;
                 f.x = in0 ? f.x : 0.f, g.x = in0 ? g.x : 0.f;
@@ -1437,13 +1525,42 @@ attend_grad(const AttnArgs a) {
     auto finish_load = [&]() {
       copy_wait<0>();
       smem_to_mma();
+      if (kScaled<T>) {
+        // of the chunks of 8 elements that this thread loaded (load_strided),
+        // the longest in each place of a row, and those of a row together
+        constexpr uint32_t kStep = 128u / kChunks;
+        const uint32_t c = role_tid % kChunks, r0 = role_tid / kChunks;
+        const char *v = smem + ((loaded % Shape::kKv) * 2u + 1u) * Shape::kKeyTile +
+                        (c >> 3) * (128u * 128u) + swizzled(r0, c & 7u);
+        float most = 0.f;
+#pragma unroll 4
+        for (uint32_t i = 0; i < 128u / kStep; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(v + i * kStep * 128u);
+          const T *e = reinterpret_cast<const T *>(&x);
+          float v2 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v2 = fmaf(to_f32(e[j]), to_f32(e[j]), v2);
+          most = fmaxf(most, v2 < INFINITY ? v2 : 0.f);
+        }
+#pragma unroll
+        for (uint32_t o = 16u; o >= kChunks; o >>= 1)
+          most = fmaxf(most, __shfl_xor_sync(kFullMask, most, o));
+#pragma unroll
+        for (uint32_t o = kChunks / 2u; o; o >>= 1) most += __shfl_xor_sync(kFullMask, most, o);
+        if (lane == 0) s_v2[loaded & 3u][warp & 3u] = most;
+      }
       __syncwarp();
       if (lane == 0) bar_arrive(kv_full(loaded));
       ++loaded;
     };
     if (load_next()) finish_load();
+    uint32_t k = 0;
     for (Items y = items(); y.w < work; advance(y)) {
       const GradItem it = item_of(y);
+      const float2 most = most_of(it);
+      float down_ds = 1.f;
+      if (kScaled<T> && it.steps) down_ds = pow2(-exponent_of(k++, most));
+      constexpr float kDownP = kScaled<T> ? 1.f / kUp : 1.f;
       // (waited for here: the products of this item's last step come after the
       // next item's scores)
       if (it.steps && Shape::kKv == 2u && load_next()) finish_load();
@@ -1457,7 +1574,7 @@ attend_grad(const AttnArgs a) {
         wait(g_done, n & 1u);
         __syncwarp();
         tmem_after_sync();
-        const float f = failed ? NAN : 1.f;
+        const float f = failed ? NAN : down_ds;
         // (places first: behind the second half the stage is given back)
         const uint32_t mine = DP == 64 ? place[at_lane] : 0u;
 #pragma unroll
@@ -1507,7 +1624,7 @@ attend_grad(const AttnArgs a) {
             __syncwarp();
             if (lane == 0) bar_arrive(acc_free);
           }
-          const float g = is_k && whole ? f * a.scale : f;
+          const float g = !is_k ? f * kDownP : whole ? f * down_ds * a.scale : f * down_ds;
           if (some) {
 #pragma unroll
             for (uint32_t y = 0; y < 32u; y += 8u) {
@@ -1645,7 +1762,7 @@ attend_grad(const AttnArgs a) {
           const uint32_t pair = a.vals[it.e0 + e];
           const uint32_t bm = pair / a.top, m = bm - it.b * a.M, h = it.g * a.R + head;
           const uint32_t row = bm * a.H + h;
-          lse[j] = a.lse_in[row] * kLog2e;
+          lse[j] = a.lse_in[row] * kLog2e - (kScaled<T> ? 15.f : 0.f);
           delta[j] = a.delta[row];
           mask[j] = r0 < it.rows ? a.mask[pair] : 0u;
           place[j] = r0 < it.rows ? pair * (a.gc * a.R) + it.gi * a.R + head : 0xffffffffu;
@@ -1806,7 +1923,8 @@ struct AttnPlan {
   uint32_t span_log2, tile_rows, least, splits, rounds;
   uint64_t pairs, spans, max_tiles;  // of one turn
   SortScratch sort;
-  uint32_t *mask, *tile_count;
+  uint32_t *mask, *tile_count, *most;
+  uint64_t most_bytes;
   uint8_t *listed;
   uint4 *span;
   unsigned long long *lead;
@@ -1872,8 +1990,11 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
   w.span = c.take<uint4>(w.spans);
   static_assert(4 * (kTileClasses + 1) <= 32, "the marks begin 32 bytes behind");
-  w.tile_count = (uint32_t *)c.take<char>(32 + 16 * w.spans);
-  w.listed = (uint8_t *)w.tile_count + (base ? 32 : 0);
+  // (cleared together, before a turn)
+  w.most_bytes = backward && d.dtype == NSFPS_F16 ? ceil_div(w.bc * (uint64_t)d.kv_heads, 2) * 16 : 0;
+  w.tile_count = (uint32_t *)c.take<char>(32 + w.most_bytes + 16 * w.spans);
+  w.most = w.tile_count + (base ? 8 : 0);
+  w.listed = (uint8_t *)w.most + (base ? w.most_bytes : 0);
   w.tiles = c.take<uint4>(kTileClasses * w.max_tiles);
   w.part = c.take<float>(w.pairs * R * w.gc * d.head_dim);
   if (backward) {
@@ -1898,6 +2019,7 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   for (int i = 0; i < 3; ++i) a.qs[i] = d.q_stride[i], a.ks[i] = d.k_stride[i], a.vs[i] = d.v_stride[i];
   a.scale = d.scale;
   a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
+  a.most = w.most;
   a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
   a.listed = (const uint4 *)w.listed;
   a.tile_stride = (uint32_t)w.max_tiles;
@@ -1933,8 +2055,9 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   const uint32_t shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
   SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
-  // (the tile counters and the spans' marks, cleared together)
-  if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + 16 * (uint64_t)spans, st))) return err;
+  // (the tile counters, the rows' maxima and the spans' marks, cleared together)
+  if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + w.most_bytes + 16 * (uint64_t)spans, st)))
+    return err;
   if (n && spans) {
     // a power of two of lanes that holds the list, up to a warp with two slots each
     const uint32_t lanes = a.top <= 8 ? 8 : a.top <= 16 ? 16 : 32;

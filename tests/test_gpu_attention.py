@@ -528,3 +528,60 @@ def test_forward_mode_derivatives_are_refused():
             torch.autograd.grad(out, leaves, forward_ad.make_dual(dout, torch.ones_like(dout)))
         assert torch.equal(attention.block_attention(*x, blocks, 16), plain)  # no tangent: as ever
     assert torch.equal(attention.block_attention(*x, blocks, 16), plain)
+
+
+@pytest.mark.parametrize("size,v_size,M,N,D", [
+    (1e-4, 1.0, 200, 2048, 64), (1e-3, 1.0, 200, 2048, 64), (1.0, 1.0, 200, 2048, 64),
+    (1e-3, 1.0, 100, 512, 128), (1e-2, 1.0, 70, 2000, 24), (8000.0, 1.0, 8, 3, 64),
+    (8000.0, 1.0, 8, 3, 128), (1e-3, 500.0, 200, 2048, 64), (10.0, 0.002, 200, 2048, 64)])
+def test_half_precision_gradients_of_any_size(size, v_size, M, N, D):
+    """float16 gradients where the incoming one is small, as it is without a
+    scaled loss, and large, as with one: dq, dk and dv are off by the roundings
+    of ds or p and of themselves alone.  A rounding error is uniform within half
+    a step, at most u of the value or 2^-25 below the smallest normal number, so
+    its square is at most a third of that on average; the two roundings are
+    independent.  ds and p keep clear of the smallest numbers, whatever the size
+    of dout; the results may lie among them.  (64 roundings of fp32 besides.)"""
+    B, H, G, block = 1, 2, 1, 128
+    q, k, v = (_normal(s, torch.float16, i) for i, s in
+               enumerate([(B, M, H, D), (B, N, G, D), (B, N, G, D)]))
+    v = (v.float() * v_size).half()
+    dout = (_normal(q.shape, torch.float32, 9) * size).half()
+    blocks = _lists(B, M, (N + block - 1) // block, 16, 4)
+    ref = Exact(q, k, v, blocks, block, None, None, dout)
+    got = _grads(q, k, v, blocks, dout, block)
+    u = 2.0 ** -11
+    for name, g in zip(("dq", "dk", "dv"), got):
+        want = getattr(ref, name)
+        assert bool(torch.isfinite(g).all()), name
+        off = float((g.double() - want).norm())
+        own = math.sqrt(2 / 3) * u * float(want.norm())
+        low = 2.0 ** -25 * math.sqrt(want.numel() / 3)
+        assert off <= math.hypot(own, low) + 64 * U32 * float(want.norm()), (name, off, own, low)
+
+
+def test_half_precision_gradients_of_unlike_rows():
+    """A query whose incoming gradient is a thousandth of its neighbours', in the
+    same tiles, keeps its dq to the roundings; an infinite one spoils its own."""
+    B, M, N, H, G, D, block = 1, 64, 1024, 2, 1, 64, 128
+    q, k, v = (_normal(s, torch.float16, i) for i, s in
+               enumerate([(B, M, H, D), (B, N, G, D), (B, N, G, D)]))
+    dout = _normal(q.shape, torch.float32, 9)
+    dout[:, ::2] *= 1e-3
+    dout = dout.half()
+    blocks = _lists(B, M, 8, 8, 4)
+    ref = Exact(q, k, v, blocks, block, None, None, dout)
+    u = 2.0 ** -11
+
+    def small(dq, rows):
+        want = ref.dq[:, rows]
+        off = float((dq[:, rows].double() - want).norm())
+        low = 2.0 ** -25 * math.sqrt(want.numel() / 3)
+        bound = math.hypot(math.sqrt(2 / 3) * u * float(want.norm()), low)
+        assert off <= bound + 64 * U32 * float(want.norm()), (off, bound)
+
+    small(_grads(q, k, v, blocks, dout, block)[0], slice(0, None, 2))
+    dout[0, 1, 0, 5] = math.inf
+    dq = _grads(q, k, v, blocks, dout, block)[0]
+    assert not bool(torch.isfinite(dq[0, 1, 0]).all())
+    small(dq, slice(2, None, 2))
