@@ -266,7 +266,11 @@ NSFPS_API int nsfps_group_points_device(const float *d_xyz, const uint64_t *poin
  * comes from the caller (`d_work`, at least the bytes the matching _workspace
  * call gives, 256-byte aligned), so calls on different streams, or captured
  * into different graphs, need only have different scratch.  Results do not
- * depend on how the work is scheduled: the same inputs give the same bits. */
+ * depend on how the work is scheduled: the same inputs give the same bits.
+ * Waits inside the attention kernels are bounded (2 s; no working call comes
+ * near).  A call that does not wait cannot report one that runs out: the out and
+ * lse of its clouds are then NaN, and of a gradient dq and every part of dk and
+ * dv that the CTA in question had in hand. */
 enum nsfps_dtype { NSFPS_F32 = 0, NSFPS_F16 = 1, NSFPS_BF16 = 2 };
 
 /* Lookup of `count` rows per batch entry in a table of `rows` rows of `width`
@@ -415,9 +419,13 @@ NSFPS_API int nsfps_last_profile(nsfps_profile *out);
  *                      (round loops) or its step-`withhold_step` proposals
  *                      (per-step loop); every wait for it then runs out and
  *                      the call returns NSFPS_ERR_TIMEOUT with the device
- *                      still usable.  -1 = none.
+ *                      still usable.  -1 = none.  In the attention kernels on
+ *                      tiles: the CTA of the grid that does not announce a
+ *                      product of its first tile or item; the results are then
+ *                      NaN, as said above.
  *   withhold_step      the round (round loops, from 0) or step (per-step loop,
- *                      from 1) at which it withholds
+ *                      from 1) at which it withholds; attention: 0 the scores,
+ *                      1 (gradient only) the products behind them
  *   fail_alloc_device  the next workspace request of an allocating entry point
  *                      on this device fails as if cudaMalloc had run out of
  *                      memory (NSFPS_ERR_OOM); it fires once.  -1 = none.

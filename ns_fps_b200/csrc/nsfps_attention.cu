@@ -62,6 +62,12 @@ struct AttnArgs {
   const uint4 *tiles;      // by cost: (span, tile within it, first pair, pairs of the span)
   uint32_t tile_stride;    // places per cost class
   const uint32_t *tile_count;
+  // waits: their limit; set when one ran out; a CTA that does not announce a
+  // product (tests), or -1, and which
+  unsigned long long wait_ns;
+  uint32_t *gave_up;
+  int hold_cta;
+  uint32_t hold_step;
   // partials of key heads g0 .. g0 + gc - 1
   uint32_t g0, gc;
   float *part;             // [pair][gc * R][D]
@@ -590,18 +596,22 @@ attend_tiles(const AttnArgs a) {
   after_previous();
   using Shape = TileShape<DP>;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2];
+  __shared__ __align__(8) uint64_t s_bar[3];
   __shared__ uint32_t s_tmem, s_any[4];
+  __shared__ volatile uint32_t s_gave_up;
   __shared__ const char *s_q[kTileRows];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = warp_value(tid >> 5);
   const uint32_t sq = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the swizzle's pattern
   const uint32_t sk = sq + Shape::kQ, sv = sk + 2u * Shape::kChunk;
   const uint32_t bar_s = smem_u32(&s_bar[0]), bar_o = smem_u32(&s_bar[1]);
+  const uint32_t bar_end = smem_u32(&s_bar[2]);
   constexpr uint32_t kChunkBits = 1u << (kSpanLog2 - 6u);
   if (warp == 0) tmem_alloc<Shape::kTmem>(smem_u32(&s_tmem));
   if (tid == 0) {
     bar_init(bar_s);
     bar_init(bar_o);
+    bar_init(bar_end);
+    s_gave_up = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tmem_before_sync();
@@ -614,7 +624,16 @@ attend_tiles(const AttnArgs a) {
   const float c2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   const float sign = a.scale == 0.f ? 0.f : a.scale < 0.f ? -1.f : 1.f;
   uint32_t phase = 0;     // of both barriers: each completes once per chunk
+  // A thread whose wait runs out goes on without waiting, so that the CTA ends;
+  // what it overwrites may be in use, for any row of its tiles.  So the mark is
+  // for the whole turn, and the join gives NaN.
   bool failed = false;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (failed || bar_wait(bar, parity, a.wait_ns)) return;
+    failed = true;
+    *(volatile uint32_t *)a.gave_up = 1u;
+    s_gave_up = 1u;
+  };
   const TileOrder order(a);
   const uint32_t work = order.size() * a.gc;
   // What this thread's row of a tile is: asked for one tile ahead, the tile
@@ -728,7 +747,7 @@ attend_tiles(const AttnArgs a) {
       if (i) {
         // the chunk before is used up: its buffers take the next but one
         buf ^= 1u;
-        if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
+        wait(bar_o, phase ^ 1u);
         __syncwarp();
         tmem_after_sync();
         load_second(now, buf ^ 1u);
@@ -744,10 +763,10 @@ attend_tiles(const AttnArgs a) {
         for (uint32_t kk = 0; kk < DP / 16; ++kk)
           mma_ss(tm_s, further(q_desc, (kk >> 2) * (kTileRows * 128u) + (kk & 3u) * 32u),
                  further(k_desc, (kk >> 2) * (64u * 128u) + (kk & 3u) * 32u), kScores, kk != 0u);
-        mma_commit(bar_s);
+        if (a.hold_cta != (int)blockIdx.x || w != blockIdx.x || i) mma_commit(bar_s);
       }
       __syncwarp();
-      if (!failed) failed = !bar_wait(bar_s, phase);
+      wait(bar_s, phase);
       __syncwarp();
       tmem_after_sync();
       uint32_t s[2][32];
@@ -843,7 +862,7 @@ attend_tiles(const AttnArgs a) {
       // so is the other buffer
       if (last) load_first(coming, buf ^ 1u);
     }
-    if (!failed) failed = !bar_wait(bar_o, phase ^ 1u);
+    wait(bar_o, phase ^ 1u);
     __syncwarp();
     tmem_after_sync();
     if (another) load_second(coming, buf);
@@ -862,15 +881,20 @@ attend_tiles(const AttnArgs a) {
           if (j * 32u + y < a.D) store8(a.part + row * a.D + j * 32u + y, &o[y], inv);
       __syncwarp();
     }
-    if (live_row)  // (a wait that ran out shows as NaN)
-      a.part_lse[row] = failed ? __int_as_float(0x7fc00000)
-                        : sum > 0.f ? fmaf(ref, c2, log2f(sum)) : -INFINITY;
+    if (live_row) a.part_lse[row] = sum > 0.f ? fmaf(ref, c2, log2f(sum)) : -INFINITY;
     now = coming;  // (the output is read before the barriers of the next chunk)
   }
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
-  if (warp == 0) tmem_free<Shape::kTmem>(tm);
+  if (warp == 0) {
+    if (s_gave_up) {  // nothing may write tensor memory that is given back
+      mma_commit(bar_end);
+      bar_wait(bar_end, 0u, a.wait_ns);
+      __syncwarp();
+    }
+    tmem_free<Shape::kTmem>(tm);
+  }
 }
 
 // Four consecutive elements of the output, rounded, and what the rounding left.
@@ -884,6 +908,10 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, uint64_t at, float4
       make_uint2(pack2<T>(x.x - to_f32(e[0]), x.y - to_f32(e[1])),
                  pack2<T>(x.z - to_f32(e[2]), x.w - to_f32(e[3])));
 }
+
+// In the joins.  (Asked for at their beginning, and as a volatile, it took 1 us
+// of each.)
+__device__ __forceinline__ bool some_gave_up(const AttnArgs &a) { return __ldg(a.gave_up) != 0u; }
 
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
 // its leading slots.  A warp takes 128 consecutive elements of a query's heads,
@@ -935,12 +963,13 @@ attend_join(const AttnArgs a, uint32_t parts) {
       acc.x += y * x[u].x; acc.y += y * x[u].y; acc.z += y * x[u].z; acc.w += y * x[u].w;
     }
   }
-  const float inv = total > 0.f ? 1.f / total : 0.f;
+  const bool gave_up = some_gave_up(a);
+  const float inv = gave_up ? NAN : total > 0.f ? 1.f / total : 0.f;
   const uint64_t out = ((uint64_t)bm * a.H + a.g0 * a.R) * a.D + d;
   store_out<T>(a, out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   if (a.lse && d == hh * a.D)
     a.lse[(uint64_t)bm * a.H + a.g0 * a.R + hh] =
-        total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
+        gave_up ? NAN : total > 0.f ? (mx + log2f(total)) * kLn2 : -INFINITY;
 }
 
 // The same for the direct path, one CTA per row: groups of LANES lanes take
@@ -1294,8 +1323,9 @@ attend_grad(const AttnArgs a) {
   using Shape = GradShape<DP>;
   constexpr uint32_t kRows = Shape::kRows, kStages = Shape::kStages, kChunks = DP / 8;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[kStages * 2 + 4 + 6];
+  __shared__ __align__(8) uint64_t s_bar[kStages * 2 + 4 + 7];
   __shared__ uint32_t s_tmem;
+  __shared__ volatile uint32_t s_gave_up;
   // |v|^2 at most, per warp that loads them, of items k & 3 (a warp that is a
   // step behind another may still read those of the item before)
   __shared__ float s_v2[4][kResultWarps];
@@ -1313,6 +1343,7 @@ attend_grad(const AttnArgs a) {
   const uint32_t s_ready = bars + kRest, s_free = s_ready + 8u;   // scores made, taken out
   const uint32_t p_ready = s_free + 8u, g_done = p_ready + 8u;    // weights there; products done
   const uint32_t dq_free = g_done + 8u, acc_free = dq_free + 8u;  // dq, dk and dv taken out
+  const uint32_t bar_end = acc_free + 8u;
   if (warp == 0) tmem_alloc<512>(smem_u32(&s_tmem));
   if (tid == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
@@ -1329,6 +1360,8 @@ attend_grad(const AttnArgs a) {
     bar_init(g_done);
     bar_init(dq_free, kResultWarps);
     bar_init(acc_free, kResultWarps);
+    bar_init(bar_end);
+    s_gave_up = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tmem_before_sync();
@@ -1373,9 +1406,16 @@ attend_grad(const AttnArgs a) {
     x.steps = steps_of(y.tile);
     return x;
   };
-  bool failed = false;  // a wait of this thread ran out: go on without waiting
+  // A thread whose wait runs out goes on without waiting, so that the CTA ends.
+  // It says so before it touches what may be in use: dk and dv that this CTA
+  // writes from then on are NaN, and by the joins all of the turn that shares
+  // make, dq among it.
+  bool failed = false;
   auto wait = [&](uint32_t bar, uint32_t phase) {
-    if (!failed) failed = !bar_wait(bar, phase);
+    if (failed || bar_wait(bar, phase, a.wait_ns)) return;
+    failed = true;
+    *(volatile uint32_t *)a.gave_up = 1u;
+    s_gave_up = 1u;
   };
   // The exponent of an item's factor of ds; `most` is asked for before the keys
   // are waited for.
@@ -1574,7 +1614,7 @@ attend_grad(const AttnArgs a) {
         wait(g_done, n & 1u);
         __syncwarp();
         tmem_after_sync();
-        const float f = failed ? NAN : down_ds;
+        const float f = down_ds;
         // (places first: behind the second half the stage is given back)
         const uint32_t mine = DP == 64 ? place[at_lane] : 0u;
 #pragma unroll
@@ -1609,7 +1649,6 @@ attend_grad(const AttnArgs a) {
       // the span's dk and dv, or this item's share of them: a lane has a key
       const bool whole = it.all_rows <= kGradItem, some = key < a.N;
       if (it.steps) {
-        const float f = failed ? NAN : 1.f;
         const uint64_t place = whole ? 0u : a.span[it.span].z + it.index;
         float *share = a.part_kv + ((place * a.gc + it.gi) * 256u + at_lane) * a.D;
 #pragma unroll
@@ -1624,7 +1663,8 @@ attend_grad(const AttnArgs a) {
             __syncwarp();
             if (lane == 0) bar_arrive(acc_free);
           }
-          const float g = !is_k ? f * kDownP : whole ? f * down_ds * a.scale : f * down_ds;
+          const float f = !is_k ? kDownP : whole ? down_ds * a.scale : down_ds;
+          const float g = s_gave_up ? NAN : f;  // (looked at behind the values)
           if (some) {
 #pragma unroll
             for (uint32_t y = 0; y < 32u; y += 8u) {
@@ -1674,6 +1714,7 @@ attend_grad(const AttnArgs a) {
         advance(x.y);
         settle(x);
       };
+      const bool hold = a.hold_cta == (int)blockIdx.x;
       // (the distance of further columns means nothing where there are none)
       const uint64_t ds_desc = tile_desc(base + Shape::kDsAt, 16384u);
       auto keys_at = [&](uint32_t k) { return base + (k % Shape::kKv) * 2u * Shape::kKeyTile; };
@@ -1695,7 +1736,7 @@ attend_grad(const AttnArgs a) {
                  further(k_desc, Shape::kKeyTile + (kk >> 2) * 16384u + (kk & 3u) * 32u),
                  further(q_desc, Shape::kRowTile + (kk >> 2) * (kRows * 128u) + (kk & 3u) * 32u),
                  kScores, kk != 0u);
-        mma_commit(s_ready);
+        if (!(hold && x.n == 0u && a.hold_step == 0u)) mma_commit(s_ready);
         next(x);
       };
       auto grads = [&](Walk &x) {
@@ -1720,7 +1761,7 @@ attend_grad(const AttnArgs a) {
           const uint64_t ds = further(ds_desc, kk * 2048u), ky = further(k_desc, kk * 2048u);
           mma_ss(tm + Shape::kDq, DP == 64 ? ds : ky, DP == 64 ? ky : ds, kDqBy, kk != 0u);
         }
-        mma_commit(g_done);
+        if (!(hold && x.n == 0u && a.hold_step == 1u)) mma_commit(g_done);
         mma_commit(empty(x.n % kStages));
         if (x.i + 1u == x.steps) mma_commit(kv_empty(x.k));
         next(x);
@@ -1809,6 +1850,13 @@ attend_grad(const AttnArgs a) {
   tmem_before_sync();
   __syncthreads();
   tmem_after_sync();
+  if (s_gave_up) {  // nothing may write tensor memory that is given back
+    if (warp == kWeightWarps + kResultWarps) {
+      mma_commit(bar_end);
+      bar_wait(bar_end, 0u, a.wait_ns);
+    }
+    __syncthreads();
+  }
   if (warp == 0) tmem_free<512>(tm);
 }
 
@@ -1833,6 +1881,7 @@ grad_join_keys(const AttnArgs a, uint32_t span) {
       k.x += y.x; k.y += y.y; v.x += z.x; v.y += z.y;
     }
     const uint64_t o = 2 * ((((uint64_t)b * a.N + key0 + r) * a.G + g) * a.D + d);
+    if (some_gave_up(a)) k.x = k.y = v.x = v.y = NAN;
     *reinterpret_cast<uint32_t *>(a.dk + o) = pack2<T>(k.x * a.scale, k.y * a.scale);
     *reinterpret_cast<uint32_t *>(a.dv + o) = pack2<T>(v.x, v.y);
   }
@@ -1867,9 +1916,9 @@ grad_join_queries(const AttnArgs a, uint32_t parts) {
     }
   }
   const uint64_t out = ((uint64_t)bm * a.H + a.g0 * a.R) * a.D + d;
+  const float f = some_gave_up(a) ? NAN : a.scale;
   *reinterpret_cast<uint2 *>(a.dq + out * 2) =
-      make_uint2(pack2<T>(acc.x * a.scale, acc.y * a.scale),
-                 pack2<T>(acc.z * a.scale, acc.w * a.scale));
+      make_uint2(pack2<T>(acc.x * f, acc.y * f), pack2<T>(acc.z * f, acc.w * f));
 }
 
 // ------------------------------------------------------------- host side
@@ -1989,7 +2038,7 @@ AttnPlan plan_attention(const nsfps_attention_desc &d, bool backward, void *base
   w.mask = c.take<uint32_t>(w.pairs);
   w.lead = c.take<unsigned long long>(w.bc * d.queries);
   w.span = c.take<uint4>(w.spans);
-  static_assert(4 * (kTileClasses + 1) <= 32, "the marks begin 32 bytes behind");
+  static_assert(4 * (kTileClasses + 2) <= 32, "the marks begin 32 bytes behind");
   // (cleared together, before a turn)
   w.most_bytes = backward && d.dtype == NSFPS_F16 ? ceil_div(w.bc * (uint64_t)d.kv_heads, 2) * 16 : 0;
   w.tile_count = (uint32_t *)c.take<char>(32 + w.most_bytes + 16 * w.spans);
@@ -2021,6 +2070,11 @@ AttnArgs common_args(const nsfps_attention_desc &d, const void *q, const void *k
   a.nsb = w.direct ? 0 : (uint32_t)ceil_div(d.keys, 1ull << w.span_log2);
   a.most = w.most;
   a.mask = w.mask; a.lead = w.lead; a.span = w.span; a.tile_count = w.tile_count;
+  a.gave_up = w.tile_count + kTileClasses + 1;
+  const WaitHooks hooks = wait_hooks();
+  a.wait_ns = (unsigned long long)hooks.limit_ns;
+  a.hold_cta = hooks.hold_cta;
+  a.hold_step = hooks.hold_step;
   a.listed = (const uint4 *)w.listed;
   a.tile_stride = (uint32_t)w.max_tiles;
   a.tiles = w.tiles; a.part = w.part; a.part_lse = w.part_lse; a.delta = w.delta;
@@ -2055,7 +2109,7 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   const uint32_t shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
   SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
-  // (the tile counters, the rows' maxima and the spans' marks, cleared together)
+  // (the tile counters and gave_up, the rows' maxima and the spans' marks, cleared together)
   if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + w.most_bytes + 16 * (uint64_t)spans, st)))
     return err;
   if (n && spans) {

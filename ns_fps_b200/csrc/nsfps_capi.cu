@@ -58,6 +58,8 @@ int set_error(int code, const char *fmt, ...) {
 
 void clear_error() { g_err.clear(); }
 
+WaitHooks wait_hooks() { return {g_wait_ns.load(), g_hold_cta.load(), g_hold_step.load()}; }
+
 #define NSFPS_CUDA(call)                                                      \
   do {                                                                        \
     cudaError_t e_ = (call);                                                  \
@@ -897,9 +899,10 @@ int run_job(DeviceCtx *ctx, cudaStream_t st, const Job &j, const float *h_xyz_pa
   la.groups = grid ? groups : 0;
   la.glist = b.glist;
   la.gbar = b.gbar;
-  la.timeout_ns = g_wait_ns.load();
-  la.hold_cta = g_hold_cta.load();
-  la.hold_step = g_hold_step.load();
+  const WaitHooks hooks = wait_hooks();
+  la.timeout_ns = hooks.limit_ns;
+  la.hold_cta = hooks.hold_cta;
+  la.hold_step = hooks.hold_step;
   if (prof) NSFPS_CUDA(cudaEventRecord(ctx->ev[2], st));
   NSFPS_CUDA(plan.rounds ? run_rounds(la, plan, st, launches) : run_loop(la, plan, st, launches));
   if (prof) NSFPS_CUDA(cudaEventRecord(ctx->ev[3], st));

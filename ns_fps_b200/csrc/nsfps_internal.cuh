@@ -153,4 +153,13 @@ int range_info(const nsfps_range &r, nsfps_range_info *info);
 int set_error(int code, const char *fmt, ...);
 void clear_error();
 
+// What nsfps_set_test_hooks set: the limit of in-kernel waits, and the CTA (or
+// -1) that withholds something its waits are for, and when.
+struct WaitHooks {
+  long long limit_ns;
+  int hold_cta;
+  uint32_t hold_step;
+};
+WaitHooks wait_hooks();
+
 }  // namespace nsfps

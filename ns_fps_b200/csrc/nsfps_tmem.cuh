@@ -160,8 +160,8 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count = 1u) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Waits for the phase of parity `phase`; false when it has not come after two
-// seconds (a product that never ends), which no working call sees.
+// Waits for the phase of parity `phase`; false when it has not come after
+// limit_ns (a product that never ends), which no working call sees.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t phase) {
   uint32_t done;
   asm volatile(
@@ -172,14 +172,15 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t phase) {
       : "memory");
   return done;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t phase) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t phase,
+                                         unsigned long long limit_ns) {
   if (bar_try(bar, phase)) return true;
   unsigned long long begin, now;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin));
   do {
     if (bar_try(bar, phase)) return true;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-  } while (now - begin < 2000000000ull);
+  } while (now - begin < limit_ns);
   return false;
 }
 
