@@ -335,7 +335,8 @@ NSFPS_API int nsfps_select_blocks_device(const nsfps_select_desc *desc, const fl
  * cloud's length, in blocks that no query of the cloud lists, or in rows of
  * queries that list nothing, is never part of a result, whatever its value;
  * what is listed has to be finite (a value that is not may also reach results
- * of queries and keys nearby that do not list it).
+ * of queries and keys nearby that do not list it), and so have its products:
+ * q . k, and that times scale * log2(e), in fp32.
  * q, k and v: F16 or BF16, elements of a head contiguous, 16-byte aligned, the
  * strides (batch, row, head, in elements) multiples of 8.  blocks (batch x
  * queries x top int64), out (batch x queries x heads x head_dim) and lse

@@ -294,7 +294,8 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
              negative, repeated, or name no block count for nothing
     lengths  None, or int32 (B,): the keys of each padded cloud; what lies
              behind them, or in blocks that no query lists, is never part of a
-             result.  Values that are listed have to be finite.
+             result.  Values that are listed have to be finite, and so have
+             their scores in float32.
     scale    a number, by default 1 / sqrt(D) (what a tensor holds is read, and
              has no gradient)
 

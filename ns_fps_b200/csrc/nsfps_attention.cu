@@ -1936,7 +1936,8 @@ int check_attention(const nsfps_attention_desc *d) {
     return set_error(NSFPS_ERR_ARG, "block must be 16, 32, 64 or 128");
   if (d->top == 0 || d->top > NSFPS_MAX_TOP)
     return set_error(NSFPS_ERR_ARG, "top must be in 1..%u", NSFPS_MAX_TOP);
-  if (!std::isfinite(d->scale)) return set_error(NSFPS_ERR_ARG, "scale must be finite");
+  if (!std::isfinite(d->scale * kLog2e))
+    return set_error(NSFPS_ERR_ARG, "scale must be finite, times log2(e) too");
   const uint64_t lim = 1ull << 30;
   if (d->batch >= lim / 8 || d->queries >= lim || d->keys >= lim || d->batch * d->keys >= lim ||
       d->batch * d->queries >= lim || d->batch * d->queries * d->top >= lim ||

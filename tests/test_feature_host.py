@@ -184,3 +184,12 @@ def test_python_entries_refuse_a_scale_that_wants_a_gradient():
         group.gather_rows(x[:, 0], idx, scale)
     with torch.no_grad(), pytest.raises(TypeError, match="CUDA"):  # a number then
         attention.block_attention(x, x, x, idx, 16, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_attention_refuses_a_scale_beyond_base_two(scale):
+    """Scores are taken in base 2: scale * log2(e) has to be finite, too."""
+    for backward in (False, True):
+        with pytest.raises(RuntimeError, match=f"rc={capi.ERR_ARG}.*scale"):
+            capi.block_attention_workspace(_attention(scale=scale), backward)
+        capi.block_attention_workspace(_attention(scale=scale / 2), backward)
