@@ -355,7 +355,13 @@ typedef struct nsfps_attention_desc {
   uint32_t reserved; /* 0 */
 } nsfps_attention_desc;
 
-/* Scratch of the forward (backward == 0) or the gradient call. */
+/* Scratch of the forward (backward == 0) or the gradient call.  Most of it are
+ * partial results: for each cloud and key head
+ *   queries * top * heads / kv_heads * 4 * (head_dim + 1) bytes
+ * (the gradient half as much again, and keys * 8 * head_dim).  Key heads and
+ * clouds are taken in turns while these pass 1 GiB; the queries of one cloud are
+ * not, so one cloud and key head may take more than that: split such a call by
+ * queries where it does not fit (the gradient's dk and dv of the parts add up). */
 NSFPS_API int nsfps_block_attention_workspace(const nsfps_attention_desc *desc, int backward,
                                               uint64_t *bytes);
 NSFPS_API int nsfps_block_attention_device(const nsfps_attention_desc *desc, const void *d_q,

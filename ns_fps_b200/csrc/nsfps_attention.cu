@@ -1959,8 +1959,12 @@ int padded_dim(uint32_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // Keys per span of the gradient.
 constexpr uint32_t kGradSpanLog2 = 7;  // one key per lane of tensor memory
 
-// Partials of a pass stay below this, by taking the key heads, then the clouds
-// of a call, in turns.  Turns small enough to keep their partials in L2 cost
+// Partials of a pass stay below this where taking the key heads, then the clouds
+// of a call, in turns brings them there.  A turn has at least one cloud and one
+// key head, with all their queries: dk and dv of a key add up over those, and the
+// gradient has no place to keep such sums between turns.  So one cloud of 65,536
+// queries, lists of 16 and eight query heads of 128 on one key head takes 4.3 GB,
+// every slot counted, as the plan cannot know how many lead a pair.  Turns small enough to keep their partials in L2 cost
 // more in launches and half-empty waves than they save: a scan's attention
 // took 199 us in one turn, 207 in two, 267 in four.
 constexpr uint64_t kMaxPartBytes = 1ull << 30;

@@ -585,3 +585,42 @@ def test_half_precision_gradients_of_unlike_rows():
     dq = _grads(q, k, v, blocks, dout, block)[0]
     assert not bool(torch.isfinite(dq[0, 1, 0]).all())
     small(dq, slice(2, None, 2))
+
+
+def test_one_cloud_beyond_the_limit_of_a_turn():
+    """One cloud and key head whose partial results pass 1 GiB stay together;
+    parts of the queries give the same within the roundings, and their dk and
+    dv add up."""
+    from ns_fps_b200 import attention, capi
+    import ctypes
+    M, N, H, D, top, block, dtype = 66_000, 400, 2, 128, 16, 16, torch.bfloat16
+    three = ctypes.c_int64 * 3
+    desc = capi.AttentionDesc(1, M, N, H, 1, D, block, top, capi.BF16, three(0, H * D, D),
+                              three(0, D, 0), three(0, D, 0), 0.1, 0)
+    assert 1 << 30 < M * top * H * 4 * (D + 1) <= capi.block_attention_workspace(desc, False)
+    q, dout = _normal((1, M, H, D), dtype, 1), _normal((1, M, H, D), dtype, 2)
+    k, v = _normal((1, N, 1, D), dtype, 3), _normal((1, N, 1, D), dtype, 4)
+    blocks = _lists(1, M, N // block, top, 5)
+
+    def step(part):
+        leaves = [t.detach().requires_grad_() for t in (q[:, part], k, v)]
+        out = attention.block_attention(*leaves, blocks[:, part], block)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout[:, part]))
+
+    out, dq, dk, dv = step(slice(None))
+    sums = [torch.zeros_like(t, dtype=torch.float64) for t in (dk, dv)]
+    offs = [torch.zeros_like(t) for t in sums]
+    for at in range(0, M, 11_000):
+        part = slice(at, at + 11_000)
+        ref = Exact(q[:, part], k, v, blocks[:, part], block, None, None, dout[:, part])
+        assert bool(((out[:, part].double() - ref.out).abs() <= ref.out_off).all())
+        assert bool(((dq[:, part].double() - ref.dq).abs() <= ref.dq_off).all())
+        for i, name in enumerate(("dk", "dv")):
+            sums[i] += getattr(ref, name)
+            offs[i] += getattr(ref, name + "_off")
+        del ref
+    # (the parts' bounds count a rounding of the result each, and fp32 sums over
+    # the part's rows: six times as many here)
+    for got, want, off in zip((dk, dv), sums, offs):
+        u = torch.finfo(dtype).eps / 2
+        assert bool(((got.double() - want).abs() <= 6 * off + u * want.abs()).all())
