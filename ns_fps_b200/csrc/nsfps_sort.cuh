@@ -10,7 +10,10 @@
 // Where a list has ten million entries this moves 20 bytes per entry and
 // digit; at the usual hundred thousand it is bound by its launches.  So the
 // offsets of few tiles are summed where they are used (two launches per
-// digit), and a list that fits one CTA takes one launch in all.
+// digit), and a list that fits one CTA takes one launch in all.  (The sampler's
+// setup has a sort of its own, by an array of keys that it keeps whole; here keys
+// come from what a caller has, entries are dropped on the way, and the short
+// lists of a call count.)
 #pragma once
 
 #include "nsfps_feature.cuh"
@@ -26,22 +29,25 @@ constexpr uint32_t kSortThreads = 256, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kSortSmall = 4096, kSmallItems = kSortSmall / 1024;
 constexpr uint32_t kSmallSmem = kSortSmall * 8u + 32u * 256u * 2u;
 
-// Tiles whose counts each CTA of the scatter sums itself.
+// Tiles whose counts each CTA of the scatter sums itself.  On the GPU alone that
+// is ahead up to some 24 tiles (two digits of 24,576 keys 14.5 us and 16.3 with
+// an offsets launch, of 65,536 keys 29.9 and 17.2); in a program that waits for
+// its launches it saves one per digit (a training lookup of 30,011 ids 100 us and
+// 104 to 107).
 constexpr uint32_t kSumTiles = 64;
 
-// Keys per tile: few enough that small lists still spread over the SMs.
-constexpr uint32_t kShortTiles = 1u << 19;  // the longest list in short tiles
-inline uint32_t sort_tile(uint32_t n) { return kSortThreads * (n <= kShortTiles ? 4u : 16u); }
+// Keys per tile.  Tiles of 4,096 are no faster for any list: two digits of 2^17
+// keys take 17 us in tiles of 1,024 and 34 in those, 2^20 43 and 43, 2^24 470
+// and 548.
+constexpr int kSortItems = 4;
+constexpr uint32_t kSortTile = kSortThreads * kSortItems;
 
-// Scratch for any list of up to n keys.  A list just short enough for short
-// tiles has more of them than one somewhat longer, so what the longest list
-// has is not enough: a call taken in turns ends with a shorter one.
+// Scratch for any list of up to n keys.
 struct SortScratch {
   uint32_t *keys0, *vals0, *keys1, *vals1, *hist, *total, *kept;
   uint32_t tiles;  // for which hist has room
   void carve(WorkCarver &w, uint32_t n) {
-    const uint32_t few = std::min(n, kShortTiles);
-    tiles = (uint32_t)std::max(ceil_div(n, sort_tile(n)), ceil_div(few, sort_tile(few)));
+    tiles = (uint32_t)ceil_div(n, kSortTile);
     keys0 = w.take<uint32_t>(n);
     vals0 = w.take<uint32_t>(n);
     keys1 = w.take<uint32_t>(n);
@@ -66,7 +72,7 @@ struct StoredKeys {
   __device__ __forceinline__ uint32_t value(uint32_t i) const { return vals[i]; }
 };
 
-template <int ITEMS, class Source>
+template <class Source>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t digit_mask,
            uint32_t *__restrict__ hist, uint32_t tiles) {
@@ -74,15 +80,15 @@ sort_count(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t
   __shared__ uint32_t s_hist[256];
   s_hist[threadIdx.x] = 0;
   __syncthreads();
-  const uint32_t m = src.count(n), first = blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
-  uint32_t key[ITEMS];
+  const uint32_t m = src.count(n), first = blockIdx.x * kSortTile + threadIdx.x;
+  uint32_t key[kSortItems];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
+  for (int i = 0; i < kSortItems; ++i) {
     const uint32_t at = first + i * kSortThreads;
     key[i] = at < m ? src.key(at) : none;
   }
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
+  for (int i = 0; i < kSortItems; ++i)
     if (key[i] != none) atomicAdd(&s_hist[(key[i] >> shift) & digit_mask], 1u);
   __syncthreads();
   if (threadIdx.x <= digit_mask) hist[(size_t)threadIdx.x * tiles + blockIdx.x] = s_hist[threadIdx.x];
@@ -129,7 +135,7 @@ sort_offsets(uint32_t *__restrict__ hist, uint32_t tiles, uint32_t *__restrict__
   if (threadIdx.x == 0) total[blockIdx.x] = base;
 }
 
-template <int ITEMS, class Source>
+template <class Source>
 __global__ void __launch_bounds__(kSortThreads)
 sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32_t digit_mask,
              const uint32_t *hist, uint32_t tiles,
@@ -139,16 +145,16 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   after_previous();
   __shared__ uint32_t s_count[kSortWarps][256];
   __shared__ uint32_t s_base[256], s_global[256], s_warp[kSortWarps];
-  __shared__ uint32_t s_key[kSortThreads * ITEMS], s_val[kSortThreads * ITEMS];
+  __shared__ uint32_t s_key[kSortTile], s_val[kSortTile];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
 #pragma unroll
   for (uint32_t w = 0; w < kSortWarps; ++w) s_count[w][tid] = 0;
   const uint32_t m = src.count(n);
   // a warp's keys are consecutive, lanes first: the order the ranks keep
-  const uint32_t first = blockIdx.x * (kSortThreads * ITEMS) + warp * (32u * ITEMS) + lane;
-  uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
+  const uint32_t first = blockIdx.x * kSortTile + warp * (32u * kSortItems) + lane;
+  uint32_t key[kSortItems], val[kSortItems], rank[kSortItems];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
+  for (int i = 0; i < kSortItems; ++i) {
     const uint32_t at = first + i * 32u;
     key[i] = at < m ? src.key(at) : none;
     val[i] = at < m ? src.value(at) : 0u;
@@ -156,7 +162,7 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   __syncthreads();
   uint32_t *cnt = s_count[warp];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
+  for (int i = 0; i < kSortItems; ++i) {
     const bool some = key[i] != none;
     const uint32_t d = some ? (key[i] >> shift) & digit_mask : 256u;
     const uint32_t peers = __match_any_sync(0xffffffffu, d);
@@ -199,7 +205,7 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   if (blockIdx.x == 0 && tid == 0 && Source::kFirst) *kept = all;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
+  for (int i = 0; i < kSortItems; ++i) {
     if (key[i] == none) continue;
     const uint32_t d = (key[i] >> shift) & digit_mask;
     const uint32_t at = s_base[d] + cnt[d] + rank[i];
@@ -208,7 +214,7 @@ sort_scatter(const Source src, uint32_t n, uint32_t none, uint32_t shift, uint32
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
+  for (int i = 0; i < kSortItems; ++i) {
     const uint32_t at = tid + i * kSortThreads;
     if (at >= in_tile) continue;
     const uint32_t k = s_key[at], d = (k >> shift) & digit_mask;
@@ -319,7 +325,7 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
   uint32_t bits = 1;
   while (bits < 32 && ((none - 1u) >> bits)) ++bits;
   const uint32_t passes = (bits + 7u) / 8u, digit = (bits + passes - 1u) / passes;
-  const uint32_t tile = sort_tile(n), tiles = (uint32_t)ceil_div(n, tile);
+  const uint32_t tiles = (uint32_t)ceil_div(n, kSortTile);
   const uint32_t dm = (1u << digit) - 1u;
   if (n <= kSortSmall) {
     const cudaError_t err = opt_in<sort_small<Source>>(kSmallSmem);
@@ -344,14 +350,8 @@ cudaError_t run_sort(const Source &src, uint32_t n, uint32_t none, const SortScr
                           tiles, few ? (uint32_t *)nullptr : w.total, keys_next, vals_next, w.kept);
       return err;
     };
-    const bool short_tiles = tile == 4u * kSortThreads;
-    cudaError_t err;
-    if (p == 0)
-      err = short_tiles ? pass(sort_count<4, Source>, sort_scatter<4, Source>, src)
-                        : pass(sort_count<16, Source>, sort_scatter<16, Source>, src);
-    else
-      err = short_tiles ? pass(sort_count<4, StoredKeys>, sort_scatter<4, StoredKeys>, stored)
-                        : pass(sort_count<16, StoredKeys>, sort_scatter<16, StoredKeys>, stored);
+    const cudaError_t err = p == 0 ? pass(sort_count<Source>, sort_scatter<Source>, src)
+                                   : pass(sort_count<StoredKeys>, sort_scatter<StoredKeys>, stored);
     if (err) return err;
     std::swap(keys, keys_next);
     std::swap(vals, vals_next);

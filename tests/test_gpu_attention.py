@@ -455,11 +455,11 @@ def test_gradients_of_few_keys_of_many_queries(N):
 
 
 @pytest.mark.parametrize("M", [16_384, 14_000])
-def test_a_last_turn_of_shorter_sort_tiles(M):
+def test_a_last_turn_of_fewer_clouds(M):
     """Three clouds whose partial results make turns of two and one: the
-    forward's (M = 16,384) or the gradient's (14,000).  A full turn's 786,432 or
-    672,000 pairs are sorted in tiles of 4,096 keys, the last one's half in more
-    tiles of 1,024.  The last cloud by itself gives the same bits."""
+    forward's (M = 16,384) or the gradient's (14,000).  The last turn sorts half
+    the pairs of a full one (786,432 or 672,000) in its scratch.  Each cloud by
+    itself gives the same bits."""
     from ns_fps_b200 import attention
     B, N, H, G, D, top, block, dtype = 3, 600, 4, 2, 128, 24, 16, torch.bfloat16
     q, dout = _normal((B, M, H, D), dtype, 1), _normal((B, M, H, D), dtype, 2)

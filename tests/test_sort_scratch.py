@@ -10,8 +10,7 @@ from ns_fps_b200 import build
 from tests.test_feature_host import _attention, _rows
 from tests import capi
 
-# pairs of a full turn and of the last one: both sides of the border at 2^19
-# keys, where the sort goes from tiles of 1,024 keys to 4,096
+# pairs of a full turn and of the last one
 TURNS = [(786_432, 393_216), ((1 << 19) + 1, 1 << 19), (1 << 21, 1 << 19), (1 << 24, 1 << 19),
          (1 << 24, 300_000), (1 << 19, 5000), (4097, 4096), (5000, 1), (1, 1)]
 
@@ -27,7 +26,7 @@ int main(int argc, char **argv) {
     WorkCarver c((void *)(1ull << 20));
     s.carve(c, n);
     const unsigned long long have = s.total - s.hist;
-    const unsigned long long want = 256ull * ceil_div(tail, sort_tile(tail));
+    const unsigned long long want = 256ull * ceil_div(tail, kSortTile);
     printf("%llu %llu\n", have, want);
   }
 }
