@@ -16,8 +16,8 @@
 // operations against 8 * D bytes of partials (written and read), so the
 // partials, the softmax and the way to the tiles, not the matrix unit, set the
 // pace (its share of the time is 13 % forward, 15 % in the gradient).  Of a
-// scan's 172 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
-// tiles take 109, the join 36 (132 MB of partials, 3.7 TB/s), the plan 33; the
+// scan's 170 us (16,384 queries, 4 heads of 64, 512 of 122,880 keys each) the
+// tiles take 107, the join 36 (132 MB of partials, 3.7 TB/s), the plan 33; the
 // floor is 22 by bytes.  Spans of 128 keys make more pairs (186 us); spans of 512
 // make that call 3 % faster, not enough for the second plan that the smaller
 // calls would then want.
@@ -522,7 +522,10 @@ struct RowsState {
 // back as 16-bit values over the scores, and o += p v takes them from there.
 // Nothing but the operands' tiles passes through shared memory.  Four CTAs an
 // SM (two with heads of 128): while one waits for its products or its loads,
-// the others compute.  A scan's 5,104 tiles take 109 us, 4,200 cycles each and
+// the others compute.  Smaller heads go through tiles of 64 elements, zeros
+// behind their own (the scan's tiles take 92 us with heads of 16, 94 with 32, 99
+// with 48, 105 with 64; 190 with 96, 228 with 128): the softmax does not depend
+// on them.  A scan's 5,104 tiles take 107 us, 4,200 cycles each and
 // SM, of which the instructions of the softmax and the loads are 45 %; with
 // mma.sync and scores in registers it was 182.
 constexpr uint32_t kTileThreads = 128;
@@ -1312,10 +1315,13 @@ struct GradItem {
 // sixteen make weights, three load a step's rows each (the loads of three steps
 // are in the air), four take dq, dk and dv out, and one issues the products,
 // the next step's scores before this step's gradients.  Four clouds (16,384
-// queries, 4 heads of 64) took 210 us without roles and take 130 (the matrix
+// queries, 4 heads of 64) took 210 us without roles and take 131 (the matrix
 // unit 15 % busy, memory 19 %: what is left is the way of a step from barrier to
 // barrier, with the gather of 128 rows of q and dout in it), shared heads
-// (2,046 queries, 8 heads of 128 over 2) 62 and 37.
+// (2,046 queries, 8 heads of 128 over 2) 62 and 38.  At 24 warps a thread has 80
+// registers; heads of 128 and half precision spill 8 to 20 bytes of them.  A call
+// of few queries pays for its whole cloud here: one query of 122,880 keys and 8
+// heads 162 us, most of it zeros written to dk and dv (252 MB).
 template <class T, int DP>
 __global__ void __launch_bounds__(kGradThreads, 1)
 attend_grad(const AttnArgs a) {

@@ -7,12 +7,13 @@
 // at the groups first: rounding is monotone, so a group's distance is never
 // above a block's of it, exactly.  The nearest groups give a bound on the
 // `top`-th distance; the blocks of all groups within it are looked at in index
-// order, and those within it are listed.  Then the minimum is taken out of the
-// list `top` times.  Distances are never negative or NaN, so their bits order
-// as integers, and a list in index order gives the lower index among equals
-// first.  What bounds it is instructions: 131,072 centres over 512 blocks and
-// top 16 take 160 us (a list kept sorted by insertion over all blocks 469, by
-// groups 260), 16,384 centres over 1,920 blocks 54 (203, 76).
+// order, and those within it are listed and ranked by comparison.  Distances
+// are never negative or NaN, so their bits order as integers, and a list in
+// index order gives the lower index among equals first.  What bounds it is
+// instructions (73 % of the issue slots) and the wait for boxes out of
+// the L1: 131,072 centres over 512 blocks of padded clouds and top 16 take 158 us
+// (a list kept sorted by insertion over all blocks 469, by groups 260), 16,384
+// centres over 1,920 blocks 54 (203, 76).
 #include <algorithm>
 
 #include "nsfps_feature.cuh"
@@ -139,10 +140,11 @@ struct Candidates {
 };
 
 // Clouds of at most this many blocks: every distance is computed once and held
-// in registers, without groups.  For 512 blocks and top 16, where most of the
-// 16 groups are within the bound, 32 clouds took 233 us so and 267 by groups;
-// for 1,920 blocks the distances alone would be more than the groups' whole
-// work.
+// in registers, without groups.  32 clouds of 4,096 centres and top 16 take, so
+// and by groups, 108 and 169 us with 128 blocks, 132 and 185 with 256, 182 and
+// 207 with 512; eight clouds of 2,048 and top 48 with 512 53 and 87, one centre
+// 10 and 6.  Twice the registers, for 1,024 blocks, cost occupancy: 252 us with
+// 512, 292 with 700 and 357 with 1,024, by groups 238 and 259.
 constexpr int kHeldRegs = 16;
 constexpr uint32_t kHeldBlocks = 32 * kHeldRegs;
 
