@@ -296,8 +296,8 @@ def block_attention(q, k, v, blocks, block: int, lengths=None, scale: float | No
              behind them, or in blocks that no query lists, is never part of a
              result.  Values that are listed have to be finite, and so have
              their scores in float32.
-    scale    a number, by default 1 / sqrt(D) (what a tensor holds is read, and
-             has no gradient)
+    scale    a number, by default 1 / sqrt(D) (what a tensor holds is read, which
+             waits for a CUDA tensor, and has no gradient)
 
     D is a multiple of 8 up to 128, H at most 256.  Returns a tensor like q,
     dense; a query without any key gets zeros.  Scores and sums are float32;

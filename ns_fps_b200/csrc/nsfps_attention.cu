@@ -766,7 +766,8 @@ attend_tiles(const AttnArgs a) {
         for (uint32_t kk = 0; kk < DP / 16; ++kk)
           mma_ss(tm_s, further(q_desc, (kk >> 2) * (kTileRows * 128u) + (kk & 3u) * 32u),
                  further(k_desc, (kk >> 2) * (64u * 128u) + (kk & 3u) * 32u), kScores, kk != 0u);
-        if (a.hold_cta != (int)blockIdx.x || w != blockIdx.x || i) mma_commit(bar_s);
+        if (a.hold_cta != (int)blockIdx.x || a.hold_step || w != blockIdx.x || i)
+          mma_commit(bar_s);
       }
       __syncwarp();
       wait(bar_s, phase);

@@ -280,7 +280,8 @@ def gather_rows(table, idx, scale: float = 1.0):
 
     table  (N, C), or (B, N, C) for B clouds: float32, float16 or bfloat16
     idx    int64: any shape for (N, C); (B, ...) for (B, N, C)
-    scale  a number (what a tensor holds is read, and has no gradient)
+    scale  a number (what a tensor holds is read, which waits for a CUDA tensor,
+           and has no gradient)
 
     Returns idx.shape + (C,) in the table's type (the product in float32,
     rounded once).  A negative index stands for no row: zeros, and no gradient.

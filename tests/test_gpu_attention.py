@@ -454,16 +454,18 @@ def test_gradients_of_few_keys_of_many_queries(N):
     assert off <= math.sqrt(2 / 3) * u + M * U32, off / u
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M", [16_384, 14_000])
-def test_a_last_turn_of_fewer_clouds(M):
+def test_a_last_turn_of_fewer_clouds(M, dtype):
     """Three clouds whose partial results make turns of two and one: the
     forward's (M = 16,384) or the gradient's (14,000).  The last turn sorts half
     the pairs of a full one (786,432 or 672,000) in its scratch.  Each cloud by
     itself gives the same bits."""
     from ns_fps_b200 import attention
-    B, N, H, G, D, top, block, dtype = 3, 600, 4, 2, 128, 24, 16, torch.bfloat16
+    B, N, H, G, D, top, block = 3, 600, 4, 2, 128, 24, 16
     q, dout = _normal((B, M, H, D), dtype, 1), _normal((B, M, H, D), dtype, 2)
     k, v = _normal((B, N, G, D), dtype, 3), _normal((B, N, G, D), dtype, 4)
+    dout[1] *= 2.0 ** -12  # (in half precision each cloud has its own factor)
     blocks = _lists(B, M, (N + block - 1) // block, top, 5)
 
     def step(*x):
@@ -624,3 +626,37 @@ def test_one_cloud_beyond_the_limit_of_a_turn():
     for got, want, off in zip((dk, dv), sums, offs):
         u = torch.finfo(dtype).eps / 2
         assert bool(((got.double() - want).abs() <= 6 * off + u * want.abs()).all())
+
+
+def test_half_precision_same_bits_again_on_another_stream_and_in_graphs():
+    """The factor of ds comes from maxima that CTAs raise in any order, in the
+    call's own scratch: two captured calls and an eager one side by side."""
+    from ns_fps_b200 import attention
+    q, k, v = _normal((2, 700, 4, 64), torch.float16, 1), _normal((2, 1500, 2, 64), torch.float16, 2), \
+        _normal((2, 1500, 2, 64), torch.float16, 3)
+    blocks, dout = _lists(2, 700, 47, 9, 4), _normal(q.shape, torch.float16, 5)
+
+    def step(size):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = attention.block_attention(*leaves, blocks, 32)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout * size))
+
+    sizes = (1.0, 1e-3)
+    first = [step(s) for s in sizes]
+    graphs = []
+    for s in sizes:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = step(s)
+        graphs.append((graph, kept))
+    side = [torch.cuda.Stream() for _ in sizes]
+    for _ in range(3):
+        for s, (graph, _) in zip(side, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = [step(s) for s in sizes]
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b, c in zip(first[i], graphs[i][1], eager[i]):
+                assert torch.equal(a, b) and torch.equal(a, c)
