@@ -915,7 +915,7 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, uint64_t at, float4
 
 // In the joins.  (Asked for at their beginning, and as a volatile, it took 1 us
 // of each.)
-__device__ __forceinline__ bool some_gave_up(const AttnArgs &a) { return __ldg(a.gave_up) != 0u; }
+__device__ __forceinline__ bool some_gave_up(const AttnArgs &a) { return *a.gave_up != 0u; }
 
 // Joins a query's partials: out = sum_s w_s o_s, w_s = exp2(lse_s - lse), over
 // its leading slots.  A warp takes 128 consecutive elements of a query's heads,
@@ -1240,9 +1240,9 @@ grad_delta(const AttnArgs a) {
   if (!kScaled<T>) return;
   // The rows' maxima: first among the CTA's 32 rows, so that a word of a key
   // head is raised by few (by every row, this kernel took 31 us of a training
-  // step of four clouds; so it takes 9, and 6 without the maxima).  Rows that move no score do not count,
-  // nor do those that are not finite: they spoil their own results, not the
-  // others' factor.
+  // step of four clouds; so it takes 9, and 6 without the maxima).  Rows that
+  // move no score do not count, nor do those that are not finite: they spoil
+  // their own results, not the others' factor.
   __shared__ uint32_t s_word[32];
   __shared__ float2 s_most[32];
   if (sub == 0) {
@@ -1971,9 +1971,10 @@ constexpr uint32_t kGradSpanLog2 = 7;  // one key per lane of tensor memory
 // key head, with all their queries: dk and dv of a key add up over those, and the
 // gradient has no place to keep such sums between turns.  So one cloud of 65,536
 // queries, lists of 16 and eight query heads of 128 on one key head takes 4.3 GB,
-// every slot counted, as the plan cannot know how many lead a pair.  Turns small enough to keep their partials in L2 cost
-// more in launches and half-empty waves than they save: a scan's attention
-// took 199 us in one turn, 207 in two, 267 in four.
+// every slot counted, as the plan cannot know how many lead a pair.  Turns small
+// enough to keep their partials in L2 cost more in launches and half-empty waves
+// than they save: a scan's attention took 199 us in one turn, 207 in two, 267 in
+// four.
 constexpr uint64_t kMaxPartBytes = 1ull << 30;
 
 // How a call is cut up, and its scratch.
@@ -2121,7 +2122,7 @@ cudaError_t run_plan(AttnArgs &a, const AttnPlan &w, cudaStream_t st) {
   const uint32_t shift = 1u << (w.span_log2 - 6);  // key bits of the chunks read
   SortedList list{w.sort.keys0, w.sort.vals0, w.sort.kept};
   cudaError_t err;
-  // (the tile counters and gave_up, the rows' maxima and the spans' marks, cleared together)
+  // (the tile counters and gave_up, the rows' maxima, the spans' marks)
   if ((err = cudaMemsetAsync(w.tile_count, 0, 32 + w.most_bytes + 16 * (uint64_t)spans, st)))
     return err;
   if (n && spans) {
